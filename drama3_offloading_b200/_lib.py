@@ -24,6 +24,7 @@ STATUS = {0: "D3_OK", -1: "D3_ERR_INVALID_ARG", -2: "D3_ERR_NOT_PINNED", -3: "D3
           -7: "D3_ERR_WORKSPACE"}
 D3_POLICY_LRU, D3_POLICY_LFU = 0, 1
 D3_MAX_BUFFERS = 4
+D3_BF16, D3_F16, D3_E4M3 = 0, 1, 2
 
 
 class D3Error(RuntimeError):
@@ -42,6 +43,33 @@ class LayerCache(ctypes.Structure):
         ("host", P * D3_MAX_BUFFERS), ("cache", P * D3_MAX_BUFFERS),
         ("bytes", I64 * D3_MAX_BUFFERS),
     ]
+
+
+class KVCache(ctypes.Structure):
+    """Mirror of ``d3_kv_cache`` (include/d3b200.h)."""
+    _fields_ = [("k", P), ("v", P), ("k_scale", P), ("v_scale", P), ("pages", I32),
+                ("kv_heads", I32), ("page_size", I32), ("head_dim", I32), ("dtype", I32)]
+
+
+class NormRope(ctypes.Structure):
+    """Mirror of ``d3_norm_rope`` (include/d3b200.h)."""
+    _fields_ = [("q", P), ("k", P), ("v", P), ("q_token", I64), ("q_head", I64),
+                ("k_token", I64), ("k_head", I64), ("v_token", I64), ("v_head", I64),
+                ("q_out", P), ("k_out", P), ("q_out_token", I64), ("q_out_head", I64),
+                ("k_out_token", I64), ("k_out_head", I64), ("q_weight", P), ("k_weight", P),
+                ("positions", P), ("inv_freq", P), ("slots", P), ("pos_bytes", I32),
+                ("slot_bytes", I32), ("tokens", I32), ("heads", I32), ("kv_heads", I32),
+                ("head_dim", I32), ("rotary_dim", I32), ("interleaved", I32), ("dtype", I32),
+                ("eps", ctypes.c_float), ("weight_offset", ctypes.c_float)]
+
+
+class Attention(ctypes.Structure):
+    """Mirror of ``d3_attention`` (include/d3b200.h)."""
+    _fields_ = [("q", P), ("q_token", I64), ("q_head", I64), ("out", P), ("out_token", I64),
+                ("out_head", I64), ("page_table", P), ("table_stride", I64), ("kv_lens", P),
+                ("cu_q", P), ("table_pages", I32), ("batch", I32), ("tokens", I32),
+                ("heads", I32), ("max_q", I32), ("max_kv", I32), ("dtype", I32),
+                ("scale", ctypes.c_float)]
 
 
 # name -> (restype, argtypes); every function declared in include/d3b200.h
@@ -85,6 +113,14 @@ SIGNATURES: dict[str, tuple] = {
                                               I64, P]),
     "d3_ep_combine_p2p": (ctypes.c_int, [P, P, P, I32, I32, I32, I32, P, I32, P, I32, P, P, I32,
                                          I64, P]),
+    "d3_kv_write": (ctypes.c_int, [ctypes.POINTER(KVCache), P, I64, I64, P, I64, I64, I32, I32, P,
+                                   I32, P]),
+    "d3_kv_read": (ctypes.c_int, [ctypes.POINTER(KVCache), P, I32, I32, I32, P, P, P]),
+    "d3_qk_norm_rope": (ctypes.c_int, [ctypes.POINTER(NormRope), ctypes.POINTER(KVCache), P]),
+    "d3_paged_attention_workspace_size": (SZ, [ctypes.POINTER(Attention),
+                                               ctypes.POINTER(KVCache)]),
+    "d3_paged_attention": (ctypes.c_int, [ctypes.POINTER(Attention), ctypes.POINTER(KVCache), P, P,
+                                          SZ, P]),
     "d3_census_add": (ctypes.c_int, [P, I32, I32, I32, I32, P, P, P]),
     "d3_trace_append": (ctypes.c_int, [P, I32, I32, I32, I32, P, P, I64, P]),
 }

@@ -50,7 +50,7 @@ def build(force: bool = False, verbose: bool = False) -> Path:
         return LIB
     srcs = [str(s) for s in sources()]
     cmd = [nvcc(), *ARCH, "-O3", "-lineinfo", "-std=c++17", "-shared", "-Xcompiler", "-fPIC",
-           "-Xcompiler", "-fvisibility=hidden", "-cudart", "static", "-Xptxas", "-v",
+           "-Xcompiler", "-fvisibility=hidden", "--threads", "0", "-cudart", "static", "-Xptxas", "-v",
            "-I", str(PKG.parent / "include"), "-o", str(LIB) + ".tmp", *srcs]
     if verbose:
         print(" ".join(cmd), flush=True)

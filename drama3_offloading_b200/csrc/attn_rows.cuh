@@ -1,0 +1,723 @@
+// Attention of few query rows over a paged K/V cache: decode tokens, or a few
+// drafted ones.
+//
+// The rows of one KV head (tokens x the G query heads that share it, at most
+// 8 * NT of them) ride along while the head's keys and values are read once,
+// so the kernel is bound by HBM: D * 2 elements per key against 4 * rows * D
+// operations.  The products are mma.sync with the KEYS as the tall side,
+//
+//   S^T [16 keys x 8 rows]  = K [16 x D] . Q^T        (A = K,   B = Q^T)
+//   O^T [16 dims x 8 rows] += V^T [16 x 16 keys] . P^T (A = V^T, B = P^T)
+//
+// because 8 rows fill the short side exactly, where the usual form would pad
+// them to 16.  (The 128-row tcgen05 form would leave 15/16 of its rows empty;
+// it takes over above 16 rows, attn_chunk.cuh.)  P^T goes from the accumulator
+// layout to the operand layout with one movmatrix per 8 x 8 block.
+//
+// Streaming: one warp issues TMA loads (128-byte swizzle) of KEYS-key tiles of
+// K and V into a ring of 32 KiB slots; each of the other warps takes 16 keys
+// of every tile with a running maximum and sum of its own, so no barrier runs
+// inside the stream; the warps' results are joined once a segment.
+//
+// Split: the tiles of all (sequence, KV head) pairs form one list that is cut
+// into gridDim.x equal parts, so ragged batches load every SM alike.  A part
+// holds whole pairs and at most two pieces of pairs, whose unnormalised sums
+// go to the workspace (two places per CTA) and are joined by
+// attn_rows_join_kernel in the order of the parts: results do not depend on
+// timing.
+//
+// e4m3 caches: codes are exact in fp16, so the products run in fp16 whatever
+// the queries' type.  bf16 queries are scaled by a power of two per row (exact
+// but for elements 2^-24 below the row's largest); a key's scale multiplies
+// its scores in fp32; a value's scale, over the largest of the warp's 16 keys,
+// multiplies the probability before it is rounded to fp16.
+#pragma once
+
+#include "kv_common.cuh"
+
+#include <cuda.h>
+
+#include <type_traits>
+
+namespace d3 {
+
+constexpr uint64_t kAttnWaitBudgetNs = 2000000000ull;
+constexpr int kAttnErrRowsLoad = 51, kAttnErrRowsUse = 52;
+
+struct AttnParams {
+  const void* q;                 // [tokens][heads][D]
+  long long q_token, q_head;     // strides in elements
+  void* out;
+  long long out_token, out_head;
+  const int* table;              // [batch][table_stride] page ids
+  long long table_stride;
+  int table_pages;               // usable entries of a table row
+  const int* kv_lens;            // [batch]
+  const int* cu_q;               // [batch + 1], or NULL: one row a sequence
+  int batch, tokens, heads, group, kv_heads;
+  int page_size, page_shift, pages;
+  const float *k_scale, *v_scale;
+  float scale_log2;              // softmax scale * log2(e)
+  int min_rows, max_rows;        // sequences this launch takes, by new tokens * group
+  float* ws_o;                   // partial sums
+  float* ws_ml;                  // their maxima and sums
+  int* err;
+};
+
+__device__ __forceinline__ void attn_error(int* err, int code) { atomicCAS(err, 0, code); }
+
+struct AttnSeq {
+  int q0, n, kv, rows;           // first query token, new tokens, keys, rows of a KV head
+};
+__device__ __forceinline__ AttnSeq attn_seq(const AttnParams& p, int b) {
+  AttnSeq s;
+  if (p.cu_q) {
+    s.q0 = p.cu_q[b];
+    s.n = p.cu_q[b + 1] - s.q0;
+  } else {
+    s.q0 = b;
+    s.n = 1;
+  }
+  // offsets outside the query tensor (a broken cu_q) are cut to it
+  if (s.q0 < 0 || s.q0 > p.tokens) s.n = 0;
+  else s.n = max(0, min(s.n, p.tokens - s.q0));
+  s.kv = max(0, min(p.kv_lens[b], p.table_pages * p.page_size));
+  s.rows = s.n * p.group;
+  return s;
+}
+
+template <typename T, int D, bool E4, int NT>
+struct RowsCfg {
+  static constexpr int ES = E4 ? 1 : 2;                     // bytes of a cached element
+  static constexpr int WARPS = (D == 256 && !E4) ? 4 : 8;   // consumer warps
+  static constexpr int KEYS = 16 * WARPS;
+  static constexpr int THREADS = 32 * (WARPS + 1);
+  static constexpr int COLS = D * ES / 128;                 // 128-byte columns of a row
+  static constexpr int ROWS = 8 * NT;
+  static constexpr int SLOT = KEYS * D * ES;                // 32 KiB, 16 KiB for D = 128 codes
+  static constexpr int SCALES = E4 ? KEYS * 4 : 0;
+  static constexpr int QFRAG = NT * D * 16;
+  // warps' results are joined DC dims at a time through 32 KiB
+  static constexpr int DC = (32 * 1024) / (WARPS * ROWS * 4) < D ? (32 * 1024) / (WARPS * ROWS * 4) : D;
+  static constexpr int JOIN_PITCH = DC + 4;
+  static constexpr int JOIN = WARPS * ROWS * JOIN_PITCH * 4;
+  static constexpr int SLOTS = (222 * 1024 - QFRAG - JOIN) / (SLOT + SCALES) < 10
+                                   ? (222 * 1024 - QFRAG - JOIN) / (SLOT + SCALES) : 10;
+  static constexpr int ML = WARPS * ROWS * 2 * 4;
+  static constexpr size_t SMEM = 1024 + (size_t)SLOTS * (SLOT + SCALES) + QFRAG + JOIN + ML + 4 * ROWS + 256;
+  static_assert(SLOTS >= 4, "the ring needs two tiles in flight");
+};
+
+// where a launch's part begins, and how the pairs lie in the list
+struct RowsWork {
+  long long total, begin;
+  int count, b;
+  long long off;                 // of `begin` inside sequence b
+};
+
+__device__ __forceinline__ int rows_tiles(int kv, int keys) { return max(1, (kv + keys - 1) / keys); }
+
+// tiles of sequence b over all of its KV heads and row groups
+__device__ __forceinline__ long long rows_units(const AttnParams& p, int b, int keys, int rows_per) {
+  const AttnSeq s = attn_seq(p, b);
+  if (s.rows == 0 || s.rows < p.min_rows || s.rows > p.max_rows) return 0;
+  return (long long)rows_tiles(s.kv, keys) * p.kv_heads * ((s.rows + rows_per - 1) / rows_per);
+}
+
+// All threads of the CTA: the list's length and, for list position `at(total)`,
+// its sequence.  s_scan: 33 long longs of shared memory.
+template <typename F>
+__device__ RowsWork rows_plan(const AttnParams& p, int keys, int rows_per, long long* s_scan, F part) {
+  const int n = blockDim.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int per = (p.batch + n - 1) / n;
+  const int b0 = min(p.batch, tid * per), b1 = min(p.batch, b0 + per);
+  long long sum = 0;
+  for (int b = b0; b < b1; ++b) sum += rows_units(p, b, keys, rows_per);
+  long long inc = sum;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const long long v = __shfl_up_sync(0xffffffffu, inc, o);
+    if (lane >= o) inc += v;
+  }
+  __shared__ int s_b;
+  __shared__ long long s_off;
+  if (lane == 31) s_scan[warp] = inc;
+  if (tid == 0) s_b = p.batch;
+  __syncthreads();
+  long long before = inc - sum, total = 0;
+  for (int w = 0; w < (n + 31) / 32; ++w) {
+    if (w < warp) before += s_scan[w];
+    total += s_scan[w];
+  }
+  RowsWork r;
+  r.total = total;
+  part(r);
+  if (r.count > 0 && before <= r.begin && r.begin < before + sum) {
+    long long at = before;
+    for (int b = b0; b < b1; ++b) {
+      const long long u = rows_units(p, b, keys, rows_per);
+      if (r.begin < at + u) {
+        s_b = b;
+        s_off = r.begin - at;
+        break;
+      }
+      at += u;
+    }
+  }
+  __syncthreads();
+  r.b = s_b;
+  r.off = s_off;
+  return r;
+}
+
+// One piece of a (sequence, KV head, row group): tiles [t0, t1) of nt.
+struct RowsPiece {
+  AttnSeq s;
+  int b, head, rg, t0, t1, nt;
+};
+// Walks a part of the list piece by piece.
+struct RowsWalk {
+  int b, left;
+  long long off;
+  __device__ __forceinline__ bool next(const AttnParams& p, int keys, int rows_per, RowsPiece& w) {
+    if (left <= 0) return false;
+    while (b < p.batch) {
+      w.s = attn_seq(p, b);
+      if (w.s.rows > 0 && w.s.rows >= p.min_rows && w.s.rows <= p.max_rows) {
+        w.nt = rows_tiles(w.s.kv, keys);
+        const int groups = (w.s.rows + rows_per - 1) / rows_per;
+        const long long units = (long long)w.nt * p.kv_heads * groups;
+        if (off < units) {
+          const int hg = (int)(off / w.nt);
+          w.b = b;
+          w.head = hg / groups;
+          w.rg = hg - w.head * groups;
+          w.t0 = (int)(off - (long long)hg * w.nt);
+          w.t1 = min(w.nt, w.t0 + left);
+          left -= w.t1 - w.t0;
+          off += w.t1 - w.t0;
+          return true;
+        }
+      }
+      ++b;
+      off = 0;
+    }
+    return false;
+  }
+};
+
+__device__ __forceinline__ void ldsm4(uint32_t addr, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void ldsm4t(uint32_t addr, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ uint32_t movm(uint32_t a) {
+  uint32_t d;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
+  return d;
+}
+template <typename T>
+__device__ __forceinline__ void mma16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2,
+                                      uint32_t a3, uint32_t b0, uint32_t b1);
+template <>
+__device__ __forceinline__ void mma16<__nv_bfloat16>(float (&c)[4], uint32_t a0, uint32_t a1,
+                                                     uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+               : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+template <>
+__device__ __forceinline__ void mma16<__half>(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2,
+                                              uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+               : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// 16-byte piece x (of 8 a 128-byte column) of a key's row in a swizzled tile
+// of `keys` rows per column
+__device__ __forceinline__ uint32_t tile_piece(uint32_t base, int keys, int key, int piece) {
+  return base + (uint32_t)(piece >> 3) * (keys * 128) + key * 128 + (((piece ^ key) & 7) << 4);
+}
+
+__device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+               ::"r"(smem_u32(dst)), "l"(src), "r"(bytes), "r"(smem_u32(bar)) : "memory");
+}
+
+__device__ __forceinline__ float ex2(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+
+template <typename T, int D, bool E4, int NT>
+__global__ void __launch_bounds__(RowsCfg<T, D, E4, NT>::THREADS, 1)
+    attn_rows_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
+                     const __grid_constant__ AttnParams p) {
+  using C = RowsCfg<T, D, E4, NT>;
+  using M = typename std::conditional<E4, __half, T>::type;   // operand type of the products
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ long long s_scan[33];
+  uint8_t* smem = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
+  uint8_t* s_slots = smem;
+  float* s_scales = reinterpret_cast<float*>(smem + (size_t)C::SLOTS * C::SLOT);   // [SLOTS][KEYS]
+  uint2* s_q = reinterpret_cast<uint2*>(smem + (size_t)C::SLOTS * (C::SLOT + C::SCALES));
+  float* s_join = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(s_q) + C::QFRAG);
+  float* s_ml = s_join + C::JOIN / 4;                          // [WARPS][ROWS][2]
+  float* s_qs = s_ml + C::ML / 4;                              // [ROWS] scale of a row's scores
+  uint64_t* full = reinterpret_cast<uint64_t*>(s_qs + C::ROWS + (C::ROWS & 1));
+  uint64_t* empty = full + C::SLOTS;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  if (tid == 0) {
+    for (int i = 0; i < C::SLOTS; ++i) {
+      mbar_init(full + i, 1);
+      mbar_init(empty + i, C::WARPS);
+    }
+    fence_barrier_init();
+    tma_prefetch_desc(&tm_k);
+    tma_prefetch_desc(&tm_v);
+  }
+  pdl_trigger();
+  pdl_wait();
+  const RowsWork work = rows_plan(p, C::KEYS, C::ROWS, s_scan, [&](RowsWork& r) {
+    // no part is empty: a pair's parts are neighbours in the workspace
+    const long long g = min((long long)gridDim.x, r.total), c = blockIdx.x;
+    r.begin = c < g ? r.total * c / g : 0;
+    r.count = c < g ? (int)(r.total * (c + 1) / g - r.begin) : 0;
+  });
+  if (work.count == 0) return;
+  RowsWalk walk{work.b, work.count, work.off};
+  RowsPiece w;
+  if (warp == C::WARPS) {
+    // ---- the loading warp: K tile, V tile, K tile, ...
+    int slot = 0;
+    uint32_t phase = 0;
+    bool ok = true;
+    const int box = min(p.page_size, C::KEYS), boxes = C::KEYS / box;
+    while (walk.next(p, C::KEYS, C::ROWS, w)) {
+      for (int t = w.t0; t < w.t1; ++t) {
+        const int key0 = t * C::KEYS;
+        // keys of this tile in whole boxes: what lies behind is never loaded
+        const int need = min(boxes, (max(0, w.s.kv - key0) + box - 1) / box);
+        // lane i: page of box i (at most KEYS / 16 = 8 boxes)
+        int row = -1;
+        if (lane < need) {
+          const int key = key0 + lane * box;
+          const int page = p.table[(long long)w.b * p.table_stride + (key >> p.page_shift)];
+          if (page >= 0 && page < p.pages)
+            row = ((page * p.kv_heads + w.head) << p.page_shift) + (key & (p.page_size - 1));
+        }
+        const int scales_ok = __popc(__ballot_sync(0xffffffffu, row >= 0));
+#pragma unroll
+        for (int kv = 0; kv < 2; ++kv) {
+          if (ok && !mbar_wait(empty + slot, phase ^ 1, kAttnWaitBudgetNs)) {
+            if (lane == 0) attn_error(p.err, kAttnErrRowsLoad);
+            ok = false;
+          }
+          ok = __all_sync(0xffffffffu, ok);
+          if (!ok) break;
+          uint8_t* dst = s_slots + (size_t)slot * C::SLOT;
+          float* sdst = s_scales + slot * C::KEYS;
+          if (E4 && lane < need && row < 0)
+            for (int i = 0; i < box; ++i) sdst[lane * box + i] = 0.f;
+          __syncwarp();
+          if (lane == 0)
+            mbar_arrive_expect_tx(full + slot, need * box * D * C::ES + (E4 ? scales_ok * box * 4 : 0));
+          __syncwarp();
+          // a page id outside the cache is loaded from outside the map: zeros
+          for (int i0 = 0; i0 < need * C::COLS; i0 += 32) {
+            const int i = i0 + lane, bx = i / C::COLS, col = i - bx * C::COLS;
+            const int r = __shfl_sync(0xffffffffu, row, bx);
+            if (bx < need)
+              tma_load_2d(dst + col * (C::KEYS * 128) + bx * box * 128, kv ? &tm_v : &tm_k, full + slot,
+                          col * (128 / C::ES), r < 0 ? -box : r);
+          }
+          __syncwarp();
+          if (E4 && lane < need && row >= 0)
+            bulk_load(sdst + lane * box, (kv ? p.v_scale : p.k_scale) + row, box * 4, full + slot);
+          if (++slot == C::SLOTS) { slot = 0; phase ^= 1; }
+        }
+        if (!ok) break;
+      }
+      if (!ok) break;
+    }
+    if (!ok) {
+      // what is still in flight has landed before the CTA's memory goes
+      for (int i = 0; i < C::SLOTS; ++i) mbar_wait(full + i, phase ^ (i < slot ? 0 : 1), kAttnWaitBudgetNs);
+    }
+    return;
+  }
+
+  // ---- the other warps: 16 keys of every tile
+  const int g = lane >> 2, t4 = lane & 3;
+  int slot = 0;
+  uint32_t phase = 0;
+  bool ok = true;
+  auto bar = [&]() { asm volatile("bar.sync 1, %0;" ::"r"(C::WARPS * 32) : "memory"); };
+  auto take = [&]() {
+    if (ok && !mbar_wait(full + slot, phase, kAttnWaitBudgetNs)) {
+      if (lane == 0) attn_error(p.err, kAttnErrRowsUse);
+      ok = false;
+    }
+    ok = __all_sync(0xffffffffu, ok);
+  };
+  auto give = [&]() {
+    __syncwarp();
+    if (lane == 0) mbar_arrive(empty + slot);
+    if (++slot == C::SLOTS) { slot = 0; phase ^= 1; }
+  };
+  while (walk.next(p, C::KEYS, C::ROWS, w)) {
+    const int row0 = w.rg * C::ROWS, rows = min(C::ROWS, w.s.rows - row0);
+    // queries in operand order: s_q[nt][kk][lane] holds the two registers of
+    // B for k-step kk.  Codes come out of ldmatrix four dims to a lane, so
+    // there the lane's k positions stand for dims 4t .. 4t + 3.
+    bar();   // the piece before has read s_q and s_join
+    for (int r = warp; r < C::ROWS; r += C::WARPS) {
+      const int gr = row0 + r, tok = w.s.q0 + gr / p.group, hd = w.head * p.group + gr % p.group;
+      const T* src = static_cast<const T*>(p.q) + (long long)tok * p.q_token + (long long)hd * p.q_head;
+      // lane's share: 8 dims at a time, D / 8 chunks
+      float amax = 0.f;
+      uint4 u = make_uint4(0, 0, 0, 0);
+      if (r < rows && lane < D / 8) u = *reinterpret_cast<const uint4*>(src + lane * 8);
+      float x[8];
+      unpack8<T>(u, x);
+      float mul = 1.f, back = 1.f;
+      if (E4 && std::is_same<T, __nv_bfloat16>::value) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) amax = fmaxf(amax, fabsf(x[i]));
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+        // amax in [2^(e-1), 2^e); the factor's exponent stays inside fp32's
+        int e = 0;
+        if (amax > 0.f && amax < INFINITY) frexpf(amax, &e);
+        e = max(-120, min(120, e));
+        mul = ldexpf(1.f, -e);
+        back = ldexpf(1.f, e);
+      }
+      if (lane == 0) s_qs[r] = p.scale_log2 * back;
+      if (lane < D / 8) {
+        const uint4 o = make_uint4(Elem<M>::from_f2(x[0] * mul, x[1] * mul), Elem<M>::from_f2(x[2] * mul, x[3] * mul),
+                                   Elem<M>::from_f2(x[4] * mul, x[5] * mul), Elem<M>::from_f2(x[6] * mul, x[7] * mul));
+        const uint32_t ow[4] = {o.x, o.y, o.z, o.w};
+        uint32_t* fr = reinterpret_cast<uint32_t*>(s_q + (r / 8) * (D / 16) * 32);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int d = lane * 8 + 2 * i, kk = d >> 4, in = (d & 15) >> 1;    // pair 0..7 of the k-step
+          const int tt = E4 ? in >> 1 : in & 3, half = E4 ? in & 1 : in >> 2;
+          fr[(kk * 32 + (r & 7) * 4 + tt) * 2 + half] = ow[i];
+        }
+      }
+    }
+    bar();
+    float o[NT][D / 16][4];
+    float mx[NT][2], sum[NT][2], cs[NT][2];
+    int last[NT][2];     // last key a row sees
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+#pragma unroll
+      for (int i = 0; i < D / 16; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) o[n][i][j] = 0.f;
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const int r = n * 8 + 2 * t4 + j;
+        mx[n][j] = -INFINITY;
+        sum[n][j] = 0.f;
+        cs[n][j] = s_qs[r];
+        last[n][j] = r < rows ? w.s.kv - w.s.n + (row0 + r) / p.group : -1;
+      }
+    }
+    const int lk = lane & 7, lm = lane >> 3;     // ldmatrix: row and matrix of this lane
+    for (int t = w.t0; t < w.t1; ++t) {
+      const int key0 = t * C::KEYS + warp * 16;  // this warp's keys
+      take();
+      const uint32_t kb = smem_u32(s_slots + (size_t)slot * C::SLOT);
+      float s[NT][4];
+      float ks0 = 1.f, ks1 = 1.f;
+      if (ok && key0 < w.s.kv) {
+        float s2[NT][2][4];
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int c = 0; c < 2; ++c)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) s2[n][c][j] = 0.f;
+        if (E4) {
+#pragma unroll
+          for (int kk = 0; kk < D / 16; kk += 2) {
+            uint32_t r[4];
+            ldsm4(tile_piece(kb, C::KEYS, warp * 16 + (lm & 1) * 8 + lk, kk + (lm >> 1)), r);
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+              const uint32_t a0 = e4m3x2_to_h2((uint16_t)r[2 * c]), a2 = e4m3x2_to_h2((uint16_t)(r[2 * c] >> 16));
+              const uint32_t a1 = e4m3x2_to_h2((uint16_t)r[2 * c + 1]), a3 = e4m3x2_to_h2((uint16_t)(r[2 * c + 1] >> 16));
+#pragma unroll
+              for (int n = 0; n < NT; ++n) {
+                const uint2 b = s_q[(n * (D / 16) + kk + c) * 32 + lane];
+                mma16<M>(s2[n][c], a0, a1, a2, a3, b.x, b.y);
+              }
+            }
+          }
+          ks0 = s_scales[slot * C::KEYS + warp * 16 + g];
+          ks1 = s_scales[slot * C::KEYS + warp * 16 + g + 8];
+        } else {
+#pragma unroll
+          for (int kk = 0; kk < D / 16; ++kk) {
+            uint32_t r[4];
+            ldsm4(tile_piece(kb, C::KEYS, warp * 16 + (lm & 1) * 8 + lk, 2 * kk + (lm >> 1)), r);
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+              const uint2 b = s_q[(n * (D / 16) + kk) * 32 + lane];
+              mma16<M>(s2[n][kk & 1], r[0], r[1], r[2], r[3], b.x, b.y);
+            }
+          }
+        }
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) s[n][j] = s2[n][0][j] + s2[n][1][j];
+      }
+      give();
+      take();
+      if (ok && key0 < w.s.kv) {
+        const uint32_t vb = smem_u32(s_slots + (size_t)slot * C::SLOT);
+        float u0 = 1.f, u1 = 1.f, vmax = 1.f;
+        if (E4) {
+          // values' scales over the largest of the 16 keys'
+          u0 = key0 + g < w.s.kv ? s_scales[slot * C::KEYS + warp * 16 + g] : 0.f;
+          u1 = key0 + g + 8 < w.s.kv ? s_scales[slot * C::KEYS + warp * 16 + g + 8] : 0.f;
+          vmax = fmaxf(u0, u1);
+#pragma unroll
+          for (int x = 4; x < 32; x <<= 1) vmax = fmaxf(vmax, __shfl_xor_sync(0xffffffffu, vmax, x));
+          const float inv = vmax > 0.f ? 1.f / vmax : 0.f;
+          u0 *= inv;
+          u1 *= inv;
+        }
+        uint32_t pb[NT][2];
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          float pr[4];
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            const float a = key0 + g <= last[n][j] ? s[n][j] * (cs[n][j] * ks0) : -INFINITY;
+            const float b = key0 + g + 8 <= last[n][j] ? s[n][2 + j] * (cs[n][j] * ks1) : -INFINITY;
+            float m = fmaxf(a, b);
+#pragma unroll
+            for (int x = 4; x < 32; x <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, x));
+            m = fmaxf(m, mx[n][j]);
+            const float base = m == -INFINITY ? 0.f : m;
+            const float keep = ex2(mx[n][j] - base);
+            mx[n][j] = m;
+            const float pa = ex2(a - base), pc = ex2(b - base);
+            sum[n][j] = fmaf(sum[n][j], keep, pa + pc);
+            pr[j] = pa * u0;
+            pr[2 + j] = pc * u1;
+            if (keep != 1.f) {
+#pragma unroll
+              for (int i = 0; i < D / 16; ++i) {
+                o[n][i][j] *= keep;
+                o[n][i][2 + j] *= keep;
+              }
+            }
+          }
+          __syncwarp();
+          pb[n][0] = movm(Elem<M>::from_f2(pr[0], pr[1]));
+          pb[n][1] = movm(Elem<M>::from_f2(pr[2], pr[3]));
+        }
+        // values of keys behind the sequence's end are whatever the page
+        // held: cut to zero, 0 * NaN is no zero
+        const bool tail = key0 + 16 > w.s.kv;
+        uint32_t cut0 = ~0u, cut1 = ~0u;
+        if (tail) {
+          const int k2 = key0 + 2 * t4;
+          cut0 = (k2 < w.s.kv ? 0xffffu : 0u) | (k2 + 1 < w.s.kv ? 0xffff0000u : 0u);
+          cut1 = (k2 + 8 < w.s.kv ? 0xffffu : 0u) | (k2 + 9 < w.s.kv ? 0xffff0000u : 0u);
+        }
+        if (E4) {
+          // one 8 x 8 block of code pairs holds 16 dims: dim 2g in the even
+          // bytes, 2g + 1 in the odd ones
+#pragma unroll
+          for (int i = 0; i < D / 16; i += 2) {
+            uint32_t r[4];
+            ldsm4t(tile_piece(vb, C::KEYS, warp * 16 + (lm & 1) * 8 + lk, i + (lm >> 1)), r);
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+              const uint32_t x = __byte_perm(r[2 * c], 0, 0x3120), y = __byte_perm(r[2 * c + 1], 0, 0x3120);
+              const uint32_t a0 = e4m3x2_to_h2((uint16_t)x) & cut0, a1 = e4m3x2_to_h2((uint16_t)(x >> 16)) & cut0;
+              const uint32_t a2 = e4m3x2_to_h2((uint16_t)y) & cut1, a3 = e4m3x2_to_h2((uint16_t)(y >> 16)) & cut1;
+#pragma unroll
+              for (int n = 0; n < NT; ++n) {
+                float z[4] = {0.f, 0.f, 0.f, 0.f};
+                mma16<M>(z, a0, a1, a2, a3, pb[n][0], pb[n][1]);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) o[n][i + c][j] = fmaf(z[j], vmax, o[n][i + c][j]);
+              }
+            }
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < D / 16; ++i) {
+            uint32_t r[4];
+            ldsm4t(tile_piece(vb, C::KEYS, warp * 16 + (lm >> 1) * 8 + lk, 2 * i + (lm & 1)), r);
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+              mma16<M>(o[n][i], r[0] & cut0, r[1] & cut0, r[2] & cut1, r[3] & cut1, pb[n][0], pb[n][1]);
+          }
+        }
+      }
+      give();
+    }
+    // ---- join the warps: out, or this CTA's place in the workspace
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        float v = sum[n][j];
+#pragma unroll
+        for (int x = 4; x < 32; x <<= 1) v += __shfl_xor_sync(0xffffffffu, v, x);
+        if (g == 0) {
+          float* ml = s_ml + (warp * C::ROWS + n * 8 + 2 * t4 + j) * 2;
+          ml[0] = mx[n][j];
+          ml[1] = v;
+        }
+      }
+    bar();
+    const bool whole = w.t0 == 0 && w.t1 == w.nt;
+    const int place = blockIdx.x * 2 + (w.t0 == 0 ? 1 : 0);
+    float* wo = p.ws_o + (size_t)place * C::ROWS * D;
+    float f[NT][2];    // this warp's factor of its rows
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const int r = n * 8 + 2 * t4 + j;
+        float m = -INFINITY;
+        for (int x = 0; x < C::WARPS; ++x) m = fmaxf(m, s_ml[(x * C::ROWS + r) * 2]);
+        float l = 0.f;
+        for (int x = 0; x < C::WARPS; ++x) {
+          const float mw = s_ml[(x * C::ROWS + r) * 2];
+          if (mw != -INFINITY) l += s_ml[(x * C::ROWS + r) * 2 + 1] * ex2(mw - m);
+        }
+        f[n][j] = mx[n][j] == -INFINITY ? 0.f : ex2(mx[n][j] - m);
+        if (whole) f[n][j] = l > 0.f ? f[n][j] / l : 0.f;
+        else if (warp == 0 && g == 0) {
+          p.ws_ml[(place * C::ROWS + r) * 2] = m;
+          p.ws_ml[(place * C::ROWS + r) * 2 + 1] = l;
+        }
+      }
+#pragma unroll
+    for (int d0 = 0; d0 < D; d0 += C::DC) {
+      if (d0) bar();
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int i = 0; i < C::DC / 16; ++i)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            // code blocks: dims 2g and 2g + 1 are rows g and g + 8
+            const int d = i * 16 + (E4 ? 2 * g + (j >> 1) : g + (j >> 1) * 8);
+            const int r = n * 8 + 2 * t4 + (j & 1);
+            const float v = o[n][d0 / 16 + i][j];
+            s_join[(warp * C::ROWS + r) * C::JOIN_PITCH + d] = f[n][j & 1] == 0.f ? 0.f : v * f[n][j & 1];
+          }
+      bar();
+      for (int i = tid; i < rows * (C::DC / 4); i += C::WARPS * 32) {
+        const int r = i / (C::DC / 4), d = (i - r * (C::DC / 4)) * 4;
+        float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int x = 0; x < C::WARPS; ++x) {
+          const float4 v = *reinterpret_cast<const float4*>(s_join + (x * C::ROWS + r) * C::JOIN_PITCH + d);
+          a.x += v.x;
+          a.y += v.y;
+          a.z += v.z;
+          a.w += v.w;
+        }
+        if (whole) {
+          const int gr = row0 + r;
+          T* dst = static_cast<T*>(p.out) + (long long)(w.s.q0 + gr / p.group) * p.out_token +
+                   (long long)(w.head * p.group + gr % p.group) * p.out_head + d0 + d;
+          *reinterpret_cast<uint2*>(dst) = make_uint2(Elem<T>::from_f2(a.x, a.y), Elem<T>::from_f2(a.z, a.w));
+        } else {
+          *reinterpret_cast<float4*>(wo + (size_t)r * D + d0 + d) = a;
+        }
+      }
+    }
+  }
+}
+
+// One CTA per (sequence, KV head, row group): those that the list was cut
+// inside of are the sum of their parts, in the parts' order.  The workspace is
+// read through L2: launched early, this kernel shares SMs with the join of the
+// call before, whose lines of the same memory may still be in L1.
+template <typename T, int D>
+__global__ void __launch_bounds__(128) attn_rows_join_kernel(const __grid_constant__ AttnParams p, int keys,
+                                                             int rows_per, int parts, int groups_max) {
+  __shared__ long long s_scan[33];
+  pdl_trigger();
+  pdl_wait();
+  const int b = blockIdx.x / (p.kv_heads * groups_max), rest = blockIdx.x - b * p.kv_heads * groups_max;
+  const int head = rest / groups_max, rg0 = rest - head * groups_max;
+  const AttnSeq s = attn_seq(p, b);
+  if (s.rows == 0 || s.rows < p.min_rows || s.rows > p.max_rows) return;
+  const int groups = (s.rows + rows_per - 1) / rows_per, nt = rows_tiles(s.kv, keys);
+  if (nt == 1 || rg0 >= groups) return;
+  // units before sequence b, and in all
+  const int tid = threadIdx.x;
+  long long mine = 0, all = 0;
+  for (int i = tid; i < p.batch; i += blockDim.x) {
+    const long long u = rows_units(p, i, keys, rows_per);
+    all += u;
+    if (i < b) mine += u;
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    mine += __shfl_xor_sync(0xffffffffu, mine, o);
+    all += __shfl_xor_sync(0xffffffffu, all, o);
+  }
+  if ((tid & 31) == 0) {
+    s_scan[tid >> 5] = mine;
+    s_scan[4 + (tid >> 5)] = all;
+  }
+  __syncthreads();
+  mine = s_scan[0] + s_scan[1] + s_scan[2] + s_scan[3];
+  all = s_scan[4] + s_scan[5] + s_scan[6] + s_scan[7];
+  const long long cut = min((long long)parts, all);
+  for (int rg = rg0; rg < groups; rg += groups_max) {
+    const long long u0 = mine + ((long long)head * groups + rg) * nt, u1 = u0 + nt - 1;
+    const int c0 = (int)(((u0 + 1) * cut - 1) / all), c1 = (int)(((u1 + 1) * cut - 1) / all);
+    if (c0 == c1) continue;          // one part held it whole
+    const int row0 = rg * rows_per, rows = min(rows_per, s.rows - row0);
+    for (int i = tid; i < rows * (D / 4); i += blockDim.x) {
+      const int r = i / (D / 4), d = (i - r * (D / 4)) * 4;
+      float m = -INFINITY;
+      for (int c = c0; c <= c1; ++c)
+        m = fmaxf(m, __ldcg(p.ws_ml + (((size_t)c * 2 + (c == c0)) * rows_per + r) * 2));
+      float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+      float l = 0.f;
+      for (int c = c0; c <= c1; ++c) {
+        const size_t at = ((size_t)c * 2 + (c == c0)) * rows_per + r;
+        const float mc = __ldcg(p.ws_ml + at * 2);
+        if (mc == -INFINITY) continue;
+        const float f = ex2(mc - m);
+        const float4 v = __ldcg(reinterpret_cast<const float4*>(p.ws_o + at * D + d));
+        l = fmaf(__ldcg(p.ws_ml + at * 2 + 1), f, l);
+        a.x = fmaf(v.x, f, a.x);
+        a.y = fmaf(v.y, f, a.y);
+        a.z = fmaf(v.z, f, a.z);
+        a.w = fmaf(v.w, f, a.w);
+      }
+      const float inv = l > 0.f ? 1.f / l : 0.f;
+      const int gr = row0 + r;
+      T* dst = static_cast<T*>(p.out) + (long long)(s.q0 + gr / p.group) * p.out_token +
+               (long long)(head * p.group + gr % p.group) * p.out_head + d;
+      *reinterpret_cast<uint2*>(dst) = make_uint2(Elem<T>::from_f2(a.x * inv, a.y * inv),
+                                                  Elem<T>::from_f2(a.z * inv, a.w * inv));
+    }
+  }
+}
+
+}  // namespace d3

@@ -2,6 +2,7 @@
 // the sm_100a PTX wrappers (mbarrier, TMA, tcgen05) the kernels use.
 #pragma once
 
+#include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
@@ -35,6 +36,13 @@ inline int launch_status(const char* what) {
   cudaError_t e = cudaGetLastError();
   return e == cudaSuccess ? D3_OK : cuda_fail(e, what);
 }
+
+// cuTensorMapEncodeTiled of the driver (NULL when it has none)
+typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*,
+                                  const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
+                                  const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                                  CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+EncodeTiledFn encode_fn();
 
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 

@@ -52,6 +52,8 @@ ERROR_CODES = {
     31: "expert parallel: a source rank's dispatch never arrived",
     32: "expert parallel: a serving rank's returned rows never arrived",
     41: "decode overlap: a fetched expert's bytes never landed",
+    51: "paged attention, few rows: the loading warp waited for a free slot",
+    52: "paged attention, few rows: a warp waited for a loaded tile",
 }
 
 

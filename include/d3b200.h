@@ -383,6 +383,101 @@ D3_API int d3_ep_combine_p2p(const void* ret, const int32_t* src_slot, const voi
                              const int64_t* epoch, int32_t* err_word, int32_t code,
                              int64_t budget_ns, d3_stream_t stream);
 
+/* ---------------------------------------------------------- paged K/V cache */
+
+enum { D3_BF16 = 0, D3_F16 = 1, D3_E4M3 = 2 };
+
+/* One layer's paged K/V cache.  Page p holds page_size tokens of every KV
+ * head; a token's slot is page * page_size + offset.  E4M3 rows are codes with
+ * one fp32 scale per (token, head): value = code * scale.  Plain data, filled
+ * by the caller; the library never stores it.
+ * Limits: head_dim 128 or 256, page_size 16, 32, 64 or 128,
+ * pages * kv_heads * page_size < 2^31.
+ * The reference keeps its K/V state in upstream fish-speech's dense buffers
+ * (snapshots of them: bin/prefix_kv.py:184-339); it has no paged or quantised
+ * cache. */
+typedef struct d3_kv_cache {
+  void* k;                  /* [pages][kv_heads][page_size][head_dim] */
+  void* v;
+  float* k_scale;           /* [pages][kv_heads][page_size], E4M3 only */
+  float* v_scale;
+  int32_t pages, kv_heads, page_size, head_dim;
+  int32_t dtype;            /* D3_BF16, D3_F16 or D3_E4M3 */
+} d3_kv_cache;
+
+/* Put the rows k, v ([tokens][kv_heads][head_dim], bf16 or fp16, strides in
+ * elements, multiples of 8, rows 16-byte aligned) into the cache's slots
+ * (int32 or int64 [tokens]).  A 16-bit cache takes rows of its own type; an
+ * E4M3 cache quantises them: scale = max|row| / 448 (1 for a row of zeros),
+ * code = e4m3(row / scale), both divisions rounded in fp32.  Slots outside the
+ * cache are skipped; the slots of one call are distinct. */
+D3_API int d3_kv_write(const d3_kv_cache* cache, const void* k, int64_t k_token, int64_t k_head,
+                       const void* v, int64_t v_token, int64_t v_head, int32_t dtype,
+                       int32_t tokens, const void* slots, int32_t slot_bytes,
+                       d3_stream_t stream);
+
+/* The rows at `slots`, as 16-bit values (code * scale rounded once), into the
+ * contiguous k_out, v_out [tokens][kv_heads][head_dim].  Slots outside the
+ * cache read as zeros. */
+D3_API int d3_kv_read(const d3_kv_cache* cache, const void* slots, int32_t slot_bytes,
+                      int32_t tokens, int32_t dtype, void* k_out, void* v_out,
+                      d3_stream_t stream);
+
+/* Norm of every query and key head, then the rotation by position:
+ *   y = x / sqrt(mean(x^2) + eps) * (weight + weight_offset)
+ * and the first rotary_dim dims of y, in pairs (i, i + rotary_dim / 2) or,
+ * interleaved, (2i, 2i + 1), turned by position * inv_freq[i] (the angle in
+ * fp64).  rotary_dim: a multiple of 16 up to head_dim.  Rows as for
+ * d3_kv_write.  With a cache, K (rounded once, from fp32) and V go into its
+ * `slots` in the same launch and k_out is not used; without one, v and slots
+ * are not.  q_out may be q itself, and k_out k.  No counterpart in the
+ * reference (upstream fish-speech's attention does it in separate torch
+ * calls). */
+typedef struct d3_norm_rope {
+  const void *q, *k, *v;
+  int64_t q_token, q_head, k_token, k_head, v_token, v_head;
+  void *q_out, *k_out;
+  int64_t q_out_token, q_out_head, k_out_token, k_out_head;
+  const void *q_weight, *k_weight;      /* [head_dim], the rows' type */
+  const void* positions;                /* int32 or int64 [tokens] */
+  const double* inv_freq;               /* [rotary_dim / 2] */
+  const void* slots;                    /* int32 or int64 [tokens] */
+  int32_t pos_bytes, slot_bytes;
+  int32_t tokens, heads, kv_heads, head_dim, rotary_dim, interleaved, dtype;
+  float eps, weight_offset;
+} d3_norm_rope;
+D3_API int d3_qk_norm_rope(const d3_norm_rope* a, const d3_kv_cache* cache, d3_stream_t stream);
+
+/* Attention of new tokens over a paged cache that holds their keys and values
+ * already.  Sequence b's query rows are cu_q[b] .. cu_q[b + 1] (cu_q NULL: row
+ * b alone), the last of its kv_lens[b] cached tokens; row i of n sees the keys
+ * [0, kv_lens[b] - n + i], and a row that sees none gives zeros.  Key j of
+ * sequence b lies in page page_table[b * table_stride + j / page_size]; a page
+ * id outside the cache reads as zeros.  out = softmax(scale * q k^T) v, bf16 or
+ * fp16 as q; query head h reads KV head h / (heads / kv_heads).  max_q and
+ * max_kv bound the new tokens and the length of any sequence (they choose the
+ * launch; a longer sequence is still computed in full, up to table_pages).
+ * Rows of out behind cu_q[batch] are left as they were.  The cache has q's
+ * type or is E4M3.  heads / kv_heads <= 128.
+ * workspace: at least d3_paged_attention_workspace_size bytes, 16-byte
+ * aligned, of this call's own until it ends.  *err_word: 51 .. 58 when a
+ * bounded wait (2 s) ran out.  No counterpart in the reference. */
+typedef struct d3_attention {
+  const void* q;                        /* [tokens][heads][head_dim] */
+  int64_t q_token, q_head;
+  void* out;
+  int64_t out_token, out_head;
+  const int32_t* page_table;
+  int64_t table_stride;
+  const int32_t* kv_lens;
+  const int32_t* cu_q;
+  int32_t table_pages, batch, tokens, heads, max_q, max_kv, dtype;
+  float scale;
+} d3_attention;
+D3_API size_t d3_paged_attention_workspace_size(const d3_attention* a, const d3_kv_cache* cache);
+D3_API int d3_paged_attention(const d3_attention* a, const d3_kv_cache* cache, int32_t* err_word,
+                              void* workspace, size_t workspace_bytes, d3_stream_t stream);
+
 /* ---------------------------------------------------------------- routing census / trace */
 
 /* counts[e] += occurrences of expert e among the rows*k ids (int32 or int64,
