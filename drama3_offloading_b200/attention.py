@@ -149,6 +149,9 @@ def paged_attention(q: torch.Tensor, cache: PagedKV, page_table: torch.Tensor,
         raise ValueError(f"the cache or page_table is not on {dev}")
     if max_q < 1:
         raise ValueError("max_q must be at least 1")
+    scale = dim ** -0.5 if scale is None else float(scale)
+    if not 0.0 < scale < float("inf"):
+        raise ValueError(f"scale {scale}: must be positive")
     top = pages * cache.page_size
     max_kv = top if max_kv is None else min(max_kv, top)
     if out is not None and (out.shape != q.shape or out.dtype != q.dtype or out.device != dev
@@ -163,7 +166,7 @@ def paged_attention(q: torch.Tensor, cache: PagedKV, page_table: torch.Tensor,
             page_table.data_ptr(), page_table.stride(0), kv_lens.data_ptr(),
             cu_q.data_ptr() if cu_q is not None else None, pages, batch, tokens, heads,
             min(max_q, max(tokens, 1)), max(max_kv, 0), code,
-            dim ** -0.5 if scale is None else scale)
+            scale)
         need = _lib.load().d3_paged_attention_workspace_size(a, cache.ref)
         ws = torch.empty(max(need, 16), dtype=torch.uint8, device=dev)
         _lib.call("d3_paged_attention", a, cache.ref, moe.error_word(dev).data_ptr(),

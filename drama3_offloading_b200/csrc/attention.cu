@@ -1,28 +1,46 @@
 // Attention over the paged K/V cache: argument checks, the choice of kernel
 // and the launches.
-#include "attn_rows.cuh"
+#include "attn_chunk.cuh"
 
 namespace d3 {
 
-// Rows of a cache buffer ([rows][D], one row per token and head) in boxes of
-// box_rows x 128 bytes, 128-byte swizzle; rows outside read as zeros.
-static int make_rows_map(CUtensorMap* m, const void* base, int dtype, uint64_t D, uint64_t rows,
-                         uint32_t box_rows) {
+// A tensor map with the 128-byte swizzle; what lies outside reads as zeros.
+static int make_map(CUtensorMap* m, const void* base, int dtype, int rank, const uint64_t* dims,
+                    const uint64_t* strides, const uint32_t* box) {
   EncodeTiledFn fn = encode_fn();
   if (!fn) return fail(D3_ERR_CUDA, "cuTensorMapEncodeTiled unavailable from the driver");
-  const uint32_t es = dtype == D3_E4M3 ? 1 : 2;
-  cuuint64_t dims[2] = {D, rows};
-  cuuint64_t strides[1] = {D * es};
-  cuuint32_t box[2] = {128 / es, box_rows};
-  cuuint32_t estr[2] = {1, 1};
+  cuuint64_t d[3], s[2];
+  cuuint32_t x[3], e[3] = {1, 1, 1};
+  for (int i = 0; i < rank; ++i) {
+    d[i] = dims[i];
+    x[i] = box[i];
+    if (i) s[i - 1] = strides[i - 1];
+  }
   const CUtensorMapDataType t = dtype == D3_BF16  ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
                                 : dtype == D3_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
                                                   : CU_TENSOR_MAP_DATA_TYPE_UINT8;
-  CUresult r = fn(m, t, 2, const_cast<void*>(base), dims, strides, box, estr,
-                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
-                  CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  CUresult r = fn(m, t, rank, const_cast<void*>(base), d, s, x, e, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                  CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) return fail(D3_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d)", (int)r);
   return D3_OK;
+}
+
+// A cache buffer as rows [pages * kv_heads * page_size][D].
+static int make_rows_map(CUtensorMap* m, const void* base, const d3_kv_cache* c, uint32_t box_rows) {
+  const uint64_t es = c->dtype == D3_E4M3 ? 1 : 2;
+  const uint64_t dims[2] = {(uint64_t)c->head_dim, (uint64_t)c->pages * c->kv_heads * c->page_size};
+  const uint64_t strides[1] = {c->head_dim * es};
+  const uint32_t box[2] = {(uint32_t)(128 / es), box_rows};
+  return make_map(m, base, c->dtype, 2, dims, strides, box);
+}
+// A 16-bit cache buffer as pages [pages * kv_heads][page_size][D]: rows before
+// or behind a page are outside the map.
+static int make_pages_map(CUtensorMap* m, const void* base, const d3_kv_cache* c, uint32_t box_rows) {
+  const uint64_t dims[3] = {(uint64_t)c->head_dim, (uint64_t)c->page_size, (uint64_t)c->pages * c->kv_heads};
+  const uint64_t strides[2] = {c->head_dim * 2ull, c->page_size * c->head_dim * 2ull};
+  const uint32_t box[3] = {64, box_rows, 1};
+  return make_map(m, base, c->dtype, 3, dims, strides, box);
 }
 
 static int check_attention(const d3_attention* a, const d3_kv_cache* c) {
@@ -43,30 +61,62 @@ static int check_attention(const d3_attention* a, const d3_kv_cache* c) {
   if ((long long)a->tokens * (a->heads / c->kv_heads) >= (1LL << 30) ||
       (long long)a->table_pages * c->page_size >= (1LL << 30) || (long long)a->batch * c->kv_heads >= (1LL << 24))
     return fail(D3_ERR_TOO_LARGE, "d3_paged_attention: tokens, table or batch too large");
-  D3_CHECK_ARG(a->scale == a->scale, "d3_paged_attention: scale is NaN");
+  D3_CHECK_ARG(a->scale > 0.f && a->scale < INFINITY, "d3_paged_attention: scale must be positive");
   return D3_OK;
 }
 
-constexpr int kJoinGroups = 4;   // row groups of a sequence's KV head with a join CTA of their own
+// Up to this many rows of a KV head (new tokens x query heads that share it) a
+// sequence goes through the row kernel.  Above it the row kernel would read
+// the keys once per 16 rows; the 256-row pairs of the chunk kernel read them
+// once and, although most of their rows may be empty, keep up with HBM.
+constexpr int kRowsMost = 16;
+
+struct Workspace {         // byte offsets
+  size_t rows_o, rows_ml, rows_desc, chunk_o, chunk_ml, chunk_desc, total;
+};
+static Workspace plan_workspace(const d3_attention* a, const d3_kv_cache* c) {
+  Workspace w{};
+  const size_t D = c->head_dim, sms = num_sms(), pairs = sms / 2;
+  size_t at = 0;
+  auto take = [&](size_t n) {
+    const size_t o = at;
+    at = (at + n + 255) / 256 * 256;
+    return o;
+  };
+  w.rows_o = take(sms * 2 * kRowsMost * D * 4);
+  w.rows_ml = take(sms * 2 * kRowsMost * 8);
+  w.rows_desc = take(sms * 16);
+  if ((long long)a->max_q * (a->heads / c->kv_heads) > kRowsMost) {
+    w.chunk_o = take(pairs * 2 * 256 * D * 4);
+    w.chunk_ml = take(pairs * 2 * 256 * 8);
+    w.chunk_desc = take(pairs * 16);
+  }
+  w.total = at;
+  return w;
+}
+
+template <typename K>
+static int set_smem(K kernel, size_t bytes, bool (&done)[64]) {
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (dev < 0 || dev >= 64 || !done[dev]) {
+    D3_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes),
+                "attention smem attribute");
+    if (dev >= 0 && dev < 64) done[dev] = true;
+  }
+  return D3_OK;
+}
 
 template <typename T, int D, bool E4, int NT>
 static int launch_rows(AttnParams p, const d3_attention* a, const d3_kv_cache* c, cudaStream_t st) {
   using C = RowsCfg<T, D, E4, NT>;
-  static bool attr_set[64] = {false};
-  int dev = 0;
-  cudaGetDevice(&dev);
-  if (dev >= 0 && dev < 64 && !attr_set[dev]) {
-    D3_CUDA_TRY(cudaFuncSetAttribute(attn_rows_kernel<T, D, E4, NT>,
-                                     cudaFuncAttributeMaxDynamicSharedMemorySize, (int)C::SMEM),
-                "attention smem attribute");
-    attr_set[dev] = true;
-  }
-  const uint32_t box = c->page_size < C::KEYS ? c->page_size : C::KEYS;
-  const uint64_t rows = (uint64_t)c->pages * c->kv_heads * c->page_size;
-  CUtensorMap tk, tv;
+  static bool done[64] = {false};
   int rc;
-  if ((rc = make_rows_map(&tk, c->k, c->dtype, D, rows, box))) return rc;
-  if ((rc = make_rows_map(&tv, c->v, c->dtype, D, rows, box))) return rc;
+  if ((rc = set_smem(attn_rows_kernel<T, D, E4, NT>, C::SMEM, done))) return rc;
+  const uint32_t box = c->page_size < C::KEYS ? c->page_size : C::KEYS;
+  CUtensorMap tk, tv;
+  if ((rc = make_rows_map(&tk, c->k, c, box))) return rc;
+  if ((rc = make_rows_map(&tv, c->v, c, box))) return rc;
   const long long groups = ((long long)a->max_q * p.group + C::ROWS - 1) / C::ROWS;
   const long long tiles = ((long long)a->max_kv + C::KEYS - 1) / C::KEYS;
   const long long most = (tiles < 1 ? 1 : tiles) * groups * a->batch * c->kv_heads;
@@ -74,16 +124,66 @@ static int launch_rows(AttnParams p, const d3_attention* a, const d3_kv_cache* c
   D3_CUDA_TRY(launch_k(attn_rows_kernel<T, D, E4, NT>, dim3(parts), dim3(C::THREADS), C::SMEM, st,
                        pdl_enabled(), tk, tv, p),
               "attn_rows_kernel launch");
-  const int jg = (int)(groups < kJoinGroups ? groups : kJoinGroups);
-  D3_CUDA_TRY(launch_k(attn_rows_join_kernel<T, D>, dim3((unsigned)(a->batch * c->kv_heads * jg)), dim3(128), 0,
-                       st, pdl_enabled(), p, (int)C::KEYS, (int)C::ROWS, parts, jg),
+  D3_CUDA_TRY(launch_k(attn_rows_join_kernel<T, D>, dim3(parts, C::ROWS), dim3(256), 0, st, pdl_enabled(), p,
+                       (int)C::ROWS),
               "attn_rows_join_kernel launch");
   return D3_OK;
 }
 
 template <typename T, int D, bool E4>
-static int launch_rows_nt(const AttnParams& p, const d3_attention* a, const d3_kv_cache* c, cudaStream_t st) {
-  return a->max_q * p.group <= 8 ? launch_rows<T, D, E4, 1>(p, a, c, st) : launch_rows<T, D, E4, 2>(p, a, c, st);
+static int launch_chunk(const AttnParams& p, const d3_attention* a, const d3_kv_cache* c, const ChunkWs& ws,
+                        cudaStream_t st) {
+  using C = ChunkCfg<T, D, E4>;
+  static bool done[64] = {false};
+  int rc;
+  if ((rc = set_smem(attn_chunk_kernel<T, D, E4>, C::SMEM, done))) return rc;
+  const int tpc = 128 / p.group;
+  CUtensorMap tq, tk, tv;
+  const uint64_t dims[3] = {(uint64_t)D, (uint64_t)a->heads, (uint64_t)a->tokens};
+  const uint64_t strides[2] = {(uint64_t)a->q_head * 2, (uint64_t)a->q_token * 2};
+  const uint32_t box[3] = {64, (uint32_t)p.group, (uint32_t)tpc};
+  if ((rc = make_map(&tq, a->q, a->dtype, 3, dims, strides, box))) return rc;
+  if (E4) {
+    tk = tv = tq;    // codes are not loaded by TMA
+  } else {
+    if ((rc = make_pages_map(&tk, c->k, c, c->page_size < 64 ? c->page_size : 64))) return rc;
+    if ((rc = make_pages_map(&tv, c->v, c, c->page_size))) return rc;
+  }
+  // row tiles at most: every sequence may have one that is not full
+  const long long tiles = a->tokens / (2 * tpc) + a->batch;
+  const long long blocks = ((long long)a->max_kv + kBlockKeys - 1) / kBlockKeys;
+  const long long most = (blocks < 1 ? 1 : blocks) * tiles * c->kv_heads;
+  const int pairs = (int)(most < num_sms() / 2 ? most : num_sms() / 2);
+  D3_CUDA_TRY(launch_k(attn_chunk_kernel<T, D, E4>, dim3(2 * pairs), dim3(C::THREADS), C::SMEM, st, pdl_enabled(),
+                       tq, tk, tv, p, ws),
+              "attn_chunk_kernel launch");
+  D3_CUDA_TRY(launch_k(attn_chunk_join_kernel<T, D>, dim3(pairs, 256 / kJoinRows), dim3(256), 0, st, pdl_enabled(),
+                       p, ws),
+              "attn_chunk_join_kernel launch");
+  return D3_OK;
+}
+
+// Which kernels run.  One launch pair for all sequences where max_q says that
+// all are short, or where tokens == batch * max_q says that none is (a shorter
+// one is still right there); otherwise each kernel takes its own.
+template <typename T, int D, bool E4>
+static int launch_attention(AttnParams p, const d3_attention* a, const d3_kv_cache* c, const ChunkWs& ws,
+                            cudaStream_t st) {
+  const long long rows = (long long)a->max_q * p.group;
+  int rc = D3_OK;
+  if (rows <= 8) return launch_rows<T, D, E4, 1>(p, a, c, st);
+  if (rows <= kRowsMost) return launch_rows<T, D, E4, 2>(p, a, c, st);
+  if ((long long)a->batch * a->max_q != a->tokens && p.group <= kRowsMost) {
+    AttnParams few = p;
+    few.max_rows = kRowsMost;
+    d3_attention one = *a;
+    one.max_q = kRowsMost / p.group;
+    if ((rc = p.group <= 8 && one.max_q == 1 ? launch_rows<T, D, E4, 1>(few, &one, c, st)
+                                             : launch_rows<T, D, E4, 2>(few, &one, c, st)))
+      return rc;
+    p.min_rows = kRowsMost + 1;
+  }
+  return launch_chunk<T, D, E4>(p, a, c, ws, st);
 }
 
 }  // namespace d3
@@ -94,8 +194,7 @@ extern "C" {
 
 size_t d3_paged_attention_workspace_size(const d3_attention* a, const d3_kv_cache* c) {
   if (check_attention(a, c)) return 0;
-  // two places per CTA of the row kernel: 16 rows of sums, maxima and sums
-  return (size_t)num_sms() * 2 * 16 * ((size_t)c->head_dim + 2) * 4 + 256;
+  return plan_workspace(a, c).total;
 }
 
 int d3_paged_attention(const d3_attention* a, const d3_kv_cache* c, int32_t* err_word, void* workspace,
@@ -108,9 +207,9 @@ int d3_paged_attention(const d3_attention* a, const d3_kv_cache* c, int32_t* err
   if (!aligned16(a->q) || !aligned16(a->out) || a->q_token % 8 || a->q_head % 8 || a->out_token % 8 || a->out_head % 8)
     return fail(D3_ERR_MISALIGNED, "d3_paged_attention: rows must start on 16-byte boundaries");
   D3_CHECK_ARG(a->cu_q || a->tokens >= a->batch, "d3_paged_attention: without cu_q every sequence has a row");
-  if (!workspace || workspace_bytes < d3_paged_attention_workspace_size(a, c))
-    return fail(D3_ERR_WORKSPACE, "d3_paged_attention: workspace of %zu bytes needed",
-                d3_paged_attention_workspace_size(a, c));
+  const Workspace w = plan_workspace(a, c);
+  if (!workspace || workspace_bytes < w.total)
+    return fail(D3_ERR_WORKSPACE, "d3_paged_attention: workspace of %zu bytes needed", w.total);
   if (!aligned16(workspace)) return fail(D3_ERR_MISALIGNED, "d3_paged_attention: workspace not 16-byte aligned");
   AttnParams p{};
   p.q = a->q;
@@ -137,19 +236,25 @@ int d3_paged_attention(const d3_attention* a, const d3_kv_cache* c, int32_t* err
   p.scale_log2 = a->scale * 1.44269504088896340736f;
   p.min_rows = 0;
   p.max_rows = 0x7fffffff;
-  p.ws_o = static_cast<float*>(workspace);
-  p.ws_ml = p.ws_o + (size_t)num_sms() * 2 * 16 * c->head_dim;
+  char* base = static_cast<char*>(workspace);
+  p.ws_o = reinterpret_cast<float*>(base + w.rows_o);
+  p.ws_ml = reinterpret_cast<float*>(base + w.rows_ml);
+  p.ws_desc = reinterpret_cast<int4*>(base + w.rows_desc);
+  const ChunkWs ws{reinterpret_cast<float*>(base + w.chunk_o), reinterpret_cast<float*>(base + w.chunk_ml),
+                   reinterpret_cast<int4*>(base + w.chunk_desc)};
+  p.k_codes = c->k;
+  p.v_codes = c->v;
   p.err = err_word;
   const cudaStream_t st = (cudaStream_t)stream;
   const bool e4 = c->dtype == D3_E4M3;
   if (a->dtype == D3_BF16) {
     if (c->head_dim == 128)
-      return e4 ? launch_rows_nt<__nv_bfloat16, 128, true>(p, a, c, st) : launch_rows_nt<__nv_bfloat16, 128, false>(p, a, c, st);
-    return e4 ? launch_rows_nt<__nv_bfloat16, 256, true>(p, a, c, st) : launch_rows_nt<__nv_bfloat16, 256, false>(p, a, c, st);
+      return e4 ? launch_attention<__nv_bfloat16, 128, true>(p, a, c, ws, st) : launch_attention<__nv_bfloat16, 128, false>(p, a, c, ws, st);
+    return e4 ? launch_attention<__nv_bfloat16, 256, true>(p, a, c, ws, st) : launch_attention<__nv_bfloat16, 256, false>(p, a, c, ws, st);
   }
   if (c->head_dim == 128)
-    return e4 ? launch_rows_nt<__half, 128, true>(p, a, c, st) : launch_rows_nt<__half, 128, false>(p, a, c, st);
-  return e4 ? launch_rows_nt<__half, 256, true>(p, a, c, st) : launch_rows_nt<__half, 256, false>(p, a, c, st);
+    return e4 ? launch_attention<__half, 128, true>(p, a, c, ws, st) : launch_attention<__half, 128, false>(p, a, c, ws, st);
+  return e4 ? launch_attention<__half, 256, true>(p, a, c, ws, st) : launch_attention<__half, 256, false>(p, a, c, ws, st);
 }
 
 }  // extern "C"

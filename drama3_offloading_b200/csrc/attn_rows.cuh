@@ -56,11 +56,13 @@ struct AttnParams {
   const int* cu_q;               // [batch + 1], or NULL: one row a sequence
   int batch, tokens, heads, group, kv_heads;
   int page_size, page_shift, pages;
+  const void *k_codes, *v_codes; // the cache's buffers
   const float *k_scale, *v_scale;
   float scale_log2;              // softmax scale * log2(e)
   int min_rows, max_rows;        // sequences this launch takes, by new tokens * group
   float* ws_o;                   // partial sums
   float* ws_ml;                  // their maxima and sums
+  int4* ws_desc;                 // of each part: the pair that begins and does not end in it (join_desc)
   int* err;
 };
 
@@ -72,8 +74,8 @@ struct AttnSeq {
 __device__ __forceinline__ AttnSeq attn_seq(const AttnParams& p, int b) {
   AttnSeq s;
   if (p.cu_q) {
-    s.q0 = p.cu_q[b];
-    s.n = p.cu_q[b + 1] - s.q0;
+    s.q0 = __ldcg(p.cu_q + b);
+    s.n = __ldcg(p.cu_q + b + 1) - s.q0;
   } else {
     s.q0 = b;
     s.n = 1;
@@ -81,7 +83,7 @@ __device__ __forceinline__ AttnSeq attn_seq(const AttnParams& p, int b) {
   // offsets outside the query tensor (a broken cu_q) are cut to it
   if (s.q0 < 0 || s.q0 > p.tokens) s.n = 0;
   else s.n = max(0, min(s.n, p.tokens - s.q0));
-  s.kv = max(0, min(p.kv_lens[b], p.table_pages * p.page_size));
+  s.kv = max(0, min(__ldcg(p.kv_lens + b), p.table_pages * p.page_size));
   s.rows = s.n * p.group;
   return s;
 }
@@ -124,15 +126,16 @@ __device__ __forceinline__ long long rows_units(const AttnParams& p, int b, int 
   return (long long)rows_tiles(s.kv, keys) * p.kv_heads * ((s.rows + rows_per - 1) / rows_per);
 }
 
-// All threads of the CTA: the list's length and, for list position `at(total)`,
-// its sequence.  s_scan: 33 long longs of shared memory.
-template <typename F>
-__device__ RowsWork rows_plan(const AttnParams& p, int keys, int rows_per, long long* s_scan, F part) {
+// All threads of the CTA: the list's length (units(b) of every sequence) and,
+// for the part that part(r) sets, the sequence it begins in.  s_scan: 33 long
+// longs of shared memory.
+template <typename U, typename F>
+__device__ RowsWork list_plan(const AttnParams& p, long long* s_scan, U units, F part) {
   const int n = blockDim.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int per = (p.batch + n - 1) / n;
   const int b0 = min(p.batch, tid * per), b1 = min(p.batch, b0 + per);
   long long sum = 0;
-  for (int b = b0; b < b1; ++b) sum += rows_units(p, b, keys, rows_per);
+  for (int b = b0; b < b1; ++b) sum += units(b);
   long long inc = sum;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
@@ -145,7 +148,7 @@ __device__ RowsWork rows_plan(const AttnParams& p, int keys, int rows_per, long 
   if (tid == 0) s_b = p.batch;
   __syncthreads();
   long long before = inc - sum, total = 0;
-  for (int w = 0; w < (n + 31) / 32; ++w) {
+  for (int w = 0; w < n / 32; ++w) {
     if (w < warp) before += s_scan[w];
     total += s_scan[w];
   }
@@ -155,7 +158,7 @@ __device__ RowsWork rows_plan(const AttnParams& p, int keys, int rows_per, long 
   if (r.count > 0 && before <= r.begin && r.begin < before + sum) {
     long long at = before;
     for (int b = b0; b < b1; ++b) {
-      const long long u = rows_units(p, b, keys, rows_per);
+      const long long u = units(b);
       if (r.begin < at + u) {
         s_b = b;
         s_off = r.begin - at;
@@ -283,13 +286,16 @@ __global__ void __launch_bounds__(RowsCfg<T, D, E4, NT>::THREADS, 1)
   }
   pdl_trigger();
   pdl_wait();
-  const RowsWork work = rows_plan(p, C::KEYS, C::ROWS, s_scan, [&](RowsWork& r) {
+  const RowsWork work = list_plan(p, s_scan, [&](int b) { return rows_units(p, b, C::KEYS, C::ROWS); }, [&](RowsWork& r) {
     // no part is empty: a pair's parts are neighbours in the workspace
     const long long g = min((long long)gridDim.x, r.total), c = blockIdx.x;
     r.begin = c < g ? r.total * c / g : 0;
     r.count = c < g ? (int)(r.total * (c + 1) / g - r.begin) : 0;
   });
-  if (work.count == 0) return;
+  if (work.count == 0) {
+    if (tid == 0) p.ws_desc[blockIdx.x] = make_int4(0, 0, 0, -1);
+    return;
+  }
   RowsWalk walk{work.b, work.count, work.off};
   RowsPiece w;
   if (warp == C::WARPS) {
@@ -307,7 +313,7 @@ __global__ void __launch_bounds__(RowsCfg<T, D, E4, NT>::THREADS, 1)
         int row = -1;
         if (lane < need) {
           const int key = key0 + lane * box;
-          const int page = p.table[(long long)w.b * p.table_stride + (key >> p.page_shift)];
+          const int page = __ldcg(p.table + (long long)w.b * p.table_stride + (key >> p.page_shift));
           if (page >= 0 && page < p.pages)
             row = ((page * p.kv_heads + w.head) << p.page_shift) + (key & (p.page_size - 1));
         }
@@ -370,6 +376,7 @@ __global__ void __launch_bounds__(RowsCfg<T, D, E4, NT>::THREADS, 1)
     if (lane == 0) mbar_arrive(empty + slot);
     if (++slot == C::SLOTS) { slot = 0; phase ^= 1; }
   };
+  int4 desc = make_int4(0, 0, 0, -1);
   while (walk.next(p, C::KEYS, C::ROWS, w)) {
     const int row0 = w.rg * C::ROWS, rows = min(C::ROWS, w.s.rows - row0);
     // queries in operand order: s_q[nt][kk][lane] holds the two registers of
@@ -382,7 +389,7 @@ __global__ void __launch_bounds__(RowsCfg<T, D, E4, NT>::THREADS, 1)
       // lane's share: 8 dims at a time, D / 8 chunks
       float amax = 0.f;
       uint4 u = make_uint4(0, 0, 0, 0);
-      if (r < rows && lane < D / 8) u = *reinterpret_cast<const uint4*>(src + lane * 8);
+      if (r < rows && lane < D / 8) u = __ldcg(reinterpret_cast<const uint4*>(src + lane * 8));
       float x[8];
       unpack8<T>(u, x);
       float mul = 1.f, back = 1.f;
@@ -589,6 +596,11 @@ __global__ void __launch_bounds__(RowsCfg<T, D, E4, NT>::THREADS, 1)
     const bool whole = w.t0 == 0 && w.t1 == w.nt;
     const int place = blockIdx.x * 2 + (w.t0 == 0 ? 1 : 0);
     float* wo = p.ws_o + (size_t)place * C::ROWS * D;
+    if (!whole && w.t0 == 0) {
+      // the part that holds the pair's last tile
+      const long long u = work.begin + work.count + (w.nt - w.t1) - 1, cut = min((long long)gridDim.x, work.total);
+      desc = make_int4(w.b, w.head, w.rg, (int)(((u + 1) * cut - 1) / work.total));
+    }
     float f[NT][2];    // this warp's factor of its rows
 #pragma unroll
     for (int n = 0; n < NT; ++n)
@@ -647,77 +659,71 @@ __global__ void __launch_bounds__(RowsCfg<T, D, E4, NT>::THREADS, 1)
       }
     }
   }
+  if (tid == 0) p.ws_desc[blockIdx.x] = desc;
 }
 
-// One CTA per (sequence, KV head, row group): those that the list was cut
-// inside of are the sum of their parts, in the parts' order.  The workspace is
-// read through L2: launched early, this kernel shares SMs with the join of the
-// call before, whose lines of the same memory may still be in L1.
+// Pairs that the parts' cuts go through: the sum of their parts, in the parts'
+// order.  blockIdx.x is the part in which the pair begins, blockIdx.y the row;
+// the threads take turns of D/4 over the parts and add up through shared
+// memory.  The workspace is read through L2: launched early, this kernel
+// shares SMs with the join of the call before, whose lines of the same memory
+// may still be in L1.
 template <typename T, int D>
-__global__ void __launch_bounds__(128) attn_rows_join_kernel(const __grid_constant__ AttnParams p, int keys,
-                                                             int rows_per, int parts, int groups_max) {
-  __shared__ long long s_scan[33];
+__global__ void __launch_bounds__(256) attn_rows_join_kernel(const __grid_constant__ AttnParams p, int rows_per) {
+  constexpr int GROUPS = 256 / (D / 4);
+  __shared__ float4 s_a[GROUPS][D / 4];
+  __shared__ float s_l[GROUPS];
   pdl_trigger();
   pdl_wait();
-  const int b = blockIdx.x / (p.kv_heads * groups_max), rest = blockIdx.x - b * p.kv_heads * groups_max;
-  const int head = rest / groups_max, rg0 = rest - head * groups_max;
-  const AttnSeq s = attn_seq(p, b);
-  if (s.rows == 0 || s.rows < p.min_rows || s.rows > p.max_rows) return;
-  const int groups = (s.rows + rows_per - 1) / rows_per, nt = rows_tiles(s.kv, keys);
-  if (nt == 1 || rg0 >= groups) return;
-  // units before sequence b, and in all
-  const int tid = threadIdx.x;
-  long long mine = 0, all = 0;
-  for (int i = tid; i < p.batch; i += blockDim.x) {
-    const long long u = rows_units(p, i, keys, rows_per);
-    all += u;
-    if (i < b) mine += u;
-  }
+  const int c0 = blockIdx.x, r = blockIdx.y;
+  const int4 de = __ldcg(p.ws_desc + c0);
+  if (de.w < 0) return;
+  const AttnSeq s = attn_seq(p, de.x);
+  const int gr = de.z * rows_per + r;
+  if (gr >= s.rows) return;
+  const int g = threadIdx.x / (D / 4), d4 = threadIdx.x % (D / 4);
+  float m = -INFINITY;
+  for (int c = c0 + (threadIdx.x & 31); c <= de.w; c += 32)
+    m = fmaxf(m, __ldcg(p.ws_ml + (((size_t)c * 2 + (c == c0)) * rows_per + r) * 2));
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    mine += __shfl_xor_sync(0xffffffffu, mine, o);
-    all += __shfl_xor_sync(0xffffffffu, all, o);
-  }
-  if ((tid & 31) == 0) {
-    s_scan[tid >> 5] = mine;
-    s_scan[4 + (tid >> 5)] = all;
-  }
-  __syncthreads();
-  mine = s_scan[0] + s_scan[1] + s_scan[2] + s_scan[3];
-  all = s_scan[4] + s_scan[5] + s_scan[6] + s_scan[7];
-  const long long cut = min((long long)parts, all);
-  for (int rg = rg0; rg < groups; rg += groups_max) {
-    const long long u0 = mine + ((long long)head * groups + rg) * nt, u1 = u0 + nt - 1;
-    const int c0 = (int)(((u0 + 1) * cut - 1) / all), c1 = (int)(((u1 + 1) * cut - 1) / all);
-    if (c0 == c1) continue;          // one part held it whole
-    const int row0 = rg * rows_per, rows = min(rows_per, s.rows - row0);
-    for (int i = tid; i < rows * (D / 4); i += blockDim.x) {
-      const int r = i / (D / 4), d = (i - r * (D / 4)) * 4;
-      float m = -INFINITY;
-      for (int c = c0; c <= c1; ++c)
-        m = fmaxf(m, __ldcg(p.ws_ml + (((size_t)c * 2 + (c == c0)) * rows_per + r) * 2));
-      float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
-      float l = 0.f;
-      for (int c = c0; c <= c1; ++c) {
-        const size_t at = ((size_t)c * 2 + (c == c0)) * rows_per + r;
-        const float mc = __ldcg(p.ws_ml + at * 2);
-        if (mc == -INFINITY) continue;
-        const float f = ex2(mc - m);
-        const float4 v = __ldcg(reinterpret_cast<const float4*>(p.ws_o + at * D + d));
-        l = fmaf(__ldcg(p.ws_ml + at * 2 + 1), f, l);
-        a.x = fmaf(v.x, f, a.x);
-        a.y = fmaf(v.y, f, a.y);
-        a.z = fmaf(v.z, f, a.z);
-        a.w = fmaf(v.w, f, a.w);
-      }
-      const float inv = l > 0.f ? 1.f / l : 0.f;
-      const int gr = row0 + r;
-      T* dst = static_cast<T*>(p.out) + (long long)(s.q0 + gr / p.group) * p.out_token +
-               (long long)(head * p.group + gr % p.group) * p.out_head + d;
-      *reinterpret_cast<uint2*>(dst) = make_uint2(Elem<T>::from_f2(a.x * inv, a.y * inv),
-                                                  Elem<T>::from_f2(a.z * inv, a.w * inv));
+  for (int x = 16; x > 0; x >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, x));
+  const float base = m == -INFINITY ? 0.f : m;
+  float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+  float l = 0.f;
+#pragma unroll 4
+  for (int c = c0 + g; c <= de.w; c += GROUPS) {
+    const size_t at = ((size_t)c * 2 + (c == c0)) * rows_per + r;
+    const float2 ml = __ldcg(reinterpret_cast<const float2*>(p.ws_ml + at * 2));
+    const float4 v = __ldcg(reinterpret_cast<const float4*>(p.ws_o + at * D) + d4);
+    const float f = ex2(ml.x - base);
+    if (f != 0.f) {
+      l = fmaf(ml.y, f, l);
+      a.x = fmaf(v.x, f, a.x);
+      a.y = fmaf(v.y, f, a.y);
+      a.z = fmaf(v.z, f, a.z);
+      a.w = fmaf(v.w, f, a.w);
     }
   }
+  s_a[g][d4] = a;
+  if (d4 == 0) s_l[g] = l;
+  __syncthreads();
+  if (g) return;
+  l = 0.f;
+  a = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+  for (int x = 0; x < GROUPS; ++x) {
+    const float4 v = s_a[x][d4];
+    l += s_l[x];
+    a.x += v.x;
+    a.y += v.y;
+    a.z += v.z;
+    a.w += v.w;
+  }
+  const float inv = l > 0.f ? 1.f / l : 0.f;
+  T* dst = static_cast<T*>(p.out) + (long long)(s.q0 + gr / p.group) * p.out_token +
+           (long long)(de.y * p.group + gr % p.group) * p.out_head + d4 * 4;
+  *reinterpret_cast<uint2*>(dst) =
+      make_uint2(Elem<T>::from_f2(a.x * inv, a.y * inv), Elem<T>::from_f2(a.z * inv, a.w * inv));
 }
 
 }  // namespace d3

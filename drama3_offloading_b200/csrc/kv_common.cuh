@@ -70,10 +70,14 @@ __device__ __forceinline__ float2 e4m3x2_to_f2(uint16_t c) {
 
 constexpr float kE4m3Max = 448.f;
 
+// Reads of what an earlier launch wrote go through L2 (__ldcg): under
+// programmatic launch a kernel may share an SM with an earlier reader of the
+// same memory, whose L1 lines are older than the write.
+
 // an index read as 4 or 8 bytes
 __device__ __forceinline__ long long load_index(const void* p, int bytes, long long i) {
-  return bytes == 8 ? static_cast<const long long*>(p)[i]
-                    : (long long)static_cast<const int*>(p)[i];
+  return bytes == 8 ? __ldcg(static_cast<const long long*>(p) + i)
+                    : (long long)__ldcg(static_cast<const int*>(p) + i);
 }
 
 // host: the checks every entry point makes of a cache descriptor

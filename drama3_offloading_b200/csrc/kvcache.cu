@@ -104,8 +104,8 @@ __global__ void __launch_bounds__(kFillThreads) kv_fill_kernel(const __grid_cons
     const long long tok = t0 + t;
     uint4 raw = make_uint4(0, 0, 0, 0);
     if (live)
-      raw = *reinterpret_cast<const uint4*>(static_cast<const T*>(in.p) + tok * in.token +
-                                            head * in.head + lane * 8);
+      raw = __ldcg(reinterpret_cast<const uint4*>(static_cast<const T*>(in.p) + tok * in.token +
+                                                  head * in.head + lane * 8));
     float x[8];
     unpack8<T>(raw, x);
     if (NORM) {
@@ -232,14 +232,14 @@ __global__ void __launch_bounds__(256) kv_read_kernel(const __grid_constant__ Re
     at[i] = (page * p.cache.kv_heads + h) * p.cache.page_size + off;
     src[i] = is_k ? p.cache.k : p.cache.v;
     if (p.cache.dtype == D3_E4M3) {
-      const uint2 c = *reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(src[i]) +
-                                                      at[i] * D + lane * 8);
+      const uint2 c = __ldcg(reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(src[i]) +
+                                                            at[i] * D + lane * 8));
       raw[i].x = c.x;
       raw[i].y = c.y;
-      sc[i] = (is_k ? p.cache.k_scale : p.cache.v_scale)[at[i]];
+      sc[i] = __ldcg((is_k ? p.cache.k_scale : p.cache.v_scale) + at[i]);
     } else {
-      raw[i] = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(src[i]) + at[i] * D +
-                                               lane * 8);
+      raw[i] = __ldcg(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(src[i]) +
+                                                     at[i] * D + lane * 8));
     }
   }
 #pragma unroll

@@ -57,7 +57,8 @@ def rows(t: torch.Tensor, name: str, heads: int, dim: int, dtype) -> torch.Tenso
 
 def aligned(t: torch.Tensor) -> bool:
     s = t.stride()
-    return s[2] == 1 and s[0] % 8 == 0 and s[1] % 8 == 0 and t.data_ptr() % 16 == 0
+    return (s[2] == 1 and s[0] % 8 == 0 and s[1] % 8 == 0 and s[0] > 0 and s[1] > 0
+            and t.data_ptr() % 16 == 0)
 
 
 def index(t: torch.Tensor, name: str, tokens: int, device) -> torch.Tensor:

@@ -54,6 +54,10 @@ ERROR_CODES = {
     41: "decode overlap: a fetched expert's bytes never landed",
     51: "paged attention, few rows: the loading warp waited for a free slot",
     52: "paged attention, few rows: a warp waited for a loaded tile",
+    53: "paged attention, chunk: the loading warp waited for a free slot",
+    54: "paged attention, chunk: the MMA issuer waited for operands or for the softmax",
+    55: "paged attention, chunk: the softmax waited for scores or for the output",
+    56: "paged attention, chunk: a widening warp waited for a free slot",
 }
 
 

@@ -453,7 +453,7 @@ D3_API int d3_qk_norm_rope(const d3_norm_rope* a, const d3_kv_cache* cache, d3_s
  * b alone), the last of its kv_lens[b] cached tokens; row i of n sees the keys
  * [0, kv_lens[b] - n + i], and a row that sees none gives zeros.  Key j of
  * sequence b lies in page page_table[b * table_stride + j / page_size]; a page
- * id outside the cache reads as zeros.  out = softmax(scale * q k^T) v, bf16 or
+ * id outside the cache reads as zeros.  out = softmax(scale * q k^T) v (scale > 0), bf16 or
  * fp16 as q; query head h reads KV head h / (heads / kv_heads).  max_q and
  * max_kv bound the new tokens and the length of any sequence (they choose the
  * launch; a longer sequence is still computed in full, up to table_pages).

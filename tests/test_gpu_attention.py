@@ -381,3 +381,21 @@ def test_streams_and_graphs_share_nothing():
         assert torch.equal(o, w)
     for o in got:
         assert torch.equal(o, want[1])
+
+
+@pytest.mark.parametrize("dtype,kind,heads,hk,dim", [(FP, E4, 16, 4, 128), (BF, BF, 8, 2, 256)])
+def test_many_calls_in_a_row_give_the_same_bits(dtype, kind, heads, hk, dim):
+    """Chunks and single tokens mixed, hundreds of launches back to back (each
+    early behind the one before): no wait runs out, no bit changes."""
+    g = gen(31)
+    lens = [(1, 2100), (140, 900), (1, 5), (65, 3500), (301, 301), (1, 800), (90, 2000)]
+    cache, table, q, cu, kv = make_batch(g, lens, heads, hk, dim, 16, dtype, kind)
+    call = lambda: attention.paged_attention(q, cache, table, kv, cu, max_q=301)
+    want = call()
+    check(want, *ref.attention(q, cache, table, kv, cu))
+    same = torch.ones((), dtype=torch.bool, device=DEV)
+    for _ in range(10):
+        for o in [call() for _ in range(40)]:
+            same &= (o == want).all()
+    assert bool(same)
+    moe.check_errors(DEV)
