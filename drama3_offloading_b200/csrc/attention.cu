@@ -4,9 +4,10 @@
 
 namespace d3 {
 
-// A tensor map with the 128-byte swizzle; what lies outside reads as zeros.
+// A tensor map, with the 128-byte swizzle unless told otherwise; what lies
+// outside reads as zeros.
 static int make_map(CUtensorMap* m, const void* base, int dtype, int rank, const uint64_t* dims,
-                    const uint64_t* strides, const uint32_t* box) {
+                    const uint64_t* strides, const uint32_t* box, bool swizzle = true) {
   EncodeTiledFn fn = encode_fn();
   if (!fn) return fail(D3_ERR_CUDA, "cuTensorMapEncodeTiled unavailable from the driver");
   cuuint64_t d[3], s[2];
@@ -20,8 +21,8 @@ static int make_map(CUtensorMap* m, const void* base, int dtype, int rank, const
                                 : dtype == D3_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
                                                   : CU_TENSOR_MAP_DATA_TYPE_UINT8;
   CUresult r = fn(m, t, rank, const_cast<void*>(base), d, s, x, e, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                  CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+                  swizzle ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE,
+                  CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) return fail(D3_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d)", (int)r);
   return D3_OK;
 }
@@ -34,13 +35,16 @@ static int make_rows_map(CUtensorMap* m, const void* base, const d3_kv_cache* c,
   const uint32_t box[2] = {(uint32_t)(128 / es), box_rows};
   return make_map(m, base, c->dtype, 2, dims, strides, box);
 }
-// A 16-bit cache buffer as pages [pages * kv_heads][page_size][D]: rows before
-// or behind a page are outside the map.
-static int make_pages_map(CUtensorMap* m, const void* base, const d3_kv_cache* c, uint32_t box_rows) {
+// A cache buffer as planes [pages * kv_heads][page_size][D]: rows before or
+// behind a page are outside the map.  16-bit rows in columns of 64 dims; codes
+// box_dims wide, unswizzled.
+static int make_pages_map(CUtensorMap* m, const void* base, const d3_kv_cache* c, uint32_t box_dims,
+                          uint32_t box_rows) {
+  const uint64_t es = c->dtype == D3_E4M3 ? 1 : 2;
   const uint64_t dims[3] = {(uint64_t)c->head_dim, (uint64_t)c->page_size, (uint64_t)c->pages * c->kv_heads};
-  const uint64_t strides[2] = {c->head_dim * 2ull, c->page_size * c->head_dim * 2ull};
-  const uint32_t box[3] = {64, box_rows, 1};
-  return make_map(m, base, c->dtype, 3, dims, strides, box);
+  const uint64_t strides[2] = {c->head_dim * es, c->page_size * c->head_dim * es};
+  const uint32_t box[3] = {box_dims, box_rows, 1};
+  return make_map(m, base, c->dtype, 3, dims, strides, box, es == 2);
 }
 
 static int check_attention(const d3_attention* a, const d3_kv_cache* c) {
@@ -143,16 +147,16 @@ static int launch_chunk(const AttnParams& p, const d3_attention* a, const d3_kv_
   const uint64_t strides[2] = {(uint64_t)a->q_head * 2, (uint64_t)a->q_token * 2};
   const uint32_t box[3] = {64, (uint32_t)p.group, (uint32_t)tpc};
   if ((rc = make_map(&tq, a->q, a->dtype, 3, dims, strides, box))) return rc;
-  if (E4) {
-    tk = tv = tq;    // codes are not loaded by TMA
-  } else {
-    if ((rc = make_pages_map(&tk, c->k, c, c->page_size < 64 ? c->page_size : 64))) return rc;
-    if ((rc = make_pages_map(&tv, c->v, c, c->page_size))) return rc;
-  }
+  const uint32_t krows = c->page_size < 64 ? c->page_size : 64;
+  if ((rc = make_pages_map(&tk, c->k, c, E4 ? D : 64, krows))) return rc;
+  if ((rc = make_pages_map(&tv, c->v, c, E4 ? D / 2 : 64, c->page_size))) return rc;
   // row tiles at most: every sequence may have one that is not full
   const long long tiles = a->tokens / (2 * tpc) + a->batch;
   const long long blocks = ((long long)a->max_kv + kBlockKeys - 1) / kBlockKeys;
   const long long most = (blocks < 1 ? 1 : blocks) * tiles * c->kv_heads;
+  // the kernel counts the list in 31 bits; the lengths it reads may be larger than max_kv says
+  if (((long long)a->table_pages * c->page_size / kBlockKeys + 1) * tiles * c->kv_heads >= (1LL << 31))
+    return fail(D3_ERR_TOO_LARGE, "d3_paged_attention: too many key blocks");
   const int pairs = (int)(most < num_sms() / 2 ? most : num_sms() / 2);
   D3_CUDA_TRY(launch_k(attn_chunk_kernel<T, D, E4>, dim3(2 * pairs), dim3(C::THREADS), C::SMEM, st, pdl_enabled(),
                        tq, tk, tv, p, ws),

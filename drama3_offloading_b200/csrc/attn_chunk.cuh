@@ -23,9 +23,10 @@
 // (in log2): P then stays below 2^8, sums are in fp32 and the quotient of the
 // two does not change.
 //
-// Roles (per CTA): warps 0-3 softmax and output, warp 4 issues the MMAs (in
-// the pair's first CTA), warp 5 the TMA loads; for codes warps 6-9 load,
-// widen and store the tiles themselves.
+// Roles (per CTA): warps 0-7 softmax and output (a row is shared by two
+// threads, 64 keys of a block and half of O each), warp 8 issues the MMAs (in
+// the pair's first CTA), warp 9 the TMA loads; for codes warp 10 brings the
+// scales and warps 12-15 widen the tiles.
 //
 // A block's last page, when the sequence ends in it, is loaded shifted: rows
 // before the page's first come from outside the tensor map and are zeros, the
@@ -36,9 +37,11 @@
 // key block) is cut into equal parts, one per pair; tiles that a cut goes
 // through are joined by attn_chunk_join_kernel in the parts' order.
 //
-// e4m3 caches: K codes are exact in 16 bits and their scale multiplies a
-// column of S in fp32; V is widened to T(code * scale), as kvcache.read gives
-// it.
+// e4m3 caches: codes are staged by TMA and widened to 16 bits in shared
+// memory.  K codes are exact there, and a key's scale multiplies a column of S
+// in fp32.  A value's scale is split into 2^e, by which the widened codes are
+// multiplied (exact again), and f in [1, 2), which multiplies a column of P in
+// fp32 before P is rounded: one rounding on the way, as with a 16-bit cache.
 #pragma once
 
 #include "attn_rows.cuh"
@@ -46,23 +49,23 @@
 namespace d3 {
 
 constexpr int kAttnErrChunkLoad = 53, kAttnErrChunkMma = 54, kAttnErrChunkSoftmax = 55,
-              kAttnErrChunkWiden = 56;
+              kAttnErrChunkWiden = 56, kAttnErrChunkAlign = 57;
 constexpr int kBlockKeys = 128;
 constexpr float kRescaleLog2 = 8.f;
 
 template <typename T, int D, bool E4>
 struct ChunkCfg {
-  static constexpr int THREADS = E4 ? 320 : 192;
+  static constexpr int THREADS = E4 ? 512 : 320;
   static constexpr int Q_BYTES = 128 * D * 2;
   static constexpr int SLOT = 64 * D * 2;                 // half a block of K or of V
-  static constexpr int SLOTS = E4 ? (D == 256 ? 4 : 8) : (D == 256 ? 5 : 10);
-  static constexpr int KS_RING = 8;                       // K scales of 8 blocks
-  static constexpr int KS_BYTES = E4 ? KS_RING * kBlockKeys * 4 : 0;
-  static constexpr size_t SMEM = 1024 + Q_BYTES + (size_t)SLOTS * SLOT + KS_BYTES + 512;
+  static constexpr int SLOTS = E4 ? (D == 256 ? 3 : 6) : (D == 256 ? 5 : 10);
+  static constexpr int RAW = E4 ? 64 * D : 0;             // the same as codes
+  static constexpr int RAWS = E4 ? (D == 256 ? 3 : 6) : 0;
+  static constexpr int SC_RING = 4;                       // scales of 4 blocks: ks, f, 2^e
+  static constexpr int SC_BYTES = E4 ? SC_RING * 3 * kBlockKeys * 4 : 0;
+  static constexpr size_t SMEM =
+      1024 + Q_BYTES + (size_t)SLOTS * SLOT + (size_t)RAWS * RAW + SC_BYTES + 2048;
   static constexpr int COL_S = 0, COL_O = 256;
-  // K scales of block j + KS_RING are written no earlier than the slot of V of
-  // block j is free, when its softmax is over
-  static_assert(2 * KS_RING >= SLOTS + 3, "K scale ring too short");
   static_assert(SMEM <= 227 * 1024, "shared memory");
 };
 
@@ -72,77 +75,129 @@ struct ChunkWs {           // carved from the call's workspace
   int4* desc;              // [pairs]: sequence, KV head, row tile, last part (-1: none)
 };
 
-// sum of floor((a i + b) / m) over i in [0, n), all arguments >= 0: the
-// Euclid-like reduction of a lattice point count
-__device__ __forceinline__ long long floor_sum(long long n, long long m, long long a, long long b) {
-  long long ans = 0;
-  if (n <= 0) return 0;
-  while (true) {
-    if (a >= m) {
-      ans += (n - 1) * n / 2 * (a / m);
-      a %= m;
-    }
-    if (b >= m) {
-      ans += n * (b / m);
-      b %= m;
-    }
-    const long long y = a * n + b;
-    if (y < m) return ans;
-    n = y / m;
-    b = y % m;
-    const long long t = m;
-    m = a;
-    a = t;
-  }
-}
-
 // key blocks that row tile i (of `per` tokens) of a sequence sees: at least one
 __device__ __forceinline__ int chunk_blocks(const AttnSeq& s, int per, int i) {
   const int vis = s.kv - s.n + min((i + 1) * per, s.n);
   return max(1, (vis + kBlockKeys - 1) / kBlockKeys);
 }
-// ... of row tiles [0, i), i below the sequence's number of tiles
-__device__ __forceinline__ long long chunk_before(const AttnSeq& s, int per, int i) {
-  const long long base = s.kv - s.n;
-  long long ones = base >= kBlockKeys ? 0 : (kBlockKeys - base) / per;
-  ones = ones < i ? ones : i;
-  return ones + floor_sum(i - ones, kBlockKeys, per, base + (ones + 1) * per + kBlockKeys - 1);
-}
 __device__ __forceinline__ int chunk_tiles(const AttnSeq& s, int per) { return (s.n + per - 1) / per; }
-__device__ __forceinline__ long long chunk_head_units(const AttnSeq& s, int per) {
-  const int nq = chunk_tiles(s, per);
-  return chunk_before(s, per, nq - 1) + chunk_blocks(s, per, nq - 1);
-}
 __device__ __forceinline__ bool chunk_takes(const AttnParams& p, const AttnSeq& s) {
   return s.rows > 0 && s.rows >= p.min_rows && s.rows <= p.max_rows;
 }
+__device__ __forceinline__ AttnSeq seq_from(const AttnSeq& s, int lane) {
+  AttnSeq r;
+  r.q0 = __shfl_sync(0xffffffffu, s.q0, lane);
+  r.n = __shfl_sync(0xffffffffu, s.n, lane);
+  r.kv = __shfl_sync(0xffffffffu, s.kv, lane);
+  r.rows = __shfl_sync(0xffffffffu, s.rows, lane);
+  return r;
+}
+// one warp: key blocks of all row tiles of a sequence, for one KV head
+__device__ __forceinline__ int warp_head_units(const AttnSeq& s, int per) {
+  int u = 0;
+  for (int i = threadIdx.x & 31; i < chunk_tiles(s, per); i += 32) u += chunk_blocks(s, per, i);
+  return __reduce_add_sync(0xffffffffu, u);
+}
+
+// A part of the list: where it begins and how long it is.
+struct ChunkPart {
+  int total, begin, count;
+  int b, head, tile, j;
+};
+// All threads of the CTA.  Each warp takes a run of sequences, 32 at a time:
+// their lanes read the lengths, and the whole warp adds up the blocks of each
+// that this launch takes.  The host has checked that the list is shorter than
+// 2^31.
+__device__ ChunkPart chunk_plan(const AttnParams& p, int per, int part, int parts, int* s_scan,
+                                ChunkPart* s_part) {
+  const int warps = blockDim.x >> 5, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int run = (p.batch + warps - 1) / warps, b0 = min(p.batch, warp * run), b1 = min(p.batch, b0 + run);
+  int sum = 0;
+  auto each = [&](auto f) {      // f(b, sequence) until it says true
+    for (int at = b0; at < b1; at += 32) {
+      AttnSeq s{0, 0, 0, 0};
+      if (at + lane < b1) s = attn_seq(p, at + lane);
+      unsigned todo = __ballot_sync(0xffffffffu, at + lane < b1 && chunk_takes(p, s));
+      while (todo) {
+        const int i = __ffs(todo) - 1;
+        todo &= todo - 1;
+        if (f(at + i, seq_from(s, i))) return;
+      }
+    }
+  };
+  each([&](int, const AttnSeq& s) {
+    sum += warp_head_units(s, per) * p.kv_heads;
+    return false;
+  });
+  if (lane == 0) s_scan[warp] = sum;
+  __syncthreads();
+  int before = 0, total = 0;
+  for (int w = 0; w < warps; ++w) {
+    before += w < warp ? s_scan[w] : 0;
+    total += s_scan[w];
+  }
+  // part c of g: [total * c / g, total * (c + 1) / g), in 32 bits
+  const int g = min(parts, total), q = g ? total / g : 0, rem = g ? total - q * g : 0;
+  const int begin = part < g ? q * part + rem * part / g : 0;
+  const int count = part < g ? q * (part + 1) + rem * (part + 1) / g - begin : 0;
+  if (count > 0 && before <= begin && begin < before + sum) {
+    int at = before;
+    each([&](int b, const AttnSeq& s) {
+      const int u = warp_head_units(s, per);
+      if (begin >= at + u * p.kv_heads) {
+        at += u * p.kv_heads;
+        return false;
+      }
+      const int head = (begin - at) / u;
+      int r = begin - at - head * u;
+      for (int i0 = 0;; i0 += 32) {          // the row tile: 32 at a time
+        const int i = i0 + lane;
+        const int n = i < chunk_tiles(s, per) ? chunk_blocks(s, per, i) : 0;
+        int inc = n;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const int v = __shfl_up_sync(0xffffffffu, inc, o);
+          if (lane >= o) inc += v;
+        }
+        const int all = __shfl_sync(0xffffffffu, inc, 31);
+        if (r < all) {
+          if (inc - n <= r && r < inc) *s_part = ChunkPart{total, begin, count, b, head, i, r - (inc - n)};
+          return true;
+        }
+        r -= all;
+      }
+    });
+  } else if (count == 0 && threadIdx.x == 0) {
+    *s_part = ChunkPart{total, 0, 0, 0, 0, 0, 0};
+  }
+  __syncthreads();
+  return *s_part;
+}
+
+struct ChunkHead {         // the first 1024 bytes of shared memory
+  uint64_t bars[64];
+  int scan[16];
+  ChunkPart part;
+  uint32_t tmem;
+  int abort;
+};
 
 struct ChunkPiece {
   AttnSeq s;
   int b, head, tile, j0, j1, nb;
 };
+// Walks a part piece by piece.
 struct ChunkWalk {
-  int b;
-  long long left, off;
-  bool fresh;             // at the start of a part: (head, tile) not known yet
-  int head, tile, j;
+  int b, left, head, tile, j;
+  bool fresh;
   AttnSeq s;
+  __device__ __forceinline__ explicit ChunkWalk(const ChunkPart& c)
+      : b(c.b), left(c.count), head(c.head), tile(c.tile), j(c.j), fresh(true) {}
   __device__ __forceinline__ bool next(const AttnParams& p, int per, ChunkPiece& w) {
     if (left <= 0) return false;
     if (fresh) {
       fresh = false;
       s = attn_seq(p, b);
-      const long long u = chunk_head_units(s, per);
-      head = (int)(off / u);
-      const long long r = off - head * u;
-      int lo = 0, hi = chunk_tiles(s, per) - 1;      // the last tile that starts at or before r
-      while (lo < hi) {
-        const int mid = (lo + hi + 1) >> 1;
-        if (chunk_before(s, per, mid) <= r) lo = mid;
-        else hi = mid - 1;
-      }
-      tile = lo;
-      j = (int)(r - chunk_before(s, per, lo));
     } else {
       j = 0;
       if (++tile >= chunk_tiles(s, per)) {
@@ -162,11 +217,45 @@ struct ChunkWalk {
     w.tile = tile;
     w.nb = chunk_blocks(s, per, tile);
     w.j0 = j;
-    w.j1 = (int)min((long long)w.nb, j + left);
+    w.j1 = min(w.nb, j + left);
     left -= w.j1 - w.j0;
     return true;
   }
 };
+// Walks it tile by tile in the order of the ring: K j0, K j0 + 1, V j0, ...,
+// K last, V last - 1, V last.
+struct ChunkTiles {
+  ChunkWalk walk;
+  ChunkPiece w;
+  int j, step;
+  bool is_v;
+  __device__ __forceinline__ explicit ChunkTiles(const ChunkPart& c) : walk(c), step(-1) { w.j0 = w.j1 = 0; }
+  __device__ __forceinline__ bool next(const AttnParams& p, int per) {
+    // steps of a piece of n blocks: 0: K0; 2k - 1: K k; 2k: V k - 1; 2n - 1: V n - 1
+    const int n = w.j1 - w.j0;
+    if (step < 0 || ++step >= 2 * n) {
+      if (!walk.next(p, per, w)) return false;
+      step = 0;
+    }
+    const int m = w.j1 - w.j0;
+    is_v = step == 2 * m - 1 || (step > 0 && (step & 1) == 0);
+    j = w.j0 + (step == 2 * m - 1 ? m - 1 : is_v ? step / 2 - 1 : (step + 1) / 2);
+    return true;
+  }
+};
+// Where rows [row, row + n) of key block j lie: the page (as a plane of the
+// tensor map; -1: none) and the row inside it.  The sequence's last page is
+// read late by what it lacks, so that its valid rows come last.
+__device__ __forceinline__ void page_row(const AttnParams& p, const ChunkPiece& w, int key, int& plane, int& row) {
+  const int pg = key >> p.page_shift, start = pg << p.page_shift;
+  plane = -1;
+  row = key - start;
+  if (start < w.s.kv) {
+    const int id = __ldcg(p.table + (long long)w.b * p.table_stride + pg);
+    if (id >= 0 && id < p.pages) plane = id * p.kv_heads + w.head;
+    row -= max(0, start + p.page_size - w.s.kv);
+  }
+}
 
 // ---------------------------------------------------------------- PTX
 
@@ -212,6 +301,13 @@ __device__ __forceinline__ void tma_pair_3d(uint32_t dst, const void* map, uint3
       "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes"
       " [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(x),
       "r"(y), "r"(z)
+      : "memory");
+}
+__device__ __forceinline__ void tma_load_3d(uint32_t dst, const void* map, uint64_t* bar, int x, int y, int z) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)),
+      "r"(x), "r"(y), "r"(z)
       : "memory");
 }
 __device__ __forceinline__ void mma_pair_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
@@ -276,6 +372,26 @@ __device__ constexpr uint32_t idesc_16(int M, int N, bool b_n_major) {
          ((uint32_t)(M >> 4) << 24);
 }
 
+// a pair of fp32 operations in one instruction
+__device__ __forceinline__ void fma2(float& x, float& y, float a, float b) {   // (x, y) * a + b
+  asm("{\n\t.reg .b64 v, m, n;\n\tmov.b64 v, {%0, %1};\n\tmov.b64 m, {%2, %2};\n\tmov.b64 n, {%3, %3};\n\t"
+      "fma.rn.f32x2 v, v, m, n;\n\tmov.b64 {%0, %1}, v;\n\t}"
+      : "+f"(x), "+f"(y)
+      : "f"(a), "f"(b));
+}
+__device__ __forceinline__ void mul2(float& x, float& y, float a, float b) {   // (x * a, y * b)
+  asm("{\n\t.reg .b64 v, m;\n\tmov.b64 v, {%0, %1};\n\tmov.b64 m, {%2, %3};\n\t"
+      "mul.rn.f32x2 v, v, m;\n\tmov.b64 {%0, %1}, v;\n\t}"
+      : "+f"(x), "+f"(y)
+      : "f"(a), "f"(b));
+}
+__device__ __forceinline__ void add2(float& x, float& y, float a, float b) {   // (x + a, y + b)
+  asm("{\n\t.reg .b64 v, m;\n\tmov.b64 v, {%0, %1};\n\tmov.b64 m, {%2, %3};\n\t"
+      "add.rn.f32x2 v, v, m;\n\tmov.b64 {%0, %1}, v;\n\t}"
+      : "+f"(x), "+f"(y)
+      : "f"(a), "f"(b));
+}
+
 // two codes as two T values
 template <typename T>
 __device__ __forceinline__ uint32_t widen2(uint16_t c);
@@ -300,14 +416,21 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(ChunkCfg<T, D, E4>::
                       const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ AttnParams p,
                       const ChunkWs ws) {
   using C = ChunkCfg<T, D, E4>;
-  extern __shared__ uint8_t smem_raw[];
-  __shared__ long long s_scan[33];
-  __shared__ uint32_t s_tmem;
-  __shared__ volatile int s_abort;
-  uint8_t* smem = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
-  const uint32_t sq = smem_u32(smem), ss = sq + C::Q_BYTES;
-  float* s_ks = reinterpret_cast<float*>(smem + C::Q_BYTES + (size_t)C::SLOTS * C::SLOT);
-  uint64_t* full = reinterpret_cast<uint64_t*>(smem + C::Q_BYTES + (size_t)C::SLOTS * C::SLOT + C::KS_BYTES);
+  // no static shared memory: the dynamic part begins on a 1024-byte boundary
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  ChunkHead& head = *reinterpret_cast<ChunkHead*>(smem_raw);
+  static_assert(sizeof(ChunkHead) <= 1024, "head of shared memory");
+  volatile int& s_abort = head.abort;
+  uint8_t* smem = smem_raw + 1024;
+  uint8_t* at = smem + C::Q_BYTES;
+  uint8_t* s_ring = at;
+  at += (size_t)C::SLOTS * C::SLOT;
+  uint8_t* s_codes = at;
+  at += (size_t)C::RAWS * C::RAW;
+  float* s_sc = reinterpret_cast<float*>(at);           // [SC_RING][ks, f, 2^e][128]
+  at += C::SC_BYTES;
+  float* s_mx = reinterpret_cast<float*>(at);           // [2][2][128]
+  uint64_t* full = head.bars;
   uint64_t* empty = full + C::SLOTS;
   uint64_t* q_full = empty + C::SLOTS;
   uint64_t* q_empty = q_full + 1;
@@ -317,152 +440,140 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(ChunkCfg<T, D, E4>::
   uint64_t* o_free = o_done + 1;
   uint64_t* o_last = o_free + 1;
   uint64_t* all_done = o_last + 1;
+  uint64_t* x_bar = all_done + 1;        // [4]: a row's two threads
+  uint64_t* raw_full = x_bar + 4;        // codes: [RAWS]
+  uint64_t* raw_empty = raw_full + C::RAWS;
+  uint64_t* sc_full = raw_empty + C::RAWS;   // [SC_RING]
+  uint64_t* sc_empty = sc_full + C::SC_RING;
+  static_assert(2 * C::SLOTS + 14 + 2 * C::RAWS + 2 * C::SC_RING <= 64, "barriers");
+  const uint32_t sq = smem_u32(smem), ss = smem_u32(s_ring);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const uint32_t rank = cluster_rank();
+  if (smem_u32(smem_raw) & 1023) {       // the swizzle counts on it
+    if (tid == 0) attn_error(p.err, kAttnErrChunkAlign);
+    return;
+  }
   if (tid == 0) {
     for (int i = 0; i < C::SLOTS; ++i) {
-      mbar_init(full + i, E4 ? 8 : 1);   // E4: four warps of either CTA
+      mbar_init(full + i, E4 ? 8 : 1);   // codes: four widening warps of either CTA
       mbar_init(empty + i, 1);
     }
     mbar_init(q_full, 1);
     mbar_init(q_empty, 1);
     for (int i = 0; i < 2; ++i) {
       mbar_init(s_full + i, 1);
-      mbar_init(p_ready + i, 8);         // four warps of either CTA
+      mbar_init(p_ready + i, 16);        // eight warps of either CTA
     }
     mbar_init(o_done, 1);
-    mbar_init(o_free, 8);
+    mbar_init(o_free, 16);
     mbar_init(o_last, 1);
     mbar_init(all_done, 1);
+    for (int i = 0; i < 4; ++i) mbar_init(x_bar + i, 2);
+    if (E4) {
+      for (int i = 0; i < C::RAWS; ++i) {
+        mbar_init(raw_full + i, 1);
+        mbar_init(raw_empty + i, 4);
+      }
+      for (int i = 0; i < C::SC_RING; ++i) {
+        mbar_init(sc_full + i, 1);
+        mbar_init(sc_empty + i, 12);     // eight softmax, four widening warps
+      }
+    }
     fence_barrier_init();
     s_abort = 0;
     tma_prefetch_desc(&tm_q);
     tma_prefetch_desc(&tm_k);
     tma_prefetch_desc(&tm_v);
   }
-  if (warp == 4) {
-    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&s_tmem)), "r"(512)
+  if (warp == 8) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&head.tmem)), "r"(512)
                  : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;");
   }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = s_tmem;
+  const uint32_t tmem = head.tmem;
   pdl_trigger();
   pdl_wait();
   const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
   const int tpc = 128 / p.group, per = 2 * tpc;      // tokens of a CTA, of the pair
-  const RowsWork work = list_plan(
-      p, s_scan,
-      [&](int b) -> long long {
-        const AttnSeq s = attn_seq(p, b);
-        return chunk_takes(p, s) ? chunk_head_units(s, per) * p.kv_heads : 0;
-      },
-      [&](RowsWork& r) {
-        const long long g = min((long long)pairs, r.total);
-        r.begin = pair < g ? r.total * pair / g : 0;
-        r.count = pair < g ? r.total * (pair + 1) / g - r.begin : 0;
-      });
+  const ChunkPart part = chunk_plan(p, per, pair, pairs, head.scan, &head.part);
   cluster_sync_all();      // both CTAs' barriers are ready
-  ChunkWalk walk;
-  walk.b = work.b;
-  walk.left = work.count;
-  walk.off = work.off;
-  walk.fresh = true;
-  ChunkPiece w;
   const int ps = p.page_size;
 
-  if (warp == 5 && !E4) {
-    // ---- TMA: Q of a piece, then K0, K1, V0, K2, V1, ..., V last
+  bool ok = true;
+  // every lane of a warp: false once a wait has run out, here or in another role
+  auto wait_warp = [&](uint64_t* bar, uint32_t par, int code) {
+    if (ok && !mbar_wait_cluster(bar, par)) {
+      attn_error(p.err, code);
+      s_abort = 1;
+      ok = false;
+    }
+    ok = __all_sync(0xffffffffu, ok && !s_abort);
+    return ok;
+  };
+
+  if (warp == 9) {
+    // ---- TMA: Q of a piece, then its tiles
+    ChunkTiles tl(part);
     int slot = 0;
     uint32_t phase = 0, qn = 0;
-    bool ok = true;
-    const int kbox = min(ps, 64), vbox = min(ps, kBlockKeys);
-    auto load = [&](const ChunkPiece& x, int j, bool is_v) {
-      if (ok && !mbar_wait(empty + slot, phase ^ 1, kAttnWaitBudgetNs)) {
-        if (lane == 0) attn_error(p.err, kAttnErrChunkLoad);
-        ok = false;
-      }
-      ok = __all_sync(0xffffffffu, ok && !s_abort);
-      if (!ok) return;
-      if (rank == 0 && lane == 0) mbar_arrive_expect_tx(full + slot, 2 * C::SLOT);
-      __syncwarp();
-      const uint32_t bar = mapa(smem_u32(full + slot), 0);
-      const uint32_t dst = ss + slot * C::SLOT;
-      // boxes of one column, columns of 64 dims
-      const int box = is_v ? vbox : kbox, rows = is_v ? kBlockKeys : 64, n = rows / box;
-      const int cols = is_v ? D / 128 : D / 64;
-      for (int i = lane; i < n * cols; i += 32) {
-        const int bx = i % n, col = i / n;
-        const int key = j * kBlockKeys + (is_v ? 0 : 64 * (int)rank) + bx * box;
-        const int pg = key >> p.page_shift, start = pg << p.page_shift;
-        int z = -1, y = key - start;
-        if (start < x.s.kv) {
-          const int id = __ldcg(p.table + (long long)x.b * p.table_stride + pg);
-          if (id >= 0 && id < p.pages) z = id * p.kv_heads + x.head;
-          if (start + ps > x.s.kv) y -= start + ps - x.s.kv;    // the last page: shifted
+    constexpr int N = E4 ? C::RAWS : C::SLOTS;
+    uint64_t* bars_full = E4 ? raw_full : full;
+    uint64_t* bars_empty = E4 ? raw_empty : empty;
+    while (tl.next(p, per)) {
+      const ChunkPiece& x = tl.w;
+      if (tl.step == 0) {
+        if (!wait_warp(q_empty, (qn & 1) ^ 1, kAttnErrChunkLoad)) break;
+        ++qn;
+        if (lane == 0) {
+          if (rank == 0) mbar_arrive_expect_tx(q_full, 2 * (D / 64) * tpc * p.group * 128);
+          const uint32_t bar = mapa(smem_u32(q_full), 0);
+          const int tok = x.s.q0 + x.tile * per + (int)rank * tpc;
+          for (int c = 0; c < D / 64; ++c)
+            tma_pair_3d(sq + c * (128 * 128), &tm_q, bar, c * 64, x.head * p.group, tok);
         }
-        // outside the map (no page, or before its first row): zeros
-        tma_pair_3d(dst + col * (rows * 128) + bx * (box * 128), is_v ? &tm_v : &tm_k, bar,
-                    (is_v ? (int)rank * (D / 2) : 0) + col * 64, y, z);
+        __syncwarp();
       }
-      if (++slot == C::SLOTS) { slot = 0; phase ^= 1; }
-    };
-    while (ok && walk.next(p, per, w)) {
-      if (!mbar_wait(q_empty, (qn & 1) ^ 1, kAttnWaitBudgetNs)) {
-        if (lane == 0) attn_error(p.err, kAttnErrChunkLoad);
-        ok = false;
-      }
-      ++qn;
-      ok = __all_sync(0xffffffffu, ok && !s_abort);
-      if (!ok) break;
-      if (lane == 0) {
-        if (rank == 0) mbar_arrive_expect_tx(q_full, 2 * (D / 64) * tpc * p.group * 128);
-        const uint32_t bar = mapa(smem_u32(q_full), 0);
-        const int tok = w.s.q0 + w.tile * per + (int)rank * tpc;
-        for (int c = 0; c < D / 64; ++c)
-          tma_pair_3d(sq + c * (128 * 128), &tm_q, bar, c * 64, w.head * p.group, tok);
+      if (!wait_warp(bars_empty + slot, phase ^ 1, kAttnErrChunkLoad)) break;
+      if (E4) {
+        if (lane == 0) mbar_arrive_expect_tx(bars_full + slot, C::RAW);
+      } else if (rank == 0 && lane == 0) {
+        mbar_arrive_expect_tx(bars_full + slot, 2 * C::SLOT);
       }
       __syncwarp();
-      for (int j = w.j0; j < w.j1; ++j) {
-        load(w, j, false);
-        if (j > w.j0) load(w, j - 1, true);
-      }
-      load(w, w.j1 - 1, true);
-    }
-    if (!ok) s_abort = 1;
-    if (!ok && rank == 0)
-      for (int i = 0; i < C::SLOTS; ++i) mbar_wait(full + i, phase ^ (i < slot ? 0 : 1), kAttnWaitBudgetNs);
-  } else if (warp == 5) {
-    // ---- codes: only Q comes by TMA
-    uint32_t qn = 0;
-    bool ok = true;
-    while (ok && walk.next(p, per, w)) {
-      if (!mbar_wait(q_empty, (qn & 1) ^ 1, kAttnWaitBudgetNs)) {
-        if (lane == 0) attn_error(p.err, kAttnErrChunkLoad);
-        ok = false;
-      }
-      ++qn;
-      ok = __all_sync(0xffffffffu, ok && !s_abort);
-      if (!ok) break;
-      if (lane == 0) {
-        if (rank == 0) mbar_arrive_expect_tx(q_full, 2 * (D / 64) * tpc * p.group * 128);
-        const uint32_t bar = mapa(smem_u32(q_full), 0);
-        const int tok = w.s.q0 + w.tile * per + (int)rank * tpc;
-        for (int c = 0; c < D / 64; ++c)
-          tma_pair_3d(sq + c * (128 * 128), &tm_q, bar, c * 64, w.head * p.group, tok);
+      // boxes of one column; columns of 64 dims, or the whole row of codes
+      const bool v = tl.is_v;
+      const int rows = v ? kBlockKeys : 64, box = min(ps, rows), n = rows / box;
+      const int cols = E4 ? 1 : v ? D / 128 : D / 64;
+      const uint32_t bar = mapa(smem_u32(bars_full + slot), 0);
+      if (lane < n * cols) {
+        const int bx = lane % n, col = lane / n;
+        int plane, row;
+        page_row(p, x, tl.j * kBlockKeys + (v ? 0 : 64 * (int)rank) + bx * box, plane, row);
+        const int x0 = (v ? (int)rank * (D / 2) : 0) + col * 64;
+        if (E4)
+          tma_load_3d(smem_u32(s_codes) + slot * C::RAW + bx * box * (v ? D / 2 : D), v ? &tm_v : &tm_k,
+                      bars_full + slot, x0, row, plane);
+        else
+          tma_pair_3d(ss + slot * C::SLOT + col * (rows * 128) + bx * (box * 128), v ? &tm_v : &tm_k, bar, x0, row,
+                      plane);
       }
       __syncwarp();
+      if (++slot == N) { slot = 0; phase ^= 1; }
     }
-    if (!ok) s_abort = 1;
-  } else if (warp == 4) {
+    // after a wait ran out: what is in flight has landed before the memory goes
+    if (!ok && (E4 || rank == 0))
+      for (int i = 0; i < N; ++i) mbar_wait(bars_full + i, phase ^ (i < slot ? 0 : 1), kAttnWaitBudgetNs);
+  } else if (warp == 8) {
     // ---- MMAs of the pair
     if (rank == 0 && lane == 0) {
       constexpr uint32_t id_s = idesc_16<T>(256, kBlockKeys, false), id_o = idesc_16<T>(256, D, true);
+      ChunkWalk walk(part);
+      ChunkPiece w;
       int slot = 0;
-      uint32_t phase = 0, it = 0, qn = 0, pieces = 0;
-      bool ok = true;
+      uint32_t phase = 0, it = 0, pieces = 0;
       auto wait = [&](uint64_t* bar, uint32_t par) {
         if (ok && !mbar_wait_cluster(bar, par)) {
           attn_error(p.err, kAttnErrChunkMma);
@@ -484,12 +595,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(ChunkCfg<T, D, E4>::
         for (int k = 0; k < D / 16; ++k)
           mma_pair_ss(d, smem_desc_k128(sq + (k >> 2) * (128 * 128) + (k & 3) * 32),
                       smem_desc_k128(kb + (k >> 2) * (64 * 128) + (k & 3) * 32), id_s, k > 0);
-        advance();
         commit_pair(s_full + (x & 1));
+        advance();
       };
       auto values = [&](uint32_t x, bool first) {
-        if (!wait(p_ready + (x & 1), (x >> 1) & 1)) return;
         if (!wait(full + slot, phase)) return;
+        if (!wait(p_ready + (x & 1), (x >> 1) & 1)) return;
         if (first && pieces > 0 && !wait(o_free, (pieces - 1) & 1)) return;
         tc_fence_after();
         const uint32_t vb = ss + slot * C::SLOT, a = tmem + C::COL_S + (x & 1) * kBlockKeys;
@@ -497,12 +608,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(ChunkCfg<T, D, E4>::
         for (int k = 0; k < kBlockKeys / 16; ++k)
           mma_pair_ts(tmem + C::COL_O, a + k * 8, smem_desc_n128(vb + k * (16 * 128), kBlockKeys * 128), id_o,
                       !first || k > 0);
-        advance();
         commit_pair(o_done);
+        advance();
       };
       while (ok && walk.next(p, per, w)) {
-        if (!wait(q_full, qn & 1)) break;
-        ++qn;
+        if (!wait(q_full, pieces & 1)) break;
         for (int j = w.j0; j < w.j1 && ok; ++j, ++it) {
           scores(it);
           if (j == w.j1 - 1 && ok) commit_pair(q_empty);
@@ -514,23 +624,31 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(ChunkCfg<T, D, E4>::
       }
       commit_pair(all_done);
     }
-  } else if (warp < 4) {
-    // ---- softmax: thread = row
-    const uint32_t lanes = tmem + ((uint32_t)(warp * 32) << 16);
-    const int rr = warp * 32 + lane, ti = rr / p.group;
-    const int hd = rr - ti * p.group;
+  } else if (warp < 8) {
+    // ---- softmax: a row's thread of half h has keys [64 h, 64 h + 64) of a
+    // block and dims [h D/2, (h + 1) D/2) of the output
+    const int h = warp >> 2, quarter = warp & 3, rr = quarter * 32 + lane;
+    const uint32_t lanes = tmem + ((uint32_t)(quarter * 32) << 16);
+    const uint32_t mine_o = lanes + C::COL_O + h * (D / 2);
+    const int ti = rr / p.group, hd = rr - ti * p.group;
+    // the value that the row's other thread gives; bounded, unlike a barrier
+    // among some of the warps.  Two buffers: a thread is one exchange ahead at
+    // most.
+    uint32_t xn = 0;
+    auto exchange = [&](float v) {
+      float* buf = s_mx + (xn & 1) * 256 + rr;
+      buf[h * 128] = v;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(x_bar + quarter);
+      wait_warp(x_bar + quarter, xn & 1, kAttnErrChunkSoftmax);
+      ++xn;
+      return buf[(h ^ 1) * 128];
+    };
+    ChunkWalk walk(part);
+    ChunkPiece w;
     uint32_t it = 0, pieces = 0;
-    bool ok = true;
     int4 desc = make_int4(0, 0, 0, -1);
     const float c = p.scale_log2;
-    auto wait = [&](uint64_t* bar, uint32_t par) {
-      if (ok && !mbar_wait_cluster(bar, par)) {
-        attn_error(p.err, kAttnErrChunkSoftmax);
-        s_abort = 1;
-        ok = false;
-      }
-      ok = __all_sync(0xffffffffu, ok && !s_abort);
-    };
     while (ok && walk.next(p, per, w)) {
       const int tok = w.tile * per + (int)rank * tpc + ti;       // of the sequence's new ones
       const bool row_ok = ti < tpc && tok < w.s.n;
@@ -538,22 +656,20 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(ChunkCfg<T, D, E4>::
       float m = -INFINITY, l = 0.f;
       for (int j = w.j0; j < w.j1; ++j, ++it) {
         const uint32_t sb = lanes + C::COL_S + (it & 1) * kBlockKeys;
-        wait(s_full + (it & 1), (it >> 1) & 1);
-        if (!ok) break;
+        const float* sc = s_sc + (it % C::SC_RING) * 3 * kBlockKeys + h * 64;
+        if (E4) wait_warp(sc_full + it % C::SC_RING, (it / C::SC_RING) & 1, kAttnErrChunkSoftmax);
+        if (!wait_warp(s_full + (it & 1), (it >> 1) & 1, kAttnErrChunkSoftmax)) break;
         tc_fence_after();
-        float s[kBlockKeys];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) tmem_ld32(sb + 32 * i, s + 32 * i);
+        float s[64];
+        tmem_ld32(sb + 64 * h, s);
+        tmem_ld32(sb + 64 * h + 32, s + 32);
         tmem_ld_wait();
         if (E4) {
-          const float4* ks = reinterpret_cast<const float4*>(s_ks + (it % C::KS_RING) * kBlockKeys);
 #pragma unroll
-          for (int i = 0; i < kBlockKeys / 4; ++i) {
-            const float4 f = ks[i];
-            s[4 * i] *= f.x;
-            s[4 * i + 1] *= f.y;
-            s[4 * i + 2] *= f.z;
-            s[4 * i + 3] *= f.w;
+          for (int i = 0; i < 16; ++i) {
+            const float4 f = reinterpret_cast<const float4*>(sc)[i];
+            mul2(s[4 * i], s[4 * i + 1], f.x, f.y);
+            mul2(s[4 * i + 2], s[4 * i + 3], f.z, f.w);
           }
         }
         const int lim = last - j * kBlockKeys;                    // last visible key of the block
@@ -561,20 +677,26 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(ChunkCfg<T, D, E4>::
           // columns from t0 hold the sequence's last page, `shift` columns late
           const int valid = w.s.kv - j * kBlockKeys;
           int t0 = kBlockKeys, shift = 0;
-          if (!E4 && valid > 0 && valid < kBlockKeys) {
+          if (valid > 0 && valid < kBlockKeys) {
             t0 = (valid - 1) / ps * ps;
             shift = t0 + ps - valid;
           }
 #pragma unroll
-          for (int i = 0; i < kBlockKeys; ++i) {
-            const int key = i < t0 ? i : (i < t0 + shift ? kBlockKeys : i - shift);
+          for (int i = 0; i < 64; ++i) {
+            const int col = 64 * h + i;
+            const int key = col < t0 ? col : (col < t0 + shift ? kBlockKeys : col - shift);
             if (key > lim) s[i] = -INFINITY;
           }
         }
         float m4[4] = {s[0], s[1], s[2], s[3]};
 #pragma unroll
-        for (int i = 4; i < kBlockKeys; ++i) m4[i & 3] = fmaxf(m4[i & 3], s[i]);
-        const float mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * c;
+        for (int i = 4; i < 64; ++i) m4[i & 3] = fmaxf(m4[i & 3], s[i]);
+        float mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * c;
+        // the other half's maximum; both threads then decide alike.  (The
+        // exchange also says that both halves of S are in registers: P of half
+        // 1 goes over S of half 0.)
+        mx = fmaxf(mx, exchange(mx));
+        if (!ok) break;
         const bool grow = mx > m + kRescaleLog2 || (m == -INFINITY && mx > m);
         if (__any_sync(0xffffffffu, grow)) {
           const float f = !grow ? 1.f : m == -INFINITY ? 0.f : ex2(m - mx);
@@ -583,71 +705,74 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(ChunkCfg<T, D, E4>::
           if (j > w.j0) {
             // one phase to wait for: P V of the block before came before this
             // S, and this block's waits for this warp
-            wait(o_done, (it - 1) & 1);
-            if (!ok) break;
+            if (!wait_warp(o_done, (it - 1) & 1, kAttnErrChunkSoftmax)) break;
             tc_fence_after();
-            // 32 columns at a time; a row that starts here holds zeros or what
-            // its factor 0 must not turn into NaN
+            // a row that starts here holds zeros, or what its factor 0 must
+            // not turn into NaN
 #pragma unroll 1
-            for (int i = 0; i < D / 32; ++i) {
+            for (int i = 0; i < D / 64; ++i) {
               float o[32];
-              tmem_ld32(lanes + C::COL_O + 32 * i, o);
+              uint32_t u[32];
+              tmem_ld32(mine_o + 32 * i, o);
               tmem_ld_wait();
 #pragma unroll
-              for (int q = 0; q < 32; ++q) o[q] = f == 0.f ? 0.f : o[q] * f;
-              uint32_t u[32];
-#pragma unroll
-              for (int q = 0; q < 32; ++q) u[q] = __float_as_uint(o[q]);
-              tmem_st32(lanes + C::COL_O + 32 * i, u);
+              for (int q = 0; q < 32; ++q) u[q] = __float_as_uint(f == 0.f ? 0.f : o[q] * f);
+              tmem_st32(mine_o + 32 * i, u);
             }
             tmem_st_wait();
           }
         }
         const float base = m == -INFINITY ? 0.f : m;
         float l2[2] = {0.f, 0.f};
+        uint32_t pk[32];
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          uint32_t pk[32];
-#pragma unroll
-          for (int q = 0; q < 32; ++q) {
-            const float a = ex2(fmaf(s[64 * i + 2 * q], c, -base)), b = ex2(fmaf(s[64 * i + 2 * q + 1], c, -base));
-            l2[0] += a;
-            l2[1] += b;
-            pk[q] = Elem<T>::from_f2(a, b);
+        for (int q = 0; q < 32; ++q) {
+          float a = s[2 * q], b = s[2 * q + 1];
+          fma2(a, b, c, -base);
+          a = ex2(a);
+          b = ex2(b);
+          add2(l2[0], l2[1], a, b);
+          if (E4) {
+            const float2 f = reinterpret_cast<const float2*>(sc + kBlockKeys)[q];
+            mul2(a, b, f.x, f.y);
           }
-          tmem_st32(sb + 32 * i, pk);
+          pk[q] = Elem<T>::from_f2(a, b);
         }
+        tmem_st32(sb + 32 * h, pk);
         l += l2[0] + l2[1];
         tmem_st_wait();
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive_cluster(mapa(smem_u32(p_ready + (it & 1)), 0));
+        if (lane == 0) {
+          mbar_arrive_cluster(mapa(smem_u32(p_ready + (it & 1)), 0));
+          if (E4) mbar_arrive(sc_empty + it % C::SC_RING);
+        }
       }
       if (!ok) break;
+      l += exchange(l);
       // a barrier of its own: o_done may be two phases behind here
-      wait(o_last, pieces & 1);
+      if (!wait_warp(o_last, pieces & 1, kAttnErrChunkSoftmax)) break;
       ++pieces;
-      if (!ok) break;
       tc_fence_after();
       const bool whole = w.j0 == 0 && w.j1 == w.nb;
       const int place = pair * 2 + (w.j0 == 0 ? 1 : 0), row = (int)rank * 128 + rr;
-      if (!whole) {
+      if (!whole && h == 0) {
         ws.ml[((size_t)place * 256 + row) * 2] = m;
         ws.ml[((size_t)place * 256 + row) * 2 + 1] = l;
-        if (w.j0 == 0) {
+        if (w.j0 == 0 && tid == 0) {
           // the part that holds the tile's last block
-          const long long u = work.begin + work.count + (w.nb - w.j1) - 1, g = min((long long)pairs, work.total);
-          desc = make_int4(w.b, w.head, w.tile, (int)(((u + 1) * g - 1) / work.total));
+          const long long u = (long long)part.begin + part.count + (w.nb - w.j1) - 1;
+          desc = make_int4(w.b, w.head, w.tile, (int)(((u + 1) * min(pairs, part.total) - 1) / part.total));
         }
       }
       const float inv = l > 0.f ? 1.f / l : 0.f;
       T* dst = static_cast<T*>(p.out) + (long long)(w.s.q0 + tok) * p.out_token +
-               (long long)(w.head * p.group + hd) * p.out_head;
-      float* wo = ws.o + ((size_t)place * 256 + row) * D;
+               (long long)(w.head * p.group + hd) * p.out_head + h * (D / 2);
+      float* wo = ws.o + ((size_t)place * 256 + row) * D + h * (D / 2);
 #pragma unroll 1
-      for (int i = 0; i < D / 32; ++i) {
+      for (int i = 0; i < D / 64; ++i) {
         float o[32];
-        tmem_ld32(lanes + C::COL_O + 32 * i, o);
+        tmem_ld32(mine_o + 32 * i, o);
         tmem_ld_wait();
         if (whole && row_ok) {
 #pragma unroll
@@ -673,106 +798,125 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(ChunkCfg<T, D, E4>::
       if (lane == 0) mbar_arrive_cluster(mapa(smem_u32(o_free), 0));
     }
     if (rank == 0 && tid == 0) ws.desc[pair] = desc;
-  } else if (E4) {
-    // ---- codes: warps 6-9 load, widen and store this CTA's halves
-    const int t = tid - 192;
+  } else if (E4 && warp == 10) {
+    // ---- scales: lane has columns lane + 32 i of every block, in the order
+    // of the loaded rows; the next block's are on their way while one is stored
+    ChunkWalk walk(part);
+    ChunkPiece w;
+    uint32_t it = 0;
+    int j = 0;
+    bool more = walk.next(p, per, w);
+    j = more ? w.j0 : 0;
+    float k[4], v[4];
+    auto load = [&]() {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        int plane, row;
+        page_row(p, w, j * kBlockKeys + lane + 32 * i, plane, row);
+        const bool have = plane >= 0 && row >= 0;
+        const long long at_row = ((long long)plane << p.page_shift) + row;
+        k[i] = have ? __ldcg(p.k_scale + at_row) : 0.f;
+        v[i] = have ? __ldcg(p.v_scale + at_row) : 0.f;
+      }
+    };
+    if (more) load();
+    while (more) {
+      float ck[4], cv[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        ck[i] = k[i];
+        cv[i] = v[i];
+      }
+      if (++j >= w.j1) {
+        more = walk.next(p, per, w);
+        j = more ? w.j0 : 0;
+      }
+      if (more) load();
+      if (!wait_warp(sc_empty + it % C::SC_RING, ((it / C::SC_RING) & 1) ^ 1, kAttnErrChunkWiden)) break;
+      float* sc = s_sc + (it % C::SC_RING) * 3 * kBlockKeys + lane;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        // v = f * 2^e; a scale without an exponent of its own stays whole
+        const uint32_t b = __float_as_uint(cv[i]);
+        const bool normal = (b & 0x7f800000u) != 0;
+        sc[32 * i] = ck[i];
+        sc[kBlockKeys + 32 * i] = normal ? __uint_as_float((b & 0x007fffffu) | 0x3f800000u) : 1.f;
+        sc[2 * kBlockKeys + 32 * i] = normal ? __uint_as_float(b & 0xff800000u) : cv[i];
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(sc_full + it % C::SC_RING);
+      ++it;
+    }
+  } else if (E4 && warp >= 12) {
+    // ---- codes to 16 bits: raw ring -> operand ring
+    const int t = tid - 384;
     constexpr int PIECES = 64 * D / 16 / 128;      // 16-code pieces of a thread
-    int slot = 0;
-    uint32_t phase = 0, kn = 0;
-    bool ok = true;
-    auto load = [&](const ChunkPiece& x, int j, bool is_v) {
-      // K: 64 keys x D; V: 128 keys x D/2
-      const int per_row = is_v ? D / 32 : D / 16;
-      uint4 u[PIECES];
-      float sc[PIECES];
+    ChunkTiles tl(part);
+    int slot = 0, raw = 0;
+    uint32_t phase = 0, raw_phase = 0, vn = 0;
+    while (tl.next(p, per)) {
+      const bool v = tl.is_v;
+      const float* e2 = s_sc + ((vn % C::SC_RING) * 3 + 2) * kBlockKeys;
+      if (!wait_warp(raw_full + raw, raw_phase, kAttnErrChunkWiden)) break;
+      if (v && !wait_warp(sc_full + vn % C::SC_RING, (vn / C::SC_RING) & 1, kAttnErrChunkWiden)) break;
+      if (!wait_warp(empty + slot, phase ^ 1, kAttnErrChunkWiden)) break;
+      const uint4* src = reinterpret_cast<const uint4*>(s_codes + (size_t)raw * C::RAW);
+      uint8_t* dst = s_ring + (size_t)slot * C::SLOT;
+      // a row is D/16 pieces of K, D/32 of V
+      const int per_row = v ? D / 32 : D / 16, rows = v ? kBlockKeys : 64;
 #pragma unroll
       for (int i = 0; i < PIECES; ++i) {
-        const int at = i * 128 + t, r = at / per_row, c = at - r * per_row;
-        const int key = j * kBlockKeys + (is_v ? 0 : 64 * (int)rank) + r;
-        u[i] = make_uint4(0, 0, 0, 0);
-        sc[i] = 0.f;
-        if (key < x.s.kv) {
-          const int id = __ldcg(p.table + (long long)x.b * p.table_stride + (key >> p.page_shift));
-          if (id >= 0 && id < p.pages) {
-            const long long row = ((long long)(id * p.kv_heads + x.head) << p.page_shift) + (key & (ps - 1));
-            u[i] = __ldcg(reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(is_v ? p.v_codes : p.k_codes) +
-                                                         row * D + (is_v ? (int)rank * (D / 2) : 0) + c * 16));
-            if (is_v) sc[i] = __ldcg(p.v_scale + row);
-          }
-        }
-      }
-      float ks = 0.f;
-      if (!is_v) {
-        // both CTAs need the scales of all 128 keys
-        const int key = j * kBlockKeys + t;
-        if (key < x.s.kv) {
-          const int id = __ldcg(p.table + (long long)x.b * p.table_stride + (key >> p.page_shift));
-          if (id >= 0 && id < p.pages)
-            ks = __ldcg(p.k_scale + ((long long)(id * p.kv_heads + x.head) << p.page_shift) + (key & (ps - 1)));
-        }
-      }
-      if (ok && !mbar_wait(empty + slot, phase ^ 1, kAttnWaitBudgetNs)) {
-        if (lane == 0) attn_error(p.err, kAttnErrChunkWiden);
-        ok = false;
-      }
-      ok = __all_sync(0xffffffffu, ok && !s_abort);
-      if (!ok) return;
-      uint8_t* dst = smem + C::Q_BYTES + (size_t)slot * C::SLOT;
-      const int rows = is_v ? kBlockKeys : 64;
-#pragma unroll
-      for (int i = 0; i < PIECES; ++i) {
-        const int at = i * 128 + t, r = at / per_row, c = at - r * per_row;
-        const uint32_t w4[4] = {u[i].x, u[i].y, u[i].z, u[i].w};
+        const int n = i * 128 + t, r = n / per_row, cpos = n - r * per_row;
+        const uint4 u = src[n];
+        const uint32_t w4[4] = {u.x, u.y, u.z, u.w};
         uint32_t o[8];
+        const float e = v ? e2[r] : 1.f;
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
-          if (is_v) {
-            o[2 * q] = widen2<T>((uint16_t)w4[q], sc[i]);
-            o[2 * q + 1] = widen2<T>((uint16_t)(w4[q] >> 16), sc[i]);
+          if (v) {
+            o[2 * q] = widen2<T>((uint16_t)w4[q], e);
+            o[2 * q + 1] = widen2<T>((uint16_t)(w4[q] >> 16), e);
           } else {
             o[2 * q] = widen2<T>((uint16_t)w4[q]);
             o[2 * q + 1] = widen2<T>((uint16_t)(w4[q] >> 16));
           }
         }
-        // 16 values: two 16-byte pieces of a 64-dim column
-        uint8_t* col = dst + (c >> 2) * (rows * 128) + r * 128;
-        const int pc = (c & 3) * 2;
-        *reinterpret_cast<uint4*>(col + (((pc ^ r) & 7) << 4)) = make_uint4(o[0], o[1], o[2], o[3]);
-        *reinterpret_cast<uint4*>(col + ((((pc + 1) ^ r) & 7) << 4)) = make_uint4(o[4], o[5], o[6], o[7]);
-      }
-      if (!is_v) {
-        s_ks[(kn % C::KS_RING) * kBlockKeys + t] = ks;
-        ++kn;
+        // 16 values: two 16-byte pieces of a 64-dim column.  Threads of the
+        // second column store theirs the other way round, so that eight
+        // threads hit eight different pieces.
+        uint8_t* col = dst + (cpos >> 2) * (rows * 128) + r * 128;
+        const int p0 = (cpos & 3) * 2, swap = (cpos >> 2) & 1;
+        const uint4 lo = make_uint4(o[0], o[1], o[2], o[3]), hi = make_uint4(o[4], o[5], o[6], o[7]);
+        *reinterpret_cast<uint4*>(col + ((((p0 + swap) ^ r) & 7) << 4)) = swap ? hi : lo;
+        *reinterpret_cast<uint4*>(col + ((((p0 + 1 - swap) ^ r) & 7) << 4)) = swap ? lo : hi;
       }
       fence_proxy_async_smem();
       __syncwarp();
-      if (lane == 0) mbar_arrive_cluster(mapa(smem_u32(full + slot), 0));
-      if (++slot == C::SLOTS) { slot = 0; phase ^= 1; }
-    };
-    while (ok && walk.next(p, per, w)) {
-      for (int j = w.j0; j < w.j1 && ok; ++j) {
-        load(w, j, false);
-        if (j > w.j0 && ok) load(w, j - 1, true);
+      if (lane == 0) {
+        mbar_arrive_cluster(mapa(smem_u32(full + slot), 0));
+        mbar_arrive(raw_empty + raw);
+        if (v) mbar_arrive(sc_empty + vn % C::SC_RING);
       }
-      if (ok) load(w, w.j1 - 1, true);
+      if (v) ++vn;
+      if (++slot == C::SLOTS) { slot = 0; phase ^= 1; }
+      if (++raw == C::RAWS) { raw = 0; raw_phase ^= 1; }
     }
-    if (!ok) s_abort = 1;
   }
   __syncwarp();
   tc_fence_before();
   __syncthreads();
   // every MMA of the pair, and every arrival that it makes here, has ended
   // before TMEM or shared memory goes
-  if (warp == 4 && !mbar_wait_cluster(all_done, 0) && lane == 0) attn_error(p.err, kAttnErrChunkMma);
+  if (warp == 8 && !mbar_wait_cluster(all_done, 0) && lane == 0) attn_error(p.err, kAttnErrChunkMma);
   __syncwarp();
   cluster_sync_all();      // no CTA leaves while its pair may still arrive at it
   tc_fence_after();
-  if (warp == 4) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
+  if (warp == 8) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
 }
 
 // Tiles that the parts' cuts go through: the sum of their parts, in order.
 // blockIdx.x is the part in which the tile begins, blockIdx.y a group of rows.
-constexpr int kJoinRows = 16;
+constexpr int kJoinRows = 4;
 template <typename T, int D>
 __global__ void __launch_bounds__(256) attn_chunk_join_kernel(const __grid_constant__ AttnParams p, const ChunkWs ws) {
   pdl_trigger();

@@ -57,7 +57,8 @@ ERROR_CODES = {
     53: "paged attention, chunk: the loading warp waited for a free slot",
     54: "paged attention, chunk: the MMA issuer waited for operands or for the softmax",
     55: "paged attention, chunk: the softmax waited for scores or for the output",
-    56: "paged attention, chunk: a widening warp waited for a free slot",
+    56: "paged attention, chunk: a widening or scale warp waited for its ring",
+    57: "paged attention, chunk: shared memory not on a 1024-byte boundary",
 }
 
 
