@@ -161,7 +161,7 @@ static int launch_chunk(const AttnParams& p, const d3_attention* a, const d3_kv_
   D3_CUDA_TRY(launch_k(attn_chunk_kernel<T, D, E4>, dim3(2 * pairs), dim3(C::THREADS), C::SMEM, st, pdl_enabled(),
                        tq, tk, tv, p, ws),
               "attn_chunk_kernel launch");
-  D3_CUDA_TRY(launch_k(attn_chunk_join_kernel<T, D>, dim3(pairs, 256 / kJoinRows), dim3(256), 0, st, pdl_enabled(),
+  D3_CUDA_TRY(launch_k(attn_chunk_join_kernel<T, D>, dim3(pairs, 8 * (D / 32)), dim3(256), 0, st, pdl_enabled(),
                        p, ws),
               "attn_chunk_join_kernel launch");
   return D3_OK;

@@ -70,7 +70,7 @@ struct ChunkCfg {
 };
 
 struct ChunkWs {           // carved from the call's workspace
-  float* o;                // [pairs][2][256][D]
+  float* o;                // [pairs][2][D / 4][256][4]
   float* ml;               // [pairs][2][256][2]
   int4* desc;              // [pairs]: sequence, KV head, row tile, last part (-1: none)
 };
@@ -243,19 +243,43 @@ struct ChunkTiles {
     return true;
   }
 };
-// Where rows [row, row + n) of key block j lie: the page (as a plane of the
-// tensor map; -1: none) and the row inside it.  The sequence's last page is
-// read late by what it lacks, so that its valid rows come last.
-__device__ __forceinline__ void page_row(const AttnParams& p, const ChunkPiece& w, int key, int& plane, int& row) {
-  const int pg = key >> p.page_shift, start = pg << p.page_shift;
-  plane = -1;
-  row = key - start;
-  if (start < w.s.kv) {
-    const int id = __ldcg(p.table + (long long)w.b * p.table_stride + pg);
-    if (id >= 0 && id < p.pages) plane = id * p.kv_heads + w.head;
-    row -= max(0, start + p.page_size - w.s.kv);
+// A warp's window of a sequence's page table: 32 entries in the lanes, the 32
+// behind them on their way.  A look-up of each tile's pages would cost the
+// loading warp an L2 round trip a tile, about as long as the tile's MMAs.
+struct PageWindow {
+  int b, base, now, then;
+  __device__ __forceinline__ PageWindow() : b(-1), base(0), now(0), then(0) {}
+  __device__ __forceinline__ int fetch(const AttnParams& p, int pg) const {
+    return pg < p.table_pages ? __ldcg(p.table + (long long)b * p.table_stride + pg) : -1;
   }
-}
+  // all lanes: makes the pages of the key block that begins at page pg of
+  // sequence nb available.  Blocks come in order, but for V of the block
+  // before the last K: a slide keeps that one.
+  __device__ __forceinline__ void reach(const AttnParams& p, int nb, int pg) {
+    const int lane = threadIdx.x & 31, need = kBlockKeys >> p.page_shift;
+    if (nb == b && pg >= base && pg + need <= base + 32) return;
+    if (nb == b && pg == base + 32) {
+      const int lo = __shfl_sync(0xffffffffu, now, (lane + 32 - need) & 31);
+      const int hi = __shfl_sync(0xffffffffu, then, (lane - need) & 31);
+      now = lane < need ? lo : hi;
+      base = pg - need;
+    } else {
+      b = nb;
+      base = pg;
+      now = fetch(p, pg + lane);
+    }
+    then = fetch(p, base + 32 + lane);
+  }
+  // all lanes: where row `key` of the sequence lies: its page, as a plane of
+  // the tensor map (-1: none), and the row inside it.  The sequence's last
+  // page is read late by what it lacks, so that its valid rows come last.
+  __device__ __forceinline__ void row(const AttnParams& p, const ChunkPiece& w, int key, int& plane, int& row) const {
+    const int pg = key >> p.page_shift, start = pg << p.page_shift;
+    const int id = __shfl_sync(0xffffffffu, now, (pg - base) & 31);
+    plane = start < w.s.kv && id >= 0 && id < p.pages ? id * p.kv_heads + w.head : -1;
+    row = key - start - max(0, start + p.page_size - w.s.kv);
+  }
+};
 
 // ---------------------------------------------------------------- PTX
 
@@ -522,6 +546,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(ChunkCfg<T, D, E4>::
     constexpr int N = E4 ? C::RAWS : C::SLOTS;
     uint64_t* bars_full = E4 ? raw_full : full;
     uint64_t* bars_empty = E4 ? raw_empty : empty;
+    PageWindow pages;
     while (tl.next(p, per)) {
       const ChunkPiece& x = tl.w;
       if (tl.step == 0) {
@@ -536,6 +561,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(ChunkCfg<T, D, E4>::
         }
         __syncwarp();
       }
+      // boxes of one column; columns of 64 dims, or the whole row of codes
+      const bool v = tl.is_v;
+      const int rows = v ? kBlockKeys : 64, box = min(ps, rows), n = rows / box;
+      const int cols = E4 ? 1 : v ? D / 128 : D / 64;
+      pages.reach(p, x.b, (tl.j * kBlockKeys) >> p.page_shift);
+      const int bx = lane % n, col = lane / n;
+      int plane, row;
+      pages.row(p, x, tl.j * kBlockKeys + (v ? 0 : 64 * (int)rank) + bx * box, plane, row);
       if (!wait_warp(bars_empty + slot, phase ^ 1, kAttnErrChunkLoad)) break;
       if (E4) {
         if (lane == 0) mbar_arrive_expect_tx(bars_full + slot, C::RAW);
@@ -543,15 +576,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(ChunkCfg<T, D, E4>::
         mbar_arrive_expect_tx(bars_full + slot, 2 * C::SLOT);
       }
       __syncwarp();
-      // boxes of one column; columns of 64 dims, or the whole row of codes
-      const bool v = tl.is_v;
-      const int rows = v ? kBlockKeys : 64, box = min(ps, rows), n = rows / box;
-      const int cols = E4 ? 1 : v ? D / 128 : D / 64;
       const uint32_t bar = mapa(smem_u32(bars_full + slot), 0);
       if (lane < n * cols) {
-        const int bx = lane % n, col = lane / n;
-        int plane, row;
-        page_row(p, x, tl.j * kBlockKeys + (v ? 0 : 64 * (int)rank) + bx * box, plane, row);
         const int x0 = (v ? (int)rank * (D / 2) : 0) + col * 64;
         if (E4)
           tma_load_3d(smem_u32(s_codes) + slot * C::RAW + bx * box * (v ? D / 2 : D), v ? &tm_v : &tm_k,
@@ -681,12 +707,15 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(ChunkCfg<T, D, E4>::
             t0 = (valid - 1) / ps * ps;
             shift = t0 + ps - valid;
           }
+          // bits of this half's visible columns
+          auto below = [&](int n) {
+            n -= 64 * h;
+            return n <= 0 ? 0ull : n >= 64 ? ~0ull : (1ull << n) - 1;
+          };
+          const unsigned long long see = below(min(t0, lim + 1)) | (below(lim + shift + 1) & ~below(t0 + shift));
+          const uint32_t see2[2] = {(uint32_t)see, (uint32_t)(see >> 32)};
 #pragma unroll
-          for (int i = 0; i < 64; ++i) {
-            const int col = 64 * h + i;
-            const int key = col < t0 ? col : (col < t0 + shift ? kBlockKeys : col - shift);
-            if (key > lim) s[i] = -INFINITY;
-          }
+          for (int i = 0; i < 64; ++i) s[i] = see2[i >> 5] & (1u << (i & 31)) ? s[i] : -INFINITY;
         }
         float m4[4] = {s[0], s[1], s[2], s[3]};
 #pragma unroll
@@ -766,32 +795,59 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(ChunkCfg<T, D, E4>::
         }
       }
       const float inv = l > 0.f ? 1.f / l : 0.f;
-      T* dst = static_cast<T*>(p.out) + (long long)(w.s.q0 + tok) * p.out_token +
-               (long long)(w.head * p.group + hd) * p.out_head + h * (D / 2);
-      float* wo = ws.o + ((size_t)place * 256 + row) * D + h * (D / 2);
-#pragma unroll 1
-      for (int i = 0; i < D / 64; ++i) {
-        float o[32];
-        tmem_ld32(mine_o + 32 * i, o);
-        tmem_ld_wait();
-        if (whole && row_ok) {
+      if (whole) {
+        // four lanes swap 16-byte pieces of their four rows, so that a store
+        // writes 64 neighbouring bytes of eight rows, not 16 bytes of 32
+        const long long mine = (long long)(w.s.q0 + tok) * p.out_token + (long long)(w.head * p.group + hd) * p.out_head;
+        T* dst[4];
 #pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            uint4 u;
-            u.x = Elem<T>::from_f2(o[8 * q] * inv, o[8 * q + 1] * inv);
-            u.y = Elem<T>::from_f2(o[8 * q + 2] * inv, o[8 * q + 3] * inv);
-            u.z = Elem<T>::from_f2(o[8 * q + 4] * inv, o[8 * q + 5] * inv);
-            u.w = Elem<T>::from_f2(o[8 * q + 6] * inv, o[8 * q + 7] * inv);
-            if (l <= 0.f) u = make_uint4(0, 0, 0, 0);
-            *reinterpret_cast<uint4*>(dst + 32 * i + 8 * q) = u;
-          }
-        } else if (row_ok) {
-#pragma unroll
-          for (int q = 0; q < 8; ++q)
-            *reinterpret_cast<float4*>(wo + 32 * i + 4 * q) =
-                make_float4(o[4 * q], o[4 * q + 1], o[4 * q + 2], o[4 * q + 3]);
+        for (int k = 0; k < 4; ++k) {
+          const long long o = __shfl_sync(0xffffffffu, row_ok ? mine : -1, (lane & ~3) + k);
+          dst[k] = o < 0 ? nullptr : static_cast<T*>(p.out) + o + h * (D / 2) + (lane & 3) * 8;
         }
-        __syncwarp();
+#pragma unroll 1
+        for (int i = 0; i < D / 64; ++i) {
+          float o[32];
+          tmem_ld32(mine_o + 32 * i, o);
+          tmem_ld_wait();
+          uint32_t u[4][4];                    // [piece][word]
+#pragma unroll
+          for (int q = 0; q < 16; ++q)
+            u[q >> 2][q & 3] = l > 0.f ? Elem<T>::from_f2(o[2 * q] * inv, o[2 * q + 1] * inv) : 0u;
+#pragma unroll
+          for (int x = 1; x <= 2; x <<= 1) {
+            const bool up = lane & x;
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+              if (!(q & x)) {
+#pragma unroll
+                for (int y = 0; y < 4; ++y) {
+                  const uint32_t got = __shfl_xor_sync(0xffffffffu, up ? u[q][y] : u[q | x][y], x);
+                  if (up) u[q][y] = got;
+                  else u[q | x][y] = got;
+                }
+              }
+          }
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            if (dst[k]) *reinterpret_cast<uint4*>(dst[k] + 32 * i) = make_uint4(u[k][0], u[k][1], u[k][2], u[k][3]);
+          __syncwarp();
+        }
+      } else {
+        // [D / 4][256 rows][4]: a store of 32 rows is 512 neighbouring bytes
+        float4* wo = reinterpret_cast<float4*>(ws.o) + ((size_t)place * (D / 4) + h * (D / 8)) * 256 + row;
+#pragma unroll 1
+        for (int i = 0; i < D / 64; ++i) {
+          float o[32];
+          tmem_ld32(mine_o + 32 * i, o);
+          tmem_ld_wait();
+          if (row_ok) {
+#pragma unroll
+            for (int q = 0; q < 8; ++q)
+              wo[(8 * i + q) * 256] = make_float4(o[4 * q], o[4 * q + 1], o[4 * q + 2], o[4 * q + 3]);
+          }
+          __syncwarp();
+        }
       }
       tc_fence_before();
       __syncwarp();
@@ -808,11 +864,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(ChunkCfg<T, D, E4>::
     bool more = walk.next(p, per, w);
     j = more ? w.j0 : 0;
     float k[4], v[4];
+    PageWindow pages;
     auto load = [&]() {
+      pages.reach(p, w.b, (j * kBlockKeys) >> p.page_shift);
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         int plane, row;
-        page_row(p, w, j * kBlockKeys + lane + 32 * i, plane, row);
+        pages.row(p, w, j * kBlockKeys + lane + 32 * i, plane, row);
         const bool have = plane >= 0 && row >= 0;
         const long long at_row = ((long long)plane << p.page_shift) + row;
         k[i] = have ? __ldcg(p.k_scale + at_row) : 0.f;
@@ -854,34 +912,31 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(ChunkCfg<T, D, E4>::
     ChunkTiles tl(part);
     int slot = 0, raw = 0;
     uint32_t phase = 0, raw_phase = 0, vn = 0;
-    while (tl.next(p, per)) {
-      const bool v = tl.is_v;
+    auto widen = [&](auto is_v) {
+      constexpr bool v = decltype(is_v)::value;
+      // a row is D/16 pieces of K, D/32 of V
+      constexpr int per_row = v ? D / 32 : D / 16, rows = v ? kBlockKeys : 64;
       const float* e2 = s_sc + ((vn % C::SC_RING) * 3 + 2) * kBlockKeys;
-      if (!wait_warp(raw_full + raw, raw_phase, kAttnErrChunkWiden)) break;
-      if (v && !wait_warp(sc_full + vn % C::SC_RING, (vn / C::SC_RING) & 1, kAttnErrChunkWiden)) break;
-      if (!wait_warp(empty + slot, phase ^ 1, kAttnErrChunkWiden)) break;
+      if (!wait_warp(raw_full + raw, raw_phase, kAttnErrChunkWiden)) return;
+      if (v && !wait_warp(sc_full + vn % C::SC_RING, (vn / C::SC_RING) & 1, kAttnErrChunkWiden)) return;
+      if (!wait_warp(empty + slot, phase ^ 1, kAttnErrChunkWiden)) return;
       const uint4* src = reinterpret_cast<const uint4*>(s_codes + (size_t)raw * C::RAW);
       uint8_t* dst = s_ring + (size_t)slot * C::SLOT;
-      // a row is D/16 pieces of K, D/32 of V
-      const int per_row = v ? D / 32 : D / 16, rows = v ? kBlockKeys : 64;
+      uint4 u[PIECES];
+#pragma unroll
+      for (int i = 0; i < PIECES; ++i) u[i] = src[i * 128 + t];
 #pragma unroll
       for (int i = 0; i < PIECES; ++i) {
-        const int n = i * 128 + t, r = n / per_row, cpos = n - r * per_row;
-        const uint4 u = src[n];
-        const uint32_t w4[4] = {u.x, u.y, u.z, u.w};
+        const int n = i * 128 + t, r = n / per_row, cpos = n % per_row;
+        const uint32_t w4[4] = {u[i].x, u[i].y, u[i].z, u[i].w};
         uint32_t o[8];
         const float e = v ? e2[r] : 1.f;
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
-          if (v) {
-            o[2 * q] = widen2<T>((uint16_t)w4[q], e);
-            o[2 * q + 1] = widen2<T>((uint16_t)(w4[q] >> 16), e);
-          } else {
-            o[2 * q] = widen2<T>((uint16_t)w4[q]);
-            o[2 * q + 1] = widen2<T>((uint16_t)(w4[q] >> 16));
-          }
+          o[2 * q] = v ? widen2<T>((uint16_t)w4[q], e) : widen2<T>((uint16_t)w4[q]);
+          o[2 * q + 1] = v ? widen2<T>((uint16_t)(w4[q] >> 16), e) : widen2<T>((uint16_t)(w4[q] >> 16));
         }
-        // 16 values: two 16-byte pieces of a 64-dim column.  Threads of the
+        // 16 values: two 16-byte pieces of a 64-dim column.  Threads of every
         // second column store theirs the other way round, so that eight
         // threads hit eight different pieces.
         uint8_t* col = dst + (cpos >> 2) * (rows * 128) + r * 128;
@@ -900,6 +955,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(ChunkCfg<T, D, E4>::
       if (v) ++vn;
       if (++slot == C::SLOTS) { slot = 0; phase ^= 1; }
       if (++raw == C::RAWS) { raw = 0; raw_phase ^= 1; }
+    };
+    while (ok && tl.next(p, per)) {
+      if (tl.is_v) widen(std::true_type{});
+      else widen(std::false_type{});
     }
   }
   __syncwarp();
@@ -915,8 +974,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(ChunkCfg<T, D, E4>::
 }
 
 // Tiles that the parts' cuts go through: the sum of their parts, in order.
-// blockIdx.x is the part in which the tile begins, blockIdx.y a group of rows.
-constexpr int kJoinRows = 4;
+// blockIdx.x is the part in which the tile begins; a block takes 32 rows and 32
+// dims, eight threads a row.
 template <typename T, int D>
 __global__ void __launch_bounds__(256) attn_chunk_join_kernel(const __grid_constant__ AttnParams p, const ChunkWs ws) {
   pdl_trigger();
@@ -927,32 +986,33 @@ __global__ void __launch_bounds__(256) attn_chunk_join_kernel(const __grid_const
   const int b = de.x, head = de.y, tile = de.z, c1 = de.w;
   const AttnSeq s = attn_seq(p, b);
   const int tpc = 128 / p.group;
-  for (int i = threadIdx.x; i < kJoinRows * (D / 4); i += 256) {
-    const int row = blockIdx.y * kJoinRows + i / (D / 4), d = (i % (D / 4)) * 4;
-    const int rr = row & 127, ti = rr / p.group, tok = tile * 2 * tpc + (row >> 7) * tpc + ti;
-    if (ti >= tpc || tok >= s.n) continue;
-    float m = -INFINITY;
-    for (int c = c0; c <= c1; ++c) m = fmaxf(m, __ldcg(ws.ml + (((size_t)c * 2 + (c == c0)) * 256 + row) * 2));
-    float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
-    float l = 0.f;
-    for (int c = c0; c <= c1; ++c) {
-      const size_t at = ((size_t)c * 2 + (c == c0)) * 256 + row;
-      const float mc = __ldcg(ws.ml + at * 2);
-      if (mc == -INFINITY) continue;
-      const float f = ex2(mc - m);
-      const float4 v = __ldcg(reinterpret_cast<const float4*>(ws.o + at * D + d));
-      l = fmaf(__ldcg(ws.ml + at * 2 + 1), f, l);
+  const int row = (blockIdx.y & 7) * 32 + (threadIdx.x >> 3), d4 = (blockIdx.y >> 3) * 8 + (threadIdx.x & 7);
+  const int rr = row & 127, ti = rr / p.group, tok = tile * 2 * tpc + (row >> 7) * tpc + ti;
+  if (ti >= tpc || tok >= s.n) return;
+  float m = -INFINITY;
+  for (int c = c0; c <= c1; ++c) m = fmaxf(m, __ldcg(ws.ml + (((size_t)c * 2 + (c == c0)) * 256 + row) * 2));
+  const float base = m == -INFINITY ? 0.f : m;
+  float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+  float l = 0.f;
+#pragma unroll 4
+  for (int c = c0; c <= c1; ++c) {
+    const size_t place = (size_t)c * 2 + (c == c0);
+    const float2 ml = __ldcg(reinterpret_cast<const float2*>(ws.ml) + place * 256 + row);
+    const float4 v = __ldcg(reinterpret_cast<const float4*>(ws.o) + (place * (D / 4) + d4) * 256 + row);
+    const float f = ex2(ml.x - base);
+    if (f != 0.f) {
+      l = fmaf(ml.y, f, l);
       a.x = fmaf(v.x, f, a.x);
       a.y = fmaf(v.y, f, a.y);
       a.z = fmaf(v.z, f, a.z);
       a.w = fmaf(v.w, f, a.w);
     }
-    const float inv = l > 0.f ? 1.f / l : 0.f;
-    T* dst = static_cast<T*>(p.out) + (long long)(s.q0 + tok) * p.out_token +
-             (long long)(head * p.group + rr - ti * p.group) * p.out_head + d;
-    *reinterpret_cast<uint2*>(dst) =
-        make_uint2(Elem<T>::from_f2(a.x * inv, a.y * inv), Elem<T>::from_f2(a.z * inv, a.w * inv));
   }
+  const float inv = l > 0.f ? 1.f / l : 0.f;
+  T* dst = static_cast<T*>(p.out) + (long long)(s.q0 + tok) * p.out_token +
+           (long long)(head * p.group + rr - ti * p.group) * p.out_head + d4 * 4;
+  *reinterpret_cast<uint2*>(dst) =
+      make_uint2(Elem<T>::from_f2(a.x * inv, a.y * inv), Elem<T>::from_f2(a.z * inv, a.w * inv));
 }
 
 }  // namespace d3
