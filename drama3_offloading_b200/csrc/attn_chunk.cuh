@@ -297,27 +297,11 @@ __device__ __forceinline__ uint32_t mapa(uint32_t addr, uint32_t rank) {
   asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
   return r;
 }
-__device__ __forceinline__ void mbar_arrive_cluster(uint32_t addr) {
-  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(addr) : "memory");
-}
-__device__ __forceinline__ bool mbar_try_wait_cluster(uint64_t* bar, uint32_t parity) {
-  uint32_t ok;
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2, %3;\n\t"
-      "selp.u32 %0, 1, 0, p;\n\t}"
-      : "=r"(ok)
-      : "r"(smem_u32(bar)), "r"(parity), "r"(20000u)
-      : "memory");
-  return ok != 0;
-}
-__device__ __forceinline__ bool mbar_wait_cluster(uint64_t* bar, uint32_t parity) {
-  if (mbar_try_wait_cluster(bar, parity)) return true;
-  const uint64_t t0 = globaltimer_ns();
-  while (true) {
-    if (mbar_try_wait_cluster(bar, parity)) return true;
-    if (globaltimer_ns() - t0 > kAttnWaitBudgetNs) return false;
-  }
+// an arrival at a barrier of either CTA.  What it publishes is in shared memory
+// or TMEM of this CTA; a release of cluster scope would also wait for the
+// thread's global stores, which cost 1300 cycles a block.
+__device__ __forceinline__ void mbar_arrive_remote(uint32_t addr) {
+  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(addr) : "memory");
 }
 // loads of a pair's CTA that complete on a barrier of either CTA; no multicast
 __device__ __forceinline__ void tma_pair_3d(uint32_t dst, const void* map, uint32_t bar, int x, int y, int z) {
@@ -529,7 +513,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(ChunkCfg<T, D, E4>::
   bool ok = true;
   // every lane of a warp: false once a wait has run out, here or in another role
   auto wait_warp = [&](uint64_t* bar, uint32_t par, int code) {
-    if (ok && !mbar_wait_cluster(bar, par)) {
+    if (ok && !mbar_wait(bar, par, kAttnWaitBudgetNs)) {
       attn_error(p.err, code);
       s_abort = 1;
       ok = false;
@@ -601,7 +585,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(ChunkCfg<T, D, E4>::
       int slot = 0;
       uint32_t phase = 0, it = 0, pieces = 0;
       auto wait = [&](uint64_t* bar, uint32_t par) {
-        if (ok && !mbar_wait_cluster(bar, par)) {
+        if (ok && !mbar_wait(bar, par, kAttnWaitBudgetNs)) {
           attn_error(p.err, kAttnErrChunkMma);
           s_abort = 1;
           ok = false;
@@ -657,34 +641,41 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(ChunkCfg<T, D, E4>::
     const uint32_t lanes = tmem + ((uint32_t)(quarter * 32) << 16);
     const uint32_t mine_o = lanes + C::COL_O + h * (D / 2);
     const int ti = rr / p.group, hd = rr - ti * p.group;
-    // the value that the row's other thread gives; bounded, unlike a barrier
-    // among some of the warps.  Two buffers: a thread is one exchange ahead at
-    // most.
+    // the value that the row's other thread gives.  Two buffers: a thread is
+    // one exchange ahead at most.  The barrier among the row's two warps is
+    // safe because both always come: after a wait has run out the loops go on
+    // to their end without waiting.
     uint32_t xn = 0;
     auto exchange = [&](float v) {
-      float* buf = s_mx + (xn & 1) * 256 + rr;
+      float* buf = s_mx + (xn++ & 1) * 256 + rr;
       buf[h * 128] = v;
-      __syncwarp();
-      if (lane == 0) mbar_arrive(x_bar + quarter);
-      wait_warp(x_bar + quarter, xn & 1, kAttnErrChunkSoftmax);
-      ++xn;
+      asm volatile("bar.sync %0, 64;" ::"r"(1 + quarter) : "memory");
       return buf[(h ^ 1) * 128];
     };
+    auto wait = [&](uint64_t* bar, uint32_t par) { wait_warp(bar, par, kAttnErrChunkSoftmax); };
     ChunkWalk walk(part);
     ChunkPiece w;
     uint32_t it = 0, pieces = 0;
     int4 desc = make_int4(0, 0, 0, -1);
     const float c = p.scale_log2;
-    while (ok && walk.next(p, per, w)) {
+    while (walk.next(p, per, w)) {
       const int tok = w.tile * per + (int)rank * tpc + ti;       // of the sequence's new ones
       const bool row_ok = ti < tpc && tok < w.s.n;
-      const int last = row_ok ? w.s.kv - w.s.n + tok : -1;
+      const int last = row_ok ? w.s.kv - w.s.n + tok : 1 << 30;
+      const bool idle = !__any_sync(0xffffffffu, row_ok);        // nothing of this warp is written
       float m = -INFINITY, l = 0.f;
       for (int j = w.j0; j < w.j1; ++j, ++it) {
         const uint32_t sb = lanes + C::COL_S + (it & 1) * kBlockKeys;
         const float* sc = s_sc + (it % C::SC_RING) * 3 * kBlockKeys + h * 64;
-        if (E4) wait_warp(sc_full + it % C::SC_RING, (it / C::SC_RING) & 1, kAttnErrChunkSoftmax);
-        if (!wait_warp(s_full + (it & 1), (it >> 1) & 1, kAttnErrChunkSoftmax)) break;
+        if (E4) wait(sc_full + it % C::SC_RING, (it / C::SC_RING) & 1);
+        wait(s_full + (it & 1), (it >> 1) & 1);
+        if (idle) {
+          if (lane == 0) {
+            mbar_arrive_remote(mapa(smem_u32(p_ready + (it & 1)), 0));
+            if (E4) mbar_arrive(sc_empty + it % C::SC_RING);
+          }
+          continue;
+        }
         tc_fence_after();
         float s[64];
         tmem_ld32(sb + 64 * h, s);
@@ -725,7 +716,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(ChunkCfg<T, D, E4>::
         // exchange also says that both halves of S are in registers: P of half
         // 1 goes over S of half 0.)
         mx = fmaxf(mx, exchange(mx));
-        if (!ok) break;
         const bool grow = mx > m + kRescaleLog2 || (m == -INFINITY && mx > m);
         if (__any_sync(0xffffffffu, grow)) {
           const float f = !grow ? 1.f : m == -INFINITY ? 0.f : ex2(m - mx);
@@ -734,7 +724,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(ChunkCfg<T, D, E4>::
           if (j > w.j0) {
             // one phase to wait for: P V of the block before came before this
             // S, and this block's waits for this warp
-            if (!wait_warp(o_done, (it - 1) & 1, kAttnErrChunkSoftmax)) break;
+            wait(o_done, (it - 1) & 1);
             tc_fence_after();
             // a row that starts here holds zeros, or what its factor 0 must
             // not turn into NaN
@@ -773,14 +763,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(ChunkCfg<T, D, E4>::
         tc_fence_before();
         __syncwarp();
         if (lane == 0) {
-          mbar_arrive_cluster(mapa(smem_u32(p_ready + (it & 1)), 0));
+          mbar_arrive_remote(mapa(smem_u32(p_ready + (it & 1)), 0));
           if (E4) mbar_arrive(sc_empty + it % C::SC_RING);
         }
       }
-      if (!ok) break;
-      l += exchange(l);
+      if (!idle) l += exchange(l);
       // a barrier of its own: o_done may be two phases behind here
-      if (!wait_warp(o_last, pieces & 1, kAttnErrChunkSoftmax)) break;
+      wait(o_last, pieces & 1);
       ++pieces;
       tc_fence_after();
       const bool whole = w.j0 == 0 && w.j1 == w.nb;
@@ -795,7 +784,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(ChunkCfg<T, D, E4>::
         }
       }
       const float inv = l > 0.f ? 1.f / l : 0.f;
-      if (whole) {
+      if (idle || !ok) {
+      } else if (whole) {
         // four lanes swap 16-byte pieces of their four rows, so that a store
         // writes 64 neighbouring bytes of eight rows, not 16 bytes of 32
         const long long mine = (long long)(w.s.q0 + tok) * p.out_token + (long long)(w.head * p.group + hd) * p.out_head;
@@ -851,7 +841,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(ChunkCfg<T, D, E4>::
       }
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive_cluster(mapa(smem_u32(o_free), 0));
+      if (lane == 0) mbar_arrive_remote(mapa(smem_u32(o_free), 0));
     }
     if (rank == 0 && tid == 0) ws.desc[pair] = desc;
   } else if (E4 && warp == 10) {
@@ -948,7 +938,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(ChunkCfg<T, D, E4>::
       fence_proxy_async_smem();
       __syncwarp();
       if (lane == 0) {
-        mbar_arrive_cluster(mapa(smem_u32(full + slot), 0));
+        mbar_arrive_remote(mapa(smem_u32(full + slot), 0));
         mbar_arrive(raw_empty + raw);
         if (v) mbar_arrive(sc_empty + vn % C::SC_RING);
       }
@@ -966,7 +956,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(ChunkCfg<T, D, E4>::
   __syncthreads();
   // every MMA of the pair, and every arrival that it makes here, has ended
   // before TMEM or shared memory goes
-  if (warp == 8 && !mbar_wait_cluster(all_done, 0) && lane == 0) attn_error(p.err, kAttnErrChunkMma);
+  if (warp == 8 && !mbar_wait(all_done, 0, kAttnWaitBudgetNs) && lane == 0) attn_error(p.err, kAttnErrChunkMma);
   __syncwarp();
   cluster_sync_all();      // no CTA leaves while its pair may still arrive at it
   tc_fence_after();
