@@ -10,8 +10,8 @@ static int make_map(CUtensorMap* m, const void* base, int dtype, int rank, const
                     const uint64_t* strides, const uint32_t* box, bool swizzle = true) {
   EncodeTiledFn fn = encode_fn();
   if (!fn) return fail(D3_ERR_CUDA, "cuTensorMapEncodeTiled unavailable from the driver");
-  cuuint64_t d[3], s[2];
-  cuuint32_t x[3], e[3] = {1, 1, 1};
+  cuuint64_t d[4], s[3];
+  cuuint32_t x[4], e[4] = {1, 1, 1, 1};
   for (int i = 0; i < rank; ++i) {
     d[i] = dims[i];
     x[i] = box[i];
@@ -35,16 +35,17 @@ static int make_rows_map(CUtensorMap* m, const void* base, const d3_kv_cache* c,
   const uint32_t box[2] = {(uint32_t)(128 / es), box_rows};
   return make_map(m, base, c->dtype, 2, dims, strides, box);
 }
-// A cache buffer as planes [pages * kv_heads][page_size][D]: rows before or
-// behind a page are outside the map.  16-bit rows in columns of 64 dims; codes
-// box_dims wide, unswizzled.
+// A cache buffer as planes [pages * kv_heads][page_size][D], the dims in
+// columns: 64 of 16 bits, swizzled, or one of all codes.  Rows before or
+// behind a page are outside the map.
 static int make_pages_map(CUtensorMap* m, const void* base, const d3_kv_cache* c, uint32_t box_dims,
-                          uint32_t box_rows) {
-  const uint64_t es = c->dtype == D3_E4M3 ? 1 : 2;
-  const uint64_t dims[3] = {(uint64_t)c->head_dim, (uint64_t)c->page_size, (uint64_t)c->pages * c->kv_heads};
-  const uint64_t strides[2] = {c->head_dim * es, c->page_size * c->head_dim * es};
-  const uint32_t box[3] = {box_dims, box_rows, 1};
-  return make_map(m, base, c->dtype, 3, dims, strides, box, es == 2);
+                          uint32_t box_rows, uint32_t box_cols) {
+  const bool e4 = c->dtype == D3_E4M3;
+  const uint64_t D = c->head_dim, es = e4 ? 1 : 2, col = e4 ? D : 64;
+  const uint64_t dims[4] = {col, (uint64_t)c->page_size, D / col, (uint64_t)c->pages * c->kv_heads};
+  const uint64_t strides[3] = {D * es, col * es, c->page_size * D * es};
+  const uint32_t box[4] = {box_dims, box_rows, box_cols, 1};
+  return make_map(m, base, c->dtype, 4, dims, strides, box, !e4);
 }
 
 static int check_attention(const d3_attention* a, const d3_kv_cache* c) {
@@ -148,8 +149,8 @@ static int launch_chunk(const AttnParams& p, const d3_attention* a, const d3_kv_
   const uint32_t box[3] = {64, (uint32_t)p.group, (uint32_t)tpc};
   if ((rc = make_map(&tq, a->q, a->dtype, 3, dims, strides, box))) return rc;
   const uint32_t krows = c->page_size < 64 ? c->page_size : 64;
-  if ((rc = make_pages_map(&tk, c->k, c, E4 ? D : 64, krows))) return rc;
-  if ((rc = make_pages_map(&tv, c->v, c, E4 ? D / 2 : 64, c->page_size))) return rc;
+  if ((rc = make_pages_map(&tk, c->k, c, E4 ? D : 64, krows, !E4 && krows == 64 ? D / 64 : 1))) return rc;
+  if ((rc = make_pages_map(&tv, c->v, c, E4 ? D / 2 : 64, c->page_size, E4 ? 1 : D / 128))) return rc;
   // row tiles at most: every sequence may have one that is not full
   const long long tiles = a->tokens / (2 * tpc) + a->batch;
   const long long blocks = ((long long)a->max_kv + kBlockKeys - 1) / kBlockKeys;

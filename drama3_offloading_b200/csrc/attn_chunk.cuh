@@ -311,11 +311,18 @@ __device__ __forceinline__ void tma_pair_3d(uint32_t dst, const void* map, uint3
       "r"(y), "r"(z)
       : "memory");
 }
-__device__ __forceinline__ void tma_load_3d(uint32_t dst, const void* map, uint64_t* bar, int x, int y, int z) {
+__device__ __forceinline__ void tma_pair_4d(uint32_t dst, const void* map, uint32_t bar, int x, int y, int z, int u) {
   asm volatile(
-      "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes"
-      " [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)),
-      "r"(x), "r"(y), "r"(z)
+      "cp.async.bulk.tensor.4d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(x),
+      "r"(y), "r"(z), "r"(u)
+      : "memory");
+}
+__device__ __forceinline__ void tma_load_4d(uint32_t dst, const void* map, uint32_t bar, int x, int y, int z, int u) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(x),
+      "r"(y), "r"(z), "r"(u)
       : "memory");
 }
 __device__ __forceinline__ void mma_pair_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
@@ -545,30 +552,38 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(ChunkCfg<T, D, E4>::
         }
         __syncwarp();
       }
-      // boxes of one column; columns of 64 dims, or the whole row of codes
+      // One box a page with all of its columns of 64 dims, but for 16-bit K of
+      // small pages, whose rows of one column have to lie together.  A TMA
+      // instruction costs the warp some 100 cycles, with operands that differ
+      // between lanes 300: one lane issues them, few and large.
       const bool v = tl.is_v;
       const int rows = v ? kBlockKeys : 64, box = min(ps, rows), n = rows / box;
-      const int cols = E4 ? 1 : v ? D / 128 : D / 64;
       pages.reach(p, x.b, (tl.j * kBlockKeys) >> p.page_shift);
-      const int bx = lane % n, col = lane / n;
       int plane, row;
-      pages.row(p, x, tl.j * kBlockKeys + (v ? 0 : 64 * (int)rank) + bx * box, plane, row);
+      pages.row(p, x, tl.j * kBlockKeys + (v ? 0 : 64 * (int)rank) + (lane & (n - 1)) * box, plane, row);
       if (!wait_warp(bars_empty + slot, phase ^ 1, kAttnErrChunkLoad)) break;
-      if (E4) {
-        if (lane == 0) mbar_arrive_expect_tx(bars_full + slot, C::RAW);
-      } else if (rank == 0 && lane == 0) {
-        mbar_arrive_expect_tx(bars_full + slot, 2 * C::SLOT);
+      if (lane == 0) {
+        if (E4) mbar_arrive_expect_tx(bars_full + slot, C::RAW);
+        else if (rank == 0) mbar_arrive_expect_tx(bars_full + slot, 2 * C::SLOT);
       }
-      __syncwarp();
-      const uint32_t bar = mapa(smem_u32(bars_full + slot), 0);
-      if (lane < n * cols) {
-        const int x0 = (v ? (int)rank * (D / 2) : 0) + col * 64;
-        if (E4)
-          tma_load_3d(smem_u32(s_codes) + slot * C::RAW + bx * box * (v ? D / 2 : D), v ? &tm_v : &tm_k,
-                      bars_full + slot, x0, row, plane);
-        else
-          tma_pair_3d(ss + slot * C::SLOT + col * (rows * 128) + bx * (box * 128), v ? &tm_v : &tm_k, bar, x0, row,
-                      plane);
+      const uint32_t bar = E4 ? smem_u32(bars_full + slot) : mapa(smem_u32(bars_full + slot), 0);
+      const uint32_t dst = E4 ? smem_u32(s_codes) + slot * C::RAW : ss + slot * C::SLOT;
+      for (int i = 0; i < n; ++i) {
+        const int y = __shfl_sync(0xffffffffu, row, i), u = __shfl_sync(0xffffffffu, plane, i);
+        if (lane == 0) {
+          if (E4) {
+            if (v) tma_load_4d(dst + i * box * (D / 2), &tm_v, bar, (int)rank * (D / 2), y, 0, u);
+            else tma_load_4d(dst + i * box * D, &tm_k, bar, 0, y, 0, u);
+          } else if (v) {
+            tma_pair_4d(dst + i * box * D, &tm_v, bar, 0, y, (int)rank * (D / 128), u);
+          } else if (n == 1) {
+            tma_pair_4d(dst, &tm_k, bar, 0, y, 0, u);
+          } else {
+#pragma unroll
+            for (int c = 0; c < D / 64; ++c)
+              tma_pair_4d(dst + c * (64 * 128) + i * (box * 128), &tm_k, bar, 0, y, c, u);
+          }
+        }
       }
       __syncwarp();
       if (++slot == N) { slot = 0; phase ^= 1; }
@@ -584,6 +599,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(ChunkCfg<T, D, E4>::
       ChunkPiece w;
       int slot = 0;
       uint32_t phase = 0, it = 0, pieces = 0;
+      // V: pages of `vrows` keys, each [D / 128 columns][vrows][128 bytes]; 16 keys a k-step
+      const int vrows = E4 ? kBlockKeys : ps;
       auto wait = [&](uint64_t* bar, uint32_t par) {
         if (ok && !mbar_wait(bar, par, kAttnWaitBudgetNs)) {
           attn_error(p.err, kAttnErrChunkMma);
@@ -616,7 +633,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(ChunkCfg<T, D, E4>::
         const uint32_t vb = ss + slot * C::SLOT, a = tmem + C::COL_S + (x & 1) * kBlockKeys;
 #pragma unroll
         for (int k = 0; k < kBlockKeys / 16; ++k)
-          mma_pair_ts(tmem + C::COL_O, a + k * 8, smem_desc_n128(vb + k * (16 * 128), kBlockKeys * 128), id_o,
+          mma_pair_ts(tmem + C::COL_O, a + k * 8,
+                      smem_desc_n128(vb + (k * 16 & -vrows) * D + (k * 16 & (vrows - 1)) * 128, vrows * 128), id_o,
                       !first || k > 0);
         commit_pair(o_done);
         advance();
