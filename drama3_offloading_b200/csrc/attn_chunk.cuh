@@ -25,8 +25,9 @@
 //
 // Roles (per CTA): warps 0-7 softmax and output (a row is shared by two
 // threads, 64 keys of a block and half of O each), warp 8 issues the MMAs (in
-// the pair's first CTA), warp 9 the TMA loads; for codes warp 10 brings the
-// scales and warps 12-15 widen the tiles.
+// the pair's first CTA), one thread each of warps 9 and 10 the TMA loads of Q
+// and K and of V; for codes warp 11 brings the scales and warps 12-15 widen
+// the tiles.
 //
 // A block's last page, when the sequence ends in it, is loaded shifted: rows
 // before the page's first come from outside the tensor map and are zeros, the
@@ -55,7 +56,7 @@ constexpr float kRescaleLog2 = 8.f;
 
 template <typename T, int D, bool E4>
 struct ChunkCfg {
-  static constexpr int THREADS = E4 ? 512 : 320;
+  static constexpr int THREADS = E4 ? 512 : 352;
   static constexpr int Q_BYTES = 128 * D * 2;
   static constexpr int SLOT = 64 * D * 2;                 // half a block of K or of V
   static constexpr int SLOTS = E4 ? (D == 256 ? 3 : 6) : (D == 256 ? 5 : 10);
@@ -278,6 +279,63 @@ struct PageWindow {
     const int id = __shfl_sync(0xffffffffu, now, (pg - base) & 31);
     plane = start < w.s.kv && id >= 0 && id < p.pages ? id * p.kv_heads + w.head : -1;
     row = key - start - max(0, start + p.page_size - w.s.kv);
+  }
+};
+
+// One thread's walk of a part block by block, a block ahead of what it loads:
+// the page ids of the next block are on their way while this one's TMA
+// instructions go out.  (An L2 round trip, or the shuffles and votes of a
+// whole warp, for every tile cost as much as the tile's MMAs.)
+struct ChunkBlocks {
+  ChunkWalk walk;
+  ChunkPiece w;
+  int j;
+  bool more;
+  int ids[8];
+  __device__ __forceinline__ explicit ChunkBlocks(const ChunkPart& c) : walk(c), j(0), more(false) {}
+  __device__ __forceinline__ void fetch(const AttnParams& p, int key0, int box, int n) {
+    const int* row = p.table + (long long)w.b * p.table_stride;
+    const int key = j * kBlockKeys + key0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (i < n) {
+        const int pg = (key + i * box) >> p.page_shift;
+        ids[i] = (pg << p.page_shift) < w.s.kv ? __ldcg(row + pg) : -1;
+      }
+  }
+  __device__ __forceinline__ void first(const AttnParams& p, int per, int key0, int box, int n) {
+    more = walk.next(p, per, w);
+    if (!more) return;
+    j = w.j0;
+    fetch(p, key0, box, n);
+  }
+  __device__ __forceinline__ void step(const AttnParams& p, int per, int key0, int box, int n) {
+    if (++j >= w.j1) {
+      more = walk.next(p, per, w);
+      if (!more) return;
+      j = w.j0;
+    }
+    fetch(p, key0, box, n);
+  }
+};
+// Where `key` of a sequence with page id `id` lies: plane of the tensor map
+// (-1: none) and row of the page.  The sequence's last page is read late by
+// what it lacks, so that its valid rows come last.
+__device__ __forceinline__ void page_place(const AttnParams& p, int id, int head, int kv, int key, int& plane, int& row) {
+  const int start = key & -p.page_size;
+  plane = id >= 0 && id < p.pages ? id * p.kv_heads + head : -1;
+  row = key - start - max(0, start + p.page_size - kv);
+}
+// A place in a ring of n slots, moved on by up to n.
+struct RingPos {
+  int slot = 0;
+  uint32_t phase = 0;
+  __device__ __forceinline__ void advance(int d, int n) {
+    slot += d;
+    if (slot >= n) {
+      slot -= n;
+      phase ^= 1;
+    }
   }
 };
 
@@ -520,77 +578,99 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(ChunkCfg<T, D, E4>::
   bool ok = true;
   // every lane of a warp: false once a wait has run out, here or in another role
   auto wait_warp = [&](uint64_t* bar, uint32_t par, int code) {
-    if (ok && !mbar_wait(bar, par, kAttnWaitBudgetNs)) {
-      attn_error(p.err, code);
-      s_abort = 1;
-      ok = false;
-    }
-    ok = __all_sync(0xffffffffu, ok && !s_abort);
-    return ok;
+    if (!ok) return false;
+    if (__all_sync(0xffffffffu, mbar_try_wait(bar, par))) return true;
+    const uint64_t t0 = globaltimer_ns();
+    while (!__all_sync(0xffffffffu, mbar_try_wait(bar, par)))
+      if (__any_sync(0xffffffffu, s_abort || globaltimer_ns() - t0 > kAttnWaitBudgetNs)) {
+        if (!s_abort) attn_error(p.err, code);
+        s_abort = 1;
+        ok = false;
+        return false;
+      }
+    return true;
+  };
+  // one thread
+  auto wait_one = [&](uint64_t* bar, uint32_t par, int code) {
+    if (!ok) return false;
+    if (mbar_try_wait(bar, par)) return true;
+    const uint64_t t0 = globaltimer_ns();
+    while (!mbar_try_wait(bar, par))
+      if (s_abort || globaltimer_ns() - t0 > kAttnWaitBudgetNs) {
+        if (!s_abort) attn_error(p.err, code);
+        s_abort = 1;
+        ok = false;
+        return false;
+      }
+    return true;
   };
 
-  if (warp == 9) {
-    // ---- TMA: Q of a piece, then its tiles
-    ChunkTiles tl(part);
-    int slot = 0;
-    uint32_t phase = 0, qn = 0;
-    constexpr int N = E4 ? C::RAWS : C::SLOTS;
-    uint64_t* bars_full = E4 ? raw_full : full;
-    uint64_t* bars_empty = E4 ? raw_empty : empty;
-    PageWindow pages;
-    while (tl.next(p, per)) {
-      const ChunkPiece& x = tl.w;
-      if (tl.step == 0) {
-        if (!wait_warp(q_empty, (qn & 1) ^ 1, kAttnErrChunkLoad)) break;
-        ++qn;
-        if (lane == 0) {
+  if (warp == 9 || warp == 10) {
+    // ---- TMA: one thread brings Q of a piece and its K tiles, one its V
+    // tiles.  The tiles of a piece of m blocks stand in the ring as K 0, K 1,
+    // V 0, K 2, V 1, ..., K m - 1, V m - 2, V m - 1.
+    if (lane == 0) {
+      constexpr int N = E4 ? C::RAWS : C::SLOTS;
+      uint64_t* bars_full = E4 ? raw_full : full;
+      uint64_t* bars_empty = E4 ? raw_empty : empty;
+      RingPos pos;
+      const bool v = warp == 10;
+      // One box a page with all of its columns of 64 dims, but for 16-bit K of
+      // small pages, whose rows of one column have to lie together.
+      const int rows = v ? kBlockKeys : 64, box = min(ps, rows), n = rows / box;
+      const int key0 = v ? 0 : 64 * (int)rank;
+      ChunkBlocks bl(part);
+      bl.first(p, per, key0, box, n);
+      uint32_t qn = 0;
+      int at_pos = 0, base = 0;
+      while (bl.more) {
+        const ChunkPiece x = bl.w;
+        const int j = bl.j, m = x.j1 - x.j0, k = j - x.j0;
+        int ids[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) ids[i] = bl.ids[i];
+        bl.step(p, per, key0, box, n);
+        const int want = base + (v ? (k == m - 1 ? 2 * m - 1 : 2 * k + 2) : (k ? 2 * k - 1 : 0));
+        for (; at_pos < want; ++at_pos) pos.advance(1, N);
+        if (k == m - 1) base += 2 * m;
+        if (!v && k == 0) {
+          if (!wait_one(q_empty, (qn & 1) ^ 1, kAttnErrChunkLoad)) break;
+          ++qn;
           if (rank == 0) mbar_arrive_expect_tx(q_full, 2 * (D / 64) * tpc * p.group * 128);
           const uint32_t bar = mapa(smem_u32(q_full), 0);
           const int tok = x.s.q0 + x.tile * per + (int)rank * tpc;
           for (int c = 0; c < D / 64; ++c)
             tma_pair_3d(sq + c * (128 * 128), &tm_q, bar, c * 64, x.head * p.group, tok);
         }
-        __syncwarp();
-      }
-      // One box a page with all of its columns of 64 dims, but for 16-bit K of
-      // small pages, whose rows of one column have to lie together.  A TMA
-      // instruction costs the warp some 100 cycles, with operands that differ
-      // between lanes 300: one lane issues them, few and large.
-      const bool v = tl.is_v;
-      const int rows = v ? kBlockKeys : 64, box = min(ps, rows), n = rows / box;
-      pages.reach(p, x.b, (tl.j * kBlockKeys) >> p.page_shift);
-      int plane, row;
-      pages.row(p, x, tl.j * kBlockKeys + (v ? 0 : 64 * (int)rank) + (lane & (n - 1)) * box, plane, row);
-      if (!wait_warp(bars_empty + slot, phase ^ 1, kAttnErrChunkLoad)) break;
-      if (lane == 0) {
-        if (E4) mbar_arrive_expect_tx(bars_full + slot, C::RAW);
-        else if (rank == 0) mbar_arrive_expect_tx(bars_full + slot, 2 * C::SLOT);
-      }
-      const uint32_t bar = E4 ? smem_u32(bars_full + slot) : mapa(smem_u32(bars_full + slot), 0);
-      const uint32_t dst = E4 ? smem_u32(s_codes) + slot * C::RAW : ss + slot * C::SLOT;
-      for (int i = 0; i < n; ++i) {
-        const int y = __shfl_sync(0xffffffffu, row, i), u = __shfl_sync(0xffffffffu, plane, i);
-        if (lane == 0) {
-          if (E4) {
-            if (v) tma_load_4d(dst + i * box * (D / 2), &tm_v, bar, (int)rank * (D / 2), y, 0, u);
-            else tma_load_4d(dst + i * box * D, &tm_k, bar, 0, y, 0, u);
-          } else if (v) {
-            tma_pair_4d(dst + i * box * D, &tm_v, bar, 0, y, (int)rank * (D / 128), u);
-          } else if (n == 1) {
-            tma_pair_4d(dst, &tm_k, bar, 0, y, 0, u);
-          } else {
+        if (!wait_one(bars_empty + pos.slot, pos.phase ^ 1, kAttnErrChunkLoad)) break;
+        if (E4) mbar_arrive_expect_tx(bars_full + pos.slot, C::RAW);
+        else if (rank == 0) mbar_arrive_expect_tx(bars_full + pos.slot, 2 * C::SLOT);
+        const uint32_t bar = E4 ? smem_u32(bars_full + pos.slot) : mapa(smem_u32(bars_full + pos.slot), 0);
+        const uint32_t dst = E4 ? smem_u32(s_codes) + pos.slot * C::RAW : ss + pos.slot * C::SLOT;
 #pragma unroll
-            for (int c = 0; c < D / 64; ++c)
-              tma_pair_4d(dst + c * (64 * 128) + i * (box * 128), &tm_k, bar, 0, y, c, u);
+        for (int i = 0; i < 8; ++i) {
+          if (i < n) {
+            int y, u;
+            page_place(p, ids[i], x.head, x.s.kv, j * kBlockKeys + key0 + i * box, u, y);
+            if (E4) {
+              if (v) tma_load_4d(dst + i * box * (D / 2), &tm_v, bar, (int)rank * (D / 2), y, 0, u);
+              else tma_load_4d(dst + i * box * D, &tm_k, bar, 0, y, 0, u);
+            } else if (v) {
+              tma_pair_4d(dst + i * box * D, &tm_v, bar, 0, y, (int)rank * (D / 128), u);
+            } else if (n == 1) {
+              tma_pair_4d(dst, &tm_k, bar, 0, y, 0, u);
+            } else {
+#pragma unroll
+              for (int c = 0; c < D / 64; ++c)
+                tma_pair_4d(dst + c * (64 * 128) + i * (box * 128), &tm_k, bar, 0, y, c, u);
+            }
           }
         }
       }
-      __syncwarp();
-      if (++slot == N) { slot = 0; phase ^= 1; }
+      // after a wait ran out: what is in flight has landed before the memory goes
+      if (!ok && (E4 || rank == 0))
+        for (int i = 0; i < N; ++i) mbar_wait(bars_full + i, pos.phase ^ (i <= pos.slot ? 0 : 1), kAttnWaitBudgetNs);
     }
-    // after a wait ran out: what is in flight has landed before the memory goes
-    if (!ok && (E4 || rank == 0))
-      for (int i = 0; i < N; ++i) mbar_wait(bars_full + i, phase ^ (i < slot ? 0 : 1), kAttnWaitBudgetNs);
   } else if (warp == 8) {
     // ---- MMAs of the pair
     if (rank == 0 && lane == 0) {
@@ -601,15 +681,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(ChunkCfg<T, D, E4>::
       uint32_t phase = 0, it = 0, pieces = 0;
       // V: pages of `vrows` keys, each [D / 128 columns][vrows][128 bytes]; 16 keys a k-step
       const int vrows = E4 ? kBlockKeys : ps;
-      auto wait = [&](uint64_t* bar, uint32_t par) {
-        if (ok && !mbar_wait(bar, par, kAttnWaitBudgetNs)) {
-          attn_error(p.err, kAttnErrChunkMma);
-          s_abort = 1;
-          ok = false;
-        }
-        ok = ok && !s_abort;
-        return ok;
-      };
+      auto wait = [&](uint64_t* bar, uint32_t par) { return wait_one(bar, par, kAttnErrChunkMma); };
       auto advance = [&]() {
         commit_pair(empty + slot);
         if (++slot == C::SLOTS) { slot = 0; phase ^= 1; }
@@ -862,7 +934,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(ChunkCfg<T, D, E4>::
       if (lane == 0) mbar_arrive_remote(mapa(smem_u32(o_free), 0));
     }
     if (rank == 0 && tid == 0) ws.desc[pair] = desc;
-  } else if (E4 && warp == 10) {
+  } else if (E4 && warp == 11) {
     // ---- scales: lane has columns lane + 32 i of every block, in the order
     // of the loaded rows; the next block's are on their way while one is stored
     ChunkWalk walk(part);
