@@ -445,26 +445,6 @@ __device__ constexpr uint32_t idesc_16(int M, int N, bool b_n_major) {
          ((uint32_t)(M >> 4) << 24);
 }
 
-// a pair of fp32 operations in one instruction
-__device__ __forceinline__ void fma2(float& x, float& y, float a, float b) {   // (x, y) * a + b
-  asm("{\n\t.reg .b64 v, m, n;\n\tmov.b64 v, {%0, %1};\n\tmov.b64 m, {%2, %2};\n\tmov.b64 n, {%3, %3};\n\t"
-      "fma.rn.f32x2 v, v, m, n;\n\tmov.b64 {%0, %1}, v;\n\t}"
-      : "+f"(x), "+f"(y)
-      : "f"(a), "f"(b));
-}
-__device__ __forceinline__ void mul2(float& x, float& y, float a, float b) {   // (x * a, y * b)
-  asm("{\n\t.reg .b64 v, m;\n\tmov.b64 v, {%0, %1};\n\tmov.b64 m, {%2, %3};\n\t"
-      "mul.rn.f32x2 v, v, m;\n\tmov.b64 {%0, %1}, v;\n\t}"
-      : "+f"(x), "+f"(y)
-      : "f"(a), "f"(b));
-}
-__device__ __forceinline__ void add2(float& x, float& y, float a, float b) {   // (x + a, y + b)
-  asm("{\n\t.reg .b64 v, m;\n\tmov.b64 v, {%0, %1};\n\tmov.b64 m, {%2, %3};\n\t"
-      "add.rn.f32x2 v, v, m;\n\tmov.b64 {%0, %1}, v;\n\t}"
-      : "+f"(x), "+f"(y)
-      : "f"(a), "f"(b));
-}
-
 // two codes as two T values
 template <typename T>
 __device__ __forceinline__ uint32_t widen2(uint16_t c);

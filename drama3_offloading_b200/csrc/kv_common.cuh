@@ -68,6 +68,32 @@ __device__ __forceinline__ float2 e4m3x2_to_f2(uint16_t c) {
   return __half22float2(*reinterpret_cast<const __half2*>(&h));
 }
 
+// a pair of fp32 operations in one instruction
+__device__ __forceinline__ void fma2(float& x, float& y, float a, float b) {   // (x, y) * a + b
+  asm("{\n\t.reg .b64 v, m, n;\n\tmov.b64 v, {%0, %1};\n\tmov.b64 m, {%2, %2};\n\tmov.b64 n, {%3, %3};\n\t"
+      "fma.rn.f32x2 v, v, m, n;\n\tmov.b64 {%0, %1}, v;\n\t}"
+      : "+f"(x), "+f"(y)
+      : "f"(a), "f"(b));
+}
+__device__ __forceinline__ void mul2(float& x, float& y, float a, float b) {   // (x * a, y * b)
+  asm("{\n\t.reg .b64 v, m;\n\tmov.b64 v, {%0, %1};\n\tmov.b64 m, {%2, %3};\n\t"
+      "mul.rn.f32x2 v, v, m;\n\tmov.b64 {%0, %1}, v;\n\t}"
+      : "+f"(x), "+f"(y)
+      : "f"(a), "f"(b));
+}
+__device__ __forceinline__ void add2(float& x, float& y, float a, float b) {   // (x + a, y + b)
+  asm("{\n\t.reg .b64 v, m;\n\tmov.b64 v, {%0, %1};\n\tmov.b64 m, {%2, %3};\n\t"
+      "add.rn.f32x2 v, v, m;\n\tmov.b64 {%0, %1}, v;\n\t}"
+      : "+f"(x), "+f"(y)
+      : "f"(a), "f"(b));
+}
+__device__ __forceinline__ void fma2v(float& x, float& y, float a, float b, float c, float e) {   // (a * b + x, c * e + y)
+  asm("{\n\t.reg .b64 v, m, n;\n\tmov.b64 v, {%0, %1};\n\tmov.b64 m, {%2, %4};\n\tmov.b64 n, {%3, %5};\n\t"
+      "fma.rn.f32x2 v, m, n, v;\n\tmov.b64 {%0, %1}, v;\n\t}"
+      : "+f"(x), "+f"(y)
+      : "f"(a), "f"(b), "f"(c), "f"(e));
+}
+
 constexpr float kE4m3Max = 448.f;
 
 // Reads of what an earlier launch wrote go through L2 (__ldcg): under

@@ -67,18 +67,85 @@ constexpr int kFillThreads = 256;
 constexpr int kMaxHalf = 128;          // rotary pairs of the widest head
 constexpr int kMaxTokensPerCta = 4;
 
-// A group of D/8 lanes holds one row; NORM: norm and rotation of q and k rows
-// (otherwise there are no q rows and K goes in as it is).
-template <typename T, int D, bool NORM>
+// x / s of a row, rounded as the division is.  With r = 1 / s rounded and
+// q = x r, the remainder x - q s is exact in one fused step and q + rem r is
+// the quotient rounded correctly (Markstein's correction): three operations
+// where a division takes about ten.  The remainder must not underflow, so
+// scales far from 1 -- and infinite ones -- take the division.
+struct RowDiv {
+  float s, r;
+  bool plain;
+  __device__ __forceinline__ explicit RowDiv(float scale) : s(scale), r(1.f / scale) {
+    plain = !(scale > 0x1p-90f && scale < 0x1p119f);
+  }
+  __device__ __forceinline__ void two(float& x, float& y) const {
+    float q0 = x, q1 = y, e0 = x, e1 = y;
+    mul2(q0, q1, r, r);
+    fma2v(e0, e1, -q0, s, -q1, s);
+    fma2v(q0, q1, e0, r, e1, r);
+    x = q0;
+    y = q1;
+  }
+};
+
+// A group of D/8 lanes holds one row, ROWS rows at a time, the next ROWS on
+// their way; NORM: norm and rotation of q and k rows (otherwise there are no q
+// rows and K goes in as it is).  E4: K and V become codes.  What a row does
+// not need (a query's largest value, a value's norm) its warp skips: the
+// kernel is as much bound by its instructions as by HBM.
+template <typename T, int D, bool NORM, bool E4>
 __global__ void __launch_bounds__(kFillThreads) kv_fill_kernel(const __grid_constant__ FillParams p) {
   constexpr int L = D / 8;                          // lanes of a row
-  __shared__ float s_cos[kMaxTokensPerCta][kMaxHalf], s_sin[kMaxTokensPerCta][kMaxHalf];
-  const int lane = threadIdx.x % L, grp = threadIdx.x / L;
+  constexpr int ROWS = 2;
   constexpr int GROUPS = kFillThreads / L;
+  __shared__ __align__(16) float s_cos[kMaxTokensPerCta][kMaxHalf], s_sin[kMaxTokensPerCta][kMaxHalf];
+  const int lane = threadIdx.x % L, grp = threadIdx.x / L;
   const int t0 = blockIdx.x * p.tokens_per_cta;
   const int nt = min(p.tokens_per_cta, p.tokens - t0);
   pdl_trigger();
+  float wq[8], wk[8];
+  if (NORM) {       // weights are no earlier launch's work
+    unpack8<T>(*reinterpret_cast<const uint4*>(static_cast<const T*>(p.q_w) + lane * 8), wq);
+    unpack8<T>(*reinterpret_cast<const uint4*>(static_cast<const T*>(p.k_w) + lane * 8), wk);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      wq[i] += p.w_offset;
+      wk[i] += p.w_offset;
+    }
+  }
   pdl_wait();
+  const bool cached = p.cache.k != nullptr;
+  const int rows = p.heads + (cached ? 2 : 1) * p.kv_heads;   // q, k and, into a cache, v
+  // a group's rows, in order: token t, row h of the token
+  struct At {
+    int t, h;
+  };
+  auto next = [&](At a) {
+    a.h += GROUPS;
+    while (a.h >= rows) {
+      a.h -= rows;
+      ++a.t;
+    }
+    return a;
+  };
+  At ahead{0, grp - GROUPS};
+  ahead = next(ahead);
+  uint4 raw[ROWS];
+  auto load = [&]() {
+#pragma unroll
+    for (int u = 0; u < ROWS; ++u) {
+      raw[u] = make_uint4(0, 0, 0, 0);
+      if (ahead.t < nt) {
+        const int k0 = ahead.h - p.heads, v0 = k0 - p.kv_heads;
+        const RowsIn& in = k0 < 0 ? p.q : v0 < 0 ? p.k : p.v;
+        raw[u] = __ldcg(reinterpret_cast<const uint4*>(static_cast<const T*>(in.p) + (long long)(t0 + ahead.t) * in.token +
+                                                       (k0 < 0 ? ahead.h : v0 < 0 ? k0 : v0) * in.head + lane * 8));
+      }
+      ahead = next(ahead);
+    }
+  };
+  At at = ahead;
+  load();
   if (NORM) {
     for (int i = threadIdx.x; i < nt * p.half; i += kFillThreads) {
       const int t = i / p.half, j = i - t * p.half;
@@ -91,100 +158,119 @@ __global__ void __launch_bounds__(kFillThreads) kv_fill_kernel(const __grid_cons
     }
     __syncthreads();
   }
-  const bool cached = p.cache.k != nullptr;
-  const int rows = p.heads + (cached ? 2 : 1) * p.kv_heads;   // q, k and, into a cache, v
-  // every lane of a warp takes the same number of turns: the shuffles are whole
-  for (int r0 = 0; r0 < nt * rows; r0 += GROUPS) {
-    const int r = r0 + grp;
-    const bool live = r < nt * rows;
-    const int t = live ? r / rows : 0, h = live ? r - t * rows : 0;
-    const int kind = h < p.heads ? 0 : h < p.heads + p.kv_heads ? 1 : 2;
-    const int head = kind == 0 ? h : kind == 1 ? h - p.heads : h - p.heads - p.kv_heads;
-    const RowsIn& in = kind == 0 ? p.q : kind == 1 ? p.k : p.v;
-    const long long tok = t0 + t;
-    uint4 raw = make_uint4(0, 0, 0, 0);
-    if (live)
-      raw = __ldcg(reinterpret_cast<const uint4*>(static_cast<const T*>(in.p) + tok * in.token +
-                                                  head * in.head + lane * 8));
-    float x[8];
-    unpack8<T>(raw, x);
-    if (NORM) {
-      float ss = 0.f;
+  const int n16 = p.half / 8;                       // lanes of one half of the rotated dims
+  const bool first = lane < n16;
+  const float sign = first ? -1.f : 1.f;
+  const int j8 = (first ? lane : lane - n16) * 8;
+  const long long slots = (long long)p.cache.pages * p.cache.page_size;
+  // the lanes of a warp leave together: the shuffles are whole
+  while (__any_sync(0xffffffffu, at.t < nt)) {
+    float x[ROWS][8];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) ss = fmaf(x[i], x[i], ss);
+    for (int u = 0; u < ROWS; ++u) unpack8<T>(raw[u], x[u]);
+    load();
 #pragma unroll
-      for (int o = L / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-      if (kind < 2) {
-        const float inv = 1.f / sqrtf(ss * (1.f / D) + p.eps);
-        float w[8];
-        unpack8<T>(*reinterpret_cast<const uint4*>(
-                       static_cast<const T*>(kind == 0 ? p.q_w : p.k_w) + lane * 8), w);
+    for (int u = 0; u < ROWS; ++u) {
+      const bool live = at.t < nt;
+      const int t = live ? at.t : 0, h = at.h, k0 = h - p.heads, v0 = k0 - p.kv_heads;
+      const bool is_q = k0 < 0, is_v = v0 >= 0;
+      at = next(at);
+      const long long tok = t0 + t;
+      long long slot = -1;
+      if (live && cached && !is_q) slot = load_index(p.slots, p.slot_bytes, tok);
+      float (&y)[8] = x[u];
+      if (NORM && __any_sync(0xffffffffu, !is_v)) {
+        float s0 = 0.f, s1 = 0.f;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = x[i] * inv * (w[i] + p.w_offset);
+        for (int i = 0; i < 8; i += 2) fma2v(s0, s1, y[i], y[i], y[i + 1], y[i + 1]);
+        float ss = s0 + s1;
+#pragma unroll
+        for (int o = L / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+        if (!is_v) {
+          const float inv = rsqrtf(ss * (1.f / D) + p.eps);
+#pragma unroll
+          for (int i = 0; i < 8; i += 2) {
+            mul2(y[i], y[i + 1], inv, inv);
+            mul2(y[i], y[i + 1], is_q ? wq[i] : wk[i], is_q ? wq[i + 1] : wk[i + 1]);
+          }
+        }
+        const float *cs = s_cos[t], *sn = s_sin[t];
+        if (p.interleaved) {
+          if (!is_v && lane * 4 < p.half) {
+            const float4 c4 = *reinterpret_cast<const float4*>(cs + lane * 4);
+            const float4 s4 = *reinterpret_cast<const float4*>(sn + lane * 4);
+            const float c[4] = {c4.x, c4.y, c4.z, c4.w}, s[4] = {s4.x, s4.y, s4.z, s4.w};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const float a = y[2 * i], b = y[2 * i + 1];
+              y[2 * i] = a * c[i] - b * s[i];
+              y[2 * i + 1] = b * c[i] + a * s[i];
+            }
+          }
+        } else {
+          // lanes [0, R/16) hold the first halves, the next R/16 the second
+          float z[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            z[i] = __shfl_sync(0xffffffffu, y[i], first ? lane + n16 : lane - n16, L);
+          if (!is_v && lane < 2 * n16) {
+#pragma unroll
+            for (int i = 0; i < 8; i += 4) {
+              const float4 c = *reinterpret_cast<const float4*>(cs + j8 + i);
+              const float4 s = *reinterpret_cast<const float4*>(sn + j8 + i);
+              mul2(y[i], y[i + 1], c.x, c.y);
+              mul2(y[i + 2], y[i + 3], c.z, c.w);
+              mul2(z[i], z[i + 1], sign, sign);
+              mul2(z[i + 2], z[i + 3], sign, sign);
+              fma2v(y[i], y[i + 1], z[i], s.x, z[i + 1], s.y);
+              fma2v(y[i + 2], y[i + 3], z[i + 2], s.z, z[i + 3], s.w);
+            }
+          }
+        }
       }
-      const float *cs = s_cos[t], *sn = s_sin[t];
-      if (p.interleaved) {
-        if (kind < 2 && lane * 4 < p.half) {
+      float amax = 0.f;
+      if (E4 && __any_sync(0xffffffffu, !is_q)) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) amax = fmaxf(amax, fabsf(y[i]));
+#pragma unroll
+        for (int o = L / 2; o > 0; o >>= 1)
+          amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+      }
+      if (!live) continue;
+      if (is_q) {
+        *reinterpret_cast<uint4*>(static_cast<T*>(p.q_out) + tok * p.q_out_token +
+                                  h * p.q_out_head + lane * 8) = pack8<T>(y);
+        continue;
+      }
+      if (!cached) {
+        *reinterpret_cast<uint4*>(static_cast<T*>(p.k_out) + tok * p.k_out_token +
+                                  k0 * p.k_out_head + lane * 8) = pack8<T>(y);
+        continue;
+      }
+      if (slot < 0 || slot >= slots) continue;
+      const int page = (int)slot / p.cache.page_size, off = (int)slot - page * p.cache.page_size;
+      const long long row = ((long long)page * p.cache.kv_heads + (is_v ? v0 : k0)) * p.cache.page_size + off;
+      void* base = is_v ? p.cache.v : p.cache.k;
+      if (E4) {
+        const float s = amax > 0.f ? amax / kE4m3Max : 1.f;
+        const RowDiv div(s);
+        uint32_t w[4];
+        if (div.plain) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) w[i] = e4m3x2(y[2 * i] / s, y[2 * i + 1] / s);
+        } else {
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            const float c = cs[lane * 4 + i], s = sn[lane * 4 + i];
-            const float a = x[2 * i], b = x[2 * i + 1];
-            x[2 * i] = a * c - b * s;
-            x[2 * i + 1] = b * c + a * s;
+            div.two(y[2 * i], y[2 * i + 1]);
+            w[i] = e4m3x2(y[2 * i], y[2 * i + 1]);
           }
         }
+        *reinterpret_cast<uint2*>(static_cast<uint8_t*>(base) + row * D + lane * 8) =
+            make_uint2(w[0] | (w[1] << 16), w[2] | (w[3] << 16));
+        if (lane == 0) (is_v ? p.cache.v_scale : p.cache.k_scale)[row] = s;
       } else {
-        // lanes [0, R/16) hold the first halves, the next R/16 the second
-        const int n = p.half / 8;
-        const bool first = lane < n;
-        float y[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-          y[i] = __shfl_sync(0xffffffffu, x[i], first ? lane + n : lane - n, L);
-        if (kind < 2 && lane < 2 * n) {
-          const int j = (first ? lane : lane - n) * 8;
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const float c = cs[j + i], s = sn[j + i];
-            x[i] = first ? x[i] * c - y[i] * s : x[i] * c + y[i] * s;
-          }
-        }
+        *reinterpret_cast<uint4*>(static_cast<T*>(base) + row * D + lane * 8) = pack8<T>(y);
       }
-    }
-    float amax = 0.f;
-    if (p.cache.dtype == D3_E4M3) {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) amax = fmaxf(amax, fabsf(x[i]));
-#pragma unroll
-      for (int o = L / 2; o > 0; o >>= 1)
-        amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
-    }
-    if (!live) continue;
-    if (kind == 0) {
-      *reinterpret_cast<uint4*>(static_cast<T*>(p.q_out) + tok * p.q_out_token +
-                                head * p.q_out_head + lane * 8) = pack8<T>(x);
-      continue;
-    }
-    if (!cached) {
-      *reinterpret_cast<uint4*>(static_cast<T*>(p.k_out) + tok * p.k_out_token +
-                                head * p.k_out_head + lane * 8) = pack8<T>(x);
-      continue;
-    }
-    const long long slot = load_index(p.slots, p.slot_bytes, tok);
-    if (slot < 0 || slot >= (long long)p.cache.pages * p.cache.page_size) continue;
-    const long long page = slot / p.cache.page_size, off = slot - page * p.cache.page_size;
-    const long long row = (page * p.cache.kv_heads + head) * p.cache.page_size + off;
-    void* base = kind == 1 ? p.cache.k : p.cache.v;
-    if (p.cache.dtype == D3_E4M3) {
-      const float s = amax > 0.f ? amax / kE4m3Max : 1.f;
-      uint32_t w[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) w[i] = e4m3x2(x[2 * i] / s, x[2 * i + 1] / s);
-      *reinterpret_cast<uint2*>(static_cast<uint8_t*>(base) + row * D + lane * 8) =
-          make_uint2(w[0] | (w[1] << 16), w[2] | (w[3] << 16));
-      if (lane == 0) (kind == 1 ? p.cache.k_scale : p.cache.v_scale)[row] = s;
-    } else {
-      *reinterpret_cast<uint4*>(static_cast<T*>(base) + row * D + lane * 8) = pack8<T>(x);
     }
   }
 }
@@ -196,68 +282,63 @@ struct ReadParams {
   d3_kv_cache cache;
 };
 
-constexpr int kReadRows = 2;   // rows a lane group has in flight
+constexpr int kReadRows = 4;   // rows a lane group has in flight
 
-// Rows of the cache back in 16 bits: T(code * s), or the row as it is.
-template <typename T, int D>
+// Rows of the cache back in 16 bits: T(code * s), or the row as it is.  A lane
+// takes 16 bytes of a row.
+template <typename T, int D, bool E4>
 __global__ void __launch_bounds__(256) kv_read_kernel(const __grid_constant__ ReadParams p) {
-  constexpr int L = D / 8, GROUPS = 256 / L;
+  constexpr int PER = E4 ? 16 : 8, L = D / PER, GROUPS = 256 / L;
   const int lane = threadIdx.x % L, grp = threadIdx.x / L;
   pdl_trigger();
   pdl_wait();
-  const long long per = 2LL * p.cache.kv_heads, rows = p.tokens * per;
+  const int per = 2 * p.cache.kv_heads;
+  const long long rows = (long long)p.tokens * per;
   const long long r0 = (long long)blockIdx.x * (GROUPS * kReadRows) + grp;
-  long long at[kReadRows];
-  const void* src[kReadRows];
   bool live[kReadRows], have[kReadRows];
   uint4 raw[kReadRows];
   float sc[kReadRows];
-  T* out[kReadRows];
+  long long to[kReadRows], slot[kReadRows];
+  int h2[kReadRows];
 #pragma unroll
   for (int i = 0; i < kReadRows; ++i) {
     const long long r = r0 + i * GROUPS;
     live[i] = r < rows;
-    have[i] = false;
+    const int t = live[i] ? (int)((unsigned)r / (unsigned)per) : 0;
+    h2[i] = (int)r - t * per;
+    to[i] = ((long long)t * p.cache.kv_heads + (h2[i] >> 1)) * D + lane * PER;
+    slot[i] = live[i] ? load_index(p.slots, p.slot_bytes, t) : -1;
+  }
+#pragma unroll
+  for (int i = 0; i < kReadRows; ++i) {
+    have[i] = slot[i] >= 0 && slot[i] < (long long)p.cache.pages * p.cache.page_size;
     raw[i] = make_uint4(0, 0, 0, 0);
-    sc[i] = 1.f;
-    if (!live[i]) continue;
-    const long long t = r / per;
-    const int h2 = (int)(r - t * per), h = h2 >> 1;
-    const bool is_k = (h2 & 1) == 0;
-    out[i] = static_cast<T*>(is_k ? p.k_out : p.v_out) + (t * p.cache.kv_heads + h) * D + lane * 8;
-    const long long slot = load_index(p.slots, p.slot_bytes, t);
-    have[i] = slot >= 0 && slot < (long long)p.cache.pages * p.cache.page_size;
+    sc[i] = 0.f;
     if (!have[i]) continue;
-    const long long page = slot / p.cache.page_size, off = slot - page * p.cache.page_size;
-    at[i] = (page * p.cache.kv_heads + h) * p.cache.page_size + off;
-    src[i] = is_k ? p.cache.k : p.cache.v;
-    if (p.cache.dtype == D3_E4M3) {
-      const uint2 c = __ldcg(reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(src[i]) +
-                                                            at[i] * D + lane * 8));
-      raw[i].x = c.x;
-      raw[i].y = c.y;
-      sc[i] = __ldcg((is_k ? p.cache.k_scale : p.cache.v_scale) + at[i]);
-    } else {
-      raw[i] = __ldcg(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(src[i]) +
-                                                     at[i] * D + lane * 8));
-    }
+    const int page = (int)slot[i] / p.cache.page_size, off = (int)slot[i] - page * p.cache.page_size;
+    const long long row = ((long long)page * p.cache.kv_heads + (h2[i] >> 1)) * p.cache.page_size + off;
+    const bool v = h2[i] & 1;
+    raw[i] = __ldcg(reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(v ? p.cache.v : p.cache.k) +
+                                                   row * (D * (E4 ? 1 : 2)) + lane * 16));
+    if (E4) sc[i] = __ldcg((v ? p.cache.v_scale : p.cache.k_scale) + row);
   }
 #pragma unroll
   for (int i = 0; i < kReadRows; ++i) {
     if (!live[i]) continue;
-    uint4 o = raw[i];
-    float x[8];
-    if (p.cache.dtype == D3_E4M3) {
+    T* out = static_cast<T*>(h2[i] & 1 ? p.v_out : p.k_out) + to[i];
+    if (E4) {
+      const uint32_t w[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
+      uint32_t o[8];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const uint32_t w = j < 2 ? raw[i].x : raw[i].y;
-        const float2 f = e4m3x2_to_f2((uint16_t)(j & 1 ? w >> 16 : w));
-        x[2 * j] = f.x * sc[i];
-        x[2 * j + 1] = f.y * sc[i];
+      for (int j = 0; j < 8; ++j) {
+        const float2 f = e4m3x2_to_f2((uint16_t)(w[j >> 1] >> (16 * (j & 1))));
+        o[j] = have[i] ? Elem<T>::from_f2(f.x * sc[i], f.y * sc[i]) : 0u;
       }
-      o = have[i] ? pack8<T>(x) : make_uint4(0, 0, 0, 0);
+      *reinterpret_cast<uint4*>(out) = make_uint4(o[0], o[1], o[2], o[3]);
+      *reinterpret_cast<uint4*>(out + 8) = make_uint4(o[4], o[5], o[6], o[7]);
+    } else {
+      *reinterpret_cast<uint4*>(out) = raw[i];
     }
-    *reinterpret_cast<uint4*>(out[i]) = o;
   }
 }
 
@@ -268,11 +349,17 @@ __global__ void __launch_bounds__(256) kv_read_kernel(const __grid_constant__ Re
 // every SM to hold several CTAs all the same.
 static int tokens_per_cta(int tokens) { return tokens >= 8 * num_sms() ? kMaxTokensPerCta : 1; }
 
+template <typename T, int D>
+static void (*fill_kernel(bool norm, bool e4))(FillParams) {
+  return norm ? (e4 ? kv_fill_kernel<T, D, true, true> : kv_fill_kernel<T, D, true, false>)
+              : (e4 ? kv_fill_kernel<T, D, false, true> : kv_fill_kernel<T, D, false, false>);
+}
+
 template <typename T>
 static int launch_fill(const FillParams& p, int D, bool norm, cudaStream_t st) {
   const dim3 grid((unsigned)((p.tokens + p.tokens_per_cta - 1) / p.tokens_per_cta));
-  void (*k)(FillParams) = D == 128 ? (norm ? kv_fill_kernel<T, 128, true> : kv_fill_kernel<T, 128, false>)
-                                   : (norm ? kv_fill_kernel<T, 256, true> : kv_fill_kernel<T, 256, false>);
+  const bool e4 = p.cache.dtype == D3_E4M3;
+  void (*k)(FillParams) = D == 128 ? fill_kernel<T, 128>(norm, e4) : fill_kernel<T, 256>(norm, e4);
   D3_CUDA_TRY(launch_k(k, grid, dim3(kFillThreads), 0, st, pdl_enabled(), p), "kv_fill_kernel launch");
   return D3_OK;
 }
@@ -331,13 +418,16 @@ int d3_kv_read(const d3_kv_cache* cache, const void* slots, int32_t slot_bytes, 
   if (!aligned16(k_out) || !aligned16(v_out))
     return fail(D3_ERR_MISALIGNED, "d3_kv_read: outputs not 16-byte aligned");
   ReadParams p{slots, slot_bytes, tokens, k_out, v_out, *cache};
-  const int D = cache->head_dim;
-  const long long rows = 2LL * cache->kv_heads * tokens, per = 256 / (D / 8) * kReadRows;
-  if ((rows + per - 1) / per >= (1LL << 31))
-    return fail(D3_ERR_TOO_LARGE, "d3_kv_read: too many rows");
+  const int D = cache->head_dim, lanes = D / (cache->dtype == D3_E4M3 ? 16 : 8);
+  const long long rows = 2LL * cache->kv_heads * tokens, per = 256 / lanes * kReadRows;
+  if (rows >= (1LL << 31)) return fail(D3_ERR_TOO_LARGE, "d3_kv_read: too many rows");
   const dim3 grid((unsigned)((rows + per - 1) / per));
-  void (*kern)(ReadParams) = dtype == D3_BF16 ? (D == 128 ? kv_read_kernel<__nv_bfloat16, 128> : kv_read_kernel<__nv_bfloat16, 256>)
-                                              : (D == 128 ? kv_read_kernel<__half, 128> : kv_read_kernel<__half, 256>);
+  const bool e4 = cache->dtype == D3_E4M3;
+  void (*kern)(ReadParams) =
+      dtype == D3_BF16 ? (D == 128 ? (e4 ? kv_read_kernel<__nv_bfloat16, 128, true> : kv_read_kernel<__nv_bfloat16, 128, false>)
+                                   : (e4 ? kv_read_kernel<__nv_bfloat16, 256, true> : kv_read_kernel<__nv_bfloat16, 256, false>))
+                       : (D == 128 ? (e4 ? kv_read_kernel<__half, 128, true> : kv_read_kernel<__half, 128, false>)
+                                   : (e4 ? kv_read_kernel<__half, 256, true> : kv_read_kernel<__half, 256, false>));
   D3_CUDA_TRY(launch_k(kern, grid, dim3(256), 0, (cudaStream_t)stream, pdl_enabled(), p),
               "kv_read_kernel launch");
   return D3_OK;
