@@ -57,7 +57,7 @@ struct FillParams {
   const void* positions;
   const double* inv_freq;
   const void* slots;
-  int pos_bytes, slot_bytes, tokens, heads, kv_heads, half, interleaved;
+  int pos_bytes, slot_bytes, tokens, heads, kv_heads, half, interleaved, page_shift;
   int tokens_per_cta;
   float eps, w_offset;
   d3_kv_cache cache;      // k == NULL: no cache
@@ -67,86 +67,150 @@ constexpr int kFillThreads = 256;
 constexpr int kMaxHalf = 128;          // rotary pairs of the widest head
 constexpr int kMaxTokensPerCta = 4;
 
-// x / s of a row, rounded as the division is.  With r = 1 / s rounded and
-// q = x r, the remainder x - q s is exact in one fused step and q + rem r is
-// the quotient rounded correctly (Markstein's correction): three operations
-// where a division takes about ten.  The remainder must not underflow, so
-// scales far from 1 -- and infinite ones -- take the division.
-struct RowDiv {
-  float s, r;
-  bool plain;
-  __device__ __forceinline__ explicit RowDiv(float scale) : s(scale), r(1.f / scale) {
-    plain = !(scale > 0x1p-90f && scale < 0x1p119f);
-  }
-  __device__ __forceinline__ void two(float& x, float& y) const {
-    float q0 = x, q1 = y, e0 = x, e1 = y;
-    mul2(q0, q1, r, r);
-    fma2v(e0, e1, -q0, s, -q1, s);
-    fma2v(q0, q1, e0, r, e1, r);
-    x = q0;
-    y = q1;
+// x / s rounded as the division is.  With r = 1 / s rounded and q = x r, the
+// remainder x - q s is exact in one fused step and q + rem r is the quotient
+// rounded correctly (Markstein's correction): three operations, two values at
+// a time, where a division takes about ten.  The remainder must not
+// underflow: the caller sees to it that s is not far from 1.
+__device__ __forceinline__ void div2(float& x, float& y, float s, float r) {
+  float q0 = x, q1 = y;
+  mul2(q0, q1, r, r);
+  fma2v(x, y, -q0, s, -q1, s);
+  fma2v(q0, q1, x, r, y, r);
+  x = q0;
+  y = q1;
+}
+
+// Where a group of lanes is among rows of `per` a token: token t, row h.
+struct At {
+  int t, h;
+  __device__ __forceinline__ void advance(int by, int per) {
+    h += by;
+    while (h >= per) {
+      h -= per;
+      ++t;
+    }
   }
 };
 
-// A group of D/8 lanes holds one row, ROWS rows at a time, the next ROWS on
-// their way; NORM: norm and rotation of q and k rows (otherwise there are no q
-// rows and K goes in as it is).  E4: K and V become codes.  What a row does
-// not need (a query's largest value, a value's norm) its warp skips: the
-// kernel is as much bound by its instructions as by HBM.
+// One cached row: 8 elements a lane of D / 8.
+template <typename T, int D, bool E4>
+__device__ __forceinline__ void put_row(void* buf, float* scales, long long row, int lane, float (&y)[8], bool live) {
+  constexpr int L = D / 8;
+  if (E4) {
+    float amax = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) amax = fmaxf(amax, fabsf(y[i]));
+#pragma unroll
+    for (int o = L / 2; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+    float s;
+    uint32_t w[4];
+    if (amax > 0x1p-80f && amax < 0x1p120f) {
+      s = amax;
+      float unused = amax;
+      div2(s, unused, kE4m3Max, 1.f / kE4m3Max);
+      const float r = __frcp_rn(s);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        div2(y[2 * i], y[2 * i + 1], s, r);
+        w[i] = e4m3x2(y[2 * i], y[2 * i + 1]);
+      }
+    } else {      // zeros, infinities, the ends of the range
+      s = amax > 0.f ? amax / kE4m3Max : 1.f;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) w[i] = e4m3x2(y[2 * i] / s, y[2 * i + 1] / s);
+    }
+    if (live) {
+      *reinterpret_cast<uint2*>(static_cast<uint8_t*>(buf) + row * D + lane * 8) =
+          make_uint2(w[0] | (w[1] << 16), w[2] | (w[3] << 16));
+      if (lane == 0) scales[row] = s;
+    }
+  } else if (live) {
+    *reinterpret_cast<uint4*>(static_cast<T*>(buf) + row * D + lane * 8) = pack8<T>(y);
+  }
+}
+
+// A group of D/8 lanes holds a row; NORM: norm and rotation of q and k rows
+// (otherwise there are no q rows and K goes in as it is).  E4: K and V become
+// codes.  Queries first, then K and V of a token and head together, which
+// share their place; what a row does not need (a query's largest value, a
+// value's norm) is not computed: the kernel is as much bound by its
+// instructions as by HBM.
 template <typename T, int D, bool NORM, bool E4>
 __global__ void __launch_bounds__(kFillThreads) kv_fill_kernel(const __grid_constant__ FillParams p) {
   constexpr int L = D / 8;                          // lanes of a row
-  constexpr int ROWS = 2;
   constexpr int GROUPS = kFillThreads / L;
   __shared__ __align__(16) float s_cos[kMaxTokensPerCta][kMaxHalf], s_sin[kMaxTokensPerCta][kMaxHalf];
   const int lane = threadIdx.x % L, grp = threadIdx.x / L;
   const int t0 = blockIdx.x * p.tokens_per_cta;
   const int nt = min(p.tokens_per_cta, p.tokens - t0);
   pdl_trigger();
-  float wq[8], wk[8];
-  if (NORM) {       // weights are no earlier launch's work
-    unpack8<T>(*reinterpret_cast<const uint4*>(static_cast<const T*>(p.q_w) + lane * 8), wq);
-    unpack8<T>(*reinterpret_cast<const uint4*>(static_cast<const T*>(p.k_w) + lane * 8), wk);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      wq[i] += p.w_offset;
-      wk[i] += p.w_offset;
-    }
-  }
   pdl_wait();
-  const bool cached = p.cache.k != nullptr;
-  const int rows = p.heads + (cached ? 2 : 1) * p.kv_heads;   // q, k and, into a cache, v
-  // a group's rows, in order: token t, row h of the token
-  struct At {
-    int t, h;
+  auto fetch = [&](const RowsIn& in, At at) {
+    uint4 u = make_uint4(0, 0, 0, 0);
+    if (at.t < nt)
+      u = __ldcg(reinterpret_cast<const uint4*>(static_cast<const T*>(in.p) + (long long)(t0 + at.t) * in.token +
+                                                at.h * in.head + lane * 8));
+    return u;
   };
-  auto next = [&](At a) {
-    a.h += GROUPS;
-    while (a.h >= rows) {
-      a.h -= rows;
-      ++a.t;
-    }
-    return a;
-  };
-  At ahead{0, grp - GROUPS};
-  ahead = next(ahead);
-  uint4 raw[ROWS];
-  auto load = [&]() {
+  const int n16 = p.half / 8;                       // lanes of one half of the rotated dims
+  const bool first = lane < n16;
+  const float sign = first ? -1.f : 1.f;
+  const int j8 = (first ? lane : lane - n16) * 8;
+  // all lanes: norm with weights w, rotation by token t
+  auto turn = [&](float (&y)[8], const float (&w)[8], int t) {
+    float s0 = 0.f, s1 = 0.f;
 #pragma unroll
-    for (int u = 0; u < ROWS; ++u) {
-      raw[u] = make_uint4(0, 0, 0, 0);
-      if (ahead.t < nt) {
-        const int k0 = ahead.h - p.heads, v0 = k0 - p.kv_heads;
-        const RowsIn& in = k0 < 0 ? p.q : v0 < 0 ? p.k : p.v;
-        raw[u] = __ldcg(reinterpret_cast<const uint4*>(static_cast<const T*>(in.p) + (long long)(t0 + ahead.t) * in.token +
-                                                       (k0 < 0 ? ahead.h : v0 < 0 ? k0 : v0) * in.head + lane * 8));
+    for (int i = 0; i < 8; i += 2) fma2v(s0, s1, y[i], y[i], y[i + 1], y[i + 1]);
+    float ss = s0 + s1;
+#pragma unroll
+    for (int o = L / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+    const float inv = rsqrtf(ss * (1.f / D) + p.eps);
+#pragma unroll
+    for (int i = 0; i < 8; i += 2) {
+      mul2(y[i], y[i + 1], inv, inv);
+      mul2(y[i], y[i + 1], w[i], w[i + 1]);
+    }
+    const float *cs = s_cos[t], *sn = s_sin[t];
+    if (p.interleaved) {
+      if (lane * 4 < p.half) {
+        const float4 c4 = *reinterpret_cast<const float4*>(cs + lane * 4);
+        const float4 s4 = *reinterpret_cast<const float4*>(sn + lane * 4);
+        const float c[4] = {c4.x, c4.y, c4.z, c4.w}, s[4] = {s4.x, s4.y, s4.z, s4.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float a = y[2 * i], b = y[2 * i + 1];
+          y[2 * i] = a * c[i] - b * s[i];
+          y[2 * i + 1] = b * c[i] + a * s[i];
+        }
       }
-      ahead = next(ahead);
+    } else {
+      // lanes [0, R/16) hold the first halves, the next R/16 the second
+      float z[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        z[i] = __shfl_sync(0xffffffffu, y[i], first ? lane + n16 : lane - n16, L);
+      if (lane < 2 * n16) {
+#pragma unroll
+        for (int i = 0; i < 8; i += 4) {
+          const float4 c = *reinterpret_cast<const float4*>(cs + j8 + i);
+          const float4 s = *reinterpret_cast<const float4*>(sn + j8 + i);
+          mul2(y[i], y[i + 1], c.x, c.y);
+          mul2(y[i + 2], y[i + 3], c.z, c.w);
+          mul2(z[i], z[i + 1], sign, sign);
+          mul2(z[i + 2], z[i + 3], sign, sign);
+          fma2v(y[i], y[i + 1], z[i], s.x, z[i + 1], s.y);
+          fma2v(y[i + 2], y[i + 3], z[i + 2], s.z, z[i + 3], s.w);
+        }
+      }
     }
   };
-  At at = ahead;
-  load();
+  float w[8];
+  // the lanes of a warp leave a loop together: the shuffles are whole
   if (NORM) {
+    At at{0, 0};
+    at.advance(grp, p.heads);
+    uint4 raw = fetch(p.q, at);
     for (int i = threadIdx.x; i < nt * p.half; i += kFillThreads) {
       const int t = i / p.half, j = i - t * p.half;
       const double turns = (double)load_index(p.positions, p.pos_bytes, t0 + t) * p.inv_freq[j] *
@@ -156,133 +220,68 @@ __global__ void __launch_bounds__(kFillThreads) kv_fill_kernel(const __grid_cons
       s_cos[t][j] = c;
       s_sin[t][j] = s;
     }
+    unpack8<T>(*reinterpret_cast<const uint4*>(static_cast<const T*>(p.q_w) + lane * 8), w);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) w[i] += p.w_offset;
     __syncthreads();
-  }
-  const int n16 = p.half / 8;                       // lanes of one half of the rotated dims
-  const bool first = lane < n16;
-  const float sign = first ? -1.f : 1.f;
-  const int j8 = (first ? lane : lane - n16) * 8;
-  const long long slots = (long long)p.cache.pages * p.cache.page_size;
-  // the lanes of a warp leave together: the shuffles are whole
-  while (__any_sync(0xffffffffu, at.t < nt)) {
-    float x[ROWS][8];
-#pragma unroll
-    for (int u = 0; u < ROWS; ++u) unpack8<T>(raw[u], x[u]);
-    load();
-#pragma unroll
-    for (int u = 0; u < ROWS; ++u) {
-      const bool live = at.t < nt;
-      const int t = live ? at.t : 0, h = at.h, k0 = h - p.heads, v0 = k0 - p.kv_heads;
-      const bool is_q = k0 < 0, is_v = v0 >= 0;
-      at = next(at);
-      const long long tok = t0 + t;
-      long long slot = -1;
-      if (live && cached && !is_q) slot = load_index(p.slots, p.slot_bytes, tok);
-      float (&y)[8] = x[u];
-      if (NORM && __any_sync(0xffffffffu, !is_v)) {
-        float s0 = 0.f, s1 = 0.f;
-#pragma unroll
-        for (int i = 0; i < 8; i += 2) fma2v(s0, s1, y[i], y[i], y[i + 1], y[i + 1]);
-        float ss = s0 + s1;
-#pragma unroll
-        for (int o = L / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-        if (!is_v) {
-          const float inv = rsqrtf(ss * (1.f / D) + p.eps);
-#pragma unroll
-          for (int i = 0; i < 8; i += 2) {
-            mul2(y[i], y[i + 1], inv, inv);
-            mul2(y[i], y[i + 1], is_q ? wq[i] : wk[i], is_q ? wq[i + 1] : wk[i + 1]);
-          }
-        }
-        const float *cs = s_cos[t], *sn = s_sin[t];
-        if (p.interleaved) {
-          if (!is_v && lane * 4 < p.half) {
-            const float4 c4 = *reinterpret_cast<const float4*>(cs + lane * 4);
-            const float4 s4 = *reinterpret_cast<const float4*>(sn + lane * 4);
-            const float c[4] = {c4.x, c4.y, c4.z, c4.w}, s[4] = {s4.x, s4.y, s4.z, s4.w};
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const float a = y[2 * i], b = y[2 * i + 1];
-              y[2 * i] = a * c[i] - b * s[i];
-              y[2 * i + 1] = b * c[i] + a * s[i];
-            }
-          }
-        } else {
-          // lanes [0, R/16) hold the first halves, the next R/16 the second
-          float z[8];
-#pragma unroll
-          for (int i = 0; i < 8; ++i)
-            z[i] = __shfl_sync(0xffffffffu, y[i], first ? lane + n16 : lane - n16, L);
-          if (!is_v && lane < 2 * n16) {
-#pragma unroll
-            for (int i = 0; i < 8; i += 4) {
-              const float4 c = *reinterpret_cast<const float4*>(cs + j8 + i);
-              const float4 s = *reinterpret_cast<const float4*>(sn + j8 + i);
-              mul2(y[i], y[i + 1], c.x, c.y);
-              mul2(y[i + 2], y[i + 3], c.z, c.w);
-              mul2(z[i], z[i + 1], sign, sign);
-              mul2(z[i + 2], z[i + 3], sign, sign);
-              fma2v(y[i], y[i + 1], z[i], s.x, z[i + 1], s.y);
-              fma2v(y[i + 2], y[i + 3], z[i + 2], s.z, z[i + 3], s.w);
-            }
-          }
-        }
-      }
-      float amax = 0.f;
-      if (E4 && __any_sync(0xffffffffu, !is_q)) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) amax = fmaxf(amax, fabsf(y[i]));
-#pragma unroll
-        for (int o = L / 2; o > 0; o >>= 1)
-          amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
-      }
-      if (!live) continue;
-      if (is_q) {
-        *reinterpret_cast<uint4*>(static_cast<T*>(p.q_out) + tok * p.q_out_token +
-                                  h * p.q_out_head + lane * 8) = pack8<T>(y);
-        continue;
-      }
-      if (!cached) {
-        *reinterpret_cast<uint4*>(static_cast<T*>(p.k_out) + tok * p.k_out_token +
-                                  k0 * p.k_out_head + lane * 8) = pack8<T>(y);
-        continue;
-      }
-      if (slot < 0 || slot >= slots) continue;
-      const int page = (int)slot / p.cache.page_size, off = (int)slot - page * p.cache.page_size;
-      const long long row = ((long long)page * p.cache.kv_heads + (is_v ? v0 : k0)) * p.cache.page_size + off;
-      void* base = is_v ? p.cache.v : p.cache.k;
-      if (E4) {
-        const float s = amax > 0.f ? amax / kE4m3Max : 1.f;
-        const RowDiv div(s);
-        uint32_t w[4];
-        if (div.plain) {
-#pragma unroll
-          for (int i = 0; i < 4; ++i) w[i] = e4m3x2(y[2 * i] / s, y[2 * i + 1] / s);
-        } else {
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            div.two(y[2 * i], y[2 * i + 1]);
-            w[i] = e4m3x2(y[2 * i], y[2 * i + 1]);
-          }
-        }
-        *reinterpret_cast<uint2*>(static_cast<uint8_t*>(base) + row * D + lane * 8) =
-            make_uint2(w[0] | (w[1] << 16), w[2] | (w[3] << 16));
-        if (lane == 0) (is_v ? p.cache.v_scale : p.cache.k_scale)[row] = s;
-      } else {
-        *reinterpret_cast<uint4*>(static_cast<T*>(base) + row * D + lane * 8) = pack8<T>(y);
-      }
+    while (__any_sync(0xffffffffu, at.t < nt)) {
+      float y[8];
+      unpack8<T>(raw, y);
+      const At now = at;
+      at.advance(GROUPS, p.heads);
+      raw = fetch(p.q, at);
+      const bool live = now.t < nt;
+      turn(y, w, live ? now.t : 0);
+      if (live)
+        *reinterpret_cast<uint4*>(static_cast<T*>(p.q_out) + (long long)(t0 + now.t) * p.q_out_token +
+                                  now.h * p.q_out_head + lane * 8) = pack8<T>(y);
     }
+    unpack8<T>(*reinterpret_cast<const uint4*>(static_cast<const T*>(p.k_w) + lane * 8), w);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) w[i] += p.w_offset;
+  }
+  const bool cached = p.cache.k != nullptr;
+  const long long slots = (long long)p.cache.pages << p.page_shift;
+  At at{0, 0};
+  at.advance(grp, p.kv_heads);
+  auto fetch_slot = [&](At a) {
+    return cached && a.t < nt ? load_index(p.slots, p.slot_bytes, t0 + a.t) : -1;
+  };
+  uint4 raw_k = fetch(p.k, at), raw_v = make_uint4(0, 0, 0, 0);
+  if (cached) raw_v = fetch(p.v, at);
+  long long next_slot = fetch_slot(at);
+  while (__any_sync(0xffffffffu, at.t < nt)) {
+    float k[8], v[8];
+    unpack8<T>(raw_k, k);
+    unpack8<T>(raw_v, v);
+    const At now = at;
+    const long long slot = next_slot;
+    at.advance(GROUPS, p.kv_heads);
+    raw_k = fetch(p.k, at);
+    if (cached) raw_v = fetch(p.v, at);
+    next_slot = fetch_slot(at);
+    if (NORM) turn(k, w, now.t < nt ? now.t : 0);
+    if (!cached) {
+      if (now.t < nt)
+        *reinterpret_cast<uint4*>(static_cast<T*>(p.k_out) + (long long)(t0 + now.t) * p.k_out_token +
+                                  now.h * p.k_out_head + lane * 8) = pack8<T>(k);
+      continue;
+    }
+    const bool live = slot >= 0 && slot < slots;
+    const long long row = (((slot >> p.page_shift) * p.cache.kv_heads + now.h) << p.page_shift) + (slot & (p.cache.page_size - 1));
+    put_row<T, D, E4>(p.cache.k, p.cache.k_scale, row, lane, k, live);
+    put_row<T, D, E4>(p.cache.v, p.cache.v_scale, row, lane, v, live);
   }
 }
 
 struct ReadParams {
   const void* slots;
-  int slot_bytes, tokens;
+  int slot_bytes, tokens, page_shift;
   void *k_out, *v_out;    // [tokens][kv_heads][D], contiguous
   d3_kv_cache cache;
 };
 
-constexpr int kReadRows = 4;   // rows a lane group has in flight
+constexpr int kReadRows = 2;   // rows a lane group has in flight
 
 // Rows of the cache back in 16 bits: T(code * s), or the row as it is.  A lane
 // takes 16 bytes of a row.
@@ -315,8 +314,8 @@ __global__ void __launch_bounds__(256) kv_read_kernel(const __grid_constant__ Re
     raw[i] = make_uint4(0, 0, 0, 0);
     sc[i] = 0.f;
     if (!have[i]) continue;
-    const int page = (int)slot[i] / p.cache.page_size, off = (int)slot[i] - page * p.cache.page_size;
-    const long long row = ((long long)page * p.cache.kv_heads + (h2[i] >> 1)) * p.cache.page_size + off;
+    const int page = (int)slot[i] >> p.page_shift, off = (int)slot[i] & (p.cache.page_size - 1);
+    const long long row = (((long long)page * p.cache.kv_heads + (h2[i] >> 1)) << p.page_shift) + off;
     const bool v = h2[i] & 1;
     raw[i] = __ldcg(reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(v ? p.cache.v : p.cache.k) +
                                                    row * (D * (E4 ? 1 : 2)) + lane * 16));
@@ -356,7 +355,8 @@ static void (*fill_kernel(bool norm, bool e4))(FillParams) {
 }
 
 template <typename T>
-static int launch_fill(const FillParams& p, int D, bool norm, cudaStream_t st) {
+static int launch_fill(FillParams p, int D, bool norm, cudaStream_t st) {
+  if (p.cache.k) p.page_shift = __builtin_ctz((unsigned)p.cache.page_size);
   const dim3 grid((unsigned)((p.tokens + p.tokens_per_cta - 1) / p.tokens_per_cta));
   const bool e4 = p.cache.dtype == D3_E4M3;
   void (*k)(FillParams) = D == 128 ? fill_kernel<T, 128>(norm, e4) : fill_kernel<T, 256>(norm, e4);
@@ -417,7 +417,7 @@ int d3_kv_read(const d3_kv_cache* cache, const void* slots, int32_t slot_bytes, 
   D3_CHECK_ARG(slots && k_out && v_out, "d3_kv_read: null pointer");
   if (!aligned16(k_out) || !aligned16(v_out))
     return fail(D3_ERR_MISALIGNED, "d3_kv_read: outputs not 16-byte aligned");
-  ReadParams p{slots, slot_bytes, tokens, k_out, v_out, *cache};
+  ReadParams p{slots, slot_bytes, tokens, __builtin_ctz((unsigned)cache->page_size), k_out, v_out, *cache};
   const int D = cache->head_dim, lanes = D / (cache->dtype == D3_E4M3 ? 16 : 8);
   const long long rows = 2LL * cache->kv_heads * tokens, per = 256 / lanes * kReadRows;
   if (rows >= (1LL << 31)) return fail(D3_ERR_TOO_LARGE, "d3_kv_read: too many rows");
