@@ -27,25 +27,16 @@ static int make_map(CUtensorMap* m, const void* base, int dtype, int rank, const
   return D3_OK;
 }
 
-// A cache buffer as rows [pages * kv_heads * page_size][D].
-static int make_rows_map(CUtensorMap* m, const void* base, const d3_kv_cache* c, uint32_t box_rows) {
-  const uint64_t es = c->dtype == D3_E4M3 ? 1 : 2;
-  const uint64_t dims[2] = {(uint64_t)c->head_dim, (uint64_t)c->pages * c->kv_heads * c->page_size};
-  const uint64_t strides[1] = {c->head_dim * es};
-  const uint32_t box[2] = {(uint32_t)(128 / es), box_rows};
-  return make_map(m, base, c->dtype, 2, dims, strides, box);
-}
 // A cache buffer as planes [pages * kv_heads][page_size][D], the dims in
-// columns: 64 of 16 bits, swizzled, or one of all codes.  Rows before or
-// behind a page are outside the map.
-static int make_pages_map(CUtensorMap* m, const void* base, const d3_kv_cache* c, uint32_t box_dims,
+// columns of 128 bytes, swizzled -- or, for codes that are to be widened, in
+// one, unswizzled.  Rows before or behind a page are outside the map.
+static int make_pages_map(CUtensorMap* m, const void* base, const d3_kv_cache* c, bool swizzle, uint32_t box_dims,
                           uint32_t box_rows, uint32_t box_cols) {
-  const bool e4 = c->dtype == D3_E4M3;
-  const uint64_t D = c->head_dim, es = e4 ? 1 : 2, col = e4 ? D : 64;
+  const uint64_t D = c->head_dim, es = c->dtype == D3_E4M3 ? 1 : 2, col = swizzle ? 128 / es : D;
   const uint64_t dims[4] = {col, (uint64_t)c->page_size, D / col, (uint64_t)c->pages * c->kv_heads};
   const uint64_t strides[3] = {D * es, col * es, c->page_size * D * es};
   const uint32_t box[4] = {box_dims, box_rows, box_cols, 1};
-  return make_map(m, base, c->dtype, 4, dims, strides, box, !e4);
+  return make_map(m, base, c->dtype, 4, dims, strides, box, swizzle);
 }
 
 static int check_attention(const d3_attention* a, const d3_kv_cache* c) {
@@ -120,8 +111,8 @@ static int launch_rows(AttnParams p, const d3_attention* a, const d3_kv_cache* c
   if ((rc = set_smem(attn_rows_kernel<T, D, E4, NT>, C::SMEM, done))) return rc;
   const uint32_t box = c->page_size < C::KEYS ? c->page_size : C::KEYS;
   CUtensorMap tk, tv;
-  if ((rc = make_rows_map(&tk, c->k, c, box))) return rc;
-  if ((rc = make_rows_map(&tv, c->v, c, box))) return rc;
+  if ((rc = make_pages_map(&tk, c->k, c, true, 128 / C::ES, box, C::COLS))) return rc;
+  if ((rc = make_pages_map(&tv, c->v, c, true, 128 / C::ES, box, C::COLS))) return rc;
   const long long groups = ((long long)a->max_q * p.group + C::ROWS - 1) / C::ROWS;
   const long long tiles = ((long long)a->max_kv + C::KEYS - 1) / C::KEYS;
   const long long most = (tiles < 1 ? 1 : tiles) * groups * a->batch * c->kv_heads;
@@ -149,8 +140,8 @@ static int launch_chunk(const AttnParams& p, const d3_attention* a, const d3_kv_
   const uint32_t box[3] = {64, (uint32_t)p.group, (uint32_t)tpc};
   if ((rc = make_map(&tq, a->q, a->dtype, 3, dims, strides, box))) return rc;
   const uint32_t krows = c->page_size < 64 ? c->page_size : 64;
-  if ((rc = make_pages_map(&tk, c->k, c, E4 ? D : 64, krows, !E4 && krows == 64 ? D / 64 : 1))) return rc;
-  if ((rc = make_pages_map(&tv, c->v, c, E4 ? D / 2 : 64, c->page_size, E4 ? 1 : D / 128))) return rc;
+  if ((rc = make_pages_map(&tk, c->k, c, !E4, E4 ? D : 64, krows, !E4 && krows == 64 ? D / 64 : 1))) return rc;
+  if ((rc = make_pages_map(&tv, c->v, c, !E4, E4 ? D / 2 : 64, c->page_size, E4 ? 1 : D / 128))) return rc;
   // row tiles at most: every sequence may have one that is not full
   const long long tiles = a->tokens / (2 * tpc) + a->batch;
   const long long blocks = ((long long)a->max_kv + kBlockKeys - 1) / kBlockKeys;

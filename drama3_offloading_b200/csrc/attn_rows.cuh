@@ -14,8 +14,8 @@
 // it takes over above 16 rows, attn_chunk.cuh.)  P^T goes from the accumulator
 // layout to the operand layout with one movmatrix per 8 x 8 block.
 //
-// Streaming: one warp issues TMA loads (128-byte swizzle) of KEYS-key tiles of
-// K and V into a ring of 32 KiB slots; each of the other warps takes 16 keys
+// Streaming: four threads issue TMA loads (128-byte swizzle) of KEYS-key tiles of
+// K and V into a ring of 32 KiB slots; each of eight (or four) warps takes 16 keys
 // of every tile with a running maximum and sum of its own, so no barrier runs
 // inside the stream; the warps' results are joined once a segment.
 //
@@ -93,20 +93,20 @@ struct RowsCfg {
   static constexpr int ES = E4 ? 1 : 2;                     // bytes of a cached element
   static constexpr int WARPS = (D == 256 && !E4) ? 4 : 8;   // consumer warps
   static constexpr int KEYS = 16 * WARPS;
-  static constexpr int THREADS = 32 * (WARPS + 1);
+  static constexpr int LOADERS = 4;                         // loading warps, one thread each
+  static constexpr int THREADS = 32 * (WARPS + LOADERS);
   static constexpr int COLS = D * ES / 128;                 // 128-byte columns of a row
   static constexpr int ROWS = 8 * NT;
   static constexpr int SLOT = KEYS * D * ES;                // 32 KiB, 16 KiB for D = 128 codes
-  static constexpr int SCALES = E4 ? KEYS * 4 : 0;
   static constexpr int QFRAG = NT * D * 16;
   // warps' results are joined DC dims at a time through 32 KiB
   static constexpr int DC = (32 * 1024) / (WARPS * ROWS * 4) < D ? (32 * 1024) / (WARPS * ROWS * 4) : D;
   static constexpr int JOIN_PITCH = DC + 4;
   static constexpr int JOIN = WARPS * ROWS * JOIN_PITCH * 4;
-  static constexpr int SLOTS = (222 * 1024 - QFRAG - JOIN) / (SLOT + SCALES) < 10
-                                   ? (222 * 1024 - QFRAG - JOIN) / (SLOT + SCALES) : 10;
+  static constexpr int SLOTS = (222 * 1024 - QFRAG - JOIN) / SLOT < 10
+                                   ? (222 * 1024 - QFRAG - JOIN) / SLOT : 10;
   static constexpr int ML = WARPS * ROWS * 2 * 4;
-  static constexpr size_t SMEM = 1024 + (size_t)SLOTS * (SLOT + SCALES) + QFRAG + JOIN + ML + 4 * ROWS + 256;
+  static constexpr size_t SMEM = 1024 + (size_t)SLOTS * SLOT + QFRAG + JOIN + ML + 4 * ROWS + 256;
   static_assert(SLOTS >= 4, "the ring needs two tiles in flight");
 };
 
@@ -240,15 +240,17 @@ __device__ __forceinline__ void mma16<__half>(float (&c)[4], uint32_t a0, uint32
                : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-// 16-byte piece x (of 8 a 128-byte column) of a key's row in a swizzled tile
-// of `keys` rows per column
-__device__ __forceinline__ uint32_t tile_piece(uint32_t base, int keys, int key, int piece) {
-  return base + (uint32_t)(piece >> 3) * (keys * 128) + key * 128 + (((piece ^ key) & 7) << 4);
+// 16-byte piece (of 8 a 128-byte column) of row `key` of a swizzled box whose
+// columns are `col` bytes apart
+__device__ __forceinline__ uint32_t tile_piece(uint32_t base, uint32_t col, int key, int piece) {
+  return base + (uint32_t)(piece >> 3) * col + key * 128 + (((piece ^ key) & 7) << 4);
 }
-
-__device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
-  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
-               ::"r"(smem_u32(dst)), "l"(src), "r"(bytes), "r"(smem_u32(bar)) : "memory");
+__device__ __forceinline__ void tma_load_4d(uint32_t dst, const void* map, uint32_t bar, int x, int y, int z, int u) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(x),
+      "r"(y), "r"(z), "r"(u)
+      : "memory");
 }
 
 __device__ __forceinline__ float ex2(float x) {
@@ -267,8 +269,7 @@ __global__ void __launch_bounds__(RowsCfg<T, D, E4, NT>::THREADS, 1)
   __shared__ long long s_scan[33];
   uint8_t* smem = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
   uint8_t* s_slots = smem;
-  float* s_scales = reinterpret_cast<float*>(smem + (size_t)C::SLOTS * C::SLOT);   // [SLOTS][KEYS]
-  uint2* s_q = reinterpret_cast<uint2*>(smem + (size_t)C::SLOTS * (C::SLOT + C::SCALES));
+  uint2* s_q = reinterpret_cast<uint2*>(smem + (size_t)C::SLOTS * C::SLOT);
   float* s_join = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(s_q) + C::QFRAG);
   float* s_ml = s_join + C::JOIN / 4;                          // [WARPS][ROWS][2]
   float* s_qs = s_ml + C::ML / 4;                              // [ROWS] scale of a row's scores
@@ -297,69 +298,79 @@ __global__ void __launch_bounds__(RowsCfg<T, D, E4, NT>::THREADS, 1)
     return;
   }
   RowsWalk walk{work.b, work.count, work.off};
-  RowsPiece w;
-  if (warp == C::WARPS) {
-    // ---- the loading warp: K tile, V tile, K tile, ...
-    int slot = 0;
-    uint32_t phase = 0;
-    bool ok = true;
-    const int box = min(p.page_size, C::KEYS), boxes = C::KEYS / box;
-    while (walk.next(p, C::KEYS, C::ROWS, w)) {
-      for (int t = w.t0; t < w.t1; ++t) {
-        const int key0 = t * C::KEYS;
+  RowsPiece w{};
+  const int box = min(p.page_size, C::KEYS), boxes = C::KEYS / box;     // rows of a TMA box, boxes of a tile
+  if (warp >= C::WARPS) {
+    // ---- loading threads: K tile, V tile, K tile, ...  A box is a page's
+    // rows with all of their columns, so a tile is [boxes][columns][box rows]
+    // [128 bytes]; thread i takes boxes i, i + 4.  (A TMA instruction holds
+    // its thread for some 300 cycles whatever its size, so small pages need
+    // several threads.)  The page ids of the next tile are on their way while
+    // this one's boxes go out.
+    if (lane == 0) {
+      const int who = warp - C::WARPS;
+      constexpr int MINE = 8 / C::LOADERS;
+      int slot = 0;
+      uint32_t phase = 0;
+      bool ok = true;
+      int t = 0, ids[MINE];
+      auto fetch = [&]() {
+        const int* row = p.table + (long long)w.b * p.table_stride;
+#pragma unroll
+        for (int i = 0; i < MINE; ++i) {
+          const int key = t * C::KEYS + (who + i * C::LOADERS) * box;
+          ids[i] = who + i * C::LOADERS < boxes && key < w.s.kv ? __ldcg(row + (key >> p.page_shift)) : -1;
+        }
+      };
+      bool more = walk.next(p, C::KEYS, C::ROWS, w);
+      if (more) {
+        t = w.t0;
+        fetch();
+      }
+      while (more && ok) {
+        const int key0 = t * C::KEYS, head = w.head;
         // keys of this tile in whole boxes: what lies behind is never loaded
         const int need = min(boxes, (max(0, w.s.kv - key0) + box - 1) / box);
-        // lane i: page of box i (at most KEYS / 16 = 8 boxes)
-        int row = -1;
-        if (lane < need) {
-          const int key = key0 + lane * box;
-          const int page = __ldcg(p.table + (long long)w.b * p.table_stride + (key >> p.page_shift));
-          if (page >= 0 && page < p.pages)
-            row = ((page * p.kv_heads + w.head) << p.page_shift) + (key & (p.page_size - 1));
+        int plane[MINE];
+#pragma unroll
+        for (int i = 0; i < MINE; ++i)
+          plane[i] = ids[i] >= 0 && ids[i] < p.pages ? ids[i] * p.kv_heads + head : -1;
+        const int in_page = key0 & (p.page_size - 1);    // of the first box, where a page is larger than a tile
+        if (++t >= w.t1) {
+          more = walk.next(p, C::KEYS, C::ROWS, w);
+          if (more) t = w.t0;
         }
-        const int scales_ok = __popc(__ballot_sync(0xffffffffu, row >= 0));
+        if (more) fetch();
 #pragma unroll
         for (int kv = 0; kv < 2; ++kv) {
-          if (ok && !mbar_wait(empty + slot, phase ^ 1, kAttnWaitBudgetNs)) {
-            if (lane == 0) attn_error(p.err, kAttnErrRowsLoad);
+          if (!mbar_wait(empty + slot, phase ^ 1, kAttnWaitBudgetNs)) {
+            attn_error(p.err, kAttnErrRowsLoad);
             ok = false;
+            break;
           }
-          ok = __all_sync(0xffffffffu, ok);
-          if (!ok) break;
-          uint8_t* dst = s_slots + (size_t)slot * C::SLOT;
-          float* sdst = s_scales + slot * C::KEYS;
-          if (E4 && lane < need && row < 0)
-            for (int i = 0; i < box; ++i) sdst[lane * box + i] = 0.f;
-          __syncwarp();
-          if (lane == 0)
-            mbar_arrive_expect_tx(full + slot, need * box * D * C::ES + (E4 ? scales_ok * box * 4 : 0));
-          __syncwarp();
+          const uint32_t dst = smem_u32(s_slots + (size_t)slot * C::SLOT);
+          if (who == 0) mbar_arrive_expect_tx(full + slot, need * box * D * C::ES);
           // a page id outside the cache is loaded from outside the map: zeros
-          for (int i0 = 0; i0 < need * C::COLS; i0 += 32) {
-            const int i = i0 + lane, bx = i / C::COLS, col = i - bx * C::COLS;
-            const int r = __shfl_sync(0xffffffffu, row, bx);
-            if (bx < need)
-              tma_load_2d(dst + col * (C::KEYS * 128) + bx * box * 128, kv ? &tm_v : &tm_k, full + slot,
-                          col * (128 / C::ES), r < 0 ? -box : r);
-          }
-          __syncwarp();
-          if (E4 && lane < need && row >= 0)
-            bulk_load(sdst + lane * box, (kv ? p.v_scale : p.k_scale) + row, box * 4, full + slot);
+#pragma unroll
+          for (int i = 0; i < MINE; ++i)
+            if (who + i * C::LOADERS < need)
+              tma_load_4d(dst + (who + i * C::LOADERS) * box * (D * C::ES), kv ? &tm_v : &tm_k, smem_u32(full + slot),
+                          0, in_page, 0, plane[i]);
           if (++slot == C::SLOTS) { slot = 0; phase ^= 1; }
         }
-        if (!ok) break;
       }
-      if (!ok) break;
-    }
-    if (!ok) {
-      // what is still in flight has landed before the CTA's memory goes
-      for (int i = 0; i < C::SLOTS; ++i) mbar_wait(full + i, phase ^ (i < slot ? 0 : 1), kAttnWaitBudgetNs);
+      if (!ok) {
+        // what is still in flight has landed before the CTA's memory goes
+        for (int i = 0; i < C::SLOTS; ++i) mbar_wait(full + i, phase ^ (i < slot ? 0 : 1), kAttnWaitBudgetNs);
+      }
     }
     return;
   }
 
   // ---- the other warps: 16 keys of every tile
   const int g = lane >> 2, t4 = lane & 3;
+  // this warp's 16 keys of a tile lie in one box
+  const uint32_t col = box * 128, mine = warp * 16 / box * (box * D * C::ES) + warp * 16 % box * 128;
   int slot = 0;
   uint32_t phase = 0;
   bool ok = true;
@@ -439,12 +450,37 @@ __global__ void __launch_bounds__(RowsCfg<T, D, E4, NT>::THREADS, 1)
       }
     }
     const int lk = lane & 7, lm = lane >> 3;     // ldmatrix: row and matrix of this lane
+    // codes: the scales of keys g and g + 8 of this warp's 16, a tile ahead,
+    // and the page id they need two ahead
+    float ks_n[2] = {0.f, 0.f}, vs_n[2] = {0.f, 0.f};
+    int id_n = -1;
+    auto fetch_id = [&](int t) {
+      const int key = t * C::KEYS + warp * 16;
+      if (E4) id_n = t < w.t1 && key < w.s.kv ? __ldcg(p.table + (long long)w.b * p.table_stride + (key >> p.page_shift)) : -1;
+    };
+    auto fetch_scales = [&](int t) {
+      if (!E4) return;
+      const bool in = id_n >= 0 && id_n < p.pages;
+      const long long row = ((long long)(in ? id_n * p.kv_heads + w.head : 0) << p.page_shift) +
+                            ((t * C::KEYS + warp * 16) & (p.page_size - 1)) + g;
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        ks_n[i] = in ? __ldcg(p.k_scale + row + 8 * i) : 0.f;
+        vs_n[i] = in ? __ldcg(p.v_scale + row + 8 * i) : 0.f;
+      }
+    };
+    fetch_id(w.t0);
+    fetch_scales(w.t0);
+    fetch_id(w.t0 + 1);
     for (int t = w.t0; t < w.t1; ++t) {
       const int key0 = t * C::KEYS + warp * 16;  // this warp's keys
+      const float ks0 = E4 ? ks_n[0] : 1.f, ks1 = E4 ? ks_n[1] : 1.f;
+      float u0 = E4 ? vs_n[0] : 1.f, u1 = E4 ? vs_n[1] : 1.f;
+      fetch_scales(t + 1);
+      fetch_id(t + 2);
       take();
-      const uint32_t kb = smem_u32(s_slots + (size_t)slot * C::SLOT);
+      const uint32_t kb = smem_u32(s_slots + (size_t)slot * C::SLOT) + mine;
       float s[NT][4];
-      float ks0 = 1.f, ks1 = 1.f;
       if (ok && key0 < w.s.kv) {
         float s2[NT][2][4];
 #pragma unroll
@@ -457,7 +493,7 @@ __global__ void __launch_bounds__(RowsCfg<T, D, E4, NT>::THREADS, 1)
 #pragma unroll
           for (int kk = 0; kk < D / 16; kk += 2) {
             uint32_t r[4];
-            ldsm4(tile_piece(kb, C::KEYS, warp * 16 + (lm & 1) * 8 + lk, kk + (lm >> 1)), r);
+            ldsm4(tile_piece(kb, col, (lm & 1) * 8 + lk, kk + (lm >> 1)), r);
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
               const uint32_t a0 = e4m3x2_to_h2((uint16_t)r[2 * c]), a2 = e4m3x2_to_h2((uint16_t)(r[2 * c] >> 16));
@@ -469,13 +505,11 @@ __global__ void __launch_bounds__(RowsCfg<T, D, E4, NT>::THREADS, 1)
               }
             }
           }
-          ks0 = s_scales[slot * C::KEYS + warp * 16 + g];
-          ks1 = s_scales[slot * C::KEYS + warp * 16 + g + 8];
         } else {
 #pragma unroll
           for (int kk = 0; kk < D / 16; ++kk) {
             uint32_t r[4];
-            ldsm4(tile_piece(kb, C::KEYS, warp * 16 + (lm & 1) * 8 + lk, 2 * kk + (lm >> 1)), r);
+            ldsm4(tile_piece(kb, col, (lm & 1) * 8 + lk, 2 * kk + (lm >> 1)), r);
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
               const uint2 b = s_q[(n * (D / 16) + kk) * 32 + lane];
@@ -491,12 +525,12 @@ __global__ void __launch_bounds__(RowsCfg<T, D, E4, NT>::THREADS, 1)
       give();
       take();
       if (ok && key0 < w.s.kv) {
-        const uint32_t vb = smem_u32(s_slots + (size_t)slot * C::SLOT);
-        float u0 = 1.f, u1 = 1.f, vmax = 1.f;
+        const uint32_t vb = smem_u32(s_slots + (size_t)slot * C::SLOT) + mine;
+        float vmax = 1.f;
         if (E4) {
           // values' scales over the largest of the 16 keys'
-          u0 = key0 + g < w.s.kv ? s_scales[slot * C::KEYS + warp * 16 + g] : 0.f;
-          u1 = key0 + g + 8 < w.s.kv ? s_scales[slot * C::KEYS + warp * 16 + g + 8] : 0.f;
+          u0 = key0 + g < w.s.kv ? u0 : 0.f;
+          u1 = key0 + g + 8 < w.s.kv ? u1 : 0.f;
           vmax = fmaxf(u0, u1);
 #pragma unroll
           for (int x = 4; x < 32; x <<= 1) vmax = fmaxf(vmax, __shfl_xor_sync(0xffffffffu, vmax, x));
@@ -550,7 +584,7 @@ __global__ void __launch_bounds__(RowsCfg<T, D, E4, NT>::THREADS, 1)
 #pragma unroll
           for (int i = 0; i < D / 16; i += 2) {
             uint32_t r[4];
-            ldsm4t(tile_piece(vb, C::KEYS, warp * 16 + (lm & 1) * 8 + lk, i + (lm >> 1)), r);
+            ldsm4t(tile_piece(vb, col, (lm & 1) * 8 + lk, i + (lm >> 1)), r);
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
               const uint32_t x = __byte_perm(r[2 * c], 0, 0x3120), y = __byte_perm(r[2 * c + 1], 0, 0x3120);
@@ -569,7 +603,7 @@ __global__ void __launch_bounds__(RowsCfg<T, D, E4, NT>::THREADS, 1)
 #pragma unroll
           for (int i = 0; i < D / 16; ++i) {
             uint32_t r[4];
-            ldsm4t(tile_piece(vb, C::KEYS, warp * 16 + (lm >> 1) * 8 + lk, 2 * i + (lm & 1)), r);
+            ldsm4t(tile_piece(vb, col, (lm >> 1) * 8 + lk, 2 * i + (lm & 1)), r);
 #pragma unroll
             for (int n = 0; n < NT; ++n)
               mma16<M>(o[n][i], r[0] & cut0, r[1] & cut0, r[2] & cut1, r[3] & cut1, pb[n][0], pb[n][1]);

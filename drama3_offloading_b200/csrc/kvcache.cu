@@ -65,7 +65,7 @@ struct FillParams {
 
 constexpr int kFillThreads = 256;
 constexpr int kMaxHalf = 128;          // rotary pairs of the widest head
-constexpr int kMaxTokensPerCta = 4;
+constexpr int kMaxTokensPerCta = 8;
 
 // x / s rounded as the division is.  With r = 1 / s rounded and q = x r, the
 // remainder x - q s is exact in one fused step and q + rem r is the quotient
@@ -137,7 +137,7 @@ __device__ __forceinline__ void put_row(void* buf, float* scales, long long row,
 // value's norm) is not computed: the kernel is as much bound by its
 // instructions as by HBM.
 template <typename T, int D, bool NORM, bool E4>
-__global__ void __launch_bounds__(kFillThreads) kv_fill_kernel(const __grid_constant__ FillParams p) {
+__global__ void __launch_bounds__(kFillThreads, 5) kv_fill_kernel(const __grid_constant__ FillParams p) {
   constexpr int L = D / 8;                          // lanes of a row
   constexpr int GROUPS = kFillThreads / L;
   __shared__ __align__(16) float s_cos[kMaxTokensPerCta][kMaxHalf], s_sin[kMaxTokensPerCta][kMaxHalf];
@@ -343,10 +343,14 @@ __global__ void __launch_bounds__(256) kv_read_kernel(const __grid_constant__ Re
 
 // ---------------------------------------------------------------- host
 
-// Tokens a CTA takes: one for small batches (as many CTAs as tokens, so that
-// a decode batch spreads over the SMs), four once there are enough tokens for
-// every SM to hold several CTAs all the same.
-static int tokens_per_cta(int tokens) { return tokens >= 8 * num_sms() ? kMaxTokensPerCta : 1; }
+// Tokens a CTA takes: one for small batches, which so spread over the SMs;
+// four, then eight, once every SM still has several CTAs (8192 tokens of 20
+// rows of 256: 53 us with two, 46 with four; 50001 of 16 rows of 128: 64 us
+// with four, 60 with eight).
+static int tokens_per_cta(int tokens) {
+  const int n = num_sms();
+  return tokens >= 64 * n ? 8 : tokens >= 8 * n ? 4 : 1;
+}
 
 template <typename T, int D>
 static void (*fill_kernel(bool norm, bool e4))(FillParams) {
