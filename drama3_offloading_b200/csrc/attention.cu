@@ -170,14 +170,15 @@ static int launch_attention(AttnParams p, const d3_attention* a, const d3_kv_cac
   if (rows <= 8) return launch_rows<T, D, E4, 1>(p, a, c, st);
   if (rows <= kRowsMost) return launch_rows<T, D, E4, 2>(p, a, c, st);
   if ((long long)a->batch * a->max_q != a->tokens && p.group <= kRowsMost) {
+    // mostly single tokens among chunks: eight rows where a token has no more
+    // (sixteen cost the row kernel twice the products)
     AttnParams few = p;
-    few.max_rows = kRowsMost;
+    few.max_rows = p.group <= 8 ? 8 : kRowsMost;
     d3_attention one = *a;
-    one.max_q = kRowsMost / p.group;
-    if ((rc = p.group <= 8 && one.max_q == 1 ? launch_rows<T, D, E4, 1>(few, &one, c, st)
-                                             : launch_rows<T, D, E4, 2>(few, &one, c, st)))
+    one.max_q = few.max_rows / p.group;
+    if ((rc = few.max_rows == 8 ? launch_rows<T, D, E4, 1>(few, &one, c, st) : launch_rows<T, D, E4, 2>(few, &one, c, st)))
       return rc;
-    p.min_rows = kRowsMost + 1;
+    p.min_rows = few.max_rows + 1;
   }
   return launch_chunk<T, D, E4>(p, a, c, ws, st);
 }

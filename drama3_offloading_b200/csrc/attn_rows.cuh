@@ -29,8 +29,9 @@
 // e4m3 caches: codes are exact in fp16, so the products run in fp16 whatever
 // the queries' type.  bf16 queries are scaled by a power of two per row (exact
 // but for elements 2^-24 below the row's largest); a key's scale multiplies
-// its scores in fp32; a value's scale, over the largest of the warp's 16 keys,
-// multiplies the probability before it is rounded to fp16.
+// its scores in fp32; a value's scale, in units of a power of two not below any
+// scale the warp has met, multiplies the probability before it is rounded to
+// fp16.
 #pragma once
 
 #include "kv_common.cuh"
@@ -431,6 +432,15 @@ __global__ void __launch_bounds__(RowsCfg<T, D, E4, NT>::THREADS, 1)
       }
     }
     bar();
+    // queries' operand, from shared memory each time where registers are short
+    constexpr bool QREG = NT == 1 && !(E4 && D == 256);
+    uint2 qr[QREG ? D / 16 : 1];
+    if (QREG) {
+#pragma unroll
+      for (int i = 0; i < D / 16; ++i) qr[QREG ? i : 0] = s_q[i * 32 + lane];
+    }
+    auto qop = [&](int n, int kk) { return QREG ? qr[QREG ? kk : 0] : s_q[(n * (D / 16) + kk) * 32 + lane]; };
+    float vref = 0.f;    // codes: the sums are in units of this power of two
     float o[NT][D / 16][4];
     float mx[NT][2], sum[NT][2], cs[NT][2];
     int last[NT][2];     // last key a row sees
@@ -500,7 +510,7 @@ __global__ void __launch_bounds__(RowsCfg<T, D, E4, NT>::THREADS, 1)
               const uint32_t a1 = e4m3x2_to_h2((uint16_t)r[2 * c + 1]), a3 = e4m3x2_to_h2((uint16_t)(r[2 * c + 1] >> 16));
 #pragma unroll
               for (int n = 0; n < NT; ++n) {
-                const uint2 b = s_q[(n * (D / 16) + kk + c) * 32 + lane];
+                const uint2 b = qop(n, kk + c);
                 mma16<M>(s2[n][c], a0, a1, a2, a3, b.x, b.y);
               }
             }
@@ -512,7 +522,7 @@ __global__ void __launch_bounds__(RowsCfg<T, D, E4, NT>::THREADS, 1)
             ldsm4(tile_piece(kb, col, (lm & 1) * 8 + lk, 2 * kk + (lm >> 1)), r);
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
-              const uint2 b = s_q[(n * (D / 16) + kk) * 32 + lane];
+              const uint2 b = qop(n, kk);
               mma16<M>(s2[n][kk & 1], r[0], r[1], r[2], r[3], b.x, b.y);
             }
           }
@@ -526,15 +536,25 @@ __global__ void __launch_bounds__(RowsCfg<T, D, E4, NT>::THREADS, 1)
       take();
       if (ok && key0 < w.s.kv) {
         const uint32_t vb = smem_u32(s_slots + (size_t)slot * C::SLOT) + mine;
-        float vmax = 1.f;
         if (E4) {
-          // values' scales over the largest of the 16 keys'
+          // values' scales in units of vref, a power of two not below any yet
           u0 = key0 + g < w.s.kv ? u0 : 0.f;
           u1 = key0 + g + 8 < w.s.kv ? u1 : 0.f;
-          vmax = fmaxf(u0, u1);
+          float vmax = fmaxf(u0, u1);
 #pragma unroll
           for (int x = 4; x < 32; x <<= 1) vmax = fmaxf(vmax, __shfl_xor_sync(0xffffffffu, vmax, x));
-          const float inv = vmax > 0.f ? 1.f / vmax : 0.f;
+          if (vmax > vref) {
+            const float up = __uint_as_float((__float_as_uint(vmax) + 0x7fffffu) & 0xff800000u);
+            const float f = vref / up;
+            vref = up;
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+              for (int i = 0; i < D / 16; ++i)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) o[n][i][j] *= f;
+          }
+          const float inv = vref > 0.f ? 1.f / vref : 0.f;
           u0 *= inv;
           u1 *= inv;
         }
@@ -569,46 +589,46 @@ __global__ void __launch_bounds__(RowsCfg<T, D, E4, NT>::THREADS, 1)
           pb[n][0] = movm(Elem<M>::from_f2(pr[0], pr[1]));
           pb[n][1] = movm(Elem<M>::from_f2(pr[2], pr[3]));
         }
-        // values of keys behind the sequence's end are whatever the page
-        // held: cut to zero, 0 * NaN is no zero
-        const bool tail = key0 + 16 > w.s.kv;
-        uint32_t cut0 = ~0u, cut1 = ~0u;
-        if (tail) {
-          const int k2 = key0 + 2 * t4;
-          cut0 = (k2 < w.s.kv ? 0xffffu : 0u) | (k2 + 1 < w.s.kv ? 0xffff0000u : 0u);
-          cut1 = (k2 + 8 < w.s.kv ? 0xffffu : 0u) | (k2 + 9 < w.s.kv ? 0xffff0000u : 0u);
-        }
-        if (E4) {
-          // one 8 x 8 block of code pairs holds 16 dims: dim 2g in the even
-          // bytes, 2g + 1 in the odd ones
+        auto products = [&](auto is_tail) {
+          // values of keys behind the sequence's end are whatever the page
+          // held: cut to zero, 0 * NaN is no zero
+          constexpr bool tail = decltype(is_tail)::value;
+          uint32_t cut0 = ~0u, cut1 = ~0u;
+          if (tail) {
+            const int k2 = key0 + 2 * t4;
+            cut0 = (k2 < w.s.kv ? 0xffffu : 0u) | (k2 + 1 < w.s.kv ? 0xffff0000u : 0u);
+            cut1 = (k2 + 8 < w.s.kv ? 0xffffu : 0u) | (k2 + 9 < w.s.kv ? 0xffff0000u : 0u);
+          }
+          if (E4) {
+            // one 8 x 8 block of code pairs holds 16 dims: dim 2g in the even
+            // bytes, 2g + 1 in the odd ones
 #pragma unroll
-          for (int i = 0; i < D / 16; i += 2) {
-            uint32_t r[4];
-            ldsm4t(tile_piece(vb, col, (lm & 1) * 8 + lk, i + (lm >> 1)), r);
+            for (int i = 0; i < D / 16; i += 2) {
+              uint32_t r[4];
+              ldsm4t(tile_piece(vb, col, (lm & 1) * 8 + lk, i + (lm >> 1)), r);
 #pragma unroll
-            for (int c = 0; c < 2; ++c) {
-              const uint32_t x = __byte_perm(r[2 * c], 0, 0x3120), y = __byte_perm(r[2 * c + 1], 0, 0x3120);
-              const uint32_t a0 = e4m3x2_to_h2((uint16_t)x) & cut0, a1 = e4m3x2_to_h2((uint16_t)(x >> 16)) & cut0;
-              const uint32_t a2 = e4m3x2_to_h2((uint16_t)y) & cut1, a3 = e4m3x2_to_h2((uint16_t)(y >> 16)) & cut1;
+              for (int c = 0; c < 2; ++c) {
+                const uint32_t x = __byte_perm(r[2 * c], 0, 0x3120), y = __byte_perm(r[2 * c + 1], 0, 0x3120);
+                uint32_t a0 = e4m3x2_to_h2((uint16_t)x), a1 = e4m3x2_to_h2((uint16_t)(x >> 16));
+                uint32_t a2 = e4m3x2_to_h2((uint16_t)y), a3 = e4m3x2_to_h2((uint16_t)(y >> 16));
+                if (tail) { a0 &= cut0; a1 &= cut0; a2 &= cut1; a3 &= cut1; }
 #pragma unroll
-              for (int n = 0; n < NT; ++n) {
-                float z[4] = {0.f, 0.f, 0.f, 0.f};
-                mma16<M>(z, a0, a1, a2, a3, pb[n][0], pb[n][1]);
-#pragma unroll
-                for (int j = 0; j < 4; ++j) o[n][i + c][j] = fmaf(z[j], vmax, o[n][i + c][j]);
+                for (int n = 0; n < NT; ++n) mma16<M>(o[n][i + c], a0, a1, a2, a3, pb[n][0], pb[n][1]);
               }
             }
-          }
-        } else {
+          } else {
 #pragma unroll
-          for (int i = 0; i < D / 16; ++i) {
-            uint32_t r[4];
-            ldsm4t(tile_piece(vb, col, (lm >> 1) * 8 + lk, 2 * i + (lm & 1)), r);
+            for (int i = 0; i < D / 16; ++i) {
+              uint32_t r[4];
+              ldsm4t(tile_piece(vb, col, (lm >> 1) * 8 + lk, 2 * i + (lm & 1)), r);
+              if (tail) { r[0] &= cut0; r[1] &= cut0; r[2] &= cut1; r[3] &= cut1; }
 #pragma unroll
-            for (int n = 0; n < NT; ++n)
-              mma16<M>(o[n][i], r[0] & cut0, r[1] & cut0, r[2] & cut1, r[3] & cut1, pb[n][0], pb[n][1]);
+              for (int n = 0; n < NT; ++n) mma16<M>(o[n][i], r[0], r[1], r[2], r[3], pb[n][0], pb[n][1]);
+            }
           }
-        }
+        };
+        if (key0 + 16 > w.s.kv) products(std::true_type{});
+        else products(std::false_type{});
       }
       give();
     }
@@ -649,6 +669,7 @@ __global__ void __launch_bounds__(RowsCfg<T, D, E4, NT>::THREADS, 1)
           if (mw != -INFINITY) l += s_ml[(x * C::ROWS + r) * 2 + 1] * ex2(mw - m);
         }
         f[n][j] = mx[n][j] == -INFINITY ? 0.f : ex2(mx[n][j] - m);
+        if (E4) f[n][j] *= vref;
         if (whole) f[n][j] = l > 0.f ? f[n][j] / l : 0.f;
         else if (warp == 0 && g == 0) {
           p.ws_ml[(place * C::ROWS + r) * 2] = m;
