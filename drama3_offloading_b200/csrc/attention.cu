@@ -115,6 +115,10 @@ static int launch_rows(AttnParams p, const d3_attention* a, const d3_kv_cache* c
   if ((rc = make_pages_map(&tv, c->v, c, true, 128 / C::ES, box, C::COLS))) return rc;
   const long long groups = ((long long)a->max_q * p.group + C::ROWS - 1) / C::ROWS;
   const long long tiles = ((long long)a->max_kv + C::KEYS - 1) / C::KEYS;
+  // the kernel counts the list in 31 bits; what it reads may be larger than max_q and max_kv say
+  if (((long long)a->tokens * p.group / C::ROWS + a->batch) * c->kv_heads *
+          ((long long)a->table_pages * c->page_size / C::KEYS + 1 + kPieceUnits) >= (1LL << 31))
+    return fail(D3_ERR_TOO_LARGE, "d3_paged_attention: too many key tiles");
   const long long most = (tiles < 1 ? 1 : tiles) * groups * a->batch * c->kv_heads;
   const int parts = (int)(most < num_sms() ? most : num_sms());
   D3_CUDA_TRY(launch_k(attn_rows_kernel<T, D, E4, NT>, dim3(parts), dim3(C::THREADS), C::SMEM, st,

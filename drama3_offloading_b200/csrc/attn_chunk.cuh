@@ -137,10 +137,9 @@ __device__ ChunkPart chunk_plan(const AttnParams& p, int per, int part, int part
     before += w < warp ? s_scan[w] : 0;
     total += s_scan[w];
   }
-  // part c of g: [total * c / g, total * (c + 1) / g), in 32 bits
-  const int g = min(parts, total), q = g ? total / g : 0, rem = g ? total - q * g : 0;
-  const int begin = part < g ? q * part + rem * part / g : 0;
-  const int count = part < g ? q * (part + 1) + rem * (part + 1) / g - begin : 0;
+  const int g = min(parts, total);
+  const int begin = part < g ? part_begin(total, g, part) : 0;
+  const int count = part < g ? part_begin(total, g, part + 1) - begin : 0;
   if (count > 0 && before <= begin && begin < before + sum) {
     int at = before;
     each([&](int b, const AttnSeq& s) {
@@ -843,7 +842,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(ChunkCfg<T, D, E4>::
         if (w.j0 == 0 && tid == 0) {
           // the part that holds the tile's last block
           const long long u = (long long)part.begin + part.count + (w.nb - w.j1) - 1;
-          desc = make_int4(w.b, w.head, w.tile, (int)(((u + 1) * min(pairs, part.total) - 1) / part.total));
+          desc = make_int4(w.b, w.head, w.tile, part_of(part.total, min(pairs, part.total), u));
         }
       }
       const float inv = l > 0.f ? 1.f / l : 0.f;

@@ -92,7 +92,7 @@ __device__ __forceinline__ AttnSeq attn_seq(const AttnParams& p, int b) {
 template <typename T, int D, bool E4, int NT>
 struct RowsCfg {
   static constexpr int ES = E4 ? 1 : 2;                     // bytes of a cached element
-  static constexpr int WARPS = (D == 256 && !E4) ? 4 : 8;   // consumer warps
+  static constexpr int WARPS = (D == 256 && (!E4 || NT == 2)) ? 4 : 8;   // consumer warps: registers for D = 256
   static constexpr int KEYS = 16 * WARPS;
   static constexpr int LOADERS = 4;                         // loading warps, one thread each
   static constexpr int THREADS = 32 * (WARPS + LOADERS);
@@ -111,55 +111,65 @@ struct RowsCfg {
   static_assert(SLOTS >= 4, "the ring needs two tiles in flight");
 };
 
-// where a launch's part begins, and how the pairs lie in the list
+// A part of the list: where it begins and how long it is.  Every pair stands
+// in the list with its tiles and kPieceUnits more in front of them, about what
+// a piece costs besides (queries in, results joined and out), so that parts of
+// many short pairs are as long as those of one.
+constexpr int kPieceUnits = 1;
 struct RowsWork {
-  long long total, begin;
-  int count, b;
-  long long off;                 // of `begin` inside sequence b
+  int total, begin, count;
+  int b, off;                    // sequence of `begin`, and its place inside it
 };
 
 __device__ __forceinline__ int rows_tiles(int kv, int keys) { return max(1, (kv + keys - 1) / keys); }
 
-// tiles of sequence b over all of its KV heads and row groups
-__device__ __forceinline__ long long rows_units(const AttnParams& p, int b, int keys, int rows_per) {
+// units of sequence b over all of its KV heads and row groups.  The host has
+// checked that the list is shorter than 2^31.
+__device__ __forceinline__ int rows_units(const AttnParams& p, int b, int keys, int rows_per) {
   const AttnSeq s = attn_seq(p, b);
   if (s.rows == 0 || s.rows < p.min_rows || s.rows > p.max_rows) return 0;
-  return (long long)rows_tiles(s.kv, keys) * p.kv_heads * ((s.rows + rows_per - 1) / rows_per);
+  return (rows_tiles(s.kv, keys) + kPieceUnits) * p.kv_heads * ((s.rows + rows_per - 1) / rows_per);
 }
+// where part c of g equal ones begins
+__device__ __forceinline__ int part_begin(int total, int g, int c) {
+  const int q = total / g;
+  return q * c + (total - q * g) * c / g;
+}
+// the part that holds unit u
+__device__ __forceinline__ int part_of(int total, int g, long long u) { return (int)(((u + 1) * g - 1) / total); }
 
-// All threads of the CTA: the list's length (units(b) of every sequence) and,
-// for the part that part(r) sets, the sequence it begins in.  s_scan: 33 long
-// longs of shared memory.
-template <typename U, typename F>
-__device__ RowsWork list_plan(const AttnParams& p, long long* s_scan, U units, F part) {
+// All threads of the CTA: part `part` of `parts`.  s_scan: 33 ints of shared memory.
+__device__ RowsWork rows_plan(const AttnParams& p, int keys, int rows_per, int part, int parts, int* s_scan) {
   const int n = blockDim.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int per = (p.batch + n - 1) / n;
   const int b0 = min(p.batch, tid * per), b1 = min(p.batch, b0 + per);
-  long long sum = 0;
-  for (int b = b0; b < b1; ++b) sum += units(b);
-  long long inc = sum;
+  int sum = 0;
+  for (int b = b0; b < b1; ++b) sum += rows_units(p, b, keys, rows_per);
+  int inc = sum;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const long long v = __shfl_up_sync(0xffffffffu, inc, o);
+    const int v = __shfl_up_sync(0xffffffffu, inc, o);
     if (lane >= o) inc += v;
   }
-  __shared__ int s_b;
-  __shared__ long long s_off;
+  __shared__ int s_b, s_off;
   if (lane == 31) s_scan[warp] = inc;
-  if (tid == 0) s_b = p.batch;
   __syncthreads();
-  long long before = inc - sum, total = 0;
+  int before = inc - sum, total = 0;
   for (int w = 0; w < n / 32; ++w) {
     if (w < warp) before += s_scan[w];
     total += s_scan[w];
   }
-  RowsWork r;
-  r.total = total;
-  part(r);
+  RowsWork r{total, 0, 0, 0, 0};
+  // no part is empty: a pair's parts are neighbours in the workspace
+  const int g = min(parts, total);
+  if (part < g) {
+    r.begin = part_begin(total, g, part);
+    r.count = part_begin(total, g, part + 1) - r.begin;
+  }
   if (r.count > 0 && before <= r.begin && r.begin < before + sum) {
-    long long at = before;
+    int at = before;
     for (int b = b0; b < b1; ++b) {
-      const long long u = units(b);
+      const int u = rows_units(p, b, keys, rows_per);
       if (r.begin < at + u) {
         s_b = b;
         s_off = r.begin - at;
@@ -181,26 +191,32 @@ struct RowsPiece {
 };
 // Walks a part of the list piece by piece.
 struct RowsWalk {
-  int b, left;
-  long long off;
+  int b, left, off;
+  int known;                     // the sequence that s holds
+  AttnSeq s;
+  __device__ __forceinline__ explicit RowsWalk(const RowsWork& r) : b(r.b), left(r.count), off(r.off), known(-1) {}
   __device__ __forceinline__ bool next(const AttnParams& p, int keys, int rows_per, RowsPiece& w) {
-    if (left <= 0) return false;
-    while (b < p.batch) {
-      w.s = attn_seq(p, b);
-      if (w.s.rows > 0 && w.s.rows >= p.min_rows && w.s.rows <= p.max_rows) {
-        w.nt = rows_tiles(w.s.kv, keys);
-        const int groups = (w.s.rows + rows_per - 1) / rows_per;
-        const long long units = (long long)w.nt * p.kv_heads * groups;
-        if (off < units) {
-          const int hg = (int)(off / w.nt);
+    while (left > 0 && b < p.batch) {
+      if (known != b) {
+        s = attn_seq(p, b);
+        known = b;
+      }
+      if (s.rows > 0 && s.rows >= p.min_rows && s.rows <= p.max_rows) {
+        const int nt = rows_tiles(s.kv, keys), len = nt + kPieceUnits;
+        const int groups = (s.rows + rows_per - 1) / rows_per;
+        if (off < len * p.kv_heads * groups) {
+          const int hg = off / len, pos = off - hg * len, take = min(left, len - pos);
+          left -= take;
+          off += take;
+          w.s = s;
           w.b = b;
+          w.nt = nt;
           w.head = hg / groups;
           w.rg = hg - w.head * groups;
-          w.t0 = (int)(off - (long long)hg * w.nt);
-          w.t1 = min(w.nt, w.t0 + left);
-          left -= w.t1 - w.t0;
-          off += w.t1 - w.t0;
-          return true;
+          w.t0 = max(0, pos - kPieceUnits);
+          w.t1 = max(0, pos + take - kPieceUnits);
+          if (w.t1 > w.t0) return true;
+          continue;              // nothing but the units in front
         }
       }
       ++b;
@@ -267,7 +283,7 @@ __global__ void __launch_bounds__(RowsCfg<T, D, E4, NT>::THREADS, 1)
   using C = RowsCfg<T, D, E4, NT>;
   using M = typename std::conditional<E4, __half, T>::type;   // operand type of the products
   extern __shared__ uint8_t smem_raw[];
-  __shared__ long long s_scan[33];
+  __shared__ int s_scan[33];
   uint8_t* smem = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
   uint8_t* s_slots = smem;
   uint2* s_q = reinterpret_cast<uint2*>(smem + (size_t)C::SLOTS * C::SLOT);
@@ -288,17 +304,12 @@ __global__ void __launch_bounds__(RowsCfg<T, D, E4, NT>::THREADS, 1)
   }
   pdl_trigger();
   pdl_wait();
-  const RowsWork work = list_plan(p, s_scan, [&](int b) { return rows_units(p, b, C::KEYS, C::ROWS); }, [&](RowsWork& r) {
-    // no part is empty: a pair's parts are neighbours in the workspace
-    const long long g = min((long long)gridDim.x, r.total), c = blockIdx.x;
-    r.begin = c < g ? r.total * c / g : 0;
-    r.count = c < g ? (int)(r.total * (c + 1) / g - r.begin) : 0;
-  });
+  const RowsWork work = rows_plan(p, C::KEYS, C::ROWS, blockIdx.x, gridDim.x, s_scan);
   if (work.count == 0) {
     if (tid == 0) p.ws_desc[blockIdx.x] = make_int4(0, 0, 0, -1);
     return;
   }
-  RowsWalk walk{work.b, work.count, work.off};
+  RowsWalk walk(work);
   RowsPiece w{};
   const int box = min(p.page_size, C::KEYS), boxes = C::KEYS / box;     // rows of a TMA box, boxes of a tile
   if (warp >= C::WARPS) {
@@ -377,11 +388,11 @@ __global__ void __launch_bounds__(RowsCfg<T, D, E4, NT>::THREADS, 1)
   bool ok = true;
   auto bar = [&]() { asm volatile("bar.sync 1, %0;" ::"r"(C::WARPS * 32) : "memory"); };
   auto take = [&]() {
-    if (ok && !mbar_wait(full + slot, phase, kAttnWaitBudgetNs)) {
-      if (lane == 0) attn_error(p.err, kAttnErrRowsUse);
-      ok = false;
+    if (ok && !__all_sync(0xffffffffu, mbar_try_wait(full + slot, phase))) {
+      const bool got = mbar_wait(full + slot, phase, kAttnWaitBudgetNs);
+      if (!got) attn_error(p.err, kAttnErrRowsUse);
+      ok = __all_sync(0xffffffffu, got);
     }
-    ok = __all_sync(0xffffffffu, ok);
   };
   auto give = [&]() {
     __syncwarp();
@@ -389,22 +400,39 @@ __global__ void __launch_bounds__(RowsCfg<T, D, E4, NT>::THREADS, 1)
     if (++slot == C::SLOTS) { slot = 0; phase ^= 1; }
   };
   int4 desc = make_int4(0, 0, 0, -1);
-  while (walk.next(p, C::KEYS, C::ROWS, w)) {
+  // a piece's queries are fetched while the one before runs: this warp's rows,
+  // 16 bytes a lane
+  constexpr int QROWS = (C::ROWS + C::WARPS - 1) / C::WARPS;
+  uint4 q_next[QROWS];
+  auto fetch_q = [&](const RowsPiece& x) {
+#pragma unroll
+    for (int k = 0; k < QROWS; ++k) {
+      const int r = warp + k * C::WARPS, gr = x.rg * C::ROWS + r;
+      q_next[k] = make_uint4(0, 0, 0, 0);
+      if (r < C::ROWS && gr < x.s.rows && lane < D / 8)
+        q_next[k] = __ldcg(reinterpret_cast<const uint4*>(
+            static_cast<const T*>(p.q) + (long long)(x.s.q0 + gr / p.group) * p.q_token +
+            (long long)(x.head * p.group + gr % p.group) * p.q_head + lane * 8));
+    }
+  };
+  RowsPiece ahead{};
+  bool more = walk.next(p, C::KEYS, C::ROWS, ahead);
+  if (more) fetch_q(ahead);
+  while (more) {
+    w = ahead;
     const int row0 = w.rg * C::ROWS, rows = min(C::ROWS, w.s.rows - row0);
     // queries in operand order: s_q[nt][kk][lane] holds the two registers of
     // B for k-step kk.  Codes come out of ldmatrix four dims to a lane, so
     // there the lane's k positions stand for dims 4t .. 4t + 3.
     bar();   // the piece before has read s_q and s_join
-    for (int r = warp; r < C::ROWS; r += C::WARPS) {
-      const int gr = row0 + r, tok = w.s.q0 + gr / p.group, hd = w.head * p.group + gr % p.group;
-      const T* src = static_cast<const T*>(p.q) + (long long)tok * p.q_token + (long long)hd * p.q_head;
-      // lane's share: 8 dims at a time, D / 8 chunks
-      float amax = 0.f;
-      uint4 u = make_uint4(0, 0, 0, 0);
-      if (r < rows && lane < D / 8) u = __ldcg(reinterpret_cast<const uint4*>(src + lane * 8));
+#pragma unroll
+    for (int k = 0; k < QROWS; ++k) {
+      const int r = warp + k * C::WARPS;
+      if (r >= C::ROWS) break;
+      const uint4 u = q_next[k];
       float x[8];
       unpack8<T>(u, x);
-      float mul = 1.f, back = 1.f;
+      float mul = 1.f, back = 1.f, amax = 0.f;
       if (E4 && std::is_same<T, __nv_bfloat16>::value) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) amax = fmaxf(amax, fabsf(x[i]));
@@ -432,6 +460,8 @@ __global__ void __launch_bounds__(RowsCfg<T, D, E4, NT>::THREADS, 1)
       }
     }
     bar();
+    more = walk.next(p, C::KEYS, C::ROWS, ahead);
+    if (more) fetch_q(ahead);
     // queries' operand, from shared memory each time where registers are short
     constexpr bool QREG = NT == 1 && !(E4 && D == 256);
     uint2 qr[QREG ? D / 16 : 1];
@@ -554,40 +584,52 @@ __global__ void __launch_bounds__(RowsCfg<T, D, E4, NT>::THREADS, 1)
 #pragma unroll
                 for (int j = 0; j < 4; ++j) o[n][i][j] *= f;
           }
-          const float inv = vref > 0.f ? 1.f / vref : 0.f;
+          // 1 / vref, a power of two as well, by its exponent
+          const float inv = vref > 0.f ? __uint_as_float(0x7f000000u - __float_as_uint(vref)) : 0.f;
           u0 *= inv;
           u1 *= inv;
         }
         uint32_t pb[NT][2];
+        float pr[NT][4], keep[NT][2], top[NT][2];
+        bool same = true;
 #pragma unroll
-        for (int n = 0; n < NT; ++n) {
-          float pr[4];
+        for (int n = 0; n < NT; ++n)
 #pragma unroll
           for (int j = 0; j < 2; ++j) {
-            const float a = key0 + g <= last[n][j] ? s[n][j] * (cs[n][j] * ks0) : -INFINITY;
-            const float b = key0 + g + 8 <= last[n][j] ? s[n][2 + j] * (cs[n][j] * ks1) : -INFINITY;
-            float m = fmaxf(a, b);
-#pragma unroll
-            for (int x = 4; x < 32; x <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, x));
-            m = fmaxf(m, mx[n][j]);
-            const float base = m == -INFINITY ? 0.f : m;
-            const float keep = ex2(mx[n][j] - base);
-            mx[n][j] = m;
-            const float pa = ex2(a - base), pc = ex2(b - base);
-            sum[n][j] = fmaf(sum[n][j], keep, pa + pc);
-            pr[j] = pa * u0;
-            pr[2 + j] = pc * u1;
-            if (keep != 1.f) {
-#pragma unroll
-              for (int i = 0; i < D / 16; ++i) {
-                o[n][i][j] *= keep;
-                o[n][i][2 + j] *= keep;
-              }
-            }
+            pr[n][j] = key0 + g <= last[n][j] ? s[n][j] * (cs[n][j] * ks0) : -INFINITY;
+            pr[n][2 + j] = key0 + g + 8 <= last[n][j] ? s[n][2 + j] * (cs[n][j] * ks1) : -INFINITY;
+            top[n][j] = fmaxf(pr[n][j], pr[n][2 + j]);
           }
-          __syncwarp();
-          pb[n][0] = movm(Elem<M>::from_f2(pr[0], pr[1]));
-          pb[n][1] = movm(Elem<M>::from_f2(pr[2], pr[3]));
+#pragma unroll
+        for (int x = 4; x < 32; x <<= 1)
+#pragma unroll
+          for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int j = 0; j < 2; ++j) top[n][j] = fmaxf(top[n][j], __shfl_xor_sync(0xffffffffu, top[n][j], x));
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            const float m = fmaxf(top[n][j], mx[n][j]);
+            const float base = m == -INFINITY ? 0.f : m;
+            keep[n][j] = ex2(mx[n][j] - base);
+            mx[n][j] = m;
+            const float pa = ex2(pr[n][j] - base), pc = ex2(pr[n][2 + j] - base);
+            sum[n][j] = fmaf(sum[n][j], keep[n][j], pa + pc);
+            pr[n][j] = pa * u0;
+            pr[n][2 + j] = pc * u1;
+            same = same && keep[n][j] == 1.f;
+          }
+          pb[n][0] = movm(Elem<M>::from_f2(pr[n][0], pr[n][1]));
+          pb[n][1] = movm(Elem<M>::from_f2(pr[n][2], pr[n][3]));
+        }
+        if (!__all_sync(0xffffffffu, same)) {
+#pragma unroll
+          for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int i = 0; i < D / 16; ++i)
+#pragma unroll
+              for (int j = 0; j < 4; ++j) o[n][i][j] *= keep[n][j & 1];
         }
         auto products = [&](auto is_tail) {
           // values of keys behind the sequence's end are whatever the page
@@ -652,8 +694,8 @@ __global__ void __launch_bounds__(RowsCfg<T, D, E4, NT>::THREADS, 1)
     float* wo = p.ws_o + (size_t)place * C::ROWS * D;
     if (!whole && w.t0 == 0) {
       // the part that holds the pair's last tile
-      const long long u = work.begin + work.count + (w.nt - w.t1) - 1, cut = min((long long)gridDim.x, work.total);
-      desc = make_int4(w.b, w.head, w.rg, (int)(((u + 1) * cut - 1) / work.total));
+      const long long u = (long long)work.begin + work.count + (w.nt - w.t1) - 1;
+      desc = make_int4(w.b, w.head, w.rg, part_of(work.total, min((int)gridDim.x, work.total), u));
     }
     float f[NT][2];    // this warp's factor of its rows
 #pragma unroll
