@@ -81,11 +81,11 @@ static Workspace plan_workspace(const d3_attention* a, const d3_kv_cache* c) {
   };
   w.rows_o = take(sms * 2 * kRowsMost * D * 4);
   w.rows_ml = take(sms * 2 * kRowsMost * 8);
-  w.rows_desc = take(sms * 16);
+  w.rows_desc = take(sms * 32);
   if ((long long)a->max_q * (a->heads / c->kv_heads) > kRowsMost) {
     w.chunk_o = take(pairs * 2 * 256 * D * 4);
     w.chunk_ml = take(pairs * 2 * 256 * 8);
-    w.chunk_desc = take(pairs * 16);
+    w.chunk_desc = take(pairs * 32);
   }
   w.total = at;
   return w;
@@ -157,7 +157,7 @@ static int launch_chunk(const AttnParams& p, const d3_attention* a, const d3_kv_
   D3_CUDA_TRY(launch_k(attn_chunk_kernel<T, D, E4>, dim3(2 * pairs), dim3(C::THREADS), C::SMEM, st, pdl_enabled(),
                        tq, tk, tv, p, ws),
               "attn_chunk_kernel launch");
-  D3_CUDA_TRY(launch_k(attn_chunk_join_kernel<T, D>, dim3(pairs, 8 * (D / 32)), dim3(256), 0, st, pdl_enabled(),
+  D3_CUDA_TRY(launch_k(attn_chunk_join_kernel<T, D>, dim3(pairs, 8), dim3(256), 0, st, pdl_enabled(),
                        p, ws),
               "attn_chunk_join_kernel launch");
   return D3_OK;

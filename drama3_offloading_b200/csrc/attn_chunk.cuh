@@ -73,7 +73,7 @@ struct ChunkCfg {
 struct ChunkWs {           // carved from the call's workspace
   float* o;                // [pairs][2][D / 4][256][4]
   float* ml;               // [pairs][2][256][2]
-  int4* desc;              // [pairs]: sequence, KV head, row tile, last part (-1: none)
+  int4* desc;              // [pairs][2]: (first query token, new tokens, KV head, row tile), (last part, or -1)
 };
 
 // key blocks that row tile i (of `per` tokens) of a sequence sees: at least one
@@ -718,7 +718,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(ChunkCfg<T, D, E4>::
     ChunkWalk walk(part);
     ChunkPiece w;
     uint32_t it = 0, pieces = 0;
-    int4 desc = make_int4(0, 0, 0, -1);
+    int4 desc = make_int4(0, 0, 0, 0);
+    int last_part = -1;
     const float c = p.scale_log2;
     while (walk.next(p, per, w)) {
       const int tok = w.tile * per + (int)rank * tpc + ti;       // of the sequence's new ones
@@ -842,7 +843,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(ChunkCfg<T, D, E4>::
         if (w.j0 == 0 && tid == 0) {
           // the part that holds the tile's last block
           const long long u = (long long)part.begin + part.count + (w.nb - w.j1) - 1;
-          desc = make_int4(w.b, w.head, w.tile, part_of(part.total, min(pairs, part.total), u));
+          desc = make_int4(w.s.q0, w.s.n, w.head, w.tile);
+          last_part = part_of(part.total, min(pairs, part.total), u);
         }
       }
       const float inv = l > 0.f ? 1.f / l : 0.f;
@@ -905,7 +907,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(ChunkCfg<T, D, E4>::
       __syncwarp();
       if (lane == 0) mbar_arrive_remote(mapa(smem_u32(o_free), 0));
     }
-    if (rank == 0 && tid == 0) ws.desc[pair] = desc;
+    if (rank == 0 && tid == 0) {
+      ws.desc[2 * pair] = desc;
+      ws.desc[2 * pair + 1] = make_int4(last_part, 0, 0, 0);
+    }
   } else if (E4 && warp == 11) {
     // ---- scales: lane has columns lane + 32 i of every block, in the order
     // of the loaded rows; the next block's are on their way while one is stored
@@ -1026,45 +1031,53 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(ChunkCfg<T, D, E4>::
 }
 
 // Tiles that the parts' cuts go through: the sum of their parts, in order.
-// blockIdx.x is the part in which the tile begins; a block takes 32 rows and 32
-// dims, eight threads a row.
+// blockIdx.x is the part in which the tile begins; a block takes 32 rows, eight
+// threads a row, each 4 dims of every 32.
 template <typename T, int D>
 __global__ void __launch_bounds__(256) attn_chunk_join_kernel(const __grid_constant__ AttnParams p, const ChunkWs ws) {
   pdl_trigger();
   pdl_wait();
   const int c0 = blockIdx.x;
-  const int4 de = __ldcg(ws.desc + c0);
-  if (de.w < 0) return;
-  const int b = de.x, head = de.y, tile = de.z, c1 = de.w;
-  const AttnSeq s = attn_seq(p, b);
+  const int4 de = __ldcg(ws.desc + 2 * c0);
+  const int c1 = __ldcg(ws.desc + 2 * c0 + 1).x;
+  if (c1 < 0) return;
   const int tpc = 128 / p.group;
-  const int row = (blockIdx.y & 7) * 32 + (threadIdx.x >> 3), d4 = (blockIdx.y >> 3) * 8 + (threadIdx.x & 7);
-  const int rr = row & 127, ti = rr / p.group, tok = tile * 2 * tpc + (row >> 7) * tpc + ti;
-  if (ti >= tpc || tok >= s.n) return;
+  const int row = blockIdx.y * 32 + (threadIdx.x >> 3), x = threadIdx.x & 7;
+  const int rr = row & 127, ti = rr / p.group, tok = de.w * 2 * tpc + (row >> 7) * tpc + ti;
+  if (ti >= tpc || tok >= de.y) return;
   float m = -INFINITY;
   for (int c = c0; c <= c1; ++c) m = fmaxf(m, __ldcg(ws.ml + (((size_t)c * 2 + (c == c0)) * 256 + row) * 2));
   const float base = m == -INFINITY ? 0.f : m;
-  float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+  float4 a[D / 32];
+#pragma unroll
+  for (int i = 0; i < D / 32; ++i) a[i] = make_float4(0.f, 0.f, 0.f, 0.f);
   float l = 0.f;
-#pragma unroll 4
   for (int c = c0; c <= c1; ++c) {
     const size_t place = (size_t)c * 2 + (c == c0);
     const float2 ml = __ldcg(reinterpret_cast<const float2*>(ws.ml) + place * 256 + row);
-    const float4 v = __ldcg(reinterpret_cast<const float4*>(ws.o) + (place * (D / 4) + d4) * 256 + row);
+    float4 v[D / 32];
+#pragma unroll
+    for (int i = 0; i < D / 32; ++i)
+      v[i] = __ldcg(reinterpret_cast<const float4*>(ws.o) + (place * (D / 4) + 8 * i + x) * 256 + row);
     const float f = ex2(ml.x - base);
     if (f != 0.f) {
       l = fmaf(ml.y, f, l);
-      a.x = fmaf(v.x, f, a.x);
-      a.y = fmaf(v.y, f, a.y);
-      a.z = fmaf(v.z, f, a.z);
-      a.w = fmaf(v.w, f, a.w);
+#pragma unroll
+      for (int i = 0; i < D / 32; ++i) {
+        a[i].x = fmaf(v[i].x, f, a[i].x);
+        a[i].y = fmaf(v[i].y, f, a[i].y);
+        a[i].z = fmaf(v[i].z, f, a[i].z);
+        a[i].w = fmaf(v[i].w, f, a[i].w);
+      }
     }
   }
   const float inv = l > 0.f ? 1.f / l : 0.f;
-  T* dst = static_cast<T*>(p.out) + (long long)(s.q0 + tok) * p.out_token +
-           (long long)(head * p.group + rr - ti * p.group) * p.out_head + d4 * 4;
-  *reinterpret_cast<uint2*>(dst) =
-      make_uint2(Elem<T>::from_f2(a.x * inv, a.y * inv), Elem<T>::from_f2(a.z * inv, a.w * inv));
+  T* dst = static_cast<T*>(p.out) + (long long)(de.x + tok) * p.out_token +
+           (long long)(de.z * p.group + rr - ti * p.group) * p.out_head + x * 4;
+#pragma unroll
+  for (int i = 0; i < D / 32; ++i)
+    *reinterpret_cast<uint2*>(dst + 32 * i) =
+        make_uint2(Elem<T>::from_f2(a[i].x * inv, a[i].y * inv), Elem<T>::from_f2(a[i].z * inv, a[i].w * inv));
 }
 
 }  // namespace d3

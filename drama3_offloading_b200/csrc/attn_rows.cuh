@@ -63,7 +63,8 @@ struct AttnParams {
   int min_rows, max_rows;        // sequences this launch takes, by new tokens * group
   float* ws_o;                   // partial sums
   float* ws_ml;                  // their maxima and sums
-  int4* ws_desc;                 // of each part: the pair that begins and does not end in it (join_desc)
+  int4* ws_desc;                 // two of each part: (first query token, rows of the sequence, KV head, row
+                                 // group), (last part or -1, ...) of the pair that begins and does not end in it
   int* err;
 };
 
@@ -119,6 +120,7 @@ constexpr int kPieceUnits = 1;
 struct RowsWork {
   int total, begin, count;
   int b, off;                    // sequence of `begin`, and its place inside it
+  AttnSeq s;
 };
 
 __device__ __forceinline__ int rows_tiles(int kv, int keys) { return max(1, (kv + keys - 1) / keys); }
@@ -138,8 +140,8 @@ __device__ __forceinline__ int part_begin(int total, int g, int c) {
 // the part that holds unit u
 __device__ __forceinline__ int part_of(int total, int g, long long u) { return (int)(((u + 1) * g - 1) / total); }
 
-// All threads of the CTA: part `part` of `parts`.  s_scan: 33 ints of shared memory.
-__device__ RowsWork rows_plan(const AttnParams& p, int keys, int rows_per, int part, int parts, int* s_scan) {
+// All threads of the CTA: part `part` of `parts`.  s_scan: 32 ints of shared memory.
+__device__ RowsWork rows_plan(const AttnParams& p, int keys, int rows_per, int part, int parts, int* s_scan, RowsWork* s_work) {
   const int n = blockDim.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int per = (p.batch + n - 1) / n;
   const int b0 = min(p.batch, tid * per), b1 = min(p.batch, b0 + per);
@@ -151,7 +153,6 @@ __device__ RowsWork rows_plan(const AttnParams& p, int keys, int rows_per, int p
     const int v = __shfl_up_sync(0xffffffffu, inc, o);
     if (lane >= o) inc += v;
   }
-  __shared__ int s_b, s_off;
   if (lane == 31) s_scan[warp] = inc;
   __syncthreads();
   int before = inc - sum, total = 0;
@@ -159,7 +160,7 @@ __device__ RowsWork rows_plan(const AttnParams& p, int keys, int rows_per, int p
     if (w < warp) before += s_scan[w];
     total += s_scan[w];
   }
-  RowsWork r{total, 0, 0, 0, 0};
+  RowsWork r{total, 0, 0, 0, 0, {0, 0, 0, 0}};
   // no part is empty: a pair's parts are neighbours in the workspace
   const int g = min(parts, total);
   if (part < g) {
@@ -171,17 +172,18 @@ __device__ RowsWork rows_plan(const AttnParams& p, int keys, int rows_per, int p
     for (int b = b0; b < b1; ++b) {
       const int u = rows_units(p, b, keys, rows_per);
       if (r.begin < at + u) {
-        s_b = b;
-        s_off = r.begin - at;
+        r.b = b;
+        r.off = r.begin - at;
+        r.s = attn_seq(p, b);
+        *s_work = r;
         break;
       }
       at += u;
     }
   }
+  if (r.count == 0 && tid == 0) *s_work = r;
   __syncthreads();
-  r.b = s_b;
-  r.off = s_off;
-  return r;
+  return *s_work;
 }
 
 // One piece of a (sequence, KV head, row group): tiles [t0, t1) of nt.
@@ -194,7 +196,7 @@ struct RowsWalk {
   int b, left, off;
   int known;                     // the sequence that s holds
   AttnSeq s;
-  __device__ __forceinline__ explicit RowsWalk(const RowsWork& r) : b(r.b), left(r.count), off(r.off), known(-1) {}
+  __device__ __forceinline__ explicit RowsWalk(const RowsWork& r) : b(r.b), left(r.count), off(r.off), known(r.b), s(r.s) {}
   __device__ __forceinline__ bool next(const AttnParams& p, int keys, int rows_per, RowsPiece& w) {
     while (left > 0 && b < p.batch) {
       if (known != b) {
@@ -283,7 +285,8 @@ __global__ void __launch_bounds__(RowsCfg<T, D, E4, NT>::THREADS, 1)
   using C = RowsCfg<T, D, E4, NT>;
   using M = typename std::conditional<E4, __half, T>::type;   // operand type of the products
   extern __shared__ uint8_t smem_raw[];
-  __shared__ int s_scan[33];
+  __shared__ int s_scan[32];
+  __shared__ RowsWork s_work;
   uint8_t* smem = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
   uint8_t* s_slots = smem;
   uint2* s_q = reinterpret_cast<uint2*>(smem + (size_t)C::SLOTS * C::SLOT);
@@ -304,9 +307,9 @@ __global__ void __launch_bounds__(RowsCfg<T, D, E4, NT>::THREADS, 1)
   }
   pdl_trigger();
   pdl_wait();
-  const RowsWork work = rows_plan(p, C::KEYS, C::ROWS, blockIdx.x, gridDim.x, s_scan);
+  const RowsWork work = rows_plan(p, C::KEYS, C::ROWS, blockIdx.x, gridDim.x, s_scan, &s_work);
   if (work.count == 0) {
-    if (tid == 0) p.ws_desc[blockIdx.x] = make_int4(0, 0, 0, -1);
+    if (tid == 0) p.ws_desc[2 * blockIdx.x + 1] = make_int4(-1, 0, 0, 0);
     return;
   }
   RowsWalk walk(work);
@@ -399,7 +402,8 @@ __global__ void __launch_bounds__(RowsCfg<T, D, E4, NT>::THREADS, 1)
     if (lane == 0) mbar_arrive(empty + slot);
     if (++slot == C::SLOTS) { slot = 0; phase ^= 1; }
   };
-  int4 desc = make_int4(0, 0, 0, -1);
+  int4 desc = make_int4(0, 0, 0, 0);
+  int last_part = -1;
   // a piece's queries are fetched while the one before runs: this warp's rows,
   // 16 bytes a lane
   constexpr int QROWS = (C::ROWS + C::WARPS - 1) / C::WARPS;
@@ -415,11 +419,37 @@ __global__ void __launch_bounds__(RowsCfg<T, D, E4, NT>::THREADS, 1)
             (long long)(x.head * p.group + gr % p.group) * p.q_head + lane * 8));
     }
   };
+  // codes: the scales of keys g and g + 8 of this warp's 16, a tile ahead, and
+  // the page id they need two ahead (a piece's first ones while the piece
+  // before runs)
+  float ks_n[2] = {0.f, 0.f}, vs_n[2] = {0.f, 0.f};
+  int id_n = -1, id_first = -1;
+  auto fetch_id = [&](const RowsPiece& x, int t) {
+    const int key = t * C::KEYS + warp * 16;
+    return E4 && t < x.t1 && key < x.s.kv
+               ? __ldcg(p.table + (long long)x.b * p.table_stride + (key >> p.page_shift)) : -1;
+  };
+  auto fetch_scales = [&](const RowsPiece& x, int t, int id) {
+    if (!E4) return;
+    const bool in = id >= 0 && id < p.pages;
+    const long long row = ((long long)(in ? id * p.kv_heads + x.head : 0) << p.page_shift) +
+                          ((t * C::KEYS + warp * 16) & (p.page_size - 1)) + g;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      ks_n[i] = in ? __ldcg(p.k_scale + row + 8 * i) : 0.f;
+      vs_n[i] = in ? __ldcg(p.v_scale + row + 8 * i) : 0.f;
+    }
+  };
   RowsPiece ahead{};
   bool more = walk.next(p, C::KEYS, C::ROWS, ahead);
-  if (more) fetch_q(ahead);
+  if (more) {
+    fetch_q(ahead);
+    id_first = fetch_id(ahead, ahead.t0);
+  }
   while (more) {
     w = ahead;
+    id_n = fetch_id(w, w.t0 + 1);
+    fetch_scales(w, w.t0, id_first);
     const int row0 = w.rg * C::ROWS, rows = min(C::ROWS, w.s.rows - row0);
     // queries in operand order: s_q[nt][kk][lane] holds the two registers of
     // B for k-step kk.  Codes come out of ldmatrix four dims to a lane, so
@@ -461,7 +491,10 @@ __global__ void __launch_bounds__(RowsCfg<T, D, E4, NT>::THREADS, 1)
     }
     bar();
     more = walk.next(p, C::KEYS, C::ROWS, ahead);
-    if (more) fetch_q(ahead);
+    if (more) {
+      fetch_q(ahead);
+      id_first = fetch_id(ahead, ahead.t0);
+    }
     // queries' operand, from shared memory each time where registers are short
     constexpr bool QREG = NT == 1 && !(E4 && D == 256);
     uint2 qr[QREG ? D / 16 : 1];
@@ -490,34 +523,12 @@ __global__ void __launch_bounds__(RowsCfg<T, D, E4, NT>::THREADS, 1)
       }
     }
     const int lk = lane & 7, lm = lane >> 3;     // ldmatrix: row and matrix of this lane
-    // codes: the scales of keys g and g + 8 of this warp's 16, a tile ahead,
-    // and the page id they need two ahead
-    float ks_n[2] = {0.f, 0.f}, vs_n[2] = {0.f, 0.f};
-    int id_n = -1;
-    auto fetch_id = [&](int t) {
-      const int key = t * C::KEYS + warp * 16;
-      if (E4) id_n = t < w.t1 && key < w.s.kv ? __ldcg(p.table + (long long)w.b * p.table_stride + (key >> p.page_shift)) : -1;
-    };
-    auto fetch_scales = [&](int t) {
-      if (!E4) return;
-      const bool in = id_n >= 0 && id_n < p.pages;
-      const long long row = ((long long)(in ? id_n * p.kv_heads + w.head : 0) << p.page_shift) +
-                            ((t * C::KEYS + warp * 16) & (p.page_size - 1)) + g;
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        ks_n[i] = in ? __ldcg(p.k_scale + row + 8 * i) : 0.f;
-        vs_n[i] = in ? __ldcg(p.v_scale + row + 8 * i) : 0.f;
-      }
-    };
-    fetch_id(w.t0);
-    fetch_scales(w.t0);
-    fetch_id(w.t0 + 1);
     for (int t = w.t0; t < w.t1; ++t) {
       const int key0 = t * C::KEYS + warp * 16;  // this warp's keys
       const float ks0 = E4 ? ks_n[0] : 1.f, ks1 = E4 ? ks_n[1] : 1.f;
       float u0 = E4 ? vs_n[0] : 1.f, u1 = E4 ? vs_n[1] : 1.f;
-      fetch_scales(t + 1);
-      fetch_id(t + 2);
+      fetch_scales(w, t + 1, id_n);
+      id_n = fetch_id(w, t + 2);
       take();
       const uint32_t kb = smem_u32(s_slots + (size_t)slot * C::SLOT) + mine;
       float s[NT][4];
@@ -695,7 +706,8 @@ __global__ void __launch_bounds__(RowsCfg<T, D, E4, NT>::THREADS, 1)
     if (!whole && w.t0 == 0) {
       // the part that holds the pair's last tile
       const long long u = (long long)work.begin + work.count + (w.nt - w.t1) - 1;
-      desc = make_int4(w.b, w.head, w.rg, part_of(work.total, min((int)gridDim.x, work.total), u));
+      desc = make_int4(w.s.q0, w.s.rows, w.head, w.rg);
+      last_part = part_of(work.total, min((int)gridDim.x, work.total), u);
     }
     float f[NT][2];    // this warp's factor of its rows
 #pragma unroll
@@ -756,7 +768,10 @@ __global__ void __launch_bounds__(RowsCfg<T, D, E4, NT>::THREADS, 1)
       }
     }
   }
-  if (tid == 0) p.ws_desc[blockIdx.x] = desc;
+  if (tid == 0) {
+    p.ws_desc[2 * blockIdx.x] = desc;
+    p.ws_desc[2 * blockIdx.x + 1] = make_int4(last_part, 0, 0, 0);
+  }
 }
 
 // Pairs that the parts' cuts go through: the sum of their parts, in the parts'
@@ -773,14 +788,14 @@ __global__ void __launch_bounds__(256) attn_rows_join_kernel(const __grid_consta
   pdl_trigger();
   pdl_wait();
   const int c0 = blockIdx.x, r = blockIdx.y;
-  const int4 de = __ldcg(p.ws_desc + c0);
-  if (de.w < 0) return;
-  const AttnSeq s = attn_seq(p, de.x);
-  const int gr = de.z * rows_per + r;
-  if (gr >= s.rows) return;
+  const int4 de = __ldcg(p.ws_desc + 2 * c0);
+  const int c1 = __ldcg(p.ws_desc + 2 * c0 + 1).x;
+  if (c1 < 0) return;
+  const int gr = de.w * rows_per + r;
+  if (gr >= de.y) return;
   const int g = threadIdx.x / (D / 4), d4 = threadIdx.x % (D / 4);
   float m = -INFINITY;
-  for (int c = c0 + (threadIdx.x & 31); c <= de.w; c += 32)
+  for (int c = c0 + (threadIdx.x & 31); c <= c1; c += 32)
     m = fmaxf(m, __ldcg(p.ws_ml + (((size_t)c * 2 + (c == c0)) * rows_per + r) * 2));
 #pragma unroll
   for (int x = 16; x > 0; x >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, x));
@@ -788,7 +803,7 @@ __global__ void __launch_bounds__(256) attn_rows_join_kernel(const __grid_consta
   float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
   float l = 0.f;
 #pragma unroll 4
-  for (int c = c0 + g; c <= de.w; c += GROUPS) {
+  for (int c = c0 + g; c <= c1; c += GROUPS) {
     const size_t at = ((size_t)c * 2 + (c == c0)) * rows_per + r;
     const float2 ml = __ldcg(reinterpret_cast<const float2*>(p.ws_ml + at * 2));
     const float4 v = __ldcg(reinterpret_cast<const float4*>(p.ws_o + at * D) + d4);
@@ -817,8 +832,8 @@ __global__ void __launch_bounds__(256) attn_rows_join_kernel(const __grid_consta
     a.w += v.w;
   }
   const float inv = l > 0.f ? 1.f / l : 0.f;
-  T* dst = static_cast<T*>(p.out) + (long long)(s.q0 + gr / p.group) * p.out_token +
-           (long long)(de.y * p.group + gr % p.group) * p.out_head + d4 * 4;
+  T* dst = static_cast<T*>(p.out) + (long long)(de.x + gr / p.group) * p.out_token +
+           (long long)(de.z * p.group + gr % p.group) * p.out_head + d4 * 4;
   *reinterpret_cast<uint2*>(dst) =
       make_uint2(Elem<T>::from_f2(a.x * inv, a.y * inv), Elem<T>::from_f2(a.z * inv, a.w * inv));
 }
