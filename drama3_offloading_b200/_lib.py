@@ -8,6 +8,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 from pathlib import Path
 
 _PKG = Path(__file__).resolve().parent
@@ -125,7 +126,20 @@ SIGNATURES: dict[str, tuple] = {
     "d3_trace_append": (ctypes.c_int, [P, I32, I32, I32, I32, P, P, I64, P]),
 }
 
+# Calls of a decode step, several per layer and token: the same functions with
+# their structs packed into bytes (``struct.pack`` of the _fields_ above), which
+# costs the host a third of filling a ctypes.Structure.
+PACKED: dict[str, list] = {
+    "d3_kv_write": [P, P, I64, I64, P, I64, I64, I32, I32, P, I32, P],
+    "d3_kv_read": [P, P, I32, I32, I32, P, P, P],
+    "d3_qk_norm_rope": [ctypes.c_char_p, P, P],
+    "d3_paged_attention": [ctypes.c_char_p, P, P, P, SZ, P],
+}
+NORM_ROPE = struct.Struct("=3Q6q2Q4q5Q9i2f4x")
+ATTENTION = struct.Struct("=Q2qQ2qQq2Q7if")
+
 _lib = None
+_packed: dict = {}
 _load_error: str | None = None
 
 
@@ -165,6 +179,24 @@ def call(name: str, *args) -> None:
     rc = getattr(lib, name)(*args)
     if rc != D3_OK:
         raise D3Error(rc, name, lib.d3_last_error().decode())
+
+
+def packed(name: str):
+    """``name`` with the argument types of PACKED; returns its status."""
+    fn = _packed.get(name)
+    if fn is None:
+        load()
+        lib = ctypes.CDLL(str(LIB_PATH))      # the same library, function objects of its own
+        for n, args in PACKED.items():
+            f = getattr(lib, n)
+            f.restype, f.argtypes = ctypes.c_int, args
+            _packed[n] = f
+        fn = _packed[name]
+    return fn
+
+
+def raise_status(rc: int, name: str) -> None:
+    raise D3Error(rc, name, load().d3_last_error().decode())
 
 
 def ptr(t) -> P:

@@ -15,8 +15,8 @@ from __future__ import annotations
 
 import torch
 
-from . import _lib, moe
-from .kvcache import DTYPES, PagedKV, aligned, index, on_device, rows
+from . import _lib
+from .kvcache import DTYPES, PagedKV, _raw_stream, aligned, elsewhere, in_place, index, place, rows
 
 
 def rope_frequencies(rotary_dim: int, theta: float = 10000.0, device="cuda") -> torch.Tensor:
@@ -25,62 +25,82 @@ def rope_frequencies(rotary_dim: int, theta: float = 10000.0, device="cuda") -> 
     return theta ** (-i / rotary_dim)
 
 
+def in_place_weight(w: torch.Tensor) -> torch.Tensor:
+    w = w.contiguous()
+    return w if w.data_ptr() % 16 == 0 else w.clone()
+
+
 def _norm_rope(q, k, v, q_weight, k_weight, positions, inv_freq, cache, slots, eps, weight_offset,
                interleaved, out, stream):
-    if q.dtype not in (torch.bfloat16, torch.float16):
-        raise TypeError(f"q must be bfloat16 or float16, got {q.dtype}")
+    dtype, dev = q.dtype, q.device
+    if dtype not in (torch.bfloat16, torch.float16):
+        raise TypeError(f"q must be bfloat16 or float16, got {dtype}")
     if q.dim() != 3 or k.dim() != 3:
         raise ValueError("q and k must be [tokens, heads, head_dim]")
     tokens, heads, dim = q.shape
-    kv_heads, dev = k.shape[1], q.device
-    q, k = rows(q, "q", heads, dim, q.dtype), rows(k, "k", kv_heads, dim, q.dtype)
+    kv_heads = k.shape[1]
+    rows(q, "q", heads, dim, dtype)
+    rows(k, "k", kv_heads, dim, dtype)
     if k.shape[0] != tokens:
         raise ValueError("q and k must have the same tokens")
     for w, name in ((q_weight, "q_weight"), (k_weight, "k_weight")):
-        if w.dtype != q.dtype or w.numel() != dim:
-            raise TypeError(f"{name} must be {q.dtype} [{dim}]")
-    q_weight, k_weight = q_weight.contiguous(), k_weight.contiguous()
+        if w.dtype != dtype or w.numel() != dim:
+            raise TypeError(f"{name} must be {dtype} [{dim}]")
     if inv_freq.dtype != torch.float64 or inv_freq.dim() != 1:
         raise TypeError("inv_freq must be float64 [rotary_dim / 2]")
-    inv_freq = inv_freq.contiguous()
-    positions = index(positions, "positions", tokens, dev)
-    for t in (k, q_weight, k_weight, inv_freq):
-        if t.device != dev:
-            raise ValueError(f"a tensor is on {t.device}, q on {dev}")
+    index(positions, "positions", tokens, dev)
+    if k.device != dev or q_weight.device != dev or k_weight.device != dev or inv_freq.device != dev:
+        raise ValueError(f"k, a weight or inv_freq is not on q's device {dev}")
     if cache is not None:
-        cache.rows_dtype(q.dtype)
-        v = rows(v, "v", kv_heads, dim, q.dtype)
+        cache.rows_dtype(dtype)
+        rows(v, "v", kv_heads, dim, dtype)
         if v.shape[0] != tokens or cache.kv_heads != kv_heads or cache.head_dim != dim:
             raise ValueError("v and the cache must have k's tokens and heads")
         if v.device != dev or cache.device != dev:
             raise ValueError(f"v or the cache is not on {dev}")
-        slots = index(slots, "slots", tokens, dev)
-
-    def take(t, like, name):
-        if t is None:
-            return torch.empty(like.shape, dtype=like.dtype, device=dev)
-        if t.shape != like.shape or t.dtype != like.dtype or t.device != dev or not aligned(t):
-            raise ValueError(f"{name} must be {like.dtype} {tuple(like.shape)} on {dev}, its rows "
-                             "contiguous on 16-byte boundaries")
-        return t
-
-    def go(st):
-        qo, ko = (out if isinstance(out, tuple) else (out, None)) if out is not None else (None, None)
-        qo = take(qo, q, "out")
-        ko = take(ko, k, "out") if cache is None else None
-        a = _lib.NormRope(
-            q.data_ptr(), k.data_ptr(), v.data_ptr() if cache is not None else None,
-            q.stride(0), q.stride(1), k.stride(0), k.stride(1),
-            v.stride(0) if cache is not None else 0, v.stride(1) if cache is not None else 0,
-            qo.data_ptr(), ko.data_ptr() if ko is not None else None, qo.stride(0), qo.stride(1),
-            ko.stride(0) if ko is not None else 0, ko.stride(1) if ko is not None else 0,
-            q_weight.data_ptr(), k_weight.data_ptr(), positions.data_ptr(), inv_freq.data_ptr(),
-            slots.data_ptr() if cache is not None else None, positions.element_size(),
-            slots.element_size() if cache is not None else 4, tokens, heads, kv_heads, dim,
-            2 * inv_freq.shape[0], 1 if interleaved else 0, DTYPES[q.dtype], eps, weight_offset)
-        _lib.call("d3_qk_norm_rope", a, cache.ref if cache is not None else None, st)
-        return qo, ko
-    return on_device(dev, go, stream=stream)
+        index(slots, "slots", tokens, dev)
+    if elsewhere(dev, stream):
+        with place(dev, stream):
+            return _norm_rope(q, k, v, q_weight, k_weight, positions, inv_freq, cache, slots, eps,
+                              weight_offset, interleaved, out, None)
+    q, k = in_place(q), in_place(k)
+    q_weight, k_weight = in_place_weight(q_weight), in_place_weight(k_weight)
+    positions, inv_freq = positions.contiguous(), inv_freq.contiguous()
+    if cache is not None:
+        v, slots = in_place(v), slots.contiguous()
+    qo, ko = out if isinstance(out, tuple) else (out, None)
+    if qo is None:
+        qo = q.new_empty(q.shape)
+    elif qo.shape != q.shape or qo.dtype != dtype or qo.device != dev or not aligned(qo):
+        raise ValueError(f"out must be {dtype} {tuple(q.shape)} on {dev}, its rows contiguous on "
+                         "16-byte boundaries")
+    qs, ks, qos = q.stride(), k.stride(), qo.stride()
+    if cache is None:
+        if ko is None:
+            ko = k.new_empty(k.shape)
+        elif ko.shape != k.shape or ko.dtype != dtype or ko.device != dev or not aligned(ko):
+            raise ValueError(f"out must be {dtype} {tuple(k.shape)} on {dev}, its rows contiguous on "
+                             "16-byte boundaries")
+        kos = ko.stride()
+        a = _lib.NORM_ROPE.pack(
+            q.data_ptr(), k.data_ptr(), 0, qs[0], qs[1], ks[0], ks[1], 0, 0, qo.data_ptr(),
+            ko.data_ptr(), qos[0], qos[1], kos[0], kos[1], q_weight.data_ptr(), k_weight.data_ptr(),
+            positions.data_ptr(), inv_freq.data_ptr(), 0, positions.element_size(), 4, tokens, heads,
+            kv_heads, dim, 2 * inv_freq.shape[0], 1 if interleaved else 0, DTYPES[dtype], eps,
+            weight_offset)
+        rc = _lib.packed("d3_qk_norm_rope")(a, None, _raw_stream(dev.index))
+    else:
+        vs = v.stride()
+        a = _lib.NORM_ROPE.pack(
+            q.data_ptr(), k.data_ptr(), v.data_ptr(), qs[0], qs[1], ks[0], ks[1], vs[0], vs[1],
+            qo.data_ptr(), 0, qos[0], qos[1], 0, 0, q_weight.data_ptr(), k_weight.data_ptr(),
+            positions.data_ptr(), inv_freq.data_ptr(), slots.data_ptr(), positions.element_size(),
+            slots.element_size(), tokens, heads, kv_heads, dim, 2 * inv_freq.shape[0],
+            1 if interleaved else 0, DTYPES[dtype], eps, weight_offset)
+        rc = _lib.packed("d3_qk_norm_rope")(a, cache.ref, _raw_stream(dev.index))
+    if rc:
+        _lib.raise_status(rc, "d3_qk_norm_rope")
+    return qo, ko
 
 
 def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor,
@@ -128,19 +148,17 @@ def paged_attention(q: torch.Tensor, cache: PagedKV, page_table: torch.Tensor,
     if q.dim() != 3:
         raise ValueError("q must be [tokens, heads, head_dim]")
     tokens, heads, dim = q.shape
-    dev = q.device
-    code = cache.rows_dtype(q.dtype)
-    q = rows(q, "q", heads, cache.head_dim, q.dtype)
+    dev, dtype = q.device, q.dtype
+    code = cache.rows_dtype(dtype)
+    rows(q, "q", heads, cache.head_dim, dtype)
     if heads % cache.kv_heads or heads // cache.kv_heads > 128:
         raise ValueError(f"{heads} heads over {cache.kv_heads} KV heads")
     if page_table.dtype != torch.int32 or page_table.dim() != 2:
         raise TypeError("page_table must be int32 [batch, pages]")
-    if page_table.stride(1) != 1:
-        page_table = page_table.contiguous()
     batch, pages = page_table.shape
-    kv_lens = index(kv_lens, "kv_lens", batch, dev)
+    index(kv_lens, "kv_lens", batch, dev)
     if cu_q is not None:
-        cu_q = index(cu_q, "cu_q", batch + 1, dev)
+        index(cu_q, "cu_q", batch + 1, dev)
     elif tokens < batch:
         raise ValueError(f"{tokens} rows for {batch} sequences of one row each")
     if kv_lens.dtype != torch.int32 or (cu_q is not None and cu_q.dtype != torch.int32):
@@ -149,27 +167,45 @@ def paged_attention(q: torch.Tensor, cache: PagedKV, page_table: torch.Tensor,
         raise ValueError(f"the cache or page_table is not on {dev}")
     if max_q < 1:
         raise ValueError("max_q must be at least 1")
-    scale = dim ** -0.5 if scale is None else float(scale)
-    if not 0.0 < scale < float("inf"):
+    if scale is None:
+        scale = dim ** -0.5
+    elif not 0.0 < scale < float("inf"):
         raise ValueError(f"scale {scale}: must be positive")
     top = pages * cache.page_size
-    max_kv = top if max_kv is None else min(max_kv, top)
-    if out is not None and (out.shape != q.shape or out.dtype != q.dtype or out.device != dev
+    max_kv = top if max_kv is None else max(0, min(max_kv, top))
+    if out is not None and (out.shape != q.shape or out.dtype != dtype or out.device != dev
                             or not aligned(out)):
-        raise ValueError(f"out must be {q.dtype} {tuple(q.shape)} on {dev}, its rows contiguous on "
+        raise ValueError(f"out must be {dtype} {tuple(q.shape)} on {dev}, its rows contiguous on "
                          "16-byte boundaries")
-
-    def go(st):
-        o = out if out is not None else torch.empty(tokens, heads, dim, dtype=q.dtype, device=dev)
-        a = _lib.Attention(
-            q.data_ptr(), q.stride(0), q.stride(1), o.data_ptr(), o.stride(0), o.stride(1),
-            page_table.data_ptr(), page_table.stride(0), kv_lens.data_ptr(),
-            cu_q.data_ptr() if cu_q is not None else None, pages, batch, tokens, heads,
-            min(max_q, max(tokens, 1)), max(max_kv, 0), code,
-            scale)
-        need = _lib.load().d3_paged_attention_workspace_size(a, cache.ref)
-        ws = torch.empty(max(need, 16), dtype=torch.uint8, device=dev)
-        _lib.call("d3_paged_attention", a, cache.ref, moe.error_word(dev).data_ptr(),
-                  ws.data_ptr(), need, st)
-        return o
-    return on_device(dev, go, stream=stream)
+    if elsewhere(dev, stream):
+        with place(dev, stream):
+            return paged_attention(q, cache, page_table, kv_lens, cu_q, max_q=max_q, max_kv=max_kv,
+                                   scale=scale, out=out)
+    q, kv_lens = in_place(q), kv_lens.contiguous()
+    if cu_q is not None:
+        cu_q = cu_q.contiguous()
+    if page_table.stride(1) != 1:
+        page_table = page_table.contiguous()
+    ts = page_table.stride()
+    if out is None:
+        out = q.new_empty((tokens, heads, dim))
+    max_q = min(max_q, max(tokens, 1))
+    qs, os = q.stride(), out.stride()
+    a = _lib.ATTENTION.pack(
+        q.data_ptr(), qs[0], qs[1], out.data_ptr(), os[0], os[1], page_table.data_ptr(), ts[0],
+        kv_lens.data_ptr(), 0 if cu_q is None else cu_q.data_ptr(), pages, batch, tokens, heads,
+        max_q, max_kv, code, scale)
+    # the workspace depends on the kernels that max_q asks for alone
+    key = max_q * (heads // cache.kv_heads) > 16
+    need = cache.workspace.get(key)
+    if need is None:
+        need = _lib.load().d3_paged_attention_workspace_size(
+            _lib.Attention.from_buffer_copy(a), _lib.KVCache.from_address(cache.ref))
+        if need:
+            cache.workspace[key] = need
+    ws = q.new_empty(max(need, 16) // 2)
+    rc = _lib.packed("d3_paged_attention")(a, cache.ref, cache.error_word.data_ptr(),
+                                           ws.data_ptr(), need, _raw_stream(dev.index))
+    if rc:
+        _lib.raise_status(rc, "d3_paged_attention")
+    return out

@@ -29,25 +29,41 @@ DTYPES = {torch.bfloat16: _lib.D3_BF16, torch.float16: _lib.D3_F16,
           torch.float8_e4m3fn: _lib.D3_E4M3}
 
 
-def on_device(device: torch.device, fn, *args, stream=None):
-    """``fn(stream_pointer, *args)`` with ``device`` current, on ``stream`` (or
-    the device's current stream); outputs it allocates belong to that stream."""
-    if stream is not None:
-        with torch.cuda.stream(stream):
-            return fn(_lib.P(stream.cuda_stream), *args)
-    if torch.cuda.current_device() != device.index:
-        with torch.cuda.device(device):
-            return fn(_lib.P(torch.cuda.current_stream().cuda_stream), *args)
-    return fn(_lib.P(torch.cuda.current_stream().cuda_stream), *args)
+_device = torch._C._cuda_getDevice if hasattr(torch._C, "_cuda_getDevice") else torch.cuda.current_device
+if hasattr(torch._C, "_cuda_getCurrentRawStream"):
+    _raw_stream = torch._C._cuda_getCurrentRawStream
+else:
+    def _raw_stream(index):
+        return torch.cuda.current_stream(index).cuda_stream
 
 
-def rows(t: torch.Tensor, name: str, heads: int, dim: int, dtype) -> torch.Tensor:
-    """``t`` checked as [tokens, heads, dim] rows the kernels can read in place:
-    contiguous dims, rows on 16-byte boundaries (others are copied)."""
+def elsewhere(device: torch.device, stream) -> bool:
+    """Whether a call on ``device`` and ``stream`` (None: the current one) needs
+    ``place`` around it -- and around the copies it may make of its arguments."""
+    if device.type != "cuda":
+        raise ValueError(f"tensors on {device}: a CUDA device is needed")
+    return stream is not None or _device() != device.index
+
+
+def place(device: torch.device, stream):
+    """Context in which ``device`` is the current device and ``stream`` (or the
+    device's current one) its current stream: outputs and workspaces made in it
+    belong to that stream."""
+    return torch.cuda.stream(stream if stream is not None else torch.cuda.current_stream(device))
+
+
+def rows(t: torch.Tensor, name: str, heads: int, dim: int, dtype) -> None:
+    """Checks ``t`` as [tokens, heads, dim] rows of ``dtype``."""
     if t.dtype != dtype:
         raise TypeError(f"{name} must be {dtype}, got {t.dtype}")
-    if t.dim() != 3 or t.shape[1] != heads or t.shape[2] != dim:
-        raise ValueError(f"{name} must be [tokens, {heads}, {dim}], got {tuple(t.shape)}")
+    shape = t.shape
+    if len(shape) != 3 or shape[1] != heads or shape[2] != dim:
+        raise ValueError(f"{name} must be [tokens, {heads}, {dim}], got {tuple(shape)}")
+
+
+def in_place(t: torch.Tensor) -> torch.Tensor:
+    """``t``, or a copy if its rows do not lie as the kernels read them:
+    contiguous dims, rows on 16-byte boundaries."""
     if not aligned(t):
         t = t.contiguous()
         if t.data_ptr() % 16:
@@ -61,14 +77,14 @@ def aligned(t: torch.Tensor) -> bool:
             and t.data_ptr() % 16 == 0)
 
 
-def index(t: torch.Tensor, name: str, tokens: int, device) -> torch.Tensor:
+def index(t: torch.Tensor, name: str, tokens: int, device) -> None:
+    """Checks ``t`` as int32 or int64 [tokens] on ``device``."""
     if t.dtype not in (torch.int32, torch.int64):
         raise TypeError(f"{name} must be int32 or int64, got {t.dtype}")
     if t.dim() != 1 or t.shape[0] != tokens:
         raise ValueError(f"{name} must be [{tokens}], got {tuple(t.shape)}")
     if t.device != device:
         raise ValueError(f"{name} is on {t.device}, not on {device}")
-    return t.contiguous()
 
 
 class PagedKV:
@@ -121,17 +137,20 @@ class PagedKV:
         self.dtype, self.device = k.dtype, k.device
         self.desc = _lib.KVCache(k.data_ptr(), v.data_ptr(), ks.data_ptr() if e4m3 else None,
                                  vs.data_ptr() if e4m3 else None, *k.shape, DTYPES[k.dtype])
-        self.ref = ctypes.byref(self.desc)
-        if k.device.type == "cuda":
-            moe.error_word(k.device)      # made here, not inside a capture
+        self.ref = ctypes.addressof(self.desc)
+        self.e4m3 = e4m3
+        self.workspace: dict = {}         # bytes an attention call needs, by its kernels
+        # made here, not inside a capture
+        self.error_word = moe.error_word(k.device) if k.device.type == "cuda" else None
 
     def rows_dtype(self, dtype) -> int:
         """The ABI's code of 16-bit rows this cache takes and gives."""
-        if dtype not in (torch.bfloat16, torch.float16):
+        code = DTYPES.get(dtype)
+        if code is None or code == _lib.D3_E4M3:
             raise TypeError(f"rows must be bfloat16 or float16, got {dtype}")
-        if self.dtype != torch.float8_e4m3fn and dtype != self.dtype:
+        if not self.e4m3 and dtype != self.dtype:
             raise TypeError(f"a {self.dtype} cache takes and gives {self.dtype} rows, not {dtype}")
-        return DTYPES[dtype]
+        return code
 
 
 def write(cache: PagedKV, k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor,
@@ -140,34 +159,44 @@ def write(cache: PagedKV, k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor,
     tensor are read in place) into ``slots`` (int32 or int64 ``[tokens]``).
     Slots outside the cache -- -1, say, for padding -- are skipped.  The slots
     of one call are distinct: a slot named twice keeps parts of either row."""
-    code = cache.rows_dtype(k.dtype)
-    k = rows(k, "k", cache.kv_heads, cache.head_dim, k.dtype)
-    v = rows(v, "v", cache.kv_heads, cache.head_dim, k.dtype)
-    if v.shape[0] != k.shape[0] or k.device != cache.device or v.device != cache.device:
+    dev = cache.device
+    dtype = k.dtype
+    code = cache.rows_dtype(dtype)
+    rows(k, "k", cache.kv_heads, cache.head_dim, dtype)
+    rows(v, "v", cache.kv_heads, cache.head_dim, dtype)
+    tokens = k.shape[0]
+    if v.shape[0] != tokens or k.device != dev or v.device != dev:
         raise ValueError("k and v must have the same tokens and the cache's device")
-    slots = index(slots, "slots", k.shape[0], cache.device)
-
-    def go(st):
-        _lib.call("d3_kv_write", cache.ref, k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(),
-                  v.stride(0), v.stride(1), code, k.shape[0], slots.data_ptr(),
-                  slots.element_size(), st)
-    on_device(cache.device, go, stream=stream)
+    index(slots, "slots", tokens, dev)
+    if elsewhere(dev, stream):
+        with place(dev, stream):
+            return write(cache, k, v, slots)
+    k, v, slots = in_place(k), in_place(v), slots.contiguous()
+    ks, vs = k.stride(), v.stride()
+    rc = _lib.packed("d3_kv_write")(cache.ref, k.data_ptr(), ks[0], ks[1], v.data_ptr(), vs[0], vs[1],
+                                    code, tokens, slots.data_ptr(), slots.element_size(),
+                                    _raw_stream(dev.index))
+    if rc:
+        _lib.raise_status(rc, "d3_kv_write")
 
 
 def read(cache: PagedKV, slots: torch.Tensor, dtype=None, stream=None):
     """(k, v) rows ``[tokens, kv_heads, head_dim]`` at ``slots`` as ``dtype``
     (the cache's own type, or bfloat16 for an e4m3 cache).  A slot outside the
     cache reads as zeros."""
+    dev = cache.device
     if dtype is None:
-        dtype = torch.bfloat16 if cache.dtype == torch.float8_e4m3fn else cache.dtype
+        dtype = torch.bfloat16 if cache.e4m3 else cache.dtype
     code = cache.rows_dtype(dtype)
-    slots = index(slots, "slots", slots.shape[0] if slots.dim() else 0, cache.device)
-
-    def go(st):
-        out = torch.empty(2, slots.shape[0], cache.kv_heads, cache.head_dim, dtype=dtype,
-                          device=cache.device)
-        k, v = out.unbind(0)
-        _lib.call("d3_kv_read", cache.ref, slots.data_ptr(), slots.element_size(), slots.shape[0],
-                  code, k.data_ptr(), v.data_ptr(), st)
-        return k, v
-    return on_device(cache.device, go, stream=stream)
+    index(slots, "slots", slots.shape[0] if slots.dim() else 0, dev)
+    if elsewhere(dev, stream):
+        with place(dev, stream):
+            return read(cache, slots, dtype)
+    slots = slots.contiguous()
+    tokens = slots.shape[0]
+    k, v = torch.empty((2, tokens, cache.kv_heads, cache.head_dim), dtype=dtype, device=dev).unbind(0)
+    rc = _lib.packed("d3_kv_read")(cache.ref, slots.data_ptr(), slots.element_size(), tokens, code,
+                                   k.data_ptr(), v.data_ptr(), _raw_stream(dev.index))
+    if rc:
+        _lib.raise_status(rc, "d3_kv_read")
+    return k, v
