@@ -16,7 +16,8 @@ from __future__ import annotations
 import torch
 
 from . import _lib
-from .kvcache import DTYPES, PagedKV, _raw_stream, aligned, elsewhere, in_place, index, place, rows
+from .kvcache import (DTYPES, PagedKV, _raw_stream, elsewhere, fresh, in_place, index, output, place,
+                      rows)
 
 
 def rope_frequencies(rotary_dim: int, theta: float = 10000.0, device="cuda") -> torch.Tensor:
@@ -25,79 +26,63 @@ def rope_frequencies(rotary_dim: int, theta: float = 10000.0, device="cuda") -> 
     return theta ** (-i / rotary_dim)
 
 
-def in_place_weight(w: torch.Tensor) -> torch.Tensor:
-    w = w.contiguous()
-    return w if w.data_ptr() % 16 == 0 else w.clone()
-
-
 def _norm_rope(q, k, v, q_weight, k_weight, positions, inv_freq, cache, slots, eps, weight_offset,
                interleaved, out, stream):
-    dtype, dev = q.dtype, q.device
-    if dtype not in (torch.bfloat16, torch.float16):
+    dtype, dev = q.dtype, q.get_device()
+    if dtype is not torch.bfloat16 and dtype is not torch.float16:
         raise TypeError(f"q must be bfloat16 or float16, got {dtype}")
     if q.dim() != 3 or k.dim() != 3:
         raise ValueError("q and k must be [tokens, heads, head_dim]")
     tokens, heads, dim = q.shape
     kv_heads = k.shape[1]
-    rows(q, "q", heads, dim, dtype)
-    rows(k, "k", kv_heads, dim, dtype)
+    rows(k, "k", kv_heads, dim, dtype, dev)
     if k.shape[0] != tokens:
         raise ValueError("q and k must have the same tokens")
-    for w, name in ((q_weight, "q_weight"), (k_weight, "k_weight")):
-        if w.dtype != dtype or w.numel() != dim:
-            raise TypeError(f"{name} must be {dtype} [{dim}]")
-    if inv_freq.dtype != torch.float64 or inv_freq.dim() != 1:
+    for w in (q_weight, k_weight):
+        if w.dtype is not dtype or w.numel() != dim:
+            raise TypeError(f"q_weight and k_weight must be {dtype} [{dim}]")
+        if w.get_device() != dev:
+            raise ValueError(f"a weight is on {w.device}, not on device {dev}")
+    if inv_freq.dtype is not torch.float64 or inv_freq.dim() != 1:
         raise TypeError("inv_freq must be float64 [rotary_dim / 2]")
+    if inv_freq.get_device() != dev:
+        raise ValueError(f"inv_freq is on {inv_freq.device}, not on device {dev}")
     index(positions, "positions", tokens, dev)
-    if k.device != dev or q_weight.device != dev or k_weight.device != dev or inv_freq.device != dev:
-        raise ValueError(f"k, a weight or inv_freq is not on q's device {dev}")
     if cache is not None:
         cache.rows_dtype(dtype)
-        rows(v, "v", kv_heads, dim, dtype)
+        rows(v, "v", kv_heads, dim, dtype, dev)
         if v.shape[0] != tokens or cache.kv_heads != kv_heads or cache.head_dim != dim:
             raise ValueError("v and the cache must have k's tokens and heads")
-        if v.device != dev or cache.device != dev:
-            raise ValueError(f"v or the cache is not on {dev}")
+        if cache.device_index != dev:
+            raise ValueError(f"the cache is on {cache.device}, not on device {dev}")
         index(slots, "slots", tokens, dev)
     if elsewhere(dev, stream):
         with place(dev, stream):
             return _norm_rope(q, k, v, q_weight, k_weight, positions, inv_freq, cache, slots, eps,
                               weight_offset, interleaved, out, None)
-    q, k = in_place(q), in_place(k)
-    q_weight, k_weight = in_place_weight(q_weight), in_place_weight(k_weight)
+    q, q_at, q0, q1 = in_place(q)
+    k, k_at, k0, k1 = in_place(k)
+    q_weight, k_weight = q_weight.contiguous(), k_weight.contiguous()
+    qw, kw = q_weight.data_ptr(), k_weight.data_ptr()
+    if (qw | kw) & 15:
+        q_weight, k_weight = q_weight.clone(), k_weight.clone()
+        qw, kw = q_weight.data_ptr(), k_weight.data_ptr()
     positions, inv_freq = positions.contiguous(), inv_freq.contiguous()
-    if cache is not None:
-        v, slots = in_place(v), slots.contiguous()
     qo, ko = out if isinstance(out, tuple) else (out, None)
-    if qo is None:
-        qo = q.new_empty(q.shape)
-    elif qo.shape != q.shape or qo.dtype != dtype or qo.device != dev or not aligned(qo):
-        raise ValueError(f"out must be {dtype} {tuple(q.shape)} on {dev}, its rows contiguous on "
-                         "16-byte boundaries")
-    qs, ks, qos = q.stride(), k.stride(), qo.stride()
+    qo, qo_at, qo0, qo1 = fresh(q, heads, dim) if qo is None else output(qo, q.shape, dtype, dev)
     if cache is None:
-        if ko is None:
-            ko = k.new_empty(k.shape)
-        elif ko.shape != k.shape or ko.dtype != dtype or ko.device != dev or not aligned(ko):
-            raise ValueError(f"out must be {dtype} {tuple(k.shape)} on {dev}, its rows contiguous on "
-                             "16-byte boundaries")
-        kos = ko.stride()
-        a = _lib.NORM_ROPE.pack(
-            q.data_ptr(), k.data_ptr(), 0, qs[0], qs[1], ks[0], ks[1], 0, 0, qo.data_ptr(),
-            ko.data_ptr(), qos[0], qos[1], kos[0], kos[1], q_weight.data_ptr(), k_weight.data_ptr(),
-            positions.data_ptr(), inv_freq.data_ptr(), 0, positions.element_size(), 4, tokens, heads,
-            kv_heads, dim, 2 * inv_freq.shape[0], 1 if interleaved else 0, DTYPES[dtype], eps,
-            weight_offset)
-        rc = _lib.packed("d3_qk_norm_rope")(a, None, _raw_stream(dev.index))
+        ko, ko_at, ko0, ko1 = fresh(k, kv_heads, dim) if ko is None else output(ko, k.shape, dtype, dev)
+        v_at, v0, v1, slots_at, slot_bytes, ref = 0, 0, 0, 0, 4, None
     else:
-        vs = v.stride()
-        a = _lib.NORM_ROPE.pack(
-            q.data_ptr(), k.data_ptr(), v.data_ptr(), qs[0], qs[1], ks[0], ks[1], vs[0], vs[1],
-            qo.data_ptr(), 0, qos[0], qos[1], 0, 0, q_weight.data_ptr(), k_weight.data_ptr(),
-            positions.data_ptr(), inv_freq.data_ptr(), slots.data_ptr(), positions.element_size(),
-            slots.element_size(), tokens, heads, kv_heads, dim, 2 * inv_freq.shape[0],
-            1 if interleaved else 0, DTYPES[dtype], eps, weight_offset)
-        rc = _lib.packed("d3_qk_norm_rope")(a, cache.ref, _raw_stream(dev.index))
+        v, v_at, v0, v1 = in_place(v)
+        slots = slots.contiguous()
+        ko_at, ko0, ko1 = 0, 0, 0
+        slots_at, slot_bytes, ref = slots.data_ptr(), slots.element_size(), cache.ref
+    rc = _lib.packed("d3_qk_norm_rope")(_lib.NORM_ROPE.pack(
+        q_at, k_at, v_at, q0, q1, k0, k1, v0, v1, qo_at, ko_at, qo0, qo1, ko0, ko1, qw, kw,
+        positions.data_ptr(), inv_freq.data_ptr(), slots_at, positions.element_size(), slot_bytes,
+        tokens, heads, kv_heads, dim, 2 * inv_freq.shape[0], 1 if interleaved else 0, DTYPES[dtype],
+        eps, weight_offset), ref, _raw_stream(dev))
     if rc:
         _lib.raise_status(rc, "d3_qk_norm_rope")
     return qo, ko
@@ -148,12 +133,14 @@ def paged_attention(q: torch.Tensor, cache: PagedKV, page_table: torch.Tensor,
     if q.dim() != 3:
         raise ValueError("q must be [tokens, heads, head_dim]")
     tokens, heads, dim = q.shape
-    dev, dtype = q.device, q.dtype
+    dev, dtype = q.get_device(), q.dtype
     code = cache.rows_dtype(dtype)
-    rows(q, "q", heads, cache.head_dim, dtype)
-    if heads % cache.kv_heads or heads // cache.kv_heads > 128:
-        raise ValueError(f"{heads} heads over {cache.kv_heads} KV heads")
-    if page_table.dtype != torch.int32 or page_table.dim() != 2:
+    kv_heads = cache.kv_heads
+    if dim != cache.head_dim:
+        raise ValueError(f"q's head_dim {dim}, the cache's {cache.head_dim}")
+    if heads % kv_heads or heads // kv_heads > 128:
+        raise ValueError(f"{heads} heads over {kv_heads} KV heads")
+    if page_table.dtype is not torch.int32 or page_table.dim() != 2:
         raise TypeError("page_table must be int32 [batch, pages]")
     batch, pages = page_table.shape
     index(kv_lens, "kv_lens", batch, dev)
@@ -161,10 +148,10 @@ def paged_attention(q: torch.Tensor, cache: PagedKV, page_table: torch.Tensor,
         index(cu_q, "cu_q", batch + 1, dev)
     elif tokens < batch:
         raise ValueError(f"{tokens} rows for {batch} sequences of one row each")
-    if kv_lens.dtype != torch.int32 or (cu_q is not None and cu_q.dtype != torch.int32):
+    if kv_lens.dtype is not torch.int32 or (cu_q is not None and cu_q.dtype is not torch.int32):
         raise TypeError("kv_lens and cu_q must be int32")
-    if cache.device != dev or page_table.device != dev:
-        raise ValueError(f"the cache or page_table is not on {dev}")
+    if cache.device_index != dev or page_table.get_device() != dev:
+        raise ValueError(f"the cache or page_table is not on q's device {q.device}")
     if max_q < 1:
         raise ValueError("max_q must be at least 1")
     if scale is None:
@@ -173,39 +160,39 @@ def paged_attention(q: torch.Tensor, cache: PagedKV, page_table: torch.Tensor,
         raise ValueError(f"scale {scale}: must be positive")
     top = pages * cache.page_size
     max_kv = top if max_kv is None else max(0, min(max_kv, top))
-    if out is not None and (out.shape != q.shape or out.dtype != dtype or out.device != dev
-                            or not aligned(out)):
-        raise ValueError(f"out must be {dtype} {tuple(q.shape)} on {dev}, its rows contiguous on "
-                         "16-byte boundaries")
+    if out is not None:
+        out, o_at, o0, o1 = output(out, q.shape, dtype, dev)
     if elsewhere(dev, stream):
         with place(dev, stream):
             return paged_attention(q, cache, page_table, kv_lens, cu_q, max_q=max_q, max_kv=max_kv,
                                    scale=scale, out=out)
-    q, kv_lens = in_place(q), kv_lens.contiguous()
+    q, q_at, q0, q1 = in_place(q)
+    kv_lens = kv_lens.contiguous()
+    cu_at = 0
     if cu_q is not None:
         cu_q = cu_q.contiguous()
-    if page_table.stride(1) != 1:
+        cu_at = cu_q.data_ptr()
+    t0, t1 = page_table.stride()
+    if t1 != 1:
         page_table = page_table.contiguous()
-    ts = page_table.stride()
+        t0 = page_table.stride(0)
     if out is None:
-        out = q.new_empty((tokens, heads, dim))
-    max_q = min(max_q, max(tokens, 1))
-    qs, os = q.stride(), out.stride()
-    a = _lib.ATTENTION.pack(
-        q.data_ptr(), qs[0], qs[1], out.data_ptr(), os[0], os[1], page_table.data_ptr(), ts[0],
-        kv_lens.data_ptr(), 0 if cu_q is None else cu_q.data_ptr(), pages, batch, tokens, heads,
-        max_q, max_kv, code, scale)
+        out, o_at, o0, o1 = fresh(q, heads, dim)
+    if max_q > tokens:
+        max_q = tokens or 1
+    a = _lib.ATTENTION.pack(q_at, q0, q1, o_at, o0, o1, page_table.data_ptr(), t0, kv_lens.data_ptr(),
+                            cu_at, pages, batch, tokens, heads, max_q, max_kv, code, scale)
     # the workspace depends on the kernels that max_q asks for alone
-    key = max_q * (heads // cache.kv_heads) > 16
+    key = max_q * (heads // kv_heads) > 16
     need = cache.workspace.get(key)
     if need is None:
         need = _lib.load().d3_paged_attention_workspace_size(
             _lib.Attention.from_buffer_copy(a), _lib.KVCache.from_address(cache.ref))
         if need:
             cache.workspace[key] = need
-    ws = q.new_empty(max(need, 16) // 2)
-    rc = _lib.packed("d3_paged_attention")(a, cache.ref, cache.error_word.data_ptr(),
-                                           ws.data_ptr(), need, _raw_stream(dev.index))
+    ws = q.new_empty(need // 2 or 8)
+    rc = _lib.packed("d3_paged_attention")(a, cache.ref, cache.error_word.data_ptr(), ws.data_ptr(),
+                                           need, _raw_stream(dev))
     if rc:
         _lib.raise_status(rc, "d3_paged_attention")
     return out

@@ -37,54 +37,73 @@ else:
         return torch.cuda.current_stream(index).cuda_stream
 
 
-def elsewhere(device: torch.device, stream) -> bool:
-    """Whether a call on ``device`` and ``stream`` (None: the current one) needs
-    ``place`` around it -- and around the copies it may make of its arguments."""
-    if device.type != "cuda":
-        raise ValueError(f"tensors on {device}: a CUDA device is needed")
-    return stream is not None or _device() != device.index
+def elsewhere(device: int, stream) -> bool:
+    """Whether a call on CUDA device ``device`` and ``stream`` (None: the current
+    one) needs ``place`` around it -- and around the copies it may make of its
+    arguments."""
+    if device < 0:
+        raise ValueError("tensors on the CPU: a CUDA device is needed")
+    return stream is not None or _device() != device
 
 
-def place(device: torch.device, stream):
+def place(device: int, stream):
     """Context in which ``device`` is the current device and ``stream`` (or the
     device's current one) its current stream: outputs and workspaces made in it
     belong to that stream."""
     return torch.cuda.stream(stream if stream is not None else torch.cuda.current_stream(device))
 
 
-def rows(t: torch.Tensor, name: str, heads: int, dim: int, dtype) -> None:
-    """Checks ``t`` as [tokens, heads, dim] rows of ``dtype``."""
-    if t.dtype != dtype:
+def rows(t: torch.Tensor, name: str, heads: int, dim: int, dtype, device: int) -> None:
+    """Checks ``t`` as [tokens, heads, dim] rows of ``dtype`` on ``device``."""
+    if t.dtype is not dtype:
         raise TypeError(f"{name} must be {dtype}, got {t.dtype}")
     shape = t.shape
     if len(shape) != 3 or shape[1] != heads or shape[2] != dim:
         raise ValueError(f"{name} must be [tokens, {heads}, {dim}], got {tuple(shape)}")
+    if t.get_device() != device:
+        raise ValueError(f"{name} is on {t.device}, not on device {device}")
 
 
-def in_place(t: torch.Tensor) -> torch.Tensor:
-    """``t``, or a copy if its rows do not lie as the kernels read them:
-    contiguous dims, rows on 16-byte boundaries."""
-    if not aligned(t):
-        t = t.contiguous()
-        if t.data_ptr() % 16:
-            t = t.clone()
-    return t
-
-
-def aligned(t: torch.Tensor) -> bool:
-    s = t.stride()
-    return (s[2] == 1 and s[0] % 8 == 0 and s[1] % 8 == 0 and s[0] > 0 and s[1] > 0
-            and t.data_ptr() % 16 == 0)
-
-
-def index(t: torch.Tensor, name: str, tokens: int, device) -> None:
+def index(t: torch.Tensor, name: str, tokens: int, device: int) -> None:
     """Checks ``t`` as int32 or int64 [tokens] on ``device``."""
-    if t.dtype not in (torch.int32, torch.int64):
+    if t.dtype is not torch.int32 and t.dtype is not torch.int64:
         raise TypeError(f"{name} must be int32 or int64, got {t.dtype}")
-    if t.dim() != 1 or t.shape[0] != tokens:
-        raise ValueError(f"{name} must be [{tokens}], got {tuple(t.shape)}")
-    if t.device != device:
-        raise ValueError(f"{name} is on {t.device}, not on {device}")
+    shape = t.shape
+    if len(shape) != 1 or shape[0] != tokens:
+        raise ValueError(f"{name} must be [{tokens}], got {tuple(shape)}")
+    if t.get_device() != device:
+        raise ValueError(f"{name} is on {t.device}, not on device {device}")
+
+
+def in_place(t: torch.Tensor):
+    """(``t``, address, token stride, head stride), or those of a copy if the
+    rows do not lie as the kernels read them: contiguous dims, rows on 16-byte
+    boundaries."""
+    s0, s1, s2 = t.stride()
+    at = t.data_ptr()
+    if s2 == 1 and s0 > 0 and s1 > 0 and not (s0 | s1) & 7 and not at & 15:
+        return t, at, s0, s1
+    t = t.contiguous()
+    if t.data_ptr() & 15:
+        t = t.clone()
+    return t, t.data_ptr(), t.stride(0), t.stride(1)
+
+
+def output(t: torch.Tensor, shape, dtype, device: int):
+    """(``t``, address, token stride, head stride) of an output the caller gives."""
+    if t.shape == shape and t.dtype is dtype and t.get_device() == device:
+        s0, s1, s2 = t.stride()
+        at = t.data_ptr()
+        if s2 == 1 and s0 > 0 and s1 > 0 and not (s0 | s1) & 7 and not at & 15:
+            return t, at, s0, s1
+    raise ValueError(f"out must be {dtype} {tuple(shape)} on device {device}, its rows contiguous on "
+                     "16-byte boundaries")
+
+
+def fresh(like: torch.Tensor, heads: int, dim: int):
+    """(new rows, address, token stride, head stride) of ``like``'s tokens."""
+    t = like.new_empty((like.shape[0], heads, dim))
+    return t, t.data_ptr(), heads * dim, dim
 
 
 class PagedKV:
@@ -134,7 +153,7 @@ class PagedKV:
             raise ValueError("pages * kv_heads * page_size must be in 1 .. 2^31 - 1")
         self.k, self.v, self.k_scale, self.v_scale = k, v, ks, vs
         self.pages, self.kv_heads, self.page_size, self.head_dim = k.shape
-        self.dtype, self.device = k.dtype, k.device
+        self.dtype, self.device, self.device_index = k.dtype, k.device, k.get_device()
         self.desc = _lib.KVCache(k.data_ptr(), v.data_ptr(), ks.data_ptr() if e4m3 else None,
                                  vs.data_ptr() if e4m3 else None, *k.shape, DTYPES[k.dtype])
         self.ref = ctypes.addressof(self.desc)
@@ -159,23 +178,22 @@ def write(cache: PagedKV, k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor,
     tensor are read in place) into ``slots`` (int32 or int64 ``[tokens]``).
     Slots outside the cache -- -1, say, for padding -- are skipped.  The slots
     of one call are distinct: a slot named twice keeps parts of either row."""
-    dev = cache.device
-    dtype = k.dtype
+    dev, dtype = cache.device_index, k.dtype
     code = cache.rows_dtype(dtype)
-    rows(k, "k", cache.kv_heads, cache.head_dim, dtype)
-    rows(v, "v", cache.kv_heads, cache.head_dim, dtype)
+    rows(k, "k", cache.kv_heads, cache.head_dim, dtype, dev)
+    rows(v, "v", cache.kv_heads, cache.head_dim, dtype, dev)
     tokens = k.shape[0]
-    if v.shape[0] != tokens or k.device != dev or v.device != dev:
-        raise ValueError("k and v must have the same tokens and the cache's device")
+    if v.shape[0] != tokens:
+        raise ValueError("k and v must have the same tokens")
     index(slots, "slots", tokens, dev)
     if elsewhere(dev, stream):
         with place(dev, stream):
             return write(cache, k, v, slots)
-    k, v, slots = in_place(k), in_place(v), slots.contiguous()
-    ks, vs = k.stride(), v.stride()
-    rc = _lib.packed("d3_kv_write")(cache.ref, k.data_ptr(), ks[0], ks[1], v.data_ptr(), vs[0], vs[1],
-                                    code, tokens, slots.data_ptr(), slots.element_size(),
-                                    _raw_stream(dev.index))
+    k, k_at, k0, k1 = in_place(k)
+    v, v_at, v0, v1 = in_place(v)
+    slots = slots.contiguous()
+    rc = _lib.packed("d3_kv_write")(cache.ref, k_at, k0, k1, v_at, v0, v1, code, tokens,
+                                    slots.data_ptr(), slots.element_size(), _raw_stream(dev))
     if rc:
         _lib.raise_status(rc, "d3_kv_write")
 
@@ -184,7 +202,7 @@ def read(cache: PagedKV, slots: torch.Tensor, dtype=None, stream=None):
     """(k, v) rows ``[tokens, kv_heads, head_dim]`` at ``slots`` as ``dtype``
     (the cache's own type, or bfloat16 for an e4m3 cache).  A slot outside the
     cache reads as zeros."""
-    dev = cache.device
+    dev = cache.device_index
     if dtype is None:
         dtype = torch.bfloat16 if cache.e4m3 else cache.dtype
     code = cache.rows_dtype(dtype)
@@ -194,9 +212,10 @@ def read(cache: PagedKV, slots: torch.Tensor, dtype=None, stream=None):
             return read(cache, slots, dtype)
     slots = slots.contiguous()
     tokens = slots.shape[0]
-    k, v = torch.empty((2, tokens, cache.kv_heads, cache.head_dim), dtype=dtype, device=dev).unbind(0)
+    k, v = torch.empty((2, tokens, cache.kv_heads, cache.head_dim), dtype=dtype,
+                       device=cache.device).unbind(0)
     rc = _lib.packed("d3_kv_read")(cache.ref, slots.data_ptr(), slots.element_size(), tokens, code,
-                                   k.data_ptr(), v.data_ptr(), _raw_stream(dev.index))
+                                   k.data_ptr(), v.data_ptr(), _raw_stream(dev))
     if rc:
         _lib.raise_status(rc, "d3_kv_read")
     return k, v
