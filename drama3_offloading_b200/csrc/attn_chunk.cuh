@@ -53,6 +53,10 @@ constexpr int kAttnErrChunkLoad = 53, kAttnErrChunkMma = 54, kAttnErrChunkSoftma
               kAttnErrChunkWiden = 56, kAttnErrChunkAlign = 57;
 constexpr int kBlockKeys = 128;
 constexpr float kRescaleLog2 = 8.f;
+// Pages below this go into the code ring by 16-byte copies of a whole warp: a
+// TMA instruction costs its thread some 500 cycles here whatever its size, and
+// a block of 16-token pages is twelve of them.
+constexpr int kSmallPage = 64;
 
 template <typename T, int D, bool E4>
 struct ChunkCfg {
@@ -62,8 +66,8 @@ struct ChunkCfg {
   static constexpr int SLOTS = E4 ? (D == 256 ? 3 : 6) : (D == 256 ? 5 : 10);
   static constexpr int RAW = E4 ? 64 * D : 0;             // the same as codes
   static constexpr int RAWS = E4 ? (D == 256 ? 3 : 6) : 0;
-  static constexpr int SC_RING = 4;                       // scales of 4 blocks: ks, f, 2^e
-  static constexpr int SC_BYTES = E4 ? SC_RING * 3 * kBlockKeys * 4 : 0;
+  static constexpr int SC_RING = 4;                       // scales of 4 blocks: ks, f, 2^e in two words
+  static constexpr int SC_BYTES = E4 ? SC_RING * 4 * kBlockKeys * 4 : 0;
   static constexpr size_t SMEM =
       1024 + Q_BYTES + (size_t)SLOTS * SLOT + (size_t)RAWS * RAW + SC_BYTES + 2048;
   static constexpr int COL_S = 0, COL_O = 256;
@@ -447,10 +451,21 @@ __device__ __forceinline__ uint32_t widen2<__nv_bfloat16>(uint16_t c) {
   const float2 f = e4m3x2_to_f2(c);
   return Elem<__nv_bfloat16>::from_f2(f.x, f.y);
 }
+// ... times a power of two: two fp16 factors, or one fp32 one
 template <typename T>
-__device__ __forceinline__ uint32_t widen2(uint16_t c, float s) {
-  const float2 f = e4m3x2_to_f2(c);
-  return Elem<T>::from_f2(f.x * s, f.y * s);
+__device__ __forceinline__ uint32_t widen2(uint16_t c, uint32_t ea, uint32_t eb);
+template <>
+__device__ __forceinline__ uint32_t widen2<__half>(uint16_t c, uint32_t ea, uint32_t eb) {
+  const uint32_t h = e4m3x2_to_h2(c);
+  __half2 x = __hmul2(*reinterpret_cast<const __half2*>(&h), *reinterpret_cast<const __half2*>(&ea));
+  x = __hmul2(x, *reinterpret_cast<const __half2*>(&eb));
+  return *reinterpret_cast<const uint32_t*>(&x);
+}
+template <>
+__device__ __forceinline__ uint32_t widen2<__nv_bfloat16>(uint16_t c, uint32_t ea, uint32_t) {
+  float2 f = e4m3x2_to_f2(c);
+  mul2(f.x, f.y, __uint_as_float(ea), __uint_as_float(ea));
+  return Elem<__nv_bfloat16>::from_f2(f.x, f.y);
 }
 
 // ---------------------------------------------------------------- kernel
@@ -472,7 +487,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(ChunkCfg<T, D, E4>::
   at += (size_t)C::SLOTS * C::SLOT;
   uint8_t* s_codes = at;
   at += (size_t)C::RAWS * C::RAW;
-  float* s_sc = reinterpret_cast<float*>(at);           // [SC_RING][ks, f, 2^e][128]
+  float* s_sc = reinterpret_cast<float*>(at);           // [SC_RING][ks, f, 2^e, 2^e][128]
   at += C::SC_BYTES;
   float* s_mx = reinterpret_cast<float*>(at);           // [2][2][128]
   uint64_t* full = head.bars;
@@ -494,6 +509,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(ChunkCfg<T, D, E4>::
   const uint32_t sq = smem_u32(smem), ss = smem_u32(s_ring);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const uint32_t rank = cluster_rank();
+  const int ps = p.page_size;
   if (smem_u32(smem_raw) & 1023) {       // the swizzle counts on it
     if (tid == 0) attn_error(p.err, kAttnErrChunkAlign);
     return;
@@ -516,7 +532,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(ChunkCfg<T, D, E4>::
     for (int i = 0; i < 4; ++i) mbar_init(x_bar + i, 2);
     if (E4) {
       for (int i = 0; i < C::RAWS; ++i) {
-        mbar_init(raw_full + i, 1);
+        mbar_init(raw_full + i, ps < kSmallPage ? 32 : 1);     // 32 lanes' copies, or TMA
         mbar_init(raw_empty + i, 4);
       }
       for (int i = 0; i < C::SC_RING; ++i) {
@@ -545,7 +561,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(ChunkCfg<T, D, E4>::
   const int tpc = 128 / p.group, per = 2 * tpc;      // tokens of a CTA, of the pair
   const ChunkPart part = chunk_plan(p, per, pair, pairs, head.scan, &head.part);
   cluster_sync_all();      // both CTAs' barriers are ready
-  const int ps = p.page_size;
 
   bool ok = true;
   // every lane of a warp: false once a wait has run out, here or in another role
@@ -577,7 +592,73 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(ChunkCfg<T, D, E4>::
     return true;
   };
 
-  if (warp == 9 || warp == 10) {
+  // Q of a piece (one thread): rows (token, head) of both CTAs
+  auto load_q = [&](const ChunkPiece& x) {
+    if (rank == 0) mbar_arrive_expect_tx(q_full, 2 * (D / 64) * tpc * p.group * 128);
+    const uint32_t bar = mapa(smem_u32(q_full), 0);
+    const int tok = x.s.q0 + x.tile * per + (int)rank * tpc;
+    for (int c = 0; c < D / 64; ++c) tma_pair_3d(sq + c * (128 * 128), &tm_q, bar, c * 64, x.head * p.group, tok);
+  };
+
+  if (E4 && ps < kSmallPage && (warp == 9 || warp == 10)) {
+    // ---- codes of small pages: a warp copies K, one V, as the TMA threads
+    // below would (same ring, same shifted last page), 512 bytes an instruction
+    auto copy = [&](auto is_v) {
+      constexpr bool v = decltype(is_v)::value;
+      constexpr int RB = v ? D / 2 : D, PPR = RB / 16, RPI = 32 / PPR, ROWS = v ? kBlockKeys : 64;
+      const uint8_t* src0 = static_cast<const uint8_t*>(v ? p.v_codes : p.k_codes) + (v ? (int)rank * RB : 0) +
+                            (lane % PPR) * 16;
+      const int n = ROWS / ps, half = v ? 0 : 64 * (int)rank;
+      ChunkWalk walk(part);
+      ChunkPiece x;
+      bool more = walk.next(p, per, x);
+      int j = more ? x.j0 : 0, id_next = -1, at_pos = 0, base = 0;
+      uint32_t qn = 0;
+      RingPos pos;
+      auto fetch = [&]() {       // lane i: page i of the tile, a block ahead
+        const int key = j * kBlockKeys + half + lane * ps;
+        id_next = lane < n && key < x.s.kv ? __ldcg(p.table + (long long)x.b * p.table_stride + (key >> p.page_shift)) : -1;
+      };
+      if (more) fetch();
+      while (more) {
+        const ChunkPiece y = x;
+        const int key0 = j * kBlockKeys + half, m = x.j1 - x.j0, k = j - x.j0;
+        const int plane = id_next >= 0 && id_next < p.pages ? id_next * p.kv_heads + x.head : -1;
+        if (++j >= x.j1) {
+          more = walk.next(p, per, x);
+          j = more ? x.j0 : 0;
+        }
+        if (more) fetch();
+        const int want = base + (v ? (k == m - 1 ? 2 * m - 1 : 2 * k + 2) : (k ? 2 * k - 1 : 0));
+        for (; at_pos < want; ++at_pos) pos.advance(1, C::RAWS);
+        if (k == m - 1) base += 2 * m;
+        if (!v && k == 0) {
+          if (!wait_warp(q_empty, (qn & 1) ^ 1, kAttnErrChunkLoad)) break;
+          ++qn;
+          if (lane == 0) load_q(y);
+          __syncwarp();
+        }
+        if (!wait_warp(raw_empty + pos.slot, pos.phase ^ 1, kAttnErrChunkLoad)) break;
+        uint32_t dst = smem_u32(s_codes) + pos.slot * C::RAW + lane * 16;
+        for (int pg = 0; pg < n; ++pg) {
+          const int pl = __shfl_sync(0xffffffffu, plane, pg);
+          const int row = lane / PPR - max(0, key0 + pg * ps + ps - y.s.kv);
+          const uint8_t* src = src0 + (((long long)pl << p.page_shift) + row) * D;
+#pragma unroll 4
+          for (int i = 0; i < ps; i += RPI) {
+            const bool in = pl >= 0 && row + i >= 0;
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(in ? src + i * D : src0), "r"(in ? 16 : 0)
+                         : "memory");
+            dst += 512;
+          }
+        }
+        asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(raw_full + pos.slot)) : "memory");
+      }
+      asm volatile("cp.async.wait_all;" ::: "memory");
+    };
+    if (warp == 9) copy(std::false_type{});
+    else copy(std::true_type{});
+  } else if (warp == 9 || warp == 10) {
     // ---- TMA: one thread brings Q of a piece and its K tiles, one its V
     // tiles.  The tiles of a piece of m blocks stand in the ring as K 0, K 1,
     // V 0, K 2, V 1, ..., K m - 1, V m - 2, V m - 1.
@@ -608,11 +689,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(ChunkCfg<T, D, E4>::
         if (!v && k == 0) {
           if (!wait_one(q_empty, (qn & 1) ^ 1, kAttnErrChunkLoad)) break;
           ++qn;
-          if (rank == 0) mbar_arrive_expect_tx(q_full, 2 * (D / 64) * tpc * p.group * 128);
-          const uint32_t bar = mapa(smem_u32(q_full), 0);
-          const int tok = x.s.q0 + x.tile * per + (int)rank * tpc;
-          for (int c = 0; c < D / 64; ++c)
-            tma_pair_3d(sq + c * (128 * 128), &tm_q, bar, c * 64, x.head * p.group, tok);
+          load_q(x);
         }
         if (!wait_one(bars_empty + pos.slot, pos.phase ^ 1, kAttnErrChunkLoad)) break;
         if (E4) mbar_arrive_expect_tx(bars_full + pos.slot, C::RAW);
@@ -729,7 +806,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(ChunkCfg<T, D, E4>::
       float m = -INFINITY, l = 0.f;
       for (int j = w.j0; j < w.j1; ++j, ++it) {
         const uint32_t sb = lanes + C::COL_S + (it & 1) * kBlockKeys;
-        const float* sc = s_sc + (it % C::SC_RING) * 3 * kBlockKeys + h * 64;
+        const float* sc = s_sc + (it % C::SC_RING) * 4 * kBlockKeys + h * 64;
         if (E4) wait(sc_full + it % C::SC_RING, (it / C::SC_RING) & 1);
         wait(s_full + (it & 1), (it >> 1) & 1);
         if (idle) {
@@ -948,7 +1025,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(ChunkCfg<T, D, E4>::
       }
       if (more) load();
       if (!wait_warp(sc_empty + it % C::SC_RING, ((it / C::SC_RING) & 1) ^ 1, kAttnErrChunkWiden)) break;
-      float* sc = s_sc + (it % C::SC_RING) * 3 * kBlockKeys + lane;
+      float* sc = s_sc + (it % C::SC_RING) * 4 * kBlockKeys + lane;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         // v = f * 2^e; a scale without an exponent of its own stays whole
@@ -956,7 +1033,18 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(ChunkCfg<T, D, E4>::
         const bool normal = (b & 0x7f800000u) != 0;
         sc[32 * i] = ck[i];
         sc[kBlockKeys + 32 * i] = normal ? __uint_as_float((b & 0x007fffffu) | 0x3f800000u) : 1.f;
-        sc[2 * kBlockKeys + 32 * i] = normal ? __uint_as_float(b & 0xff800000u) : cv[i];
+        uint32_t* e = reinterpret_cast<uint32_t*>(sc) + 2 * kBlockKeys + 32 * i;
+        if (std::is_same<T, __half>::value) {
+          // 2^e as two fp16 factors, each twice: fp16 codes are multiplied by
+          // them (a scale without an exponent is below fp16's least)
+          const int x = (int)(b >> 23 & 0xff) - 127, x1 = max(-14, min(15, x)), x2 = max(-24, min(15, x - x1));
+          const uint32_t h1 = normal ? ((uint32_t)(x1 + 15) << 10) | (b >> 16 & 0x8000u) : 0u;
+          const uint32_t h2 = x2 >= -14 ? (uint32_t)(x2 + 15) << 10 : 1u << (x2 + 24);
+          e[0] = h1 | h1 << 16;
+          e[kBlockKeys] = h2 | h2 << 16;
+        } else {
+          e[0] = normal ? b & 0xff800000u : b;
+        }
       }
       __syncwarp();
       if (lane == 0) mbar_arrive(sc_full + it % C::SC_RING);
@@ -973,7 +1061,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(ChunkCfg<T, D, E4>::
       constexpr bool v = decltype(is_v)::value;
       // a row is D/16 pieces of K, D/32 of V
       constexpr int per_row = v ? D / 32 : D / 16, rows = v ? kBlockKeys : 64;
-      const float* e2 = s_sc + ((vn % C::SC_RING) * 3 + 2) * kBlockKeys;
+      const uint32_t* e2 = reinterpret_cast<const uint32_t*>(s_sc) + ((vn % C::SC_RING) * 4 + 2) * kBlockKeys;
       if (!wait_warp(raw_full + raw, raw_phase, kAttnErrChunkWiden)) return;
       if (v && !wait_warp(sc_full + vn % C::SC_RING, (vn / C::SC_RING) & 1, kAttnErrChunkWiden)) return;
       if (!wait_warp(empty + slot, phase ^ 1, kAttnErrChunkWiden)) return;
@@ -987,11 +1075,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(ChunkCfg<T, D, E4>::
         const int n = i * 128 + t, r = n / per_row, cpos = n % per_row;
         const uint32_t w4[4] = {u[i].x, u[i].y, u[i].z, u[i].w};
         uint32_t o[8];
-        const float e = v ? e2[r] : 1.f;
+        const uint32_t ea = v ? e2[r] : 0u, eb = v && std::is_same<T, __half>::value ? e2[r + kBlockKeys] : 0u;
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
-          o[2 * q] = v ? widen2<T>((uint16_t)w4[q], e) : widen2<T>((uint16_t)w4[q]);
-          o[2 * q + 1] = v ? widen2<T>((uint16_t)(w4[q] >> 16), e) : widen2<T>((uint16_t)(w4[q] >> 16));
+          o[2 * q] = v ? widen2<T>((uint16_t)w4[q], ea, eb) : widen2<T>((uint16_t)w4[q]);
+          o[2 * q + 1] = v ? widen2<T>((uint16_t)(w4[q] >> 16), ea, eb) : widen2<T>((uint16_t)(w4[q] >> 16));
         }
         // 16 values: two 16-byte pieces of a 64-dim column.  Threads of every
         // second column store theirs the other way round, so that eight
@@ -1045,29 +1133,42 @@ __global__ void __launch_bounds__(256) attn_chunk_join_kernel(const __grid_const
   const int row = blockIdx.y * 32 + (threadIdx.x >> 3), x = threadIdx.x & 7;
   const int rr = row & 127, ti = rr / p.group, tok = de.w * 2 * tpc + (row >> 7) * tpc + ti;
   if (ti >= tpc || tok >= de.y) return;
-  float m = -INFINITY;
-  for (int c = c0; c <= c1; ++c) m = fmaxf(m, __ldcg(ws.ml + (((size_t)c * 2 + (c == c0)) * 256 + row) * 2));
-  const float base = m == -INFINITY ? 0.f : m;
+  // two parts at a time (a tile seldom has more), all of their loads at once
+  float m = -INFINITY, l = 0.f;
   float4 a[D / 32];
 #pragma unroll
   for (int i = 0; i < D / 32; ++i) a[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-  float l = 0.f;
-  for (int c = c0; c <= c1; ++c) {
-    const size_t place = (size_t)c * 2 + (c == c0);
-    const float2 ml = __ldcg(reinterpret_cast<const float2*>(ws.ml) + place * 256 + row);
-    float4 v[D / 32];
+  for (int c = c0; c <= c1; c += 2) {
+    float2 ml[2];
+    float4 v[2][D / 32];
 #pragma unroll
-    for (int i = 0; i < D / 32; ++i)
-      v[i] = __ldcg(reinterpret_cast<const float4*>(ws.o) + (place * (D / 4) + 8 * i + x) * 256 + row);
-    const float f = ex2(ml.x - base);
-    if (f != 0.f) {
-      l = fmaf(ml.y, f, l);
+    for (int k = 0; k < 2; ++k) {
+      ml[k] = make_float2(-INFINITY, 0.f);
+      if (c + k <= c1) {
+        const size_t place = (size_t)(c + k) * 2 + (c + k == c0);
+        ml[k] = __ldcg(reinterpret_cast<const float2*>(ws.ml) + place * 256 + row);
+#pragma unroll
+        for (int i = 0; i < D / 32; ++i)
+          v[k][i] = __ldcg(reinterpret_cast<const float4*>(ws.o) + (place * (D / 4) + 8 * i + x) * 256 + row);
+      }
+    }
+    const float top = fmaxf(m, fmaxf(ml[0].x, ml[1].x)), base = top == -INFINITY ? 0.f : top;
+    const float keep = ex2(m - base);
+    m = top;
+    l *= keep;
+#pragma unroll
+    for (int i = 0; i < D / 32; ++i) a[i] = make_float4(a[i].x * keep, a[i].y * keep, a[i].z * keep, a[i].w * keep);
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      const float f = ex2(ml[k].x - base);
+      if (f == 0.f) continue;
+      l = fmaf(ml[k].y, f, l);
 #pragma unroll
       for (int i = 0; i < D / 32; ++i) {
-        a[i].x = fmaf(v[i].x, f, a[i].x);
-        a[i].y = fmaf(v[i].y, f, a[i].y);
-        a[i].z = fmaf(v[i].z, f, a[i].z);
-        a[i].w = fmaf(v[i].w, f, a[i].w);
+        a[i].x = fmaf(v[k][i].x, f, a[i].x);
+        a[i].y = fmaf(v[k][i].y, f, a[i].y);
+        a[i].z = fmaf(v[k][i].z, f, a[i].z);
+        a[i].w = fmaf(v[k][i].w, f, a[i].w);
       }
     }
   }

@@ -784,7 +784,7 @@ template <typename T, int D>
 __global__ void __launch_bounds__(256) attn_rows_join_kernel(const __grid_constant__ AttnParams p, int rows_per) {
   constexpr int GROUPS = 256 / (D / 4);
   __shared__ float4 s_a[GROUPS][D / 4];
-  __shared__ float s_l[GROUPS];
+  __shared__ float2 s_ml[GROUPS];
   pdl_trigger();
   pdl_wait();
   const int c0 = blockIdx.x, r = blockIdx.y;
@@ -794,42 +794,59 @@ __global__ void __launch_bounds__(256) attn_rows_join_kernel(const __grid_consta
   const int gr = de.w * rows_per + r;
   if (gr >= de.y) return;
   const int g = threadIdx.x / (D / 4), d4 = threadIdx.x % (D / 4);
-  float m = -INFINITY;
-  for (int c = c0 + (threadIdx.x & 31); c <= c1; c += 32)
-    m = fmaxf(m, __ldcg(p.ws_ml + (((size_t)c * 2 + (c == c0)) * rows_per + r) * 2));
-#pragma unroll
-  for (int x = 16; x > 0; x >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, x));
-  const float base = m == -INFINITY ? 0.f : m;
+  // a group's parts four at a time, all of their loads at once
+  float m = -INFINITY, l = 0.f;
   float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
-  float l = 0.f;
-#pragma unroll 4
-  for (int c = c0 + g; c <= c1; c += GROUPS) {
-    const size_t at = ((size_t)c * 2 + (c == c0)) * rows_per + r;
-    const float2 ml = __ldcg(reinterpret_cast<const float2*>(p.ws_ml + at * 2));
-    const float4 v = __ldcg(reinterpret_cast<const float4*>(p.ws_o + at * D) + d4);
-    const float f = ex2(ml.x - base);
-    if (f != 0.f) {
-      l = fmaf(ml.y, f, l);
-      a.x = fmaf(v.x, f, a.x);
-      a.y = fmaf(v.y, f, a.y);
-      a.z = fmaf(v.z, f, a.z);
-      a.w = fmaf(v.w, f, a.w);
+  for (int c = c0 + g; c <= c1; c += 4 * GROUPS) {
+    float2 ml[4];
+    float4 v[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int ck = c + k * GROUPS;
+      ml[k] = make_float2(-INFINITY, 0.f);
+      v[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (ck <= c1) {
+        const size_t at = ((size_t)ck * 2 + (ck == c0)) * rows_per + r;
+        ml[k] = __ldcg(reinterpret_cast<const float2*>(p.ws_ml + at * 2));
+        v[k] = __ldcg(reinterpret_cast<const float4*>(p.ws_o + at * D) + d4);
+      }
+    }
+    const float top = fmaxf(fmaxf(m, fmaxf(ml[0].x, ml[1].x)), fmaxf(ml[2].x, ml[3].x));
+    const float base = top == -INFINITY ? 0.f : top, keep = ex2(m - base);
+    m = top;
+    l *= keep;
+    a = make_float4(a.x * keep, a.y * keep, a.z * keep, a.w * keep);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const float f = ex2(ml[k].x - base);
+      if (f == 0.f) continue;
+      l = fmaf(ml[k].y, f, l);
+      a.x = fmaf(v[k].x, f, a.x);
+      a.y = fmaf(v[k].y, f, a.y);
+      a.z = fmaf(v[k].z, f, a.z);
+      a.w = fmaf(v[k].w, f, a.w);
     }
   }
   s_a[g][d4] = a;
-  if (d4 == 0) s_l[g] = l;
+  if (d4 == 0) s_ml[g] = make_float2(m, l);
   __syncthreads();
   if (g) return;
+  float top = -INFINITY;
+#pragma unroll
+  for (int x = 0; x < GROUPS; ++x) top = fmaxf(top, s_ml[x].x);
+  const float base = top == -INFINITY ? 0.f : top;
   l = 0.f;
   a = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
   for (int x = 0; x < GROUPS; ++x) {
+    const float f = ex2(s_ml[x].x - base);
+    if (f == 0.f) continue;
     const float4 v = s_a[x][d4];
-    l += s_l[x];
-    a.x += v.x;
-    a.y += v.y;
-    a.z += v.z;
-    a.w += v.w;
+    l = fmaf(s_ml[x].y, f, l);
+    a.x = fmaf(v.x, f, a.x);
+    a.y = fmaf(v.y, f, a.y);
+    a.z = fmaf(v.z, f, a.z);
+    a.w = fmaf(v.w, f, a.w);
   }
   const float inv = l > 0.f ? 1.f / l : 0.f;
   T* dst = static_cast<T*>(p.out) + (long long)(de.x + gr / p.group) * p.out_token +
