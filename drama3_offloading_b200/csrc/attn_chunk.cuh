@@ -565,31 +565,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(ChunkCfg<T, D, E4>::
   bool ok = true;
   // every lane of a warp: false once a wait has run out, here or in another role
   auto wait_warp = [&](uint64_t* bar, uint32_t par, int code) {
-    if (!ok) return false;
-    if (__all_sync(0xffffffffu, mbar_try_wait(bar, par))) return true;
-    const uint64_t t0 = globaltimer_ns();
-    while (!__all_sync(0xffffffffu, mbar_try_wait(bar, par)))
-      if (__any_sync(0xffffffffu, s_abort || globaltimer_ns() - t0 > kAttnWaitBudgetNs)) {
-        if (!s_abort) attn_error(p.err, code);
-        s_abort = 1;
-        ok = false;
-        return false;
-      }
-    return true;
+    if (ok && !__all_sync(0xffffffffu, mbar_try_wait(bar, par)))
+      ok = __all_sync(0xffffffffu, wait_on(smem_u32(bar), par, p.err, code, &s_abort));
+    return ok;
   };
   // one thread
   auto wait_one = [&](uint64_t* bar, uint32_t par, int code) {
-    if (!ok) return false;
-    if (mbar_try_wait(bar, par)) return true;
-    const uint64_t t0 = globaltimer_ns();
-    while (!mbar_try_wait(bar, par))
-      if (s_abort || globaltimer_ns() - t0 > kAttnWaitBudgetNs) {
-        if (!s_abort) attn_error(p.err, code);
-        s_abort = 1;
-        ok = false;
-        return false;
-      }
-    return true;
+    if (ok && !mbar_try_wait(bar, par)) ok = wait_on(smem_u32(bar), par, p.err, code, &s_abort);
+    return ok;
   };
 
   // Q of a piece (one thread): rows (token, head) of both CTAs
@@ -597,6 +580,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(ChunkCfg<T, D, E4>::
     if (rank == 0) mbar_arrive_expect_tx(q_full, 2 * (D / 64) * tpc * p.group * 128);
     const uint32_t bar = mapa(smem_u32(q_full), 0);
     const int tok = x.s.q0 + x.tile * per + (int)rank * tpc;
+#pragma unroll 1
     for (int c = 0; c < D / 64; ++c) tma_pair_3d(sq + c * (128 * 128), &tm_q, bar, c * 64, x.head * p.group, tok);
   };
 
@@ -718,6 +702,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(ChunkCfg<T, D, E4>::
       }
       // after a wait ran out: what is in flight has landed before the memory goes
       if (!ok && (E4 || rank == 0))
+#pragma unroll 1
         for (int i = 0; i < N; ++i) mbar_wait(bars_full + i, pos.phase ^ (i <= pos.slot ? 0 : 1), kAttnWaitBudgetNs);
     }
   } else if (warp == 8) {

@@ -70,6 +70,33 @@ struct AttnParams {
 
 __device__ __forceinline__ void attn_error(int* err, int code) { atomicCAS(err, 0, code); }
 
+// The rest of a wait whose first try failed, for one thread or all lanes of a
+// warp: false once it has run out, with the error recorded, or *abort is set.
+// Out of line: a kernel's roles run from different places of its code at once
+// and its many waits in line cost it instruction-cache misses (a chunk of 2048
+// over 30720: 796 us in line, 728 so; the walks out of line, with their state
+// in local memory, made everything slower).
+__device__ __noinline__ bool wait_on(uint32_t bar, uint32_t parity, int* err, int code, volatile int* abort) {
+  const uint64_t t0 = globaltimer_ns();
+  while (true) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(bar), "r"(parity), "r"(20000u)
+        : "memory");
+    if (ok) return true;
+    if (*abort) return false;
+    if (globaltimer_ns() - t0 > kAttnWaitBudgetNs) {
+      attn_error(err, code);
+      *abort = 1;
+      return false;
+    }
+  }
+}
+
 struct AttnSeq {
   int q0, n, kv, rows;           // first query token, new tokens, keys, rows of a KV head
 };
@@ -287,6 +314,7 @@ __global__ void __launch_bounds__(RowsCfg<T, D, E4, NT>::THREADS, 1)
   extern __shared__ uint8_t smem_raw[];
   __shared__ int s_scan[32];
   __shared__ RowsWork s_work;
+  __shared__ volatile int s_abort;
   uint8_t* smem = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
   uint8_t* s_slots = smem;
   uint2* s_q = reinterpret_cast<uint2*>(smem + (size_t)C::SLOTS * C::SLOT);
@@ -298,10 +326,11 @@ __global__ void __launch_bounds__(RowsCfg<T, D, E4, NT>::THREADS, 1)
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   if (tid == 0) {
     for (int i = 0; i < C::SLOTS; ++i) {
-      mbar_init(full + i, 1);
+      mbar_init(full + i, C::LOADERS);
       mbar_init(empty + i, C::WARPS);
     }
     fence_barrier_init();
+    s_abort = 0;
     tma_prefetch_desc(&tm_k);
     tma_prefetch_desc(&tm_v);
   }
@@ -358,13 +387,17 @@ __global__ void __launch_bounds__(RowsCfg<T, D, E4, NT>::THREADS, 1)
         if (more) fetch();
 #pragma unroll
         for (int kv = 0; kv < 2; ++kv) {
-          if (!mbar_wait(empty + slot, phase ^ 1, kAttnWaitBudgetNs)) {
-            attn_error(p.err, kAttnErrRowsLoad);
+          if (!mbar_try_wait(empty + slot, phase ^ 1) &&
+              !wait_on(smem_u32(empty + slot), phase ^ 1, p.err, kAttnErrRowsLoad, &s_abort)) {
             ok = false;
             break;
           }
           const uint32_t dst = smem_u32(s_slots + (size_t)slot * C::SLOT);
+          // every thread arrives, boxes or not: a thread that has none in some
+          // tiles would else be overtaken by two turns of the ring, and wait
+          // for a phase that has come and gone
           if (who == 0) mbar_arrive_expect_tx(full + slot, need * box * D * C::ES);
+          else mbar_arrive(full + slot);
           // a page id outside the cache is loaded from outside the map: zeros
 #pragma unroll
           for (int i = 0; i < MINE; ++i)
@@ -376,6 +409,7 @@ __global__ void __launch_bounds__(RowsCfg<T, D, E4, NT>::THREADS, 1)
       }
       if (!ok) {
         // what is still in flight has landed before the CTA's memory goes
+#pragma unroll 1
         for (int i = 0; i < C::SLOTS; ++i) mbar_wait(full + i, phase ^ (i < slot ? 0 : 1), kAttnWaitBudgetNs);
       }
     }
@@ -391,11 +425,8 @@ __global__ void __launch_bounds__(RowsCfg<T, D, E4, NT>::THREADS, 1)
   bool ok = true;
   auto bar = [&]() { asm volatile("bar.sync 1, %0;" ::"r"(C::WARPS * 32) : "memory"); };
   auto take = [&]() {
-    if (ok && !__all_sync(0xffffffffu, mbar_try_wait(full + slot, phase))) {
-      const bool got = mbar_wait(full + slot, phase, kAttnWaitBudgetNs);
-      if (!got) attn_error(p.err, kAttnErrRowsUse);
-      ok = __all_sync(0xffffffffu, got);
-    }
+    if (ok && !__all_sync(0xffffffffu, mbar_try_wait(full + slot, phase)))
+      ok = __all_sync(0xffffffffu, wait_on(smem_u32(full + slot), phase, p.err, kAttnErrRowsUse, &s_abort));
   };
   auto give = [&]() {
     __syncwarp();
@@ -642,46 +673,39 @@ __global__ void __launch_bounds__(RowsCfg<T, D, E4, NT>::THREADS, 1)
 #pragma unroll
               for (int j = 0; j < 4; ++j) o[n][i][j] *= keep[n][j & 1];
         }
-        auto products = [&](auto is_tail) {
+        if (key0 + 16 > w.s.kv) {
           // values of keys behind the sequence's end are whatever the page
-          // held: cut to zero, 0 * NaN is no zero
-          constexpr bool tail = decltype(is_tail)::value;
-          uint32_t cut0 = ~0u, cut1 = ~0u;
-          if (tail) {
-            const int k2 = key0 + 2 * t4;
-            cut0 = (k2 < w.s.kv ? 0xffffu : 0u) | (k2 + 1 < w.s.kv ? 0xffff0000u : 0u);
-            cut1 = (k2 + 8 < w.s.kv ? 0xffffu : 0u) | (k2 + 9 < w.s.kv ? 0xffff0000u : 0u);
-          }
-          if (E4) {
-            // one 8 x 8 block of code pairs holds 16 dims: dim 2g in the even
-            // bytes, 2g + 1 in the odd ones
+          // held, and 0 * NaN is no zero: this warp's rows are its own to clear
+          for (int r = w.s.kv - key0; r < 16; ++r)
+            for (int x = lane; x < D * C::ES / 16; x += 32)
+              asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(tile_piece(vb, col, r, x)), "r"(0) : "memory");
+          __syncwarp();
+        }
+        if (E4) {
+          // one 8 x 8 block of code pairs holds 16 dims: dim 2g in the even
+          // bytes, 2g + 1 in the odd ones
 #pragma unroll
-            for (int i = 0; i < D / 16; i += 2) {
-              uint32_t r[4];
-              ldsm4t(tile_piece(vb, col, (lm & 1) * 8 + lk, i + (lm >> 1)), r);
+          for (int i = 0; i < D / 16; i += 2) {
+            uint32_t r[4];
+            ldsm4t(tile_piece(vb, col, (lm & 1) * 8 + lk, i + (lm >> 1)), r);
 #pragma unroll
-              for (int c = 0; c < 2; ++c) {
-                const uint32_t x = __byte_perm(r[2 * c], 0, 0x3120), y = __byte_perm(r[2 * c + 1], 0, 0x3120);
-                uint32_t a0 = e4m3x2_to_h2((uint16_t)x), a1 = e4m3x2_to_h2((uint16_t)(x >> 16));
-                uint32_t a2 = e4m3x2_to_h2((uint16_t)y), a3 = e4m3x2_to_h2((uint16_t)(y >> 16));
-                if (tail) { a0 &= cut0; a1 &= cut0; a2 &= cut1; a3 &= cut1; }
+            for (int c = 0; c < 2; ++c) {
+              const uint32_t x = __byte_perm(r[2 * c], 0, 0x3120), y = __byte_perm(r[2 * c + 1], 0, 0x3120);
+              const uint32_t a0 = e4m3x2_to_h2((uint16_t)x), a1 = e4m3x2_to_h2((uint16_t)(x >> 16));
+              const uint32_t a2 = e4m3x2_to_h2((uint16_t)y), a3 = e4m3x2_to_h2((uint16_t)(y >> 16));
 #pragma unroll
-                for (int n = 0; n < NT; ++n) mma16<M>(o[n][i + c], a0, a1, a2, a3, pb[n][0], pb[n][1]);
-              }
-            }
-          } else {
-#pragma unroll
-            for (int i = 0; i < D / 16; ++i) {
-              uint32_t r[4];
-              ldsm4t(tile_piece(vb, col, (lm >> 1) * 8 + lk, 2 * i + (lm & 1)), r);
-              if (tail) { r[0] &= cut0; r[1] &= cut0; r[2] &= cut1; r[3] &= cut1; }
-#pragma unroll
-              for (int n = 0; n < NT; ++n) mma16<M>(o[n][i], r[0], r[1], r[2], r[3], pb[n][0], pb[n][1]);
+              for (int n = 0; n < NT; ++n) mma16<M>(o[n][i + c], a0, a1, a2, a3, pb[n][0], pb[n][1]);
             }
           }
-        };
-        if (key0 + 16 > w.s.kv) products(std::true_type{});
-        else products(std::false_type{});
+        } else {
+#pragma unroll
+          for (int i = 0; i < D / 16; ++i) {
+            uint32_t r[4];
+            ldsm4t(tile_piece(vb, col, (lm >> 1) * 8 + lk, 2 * i + (lm & 1)), r);
+#pragma unroll
+            for (int n = 0; n < NT; ++n) mma16<M>(o[n][i], r[0], r[1], r[2], r[3], pb[n][0], pb[n][1]);
+          }
+        }
       }
       give();
     }
