@@ -17,7 +17,7 @@
 // for the exponentials of 128 x 128 scores on one warpgroup); the
 // exponentials for D = 128.
 //
-// TMEM, 512 columns: two S blocks (P overwrites its own S) and O.  S of block
+// TMEM, 512 columns: two S blocks (P of each half goes over its S) and O.  S of block
 // j + 1 is issued before P V of block j, so the tensor core works while the
 // softmax does.  O is only rescaled when a row's maximum grows by more than 8
 // (in log2): P then stays below 2^8, sums are in fp32 and the quotient of the
@@ -419,6 +419,18 @@ __device__ __forceinline__ void tmem_st32(uint32_t a, const uint32_t* u) {
       "r"(u[28]), "r"(u[29]), "r"(u[30]), "r"(u[31])
       : "memory");
 }
+__device__ __forceinline__ void tmem_ld16f(uint32_t a, float* r) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+      : "=f"(r[0]), "=f"(r[1]), "=f"(r[2]), "=f"(r[3]), "=f"(r[4]), "=f"(r[5]), "=f"(r[6]), "=f"(r[7]), "=f"(r[8]),
+        "=f"(r[9]), "=f"(r[10]), "=f"(r[11]), "=f"(r[12]), "=f"(r[13]), "=f"(r[14]), "=f"(r[15])
+      : "r"(a));
+}
+__device__ __forceinline__ void tmem_st8(uint32_t a, const uint32_t* u) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(a), "r"(u[0]), "r"(u[1]),
+               "r"(u[2]), "r"(u[3]), "r"(u[4]), "r"(u[5]), "r"(u[6]), "r"(u[7])
+               : "memory");
+}
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
 // Descriptor of an operand whose contiguous dim is the MMA's N (V: dims), with
@@ -715,6 +727,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(ChunkCfg<T, D, E4>::
       uint32_t phase = 0, it = 0, pieces = 0;
       // V: pages of `vrows` keys, each [D / 128 columns][vrows][128 bytes]; 16 keys a k-step
       const int vrows = E4 ? kBlockKeys : ps;
+      const uint64_t qd = smem_desc_k128(sq);
       auto wait = [&](uint64_t* bar, uint32_t par) { return wait_one(bar, par, kAttnErrChunkMma); };
       auto advance = [&]() {
         commit_pair(empty + slot);
@@ -723,11 +736,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(ChunkCfg<T, D, E4>::
       auto scores = [&](uint32_t x) {
         if (!wait(full + slot, phase)) return;
         tc_fence_after();
-        const uint32_t kb = ss + slot * C::SLOT, d = tmem + C::COL_S + (x & 1) * kBlockKeys;
+        // descriptors count in 16 bytes: a k-step is an addition
+        const uint64_t kd = smem_desc_k128(ss + slot * C::SLOT);
+        const uint32_t d = tmem + C::COL_S + (x & 1) * kBlockKeys;
 #pragma unroll
         for (int k = 0; k < D / 16; ++k)
-          mma_pair_ss(d, smem_desc_k128(sq + (k >> 2) * (128 * 128) + (k & 3) * 32),
-                      smem_desc_k128(kb + (k >> 2) * (64 * 128) + (k & 3) * 32), id_s, k > 0);
+          mma_pair_ss(d, qd + ((k >> 2) * (128 * 128) + (k & 3) * 32) / 16,
+                      kd + ((k >> 2) * (64 * 128) + (k & 3) * 32) / 16, id_s, k > 0);
         commit_pair(s_full + (x & 1));
         advance();
       };
@@ -736,12 +751,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(ChunkCfg<T, D, E4>::
         if (!wait(p_ready + (x & 1), (x >> 1) & 1)) return;
         if (first && pieces > 0 && !wait(o_free, (pieces - 1) & 1)) return;
         tc_fence_after();
-        const uint32_t vb = ss + slot * C::SLOT, a = tmem + C::COL_S + (x & 1) * kBlockKeys;
+        const uint64_t vd = smem_desc_n128(ss + slot * C::SLOT, vrows * 128);
+        const uint32_t a = tmem + C::COL_S + (x & 1) * kBlockKeys;
 #pragma unroll
         for (int k = 0; k < kBlockKeys / 16; ++k)
-          mma_pair_ts(tmem + C::COL_O, a + k * 8,
-                      smem_desc_n128(vb + (k * 16 & -vrows) * D + (k * 16 & (vrows - 1)) * 128, vrows * 128), id_o,
-                      !first || k > 0);
+          mma_pair_ts(tmem + C::COL_O, a + (k >> 2) * 64 + (k & 3) * 8,
+                      vd + ((k * 16 & -vrows) * D + (k * 16 & (vrows - 1)) * 128) / 16, id_o, !first || k > 0);
         commit_pair(o_done);
         advance();
       };
@@ -802,20 +817,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(ChunkCfg<T, D, E4>::
           continue;
         }
         tc_fence_after();
-        float s[64];
-        tmem_ld32(sb + 64 * h, s);
-        tmem_ld32(sb + 64 * h + 32, s + 32);
-        tmem_ld_wait();
-        if (E4) {
-#pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            const float4 f = reinterpret_cast<const float4*>(sc)[i];
-            mul2(s[4 * i], s[4 * i + 1], f.x, f.y);
-            mul2(s[4 * i + 2], s[4 * i + 3], f.z, f.w);
-          }
-        }
         const int lim = last - j * kBlockKeys;                    // last visible key of the block
-        if (__any_sync(0xffffffffu, lim < kBlockKeys - 1)) {
+        const bool masked = __any_sync(0xffffffffu, lim < kBlockKeys - 1);
+        unsigned long long see = ~0ull;                           // this half's visible columns
+        if (masked) {
           // columns from t0 hold the sequence's last page, `shift` columns late
           const int valid = w.s.kv - j * kBlockKeys;
           int t0 = kBlockKeys, shift = 0;
@@ -823,23 +828,49 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(ChunkCfg<T, D, E4>::
             t0 = (valid - 1) / ps * ps;
             shift = t0 + ps - valid;
           }
-          // bits of this half's visible columns
           auto below = [&](int n) {
             n -= 64 * h;
             return n <= 0 ? 0ull : n >= 64 ? ~0ull : (1ull << n) - 1;
           };
-          const unsigned long long see = below(min(t0, lim + 1)) | (below(lim + shift + 1) & ~below(t0 + shift));
-          const uint32_t see2[2] = {(uint32_t)see, (uint32_t)(see >> 32)};
-#pragma unroll
-          for (int i = 0; i < 64; ++i) s[i] = see2[i >> 5] & (1u << (i & 31)) ? s[i] : -INFINITY;
+          see = below(min(t0, lim + 1)) | (below(lim + shift + 1) & ~below(t0 + shift));
         }
-        float m4[4] = {s[0], s[1], s[2], s[3]};
+        // STEP columns at a time: all 64 stay in registers from the maximum to
+        // the exponentials, or, with codes, where the widening warps' code
+        // fills the instruction cache, a short loop reads them from TMEM twice
+        constexpr int STEP = E4 ? 16 : 64;
+        float s[STEP];
+        auto columns = [&](int c0) {
+          if (STEP == 64) {
+            tmem_ld32(sb + 64 * h, s);
+            tmem_ld32(sb + 64 * h + 32, s + STEP / 2);
+          } else {
+            tmem_ld16f(sb + 64 * h + c0, s);
+          }
+          tmem_ld_wait();
+          if (E4) {
 #pragma unroll
-        for (int i = 4; i < 64; ++i) m4[i & 3] = fmaxf(m4[i & 3], s[i]);
+            for (int i = 0; i < STEP / 4; ++i) {
+              const float4 f = reinterpret_cast<const float4*>(sc + c0)[i];
+              mul2(s[4 * i], s[4 * i + 1], f.x, f.y);
+              mul2(s[4 * i + 2], s[4 * i + 3], f.z, f.w);
+            }
+          }
+          if (masked) {
+            const unsigned long long bits = see >> c0;
+            const uint32_t see2[2] = {(uint32_t)bits, (uint32_t)(bits >> 32)};
+#pragma unroll
+            for (int i = 0; i < STEP; ++i) s[i] = see2[i >> 5] & (1u << (i & 31)) ? s[i] : -INFINITY;
+          }
+        };
+        float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll 1
+        for (int c0 = 0; c0 < 64; c0 += STEP) {
+          columns(c0);
+#pragma unroll
+          for (int i = 0; i < STEP; ++i) m4[i & 3] = fmaxf(m4[i & 3], s[i]);
+        }
         float mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * c;
-        // the other half's maximum; both threads then decide alike.  (The
-        // exchange also says that both halves of S are in registers: P of half
-        // 1 goes over S of half 0.)
+        // the other half's maximum: both threads then decide alike
         mx = fmaxf(mx, exchange(mx));
         const bool grow = mx > m + kRescaleLog2 || (m == -INFINITY && mx > m);
         if (__any_sync(0xffffffffu, grow)) {
@@ -868,21 +899,27 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(ChunkCfg<T, D, E4>::
         }
         const float base = m == -INFINITY ? 0.f : m;
         float l2[2] = {0.f, 0.f};
-        uint32_t pk[32];
+#pragma unroll 1
+        for (int c0 = 0; c0 < 64; c0 += STEP) {
+          if (STEP < 64) columns(c0);
+          uint32_t pk[STEP / 2];
 #pragma unroll
-        for (int q = 0; q < 32; ++q) {
-          float a = s[2 * q], b = s[2 * q + 1];
-          fma2(a, b, c, -base);
-          a = ex2(a);
-          b = ex2(b);
-          add2(l2[0], l2[1], a, b);
-          if (E4) {
-            const float2 f = reinterpret_cast<const float2*>(sc + kBlockKeys)[q];
-            mul2(a, b, f.x, f.y);
+          for (int q = 0; q < STEP / 2; ++q) {
+            float a = s[2 * q], b = s[2 * q + 1];
+            fma2(a, b, c, -base);
+            a = ex2(a);
+            b = ex2(b);
+            add2(l2[0], l2[1], a, b);
+            if (E4) {
+              const float2 f = reinterpret_cast<const float2*>(sc + kBlockKeys + c0)[q];
+              mul2(a, b, f.x, f.y);
+            }
+            pk[q] = Elem<T>::from_f2(a, b);
           }
-          pk[q] = Elem<T>::from_f2(a, b);
+          // P of a half goes over the S columns that its own threads have read
+          if (STEP == 64) tmem_st32(sb + 64 * h, pk);
+          else tmem_st8(sb + 64 * h + c0 / 2, pk);
         }
-        tmem_st32(sb + 32 * h, pk);
         l += l2[0] + l2[1];
         tmem_st_wait();
         tc_fence_before();
@@ -1052,13 +1089,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(ChunkCfg<T, D, E4>::
       if (!wait_warp(empty + slot, phase ^ 1, kAttnErrChunkWiden)) return;
       const uint4* src = reinterpret_cast<const uint4*>(s_codes + (size_t)raw * C::RAW);
       uint8_t* dst = s_ring + (size_t)slot * C::SLOT;
-      uint4 u[PIECES];
-#pragma unroll
-      for (int i = 0; i < PIECES; ++i) u[i] = src[i * 128 + t];
-#pragma unroll
+#pragma unroll 2
       for (int i = 0; i < PIECES; ++i) {
+        const uint4 u = src[i * 128 + t];
         const int n = i * 128 + t, r = n / per_row, cpos = n % per_row;
-        const uint32_t w4[4] = {u[i].x, u[i].y, u[i].z, u[i].w};
+        const uint32_t w4[4] = {u.x, u.y, u.z, u.w};
         uint32_t o[8];
         const uint32_t ea = v ? e2[r] : 0u, eb = v && std::is_same<T, __half>::value ? e2[r + kBlockKeys] : 0u;
 #pragma unroll
