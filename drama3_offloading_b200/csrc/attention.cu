@@ -104,7 +104,7 @@ static int set_smem(K kernel, size_t bytes, bool (&done)[64]) {
 }
 
 template <typename T, int D, bool E4, int NT>
-static int launch_rows(AttnParams p, const d3_attention* a, const d3_kv_cache* c, cudaStream_t st) {
+static int launch_rows(const AttnParams& p, const d3_attention* a, const d3_kv_cache* c, int* parts_out, cudaStream_t st) {
   using C = RowsCfg<T, D, E4, NT>;
   static bool done[64] = {false};
   int rc;
@@ -124,15 +124,13 @@ static int launch_rows(AttnParams p, const d3_attention* a, const d3_kv_cache* c
   D3_CUDA_TRY(launch_k(attn_rows_kernel<T, D, E4, NT>, dim3(parts), dim3(C::THREADS), C::SMEM, st,
                        pdl_enabled(), tk, tv, p),
               "attn_rows_kernel launch");
-  D3_CUDA_TRY(launch_k(attn_rows_join_kernel<T, D>, dim3(parts, C::ROWS), dim3(256), 0, st, pdl_enabled(), p,
-                       (int)C::ROWS),
-              "attn_rows_join_kernel launch");
+  *parts_out = parts;
   return D3_OK;
 }
 
 template <typename T, int D, bool E4>
 static int launch_chunk(const AttnParams& p, const d3_attention* a, const d3_kv_cache* c, const ChunkWs& ws,
-                        cudaStream_t st) {
+                        int* pairs_out, cudaStream_t st) {
   using C = ChunkCfg<T, D, E4>;
   static bool done[64] = {false};
   int rc;
@@ -157,9 +155,7 @@ static int launch_chunk(const AttnParams& p, const d3_attention* a, const d3_kv_
   D3_CUDA_TRY(launch_k(attn_chunk_kernel<T, D, E4>, dim3(2 * pairs), dim3(C::THREADS), C::SMEM, st, pdl_enabled(),
                        tq, tk, tv, p, ws),
               "attn_chunk_kernel launch");
-  D3_CUDA_TRY(launch_k(attn_chunk_join_kernel<T, D>, dim3(pairs, 8), dim3(256), 0, st, pdl_enabled(),
-                       p, ws),
-              "attn_chunk_join_kernel launch");
+  *pairs_out = pairs;
   return D3_OK;
 }
 
@@ -170,21 +166,31 @@ template <typename T, int D, bool E4>
 static int launch_attention(AttnParams p, const d3_attention* a, const d3_kv_cache* c, const ChunkWs& ws,
                             cudaStream_t st) {
   const long long rows = (long long)a->max_q * p.group;
-  int rc = D3_OK;
-  if (rows <= 8) return launch_rows<T, D, E4, 1>(p, a, c, st);
-  if (rows <= kRowsMost) return launch_rows<T, D, E4, 2>(p, a, c, st);
-  if ((long long)a->batch * a->max_q != a->tokens && p.group <= kRowsMost) {
-    // mostly single tokens among chunks: eight rows where a token has no more
-    // (sixteen cost the row kernel twice the products)
-    AttnParams few = p;
-    few.max_rows = p.group <= 8 ? 8 : kRowsMost;
-    d3_attention one = *a;
-    one.max_q = few.max_rows / p.group;
-    if ((rc = few.max_rows == 8 ? launch_rows<T, D, E4, 1>(few, &one, c, st) : launch_rows<T, D, E4, 2>(few, &one, c, st)))
-      return rc;
-    p.min_rows = few.max_rows + 1;
+  int rc = D3_OK, parts = 0, pairs = 0, rows_per = 8;
+  if (rows <= kRowsMost) {
+    rows_per = rows <= 8 ? 8 : 16;
+    rc = rows_per == 8 ? launch_rows<T, D, E4, 1>(p, a, c, &parts, st) : launch_rows<T, D, E4, 2>(p, a, c, &parts, st);
+  } else {
+    if ((long long)a->batch * a->max_q != a->tokens && p.group <= kRowsMost) {
+      // mostly single tokens among chunks: eight rows where a token has no more
+      // (sixteen cost the row kernel twice the products)
+      AttnParams few = p;
+      few.max_rows = rows_per = p.group <= 8 ? 8 : kRowsMost;
+      d3_attention one = *a;
+      one.max_q = few.max_rows / p.group;
+      if ((rc = rows_per == 8 ? launch_rows<T, D, E4, 1>(few, &one, c, &parts, st)
+                              : launch_rows<T, D, E4, 2>(few, &one, c, &parts, st)))
+        return rc;
+      p.min_rows = few.max_rows + 1;
+    }
+    rc = launch_chunk<T, D, E4>(p, a, c, ws, &pairs, st);
   }
-  return launch_chunk<T, D, E4>(p, a, c, ws, st);
+  if (rc) return rc;
+  const unsigned y = parts ? (unsigned)rows_per : 8u;
+  D3_CUDA_TRY(launch_k(attn_join_kernel<T, D>, dim3(parts + pairs, y < 8 ? 8 : y), dim3(256), 0, st, pdl_enabled(), p,
+                       rows_per, parts, ws),
+              "attn_join_kernel launch");
+  return D3_OK;
 }
 
 }  // namespace d3

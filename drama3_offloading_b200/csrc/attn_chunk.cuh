@@ -97,23 +97,28 @@ __device__ __forceinline__ AttnSeq seq_from(const AttnSeq& s, int lane) {
   r.rows = __shfl_sync(0xffffffffu, s.rows, lane);
   return r;
 }
-// one warp: key blocks of all row tiles of a sequence, for one KV head
-__device__ __forceinline__ int warp_head_units(const AttnSeq& s, int per) {
+// Every row tile stands in the list with its key blocks and `more` units in
+// front of them, about what a piece costs besides (queries in, output out): a
+// prompt's first tiles have one block each.
+template <int D>
+constexpr int kTileUnits = D == 256 ? 2 : 3;
+// one warp: units of all row tiles of a sequence, for one KV head
+__device__ __forceinline__ int warp_head_units(const AttnSeq& s, int per, int more) {
   int u = 0;
-  for (int i = threadIdx.x & 31; i < chunk_tiles(s, per); i += 32) u += chunk_blocks(s, per, i);
+  for (int i = threadIdx.x & 31; i < chunk_tiles(s, per); i += 32) u += chunk_blocks(s, per, i) + more;
   return __reduce_add_sync(0xffffffffu, u);
 }
 
 // A part of the list: where it begins and how long it is.
 struct ChunkPart {
   int total, begin, count;
-  int b, head, tile, j;
+  int b, head, tile, pos;        // place in the tile's units
 };
 // All threads of the CTA.  Each warp takes a run of sequences, 32 at a time:
 // their lanes read the lengths, and the whole warp adds up the blocks of each
 // that this launch takes.  The host has checked that the list is shorter than
 // 2^31.
-__device__ ChunkPart chunk_plan(const AttnParams& p, int per, int part, int parts, int* s_scan,
+__device__ ChunkPart chunk_plan(const AttnParams& p, int per, int more, int part, int parts, int* s_scan,
                                 ChunkPart* s_part) {
   const int warps = blockDim.x >> 5, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int run = (p.batch + warps - 1) / warps, b0 = min(p.batch, warp * run), b1 = min(p.batch, b0 + run);
@@ -131,7 +136,7 @@ __device__ ChunkPart chunk_plan(const AttnParams& p, int per, int part, int part
     }
   };
   each([&](int, const AttnSeq& s) {
-    sum += warp_head_units(s, per) * p.kv_heads;
+    sum += warp_head_units(s, per, more) * p.kv_heads;
     return false;
   });
   if (lane == 0) s_scan[warp] = sum;
@@ -147,7 +152,7 @@ __device__ ChunkPart chunk_plan(const AttnParams& p, int per, int part, int part
   if (count > 0 && before <= begin && begin < before + sum) {
     int at = before;
     each([&](int b, const AttnSeq& s) {
-      const int u = warp_head_units(s, per);
+      const int u = warp_head_units(s, per, more);
       if (begin >= at + u * p.kv_heads) {
         at += u * p.kv_heads;
         return false;
@@ -156,7 +161,7 @@ __device__ ChunkPart chunk_plan(const AttnParams& p, int per, int part, int part
       int r = begin - at - head * u;
       for (int i0 = 0;; i0 += 32) {          // the row tile: 32 at a time
         const int i = i0 + lane;
-        const int n = i < chunk_tiles(s, per) ? chunk_blocks(s, per, i) : 0;
+        const int n = i < chunk_tiles(s, per) ? chunk_blocks(s, per, i) + more : 0;
         int inc = n;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -192,38 +197,41 @@ struct ChunkPiece {
 };
 // Walks a part piece by piece.
 struct ChunkWalk {
-  int b, left, head, tile, j;
+  int b, left, head, tile, pos, more;
   bool fresh;
   AttnSeq s;
-  __device__ __forceinline__ explicit ChunkWalk(const ChunkPart& c)
-      : b(c.b), left(c.count), head(c.head), tile(c.tile), j(c.j), fresh(true) {}
+  __device__ __forceinline__ ChunkWalk(const ChunkPart& c, int more_)
+      : b(c.b), left(c.count), head(c.head), tile(c.tile), pos(c.pos), more(more_), fresh(true) {}
   __device__ __forceinline__ bool next(const AttnParams& p, int per, ChunkPiece& w) {
-    if (left <= 0) return false;
-    if (fresh) {
-      fresh = false;
-      s = attn_seq(p, b);
-    } else {
-      j = 0;
-      if (++tile >= chunk_tiles(s, per)) {
-        tile = 0;
-        if (++head >= p.kv_heads) {
-          head = 0;
-          do {
-            if (++b >= p.batch) return false;
-            s = attn_seq(p, b);
-          } while (!chunk_takes(p, s));
+    while (left > 0) {
+      if (fresh) {
+        fresh = false;
+        s = attn_seq(p, b);
+      } else {
+        pos = 0;
+        if (++tile >= chunk_tiles(s, per)) {
+          tile = 0;
+          if (++head >= p.kv_heads) {
+            head = 0;
+            do {
+              if (++b >= p.batch) return false;
+              s = attn_seq(p, b);
+            } while (!chunk_takes(p, s));
+          }
         }
       }
+      const int nb = chunk_blocks(s, per, tile), take = min(left, nb + more - pos);
+      left -= take;
+      w.s = s;
+      w.b = b;
+      w.head = head;
+      w.tile = tile;
+      w.nb = nb;
+      w.j0 = max(0, pos - more);
+      w.j1 = max(0, pos + take - more);
+      if (w.j1 > w.j0) return true;      // else nothing but the units in front
     }
-    w.s = s;
-    w.b = b;
-    w.head = head;
-    w.tile = tile;
-    w.nb = chunk_blocks(s, per, tile);
-    w.j0 = j;
-    w.j1 = min(w.nb, j + left);
-    left -= w.j1 - w.j0;
-    return true;
+    return false;
   }
 };
 // Walks it tile by tile in the order of the ring: K j0, K j0 + 1, V j0, ...,
@@ -233,7 +241,7 @@ struct ChunkTiles {
   ChunkPiece w;
   int j, step;
   bool is_v;
-  __device__ __forceinline__ explicit ChunkTiles(const ChunkPart& c) : walk(c), step(-1) { w.j0 = w.j1 = 0; }
+  __device__ __forceinline__ ChunkTiles(const ChunkPart& c, int more) : walk(c, more), step(-1) { w.j0 = w.j1 = 0; }
   __device__ __forceinline__ bool next(const AttnParams& p, int per) {
     // steps of a piece of n blocks: 0: K0; 2k - 1: K k; 2k: V k - 1; 2n - 1: V n - 1
     const int n = w.j1 - w.j0;
@@ -295,7 +303,7 @@ struct ChunkBlocks {
   int j;
   bool more;
   int ids[8];
-  __device__ __forceinline__ explicit ChunkBlocks(const ChunkPart& c) : walk(c), j(0), more(false) {}
+  __device__ __forceinline__ ChunkBlocks(const ChunkPart& c, int units) : walk(c, units), j(0), more(false) {}
   __device__ __forceinline__ void fetch(const AttnParams& p, int key0, int box, int n) {
     const int* row = p.table + (long long)w.b * p.table_stride;
     const int key = j * kBlockKeys + key0;
@@ -488,6 +496,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(ChunkCfg<T, D, E4>::
                       const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ AttnParams p,
                       const ChunkWs ws) {
   using C = ChunkCfg<T, D, E4>;
+  constexpr int MORE = kTileUnits<D>;
   // no static shared memory: the dynamic part begins on a 1024-byte boundary
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   ChunkHead& head = *reinterpret_cast<ChunkHead*>(smem_raw);
@@ -571,7 +580,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(ChunkCfg<T, D, E4>::
   pdl_wait();
   const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
   const int tpc = 128 / p.group, per = 2 * tpc;      // tokens of a CTA, of the pair
-  const ChunkPart part = chunk_plan(p, per, pair, pairs, head.scan, &head.part);
+  const ChunkPart part = chunk_plan(p, per, MORE, pair, pairs, head.scan, &head.part);
   cluster_sync_all();      // both CTAs' barriers are ready
 
   bool ok = true;
@@ -605,7 +614,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(ChunkCfg<T, D, E4>::
       const uint8_t* src0 = static_cast<const uint8_t*>(v ? p.v_codes : p.k_codes) + (v ? (int)rank * RB : 0) +
                             (lane % PPR) * 16;
       const int n = ROWS / ps, half = v ? 0 : 64 * (int)rank;
-      ChunkWalk walk(part);
+      ChunkWalk walk(part, MORE);
       ChunkPiece x;
       bool more = walk.next(p, per, x);
       int j = more ? x.j0 : 0, id_next = -1, at_pos = 0, base = 0;
@@ -668,7 +677,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(ChunkCfg<T, D, E4>::
       // small pages, whose rows of one column have to lie together.
       const int rows = v ? kBlockKeys : 64, box = min(ps, rows), n = rows / box;
       const int key0 = v ? 0 : 64 * (int)rank;
-      ChunkBlocks bl(part);
+      ChunkBlocks bl(part, MORE);
       bl.first(p, per, key0, box, n);
       uint32_t qn = 0;
       int at_pos = 0, base = 0;
@@ -721,7 +730,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(ChunkCfg<T, D, E4>::
     // ---- MMAs of the pair
     if (rank == 0 && lane == 0) {
       constexpr uint32_t id_s = idesc_16<T>(256, kBlockKeys, false), id_o = idesc_16<T>(256, D, true);
-      ChunkWalk walk(part);
+      ChunkWalk walk(part, MORE);
       ChunkPiece w;
       int slot = 0;
       uint32_t phase = 0, it = 0, pieces = 0;
@@ -792,7 +801,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(ChunkCfg<T, D, E4>::
       return buf[(h ^ 1) * 128];
     };
     auto wait = [&](uint64_t* bar, uint32_t par) { wait_warp(bar, par, kAttnErrChunkSoftmax); };
-    ChunkWalk walk(part);
+    ChunkWalk walk(part, MORE);
     ChunkPiece w;
     uint32_t it = 0, pieces = 0;
     int4 desc = make_int4(0, 0, 0, 0);
@@ -1013,7 +1022,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(ChunkCfg<T, D, E4>::
   } else if (E4 && warp == 11) {
     // ---- scales: lane has columns lane + 32 i of every block, in the order
     // of the loaded rows; the next block's are on their way while one is stored
-    ChunkWalk walk(part);
+    ChunkWalk walk(part, MORE);
     ChunkPiece w;
     uint32_t it = 0;
     int j = 0;
@@ -1076,7 +1085,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(ChunkCfg<T, D, E4>::
     // ---- codes to 16 bits: raw ring -> operand ring
     const int t = tid - 384;
     constexpr int PIECES = 64 * D / 16 / 128;      // 16-code pieces of a thread
-    ChunkTiles tl(part);
+    ChunkTiles tl(part, MORE);
     int slot = 0, raw = 0;
     uint32_t phase = 0, raw_phase = 0, vn = 0;
     auto widen = [&](auto is_v) {
@@ -1139,18 +1148,15 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(ChunkCfg<T, D, E4>::
 }
 
 // Tiles that the parts' cuts go through: the sum of their parts, in order.
-// blockIdx.x is the part in which the tile begins; a block takes 32 rows, eight
-// threads a row, each 4 dims of every 32.
+// c0 is the part in which the tile begins; a block takes 32 rows, eight threads
+// a row, each 4 dims of every 32.
 template <typename T, int D>
-__global__ void __launch_bounds__(256) attn_chunk_join_kernel(const __grid_constant__ AttnParams p, const ChunkWs ws) {
-  pdl_trigger();
-  pdl_wait();
-  const int c0 = blockIdx.x;
+__device__ __forceinline__ void chunk_join(const AttnParams& p, const ChunkWs& ws, int c0, int group) {
   const int4 de = __ldcg(ws.desc + 2 * c0);
   const int c1 = __ldcg(ws.desc + 2 * c0 + 1).x;
   if (c1 < 0) return;
   const int tpc = 128 / p.group;
-  const int row = blockIdx.y * 32 + (threadIdx.x >> 3), x = threadIdx.x & 7;
+  const int row = group * 32 + (threadIdx.x >> 3), x = threadIdx.x & 7;
   const int rr = row & 127, ti = rr / p.group, tok = de.w * 2 * tpc + (row >> 7) * tpc + ti;
   if (ti >= tpc || tok >= de.y) return;
   // two parts at a time (a tile seldom has more), all of their loads at once
@@ -1199,6 +1205,19 @@ __global__ void __launch_bounds__(256) attn_chunk_join_kernel(const __grid_const
   for (int i = 0; i < D / 32; ++i)
     *reinterpret_cast<uint2*>(dst + 32 * i) =
         make_uint2(Elem<T>::from_f2(a[i].x * inv, a[i].y * inv), Elem<T>::from_f2(a[i].z * inv, a[i].w * inv));
+}
+
+// What the row kernel (blocks [0, rows_parts) of x) and the chunk kernel cut.
+template <typename T, int D>
+__global__ void __launch_bounds__(256) attn_join_kernel(const __grid_constant__ AttnParams p, int rows_per,
+                                                        int rows_parts, const ChunkWs ws) {
+  pdl_trigger();
+  pdl_wait();
+  if ((int)blockIdx.x < rows_parts) {
+    if ((int)blockIdx.y < rows_per) rows_join<T, D>(p, rows_per, blockIdx.x, blockIdx.y);
+  } else if (blockIdx.y < 8) {
+    chunk_join<T, D>(p, ws, blockIdx.x - rows_parts, blockIdx.y);
+  }
 }
 
 }  // namespace d3

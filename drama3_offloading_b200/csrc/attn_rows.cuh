@@ -799,19 +799,16 @@ __global__ void __launch_bounds__(RowsCfg<T, D, E4, NT>::THREADS, 1)
 }
 
 // Pairs that the parts' cuts go through: the sum of their parts, in the parts'
-// order.  blockIdx.x is the part in which the pair begins, blockIdx.y the row;
+// order.  c0 is the part in which the pair begins, r the row;
 // the threads take turns of D/4 over the parts and add up through shared
 // memory.  The workspace is read through L2: launched early, this kernel
 // shares SMs with the join of the call before, whose lines of the same memory
 // may still be in L1.
 template <typename T, int D>
-__global__ void __launch_bounds__(256) attn_rows_join_kernel(const __grid_constant__ AttnParams p, int rows_per) {
+__device__ __forceinline__ void rows_join(const AttnParams& p, int rows_per, int c0, int r) {
   constexpr int GROUPS = 256 / (D / 4);
   __shared__ float4 s_a[GROUPS][D / 4];
   __shared__ float2 s_ml[GROUPS];
-  pdl_trigger();
-  pdl_wait();
-  const int c0 = blockIdx.x, r = blockIdx.y;
   const int4 de = __ldcg(p.ws_desc + 2 * c0);
   const int c1 = __ldcg(p.ws_desc + 2 * c0 + 1).x;
   if (c1 < 0) return;
