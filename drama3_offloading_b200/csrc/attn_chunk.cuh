@@ -113,6 +113,7 @@ __device__ __forceinline__ int warp_head_units(const AttnSeq& s, int per, int mo
 struct ChunkPart {
   int total, begin, count;
   int b, head, tile, pos;        // place in the tile's units
+  AttnSeq s;
 };
 // All threads of the CTA.  Each warp takes a run of sequences, 32 at a time:
 // their lanes read the lengths, and the whole warp adds up the blocks of each
@@ -123,10 +124,12 @@ __device__ ChunkPart chunk_plan(const AttnParams& p, int per, int more, int part
   const int warps = blockDim.x >> 5, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int run = (p.batch + warps - 1) / warps, b0 = min(p.batch, warp * run), b1 = min(p.batch, b0 + run);
   int sum = 0;
+  AttnSeq held{0, 0, 0, 0};      // the lane's first sequence, read once
+  if (b0 + lane < b1) held = attn_seq(p, b0 + lane);
   auto each = [&](auto f) {      // f(b, sequence) until it says true
     for (int at = b0; at < b1; at += 32) {
-      AttnSeq s{0, 0, 0, 0};
-      if (at + lane < b1) s = attn_seq(p, at + lane);
+      AttnSeq s = held;
+      if (at > b0 && at + lane < b1) s = attn_seq(p, at + lane);
       unsigned todo = __ballot_sync(0xffffffffu, at + lane < b1 && chunk_takes(p, s));
       while (todo) {
         const int i = __ffs(todo) - 1;
@@ -170,14 +173,14 @@ __device__ ChunkPart chunk_plan(const AttnParams& p, int per, int more, int part
         }
         const int all = __shfl_sync(0xffffffffu, inc, 31);
         if (r < all) {
-          if (inc - n <= r && r < inc) *s_part = ChunkPart{total, begin, count, b, head, i, r - (inc - n)};
+          if (inc - n <= r && r < inc) *s_part = ChunkPart{total, begin, count, b, head, i, r - (inc - n), s};
           return true;
         }
         r -= all;
       }
     });
   } else if (count == 0 && threadIdx.x == 0) {
-    *s_part = ChunkPart{total, 0, 0, 0, 0, 0, 0};
+    *s_part = ChunkPart{total, 0, 0, 0, 0, 0, 0, {0, 0, 0, 0}};
   }
   __syncthreads();
   return *s_part;
@@ -201,12 +204,11 @@ struct ChunkWalk {
   bool fresh;
   AttnSeq s;
   __device__ __forceinline__ ChunkWalk(const ChunkPart& c, int more_)
-      : b(c.b), left(c.count), head(c.head), tile(c.tile), pos(c.pos), more(more_), fresh(true) {}
+      : b(c.b), left(c.count), head(c.head), tile(c.tile), pos(c.pos), more(more_), fresh(true), s(c.s) {}
   __device__ __forceinline__ bool next(const AttnParams& p, int per, ChunkPiece& w) {
     while (left > 0) {
       if (fresh) {
         fresh = false;
-        s = attn_seq(p, b);
       } else {
         pos = 0;
         if (++tile >= chunk_tiles(s, per)) {
