@@ -72,6 +72,9 @@ def parse():
     ap.add_argument("--one-host-copy", action="store_true",
                     help="decode: one copy of the host store for all local ranks instead of "
                          "one per NUMA node of their GPUs")
+    ap.add_argument("--kv-cache", choices=("dense", "bf16", "e4m3"), default="dense",
+                    help="decode workload: the full-attention layers' K/V (dense: the stand-in's "
+                         "GEMVs; bf16, e4m3: the paged cache and its kernels)")
     ap.add_argument("--l2-warm-mib", type=float, default=85.0,
                     help="decode: MiB of the next layer's first dense weight hinted into L2 "
                          "during each layer's fetch (85 = all of it; 0 = off)")
@@ -252,14 +255,15 @@ def decode_config(args, capacity: int | None = None) -> dict:
     """The decode workload's ``config`` (the same dict for both arms)."""
     from drama3_offloading_b200 import decode as dec
     cap = capacity or max(1, int(args.cache_gib * (1 << 30)) // (args.layers * EXPERT_BYTES))
-    dense = dec.dense_bytes_per_token(args.layers)
+    kind = args.kv_cache if args.impl == "ours" else "dense"
+    dense = dec.dense_bytes_per_token(args.layers, kv_cache=kind)
     return {"workload": "decode-40L-bs1-offloaded", "layers": args.layers, "hidden": 2048,
             "experts": 256, "topk": 8, "shared_expert": True, "cache_gib": args.cache_gib,
             "slots_per_layer": cap, "policy": args.policy, "fetch_overlap": not args.no_overlap,
             "kv_context": dec.KV_CONTEXT, "l2_warm_mib": args.l2_warm_mib,
             "l2_warm_gate": not args.no_l2_warm_gate,
-            "kv_mib_per_token": len(dec.full_attention_layers(args.layers)) * 2 *
-            dec.KV_CONTEXT * dec.KV_HEADS * dec.HEAD_DIM * 2 / 2**20,
+            "kv_mib_per_token": dec.kv_bytes_per_token(args.layers, kv_cache=kind) / 2**20,
+            **({} if kind == "dense" else {"kv_cache": kind}),
             "dense_gib_per_token": dense / 2**30,
             "cache_warm_steps": args.cache_warm_steps,
             "l2": "inputs > L2 (30 GiB host store, 6.9 GiB dense, 8 GiB cache)",
@@ -293,7 +297,7 @@ def run_decode(args, rank, world, local):
                         policy=args.policy, group=local_group(world), local_rank=local,
                         trace_offset=512 * rank, overlap=not args.no_overlap,
                         host_per_node=not args.one_host_copy, l2_warm_mib=args.l2_warm_mib,
-                        l2_warm_gate=not args.no_l2_warm_gate)
+                        l2_warm_gate=not args.no_l2_warm_gate, kv_cache=args.kv_cache)
     from drama3_offloading_b200 import devcache
     devcache.FETCH_CTAS = args.fetch_ctas
     if args.fetch_ctas > 0:

@@ -27,6 +27,13 @@ attends the layer's hidden state (as 2 KV groups x 4 query rows) over a
 resident bf16 K/V cache of that size with two batched GEMVs and a softmax
 (cuBLAS / torch), so those bytes are read every token too.
 
+``kv_cache="bf16"`` or ``"e4m3"`` puts this library's own cache and kernels in
+the place of those GEMVs: every full-attention layer projects the token's K
+and V, ``attention.qk_norm_rope_write`` norms and turns them into a
+``kvcache.PagedKV`` and ``attention.paged_attention`` reads it.  The cache is a
+ring of ``kv_context`` tokens -- each token replaces the oldest one -- in pages
+whose order is shuffled; e4m3 halves the bytes that are read.
+
 Routing: the router runs every layer (its cost is real), but the expert ids
 fed to the cache come from the seeded Zipf(1.1) trace so hit rates are those
 of skewed real routing rather than of a random-init gate (which routes almost
@@ -40,12 +47,15 @@ from __future__ import annotations
 import numpy as np
 import torch
 
-from . import _lib, devcache, moe
+from . import _lib, attention, devcache, kvcache, moe
 from .stack import OffloadedExperts
 
 DENSE_GIB = 6.9
 KV_CONTEXT = 2048        # cached tokens of every full-attention layer
 KV_HEADS, HEAD_DIM = 2, 256
+KV_PAGE = 64             # tokens of a page of the paged cache
+ROTARY_DIM, ROPE_THETA = 64, 1e7
+KV_CACHES = {"dense": None, "bf16": torch.bfloat16, "e4m3": torch.float8_e4m3fn}
 
 
 def full_attention_layers(layers: int) -> list:
@@ -61,13 +71,23 @@ def dense_stand_in_rows(layers: int, hidden: int, inter: int, dense_gib: float) 
     return max(128, int(per_layer / (2 * hidden * 2)) // 128 * 128)
 
 
+def kv_bytes_per_token(layers: int = 40, kv_context: int = KV_CONTEXT, kv_cache: str = "dense") -> int:
+    """Bytes of K and V the full-attention layers read per decode token."""
+    row = HEAD_DIM + 4 if kv_cache == "e4m3" else HEAD_DIM * 2
+    return len(full_attention_layers(layers)) * 2 * kv_context * KV_HEADS * row
+
+
 def dense_bytes_per_token(layers: int = 40, hidden: int = 2048, inter: int = 512,
-                          dense_gib: float = DENSE_GIB, kv_context: int = KV_CONTEXT) -> int:
-    """bf16 bytes the non-routed part of one decode token reads: the dense
-    stand-in, the shared experts and the full-attention layers' KV context."""
+                          dense_gib: float = DENSE_GIB, kv_context: int = KV_CONTEXT,
+                          kv_cache: str = "dense") -> int:
+    """Bytes the non-routed part of one decode token reads: the dense stand-in,
+    the shared experts and the full-attention layers' KV context (with a paged
+    cache also their K and V projection)."""
     R = dense_stand_in_rows(layers, hidden, inter, dense_gib)
     shared_bytes = (3 * inter * hidden + hidden) * 2
-    kv = len(full_attention_layers(layers)) * 2 * kv_context * KV_HEADS * HEAD_DIM * 2
+    kv = kv_bytes_per_token(layers, kv_context, kv_cache)
+    if kv_cache != "dense":
+        kv += len(full_attention_layers(layers)) * 2 * KV_HEADS * HEAD_DIM * hidden * 2
     return layers * (2 * R * hidden * 2 + shared_bytes) + kv
 
 
@@ -78,7 +98,9 @@ class DecodeStack:
                  policy: str = "lru", seed: int = 0, fill: str = "random", group=None,
                  local_rank: int = 0, trace_offset: int = 0, overlap: bool = True,
                  kv_context: int = KV_CONTEXT, host_per_node: bool = True,
-                 l2_warm_mib: float = 85.0, l2_warm_gate: bool = True):
+                 l2_warm_mib: float = 85.0, l2_warm_gate: bool = True, kv_cache: str = "dense"):
+        if kv_cache not in KV_CACHES:
+            raise ValueError(f"kv_cache {kv_cache!r}: {', '.join(KV_CACHES)}")
         self.device = dev = torch.device(device)
         self.overlap = overlap
         # with the overlapped fetch: MiB of the next layer's first dense weight
@@ -111,15 +133,20 @@ class DecodeStack:
         self.down = [torch.randn(hidden, R, generator=g, device=dev, dtype=torch.bfloat16) * (R ** -0.5 * 0.5)
                      for _ in range(layers)]
         # the full-attention layers' KV context: K and V [KV_HEADS, ctx, HEAD_DIM]
-        self.kv_context = kv_context
-        self.kv = {}
+        self.kv_context, self.kv_cache = kv_context, kv_cache
+        self.kv, self.paged, self.kv_proj = {}, {}, {}
         if kv_context > 0 and hidden % (KV_HEADS * HEAD_DIM) == 0:
-            for l in full_attention_layers(layers):
-                k = torch.randn(KV_HEADS, kv_context, HEAD_DIM, generator=g, device=dev) * 0.5
-                v = torch.randn(KV_HEADS, kv_context, HEAD_DIM, generator=g, device=dev)
-                self.kv[l] = (k.to(torch.bfloat16), v.to(torch.bfloat16))
-        self.kv_bytes = sum(k.numel() * 2 + v.numel() * 2 for k, v in self.kv.values())
+            if kv_cache == "dense":
+                for l in full_attention_layers(layers):
+                    k = torch.randn(KV_HEADS, kv_context, HEAD_DIM, generator=g, device=dev) * 0.5
+                    v = torch.randn(KV_HEADS, kv_context, HEAD_DIM, generator=g, device=dev)
+                    self.kv[l] = (k.to(torch.bfloat16), v.to(torch.bfloat16))
+            else:
+                self._init_paged(seed)
+        self.kv_bytes = (kv_bytes_per_token(layers, kv_context, kv_cache)
+                         if self.kv or self.paged else 0)
         self.dense_bytes = (sum(t.numel() * 2 for t in self.up + self.down) +
+                            sum(t.numel() * 2 for t in self.kv_proj.values()) +
                             layers * shared_bytes + self.kv_bytes)
         self.gate = [(torch.randn(experts, hidden, generator=g, device=dev) * 0.02).to(torch.bfloat16)
                      for _ in range(layers)]
@@ -138,8 +165,60 @@ class DecodeStack:
         # warm the library (workspaces, smem attributes) outside any capture
         moe.router_topk(self.h, self.gate[0], topk, out_ids=self.ids, out_w=self.wts)
 
+    # ---------------------------------------------------------------- paged K/V
+    def _init_paged(self, seed: int) -> None:
+        dev, ctx = self.device, self.kv_context
+        g = torch.Generator(device=dev).manual_seed(seed + 11)
+        pages = -(-ctx // KV_PAGE)
+        self.kv_table = torch.randperm(pages, generator=g, device=dev).to(torch.int32).view(1, -1)
+        at = torch.arange(ctx, device=dev)
+        self.kv_slots = (self.kv_table[0].long()[at // KV_PAGE] * KV_PAGE + at % KV_PAGE).to(torch.int32)
+        self.kv_lens = torch.full((1,), ctx, dtype=torch.int32, device=dev)
+        self.kv_pos = torch.empty(1, dtype=torch.int64, device=dev)
+        self.inv_freq = attention.rope_frequencies(ROTARY_DIM, ROPE_THETA, dev)
+        self.qk_norm = torch.ones(HEAD_DIM, dtype=torch.bfloat16, device=dev)
+        self._kv_seed = seed + 13
+        for l in full_attention_layers(self.L):
+            self.paged[l] = kvcache.PagedKV(pages, KV_PAGE, KV_HEADS, HEAD_DIM,
+                                            KV_CACHES[self.kv_cache], dev)
+            w = torch.randn(2 * KV_HEADS * HEAD_DIM, self.H, generator=g, device=dev) * self.H ** -0.5
+            self.kv_proj[l] = w.to(torch.bfloat16)
+        self._fill_paged()
+
+    def _fill_paged(self) -> None:
+        """The context before the first token, always the same."""
+        g = torch.Generator(device=self.device).manual_seed(self._kv_seed)
+        for cache in self.paged.values():
+            kv = torch.randn(self.kv_context, 2 * KV_HEADS, HEAD_DIM, generator=g, device=self.device)
+            kv[:, :KV_HEADS] *= 0.5
+            kv = kv.to(torch.bfloat16)
+            kvcache.write(cache, kv[:, :KV_HEADS], kv[:, KV_HEADS:], self.kv_slots)
+        self.kv_pos.fill_(self.kv_context)
+
+    def _paged_attention(self, l: int, slot: torch.Tensor) -> None:
+        """h += attention of the token over the ring, its own K and V in it."""
+        h, cache = self.h, self.paged[l]
+        kv = (h @ self.kv_proj[l].t()).view(1, 2 * KV_HEADS, HEAD_DIM)
+        q = attention.qk_norm_rope_write(h.view(1, -1, HEAD_DIM), kv[:, :KV_HEADS], kv[:, KV_HEADS:],
+                                         self.qk_norm, self.qk_norm, self.kv_pos, self.inv_freq,
+                                         cache, slot)
+        # (a ring's order does not matter: the rotation is in the keys)
+        a = attention.paged_attention(q, cache, self.kv_table, self.kv_lens, max_kv=self.kv_context)
+        h.add_(a.view(1, -1), alpha=0.25)
+
     # ---------------------------------------------------------------- one token
-    def _layer(self, l: int, cur_ids: torch.Tensor, events: list | None = None) -> None:
+    def _next(self):
+        """(this token's expert ids of every layer, its slot of the K/V ring);
+        moves both counters on."""
+        cur = self.trace_dev.index_select(0, self.step_idx)[0]
+        self.step_idx.add_(1).remainder_(self.trace_steps)
+        slot = None
+        if self.paged:
+            slot = self.kv_slots.index_select(0, self.kv_pos % self.kv_context)
+        return cur, slot
+
+    def _layer(self, l: int, cur_ids: torch.Tensor, slot: torch.Tensor | None = None,
+               events: list | None = None) -> None:
         """h += dense(h); route; resolve + fetch; h += moe(h) -- all in place."""
         h = self.h
         a = torch.nn.functional.silu(h @ self.up[l].t())
@@ -152,6 +231,8 @@ class DecodeStack:
             p = torch.softmax(torch.bmm(q, k.transpose(1, 2)).float() * HEAD_DIM ** -0.5,
                               dim=-1).to(torch.bfloat16)
             h.add_(torch.bmm(p, v).view(1, -1), alpha=0.25)
+        elif l in self.paged:
+            self._paged_attention(l, slot)
         moe.router_topk(h, self.gate[l], self.k, out_ids=self.ids, out_w=self.wts)
         ex = self.store.layers[l]
         if events is not None:
@@ -190,10 +271,11 @@ class DecodeStack:
 
     def step(self) -> None:
         """One decode token through all layers (eager; capturable)."""
-        cur = self.trace_dev.index_select(0, self.step_idx)[0]
-        self.step_idx.add_(1).remainder_(self.trace_steps)
+        cur, slot = self._next()
         for l in range(self.L):
-            self._layer(l, cur)
+            self._layer(l, cur, slot)
+        if self.paged:
+            self.kv_pos.add_(1)
 
     def capture(self) -> torch.cuda.CUDAGraph:
         s = torch.cuda.Stream(device=self.device)
@@ -214,13 +296,21 @@ class DecodeStack:
 
     def snapshot(self) -> dict:
         """A device copy of everything a replay changes -- every layer's slot
-        tables, job table, counters and cache bytes, the hidden state and the
-        trace position -- so the same window of tokens can be run again from
+        tables, job table, counters and cache bytes, the hidden state, the
+        trace position and the paged K/V -- so the same window of tokens can be run again from
         the same state (``restore``)."""
         torch.cuda.synchronize(self.device)
         return {"layers": [[getattr(ex, n).clone() for n in self._TABLES]
                            for ex in self.store.layers],
-                "h": self.h.clone(), "step_idx": self.step_idx.clone()}
+                "h": self.h.clone(), "step_idx": self.step_idx.clone(),
+                "kv": [t.clone() for t in self._paged_state()]}
+
+    def _paged_state(self) -> list:
+        """The tensors of the paged K/V that a step changes."""
+        if not self.paged:
+            return []
+        return [self.kv_pos] + [t for c in self.paged.values()
+                                for t in (c.k, c.v, c.k_scale, c.v_scale) if t is not None]
 
     def restore(self, snap: dict) -> None:
         """Copy a ``snapshot`` back in place (addresses unchanged, so captured
@@ -230,13 +320,18 @@ class DecodeStack:
                 getattr(ex, n).copy_(t)
         self.h.copy_(snap["h"])
         self.step_idx.copy_(snap["step_idx"])
+        for t, saved in zip(self._paged_state(), snap["kv"]):
+            t.copy_(saved)
         torch.cuda.synchronize(self.device)
 
     def reset(self) -> None:
-        """Cold caches, trace at its start, zero hidden state (addresses unchanged)."""
+        """Cold caches, trace at its start, zero hidden state, the K/V context as
+        it was (addresses unchanged)."""
         self.store.reset_caches()
         self.step_idx.fill_(self.trace_offset % self.trace_steps)
         self.h.zero_()
+        if self.paged:
+            self._fill_paged()
         torch.cuda.synchronize(self.device)
 
     def sample_fetch_timing(self, steps: int) -> dict:
@@ -247,10 +342,11 @@ class DecodeStack:
         evs = []
         c0 = self.store.counters()
         for _ in range(steps):
-            cur = self.trace_dev.index_select(0, self.step_idx)[0]
-            self.step_idx.add_(1).remainder_(self.trace_steps)
+            cur, slot = self._next()
             for l in range(self.L):
-                self._layer(l, cur, evs)
+                self._layer(l, cur, slot, evs)
+            if self.paged:
+                self.kv_pos.add_(1)
         torch.cuda.synchronize(self.device)
         c1 = self.store.counters()
         ms = sum(a.elapsed_time(b) for a, b in evs)
@@ -260,8 +356,10 @@ class DecodeStack:
     def launches_per_step(self) -> int:
         """Kernels of this library launched per token: router, allocator, fetch,
         and the batch-1 expert path's gate/up and down launches per layer
-        (with overlap the fetch and the gate/up products are one launch)."""
-        return (4 if self.overlap else 5) * self.L
+        (with overlap the fetch and the gate/up products are one launch); over a
+        paged cache also the norm and rotation, the attention and its join per
+        full-attention layer."""
+        return (4 if self.overlap else 5) * self.L + 3 * len(self.paged)
 
     def roofline_ms(self, hits: float, misses: float, hbm_gbs: float, host_gbs: float) -> float:
         """t >= dense/HBM + hits*expert/HBM + misses*expert/host per token."""
