@@ -67,12 +67,19 @@ static int check_attention(const d3_attention* a, const d3_kv_cache* c) {
 // once and, although most of their rows may be empty, keep up with HBM.
 constexpr int kRowsMost = 16;
 
+// SMs that the kernels' parts are counted for: a part of either kernel has a
+// thread of a joining block.
+static int part_sms() {
+  const int n = num_sms();
+  return n < kJoinThreads * 2 / 3 ? n : kJoinThreads * 2 / 3;
+}
+
 struct Workspace {         // byte offsets
   size_t rows_o, rows_ml, rows_desc, chunk_o, chunk_ml, chunk_desc, total;
 };
 static Workspace plan_workspace(const d3_attention* a, const d3_kv_cache* c) {
   Workspace w{};
-  const size_t D = c->head_dim, sms = num_sms(), pairs = sms / 2;
+  const size_t D = c->head_dim, sms = part_sms(), pairs = sms / 2;
   size_t at = 0;
   auto take = [&](size_t n) {
     const size_t o = at;
@@ -120,7 +127,7 @@ static int launch_rows(const AttnParams& p, const d3_attention* a, const d3_kv_c
           ((long long)a->table_pages * c->page_size / C::KEYS + 1 + kPieceUnits) >= (1LL << 31))
     return fail(D3_ERR_TOO_LARGE, "d3_paged_attention: too many key tiles");
   const long long most = (tiles < 1 ? 1 : tiles) * groups * a->batch * c->kv_heads;
-  const int parts = (int)(most < num_sms() ? most : num_sms());
+  const int parts = (int)(most < part_sms() ? most : part_sms());
   D3_CUDA_TRY(launch_k(attn_rows_kernel<T, D, E4, NT>, dim3(parts), dim3(C::THREADS), C::SMEM, st,
                        pdl_enabled(), tk, tv, p),
               "attn_rows_kernel launch");
@@ -151,7 +158,7 @@ static int launch_chunk(const AttnParams& p, const d3_attention* a, const d3_kv_
   // the kernel counts the list in 31 bits; the lengths it reads may be larger than max_kv says
   if (((long long)a->table_pages * c->page_size / kBlockKeys + 1) * tiles * c->kv_heads >= (1LL << 31))
     return fail(D3_ERR_TOO_LARGE, "d3_paged_attention: too many key blocks");
-  const int pairs = (int)(most < num_sms() / 2 ? most : num_sms() / 2);
+  const int pairs = (int)(most < part_sms() / 2 ? most : part_sms() / 2);
   D3_CUDA_TRY(launch_k(attn_chunk_kernel<T, D, E4>, dim3(2 * pairs), dim3(C::THREADS), C::SMEM, st, pdl_enabled(),
                        tq, tk, tv, p, ws),
               "attn_chunk_kernel launch");
@@ -182,13 +189,15 @@ static int launch_attention(AttnParams p, const d3_attention* a, const d3_kv_cac
                               : launch_rows<T, D, E4, 2>(few, &one, c, &parts, st)))
         return rc;
       p.min_rows = few.max_rows + 1;
+      p.beside = 1;
     }
     rc = launch_chunk<T, D, E4>(p, a, c, ws, &pairs, st);
   }
   if (rc) return rc;
-  const unsigned y = parts ? (unsigned)rows_per : 8u;
-  D3_CUDA_TRY(launch_k(attn_join_kernel<T, D>, dim3(parts + pairs, y < 8 ? 8 : y), dim3(256), 0, st, pdl_enabled(), p,
-                       rows_per, parts, ws),
+  const int items = parts * rows_per + pairs * (256 / kJoinRows), most = kJoinBlocks * num_sms();
+  const dim3 grid = pairs ? dim3(items < most ? items : most) : dim3(parts, rows_per);
+  D3_CUDA_TRY(launch_k(attn_join_kernel<T, D>, grid, dim3(kJoinThreads), 0, st,
+                       pdl_enabled(), p, rows_per, parts, parts + pairs, ws),
               "attn_join_kernel launch");
   return D3_OK;
 }

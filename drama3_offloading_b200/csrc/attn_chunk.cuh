@@ -579,7 +579,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(ChunkCfg<T, D, E4>::
   tc_fence_after();
   const uint32_t tmem = head.tmem;
   pdl_trigger();
-  pdl_wait();
+  if (!p.beside) pdl_wait();
   const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
   const int tpc = 128 / p.group, per = 2 * tpc;      // tokens of a CTA, of the pair
   const ChunkPart part = chunk_plan(p, per, MORE, pair, pairs, head.scan, &head.part);
@@ -1144,31 +1144,40 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(ChunkCfg<T, D, E4>::
   // before TMEM or shared memory goes
   if (warp == 8 && !mbar_wait(all_done, 0, kAttnWaitBudgetNs) && lane == 0) attn_error(p.err, kAttnErrChunkMma);
   __syncwarp();
+  if (p.beside) pdl_wait();
   cluster_sync_all();      // no CTA leaves while its pair may still arrive at it
   tc_fence_after();
   if (warp == 8) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
 }
 
 // Tiles that the parts' cuts go through: the sum of their parts, in order.
-// c0 is the part in which the tile begins; a block takes 32 rows, eight threads
-// a row, each 4 dims of every 32.
+// c0 and c1 are the first and the last of a tile's parts.  A block takes 16
+// rows: a warp eight of them (a load of eight rows' 16 bytes is a whole line)
+// and a quarter of the dims.
+constexpr int kJoinRows = 16;
+// those of a tile with rows in CTA `half` of the pair
+__device__ __forceinline__ int chunk_join_groups(const AttnParams& p, const int4& de, int half) {
+  const int tpc = 128 / p.group, toks = min(de.y - (de.w * 2 + half) * tpc, tpc);
+  return toks > 0 ? (toks * p.group + kJoinRows - 1) / kJoinRows : 0;
+}
 template <typename T, int D>
-__device__ __forceinline__ void chunk_join(const AttnParams& p, const ChunkWs& ws, int c0, int group) {
-  const int4 de = __ldcg(ws.desc + 2 * c0);
-  const int c1 = __ldcg(ws.desc + 2 * c0 + 1).x;
-  if (c1 < 0) return;
-  const int tpc = 128 / p.group;
-  const int row = group * 32 + (threadIdx.x >> 3), x = threadIdx.x & 7;
-  const int rr = row & 127, ti = rr / p.group, tok = de.w * 2 * tpc + (row >> 7) * tpc + ti;
+__device__ __forceinline__ void chunk_join(const AttnParams& p, const ChunkWs& ws, const int4& de, int c0, int c1,
+                                           int group) {
+  constexpr int N = D / 64;
+  const int g0 = chunk_join_groups(p, de, 0), half = group >= g0, tpc = 128 / p.group;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int rr = (half ? group - g0 : group) * kJoinRows + (warp & 1) * 8 + (lane & 7), row = half * 128 + rr;
+  const int x = (warp >> 1) * (D / 16) + (lane >> 3);
+  const int ti = rr / p.group, tok = (de.w * 2 + half) * tpc + ti;
   if (ti >= tpc || tok >= de.y) return;
   // two parts at a time (a tile seldom has more), all of their loads at once
   float m = -INFINITY, l = 0.f;
-  float4 a[D / 32];
+  float4 a[N];
 #pragma unroll
-  for (int i = 0; i < D / 32; ++i) a[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int i = 0; i < N; ++i) a[i] = make_float4(0.f, 0.f, 0.f, 0.f);
   for (int c = c0; c <= c1; c += 2) {
     float2 ml[2];
-    float4 v[2][D / 32];
+    float4 v[2][N];
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
       ml[k] = make_float2(-INFINITY, 0.f);
@@ -1176,8 +1185,8 @@ __device__ __forceinline__ void chunk_join(const AttnParams& p, const ChunkWs& w
         const size_t place = (size_t)(c + k) * 2 + (c + k == c0);
         ml[k] = __ldcg(reinterpret_cast<const float2*>(ws.ml) + place * 256 + row);
 #pragma unroll
-        for (int i = 0; i < D / 32; ++i)
-          v[k][i] = __ldcg(reinterpret_cast<const float4*>(ws.o) + (place * (D / 4) + 8 * i + x) * 256 + row);
+        for (int i = 0; i < N; ++i)
+          v[k][i] = __ldcg(reinterpret_cast<const float4*>(ws.o) + (place * (D / 4) + x + 4 * i) * 256 + row);
       }
     }
     const float top = fmaxf(m, fmaxf(ml[0].x, ml[1].x)), base = top == -INFINITY ? 0.f : top;
@@ -1185,14 +1194,14 @@ __device__ __forceinline__ void chunk_join(const AttnParams& p, const ChunkWs& w
     m = top;
     l *= keep;
 #pragma unroll
-    for (int i = 0; i < D / 32; ++i) a[i] = make_float4(a[i].x * keep, a[i].y * keep, a[i].z * keep, a[i].w * keep);
+    for (int i = 0; i < N; ++i) a[i] = make_float4(a[i].x * keep, a[i].y * keep, a[i].z * keep, a[i].w * keep);
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
       const float f = ex2(ml[k].x - base);
       if (f == 0.f) continue;
       l = fmaf(ml[k].y, f, l);
 #pragma unroll
-      for (int i = 0; i < D / 32; ++i) {
+      for (int i = 0; i < N; ++i) {
         a[i].x = fmaf(v[k][i].x, f, a[i].x);
         a[i].y = fmaf(v[k][i].y, f, a[i].y);
         a[i].z = fmaf(v[k][i].z, f, a[i].z);
@@ -1204,21 +1213,70 @@ __device__ __forceinline__ void chunk_join(const AttnParams& p, const ChunkWs& w
   T* dst = static_cast<T*>(p.out) + (long long)(de.x + tok) * p.out_token +
            (long long)(de.z * p.group + rr - ti * p.group) * p.out_head + x * 4;
 #pragma unroll
-  for (int i = 0; i < D / 32; ++i)
-    *reinterpret_cast<uint2*>(dst + 32 * i) =
+  for (int i = 0; i < N; ++i)
+    *reinterpret_cast<uint2*>(dst + 16 * i) =
         make_uint2(Elem<T>::from_f2(a[i].x * inv, a[i].y * inv), Elem<T>::from_f2(a[i].z * inv, a[i].w * inv));
 }
 
-// What the row kernel (blocks [0, rows_parts) of x) and the chunk kernel cut.
+// What the row kernel (parts [0, rows_parts)) and the chunk kernel cut.  After
+// the row kernel alone a block has one part's row, if there is one (x: part, y:
+// row): the least latency.  Else every block reads the list of all parts, at
+// most one a thread, and takes its share of the rows to be joined: a block for
+// each 32 rows that might be cut spent more on blocks without work (24
+// sequences of 3 to 7 tokens: 55.1 us in all, 51.9 with the list; 12 mixed
+// ones 146 and 139; 2048 tokens 40.1 and 35.9; but one single token 9.1 and
+// 10.0).
 template <typename T, int D>
-__global__ void __launch_bounds__(256) attn_join_kernel(const __grid_constant__ AttnParams p, int rows_per,
-                                                        int rows_parts, const ChunkWs ws) {
+__global__ void __launch_bounds__(kJoinThreads, kJoinBlocks) attn_join_kernel(const __grid_constant__ AttnParams p, int rows_per,
+                                                                    int rows_parts, int parts, const ChunkWs ws) {
+  __shared__ int s_sum[kJoinThreads / 32], s_c0, s_c1, s_at;
+  __shared__ int4 s_de;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   pdl_trigger();
   pdl_wait();
-  if ((int)blockIdx.x < rows_parts) {
-    if ((int)blockIdx.y < rows_per) rows_join<T, D>(p, rows_per, blockIdx.x, blockIdx.y);
-  } else if (blockIdx.y < 8) {
-    chunk_join<T, D>(p, ws, blockIdx.x - rows_parts, blockIdx.y);
+  int4 de = make_int4(0, 0, 0, 0);
+  int c1 = -1, n = 0;
+  if (gridDim.y > 1) {
+    const int part = blockIdx.x, row = blockIdx.y;
+    de = __ldcg(p.ws_desc + 2 * part);
+    c1 = __ldcg(p.ws_desc + 2 * part + 1).x;
+    if (c1 >= 0 && de.w * rows_per + row < de.y) rows_join<T, D>(p, rows_per, de, part, c1, row);
+    return;
+  }
+  const int c0 = tid < rows_parts ? tid : tid - rows_parts;
+  if (tid < parts) {
+    const int4* at = (tid < rows_parts ? p.ws_desc : ws.desc) + 2 * c0;
+    de = __ldcg(at);
+    c1 = __ldcg(at + 1).x;
+    if (c1 >= 0)
+      n = tid < rows_parts ? min(rows_per, de.y - de.w * rows_per)
+                           : chunk_join_groups(p, de, 0) + chunk_join_groups(p, de, 1);
+  }
+  int before = n, total = 0;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int v = __shfl_up_sync(0xffffffffu, before, o);
+    if (lane >= o) before += v;
+  }
+  if (lane == 31) s_sum[warp] = before;
+  __syncthreads();
+  before -= n;
+#pragma unroll
+  for (int w = 0; w < kJoinThreads / 32; ++w) {
+    if (w < warp) before += s_sum[w];
+    total += s_sum[w];
+  }
+  for (int i = blockIdx.x; i < total; i += gridDim.x) {
+    if (i >= before && i < before + n) {
+      s_de = de;
+      s_c0 = c0 + (tid < rows_parts ? 0 : rows_parts);
+      s_c1 = c1;
+      s_at = i - before;
+    }
+    __syncthreads();
+    if (s_c0 < rows_parts) rows_join<T, D>(p, rows_per, s_de, s_c0, s_c1, s_at);
+    else chunk_join<T, D>(p, ws, s_de, s_c0 - rows_parts, s_c1, s_at);
+    __syncthreads();
   }
 }
 

@@ -43,6 +43,7 @@
 namespace d3 {
 
 constexpr uint64_t kAttnWaitBudgetNs = 2000000000ull;
+constexpr int kJoinThreads = 256, kJoinBlocks = 3;   // of the joining kernel: threads, blocks an SM
 constexpr int kAttnErrRowsLoad = 51, kAttnErrRowsUse = 52;
 
 struct AttnParams {
@@ -61,6 +62,8 @@ struct AttnParams {
   const float *k_scale, *v_scale;
   float scale_log2;              // softmax scale * log2(e)
   int min_rows, max_rows;        // sequences this launch takes, by new tokens * group
+  int beside;                    // the launch before is the row kernel of the same call: what that one
+                                 // waited for has ended, and it itself is waited for at the end
   float* ws_o;                   // partial sums
   float* ws_ml;                  // their maxima and sums
   int4* ws_desc;                 // two of each part: (first query token, rows of the sequence, KV head, row
@@ -334,8 +337,9 @@ __global__ void __launch_bounds__(RowsCfg<T, D, E4, NT>::THREADS, 1)
     tma_prefetch_desc(&tm_k);
     tma_prefetch_desc(&tm_v);
   }
-  pdl_trigger();
+  // in this order: the chunk kernel behind may then run beside this one
   pdl_wait();
+  pdl_trigger();
   const RowsWork work = rows_plan(p, C::KEYS, C::ROWS, blockIdx.x, gridDim.x, s_scan, &s_work);
   if (work.count == 0) {
     if (tid == 0) p.ws_desc[2 * blockIdx.x + 1] = make_int4(-1, 0, 0, 0);
@@ -799,21 +803,17 @@ __global__ void __launch_bounds__(RowsCfg<T, D, E4, NT>::THREADS, 1)
 }
 
 // Pairs that the parts' cuts go through: the sum of their parts, in the parts'
-// order.  c0 is the part in which the pair begins, r the row;
-// the threads take turns of D/4 over the parts and add up through shared
+// order.  c0 and c1 are the first and the last of its parts, r the row; the
+// threads take turns of D/4 over the parts and add up through shared
 // memory.  The workspace is read through L2: launched early, this kernel
 // shares SMs with the join of the call before, whose lines of the same memory
 // may still be in L1.
 template <typename T, int D>
-__device__ __forceinline__ void rows_join(const AttnParams& p, int rows_per, int c0, int r) {
-  constexpr int GROUPS = 256 / (D / 4);
+__device__ __forceinline__ void rows_join(const AttnParams& p, int rows_per, const int4& de, int c0, int c1, int r) {
+  constexpr int GROUPS = kJoinThreads / (D / 4);
   __shared__ float4 s_a[GROUPS][D / 4];
   __shared__ float2 s_ml[GROUPS];
-  const int4 de = __ldcg(p.ws_desc + 2 * c0);
-  const int c1 = __ldcg(p.ws_desc + 2 * c0 + 1).x;
-  if (c1 < 0) return;
   const int gr = de.w * rows_per + r;
-  if (gr >= de.y) return;
   const int g = threadIdx.x / (D / 4), d4 = threadIdx.x % (D / 4);
   // a group's parts four at a time, all of their loads at once
   float m = -INFINITY, l = 0.f;
