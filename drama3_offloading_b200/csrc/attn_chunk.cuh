@@ -429,13 +429,6 @@ __device__ __forceinline__ void tmem_st32(uint32_t a, const uint32_t* u) {
       "r"(u[28]), "r"(u[29]), "r"(u[30]), "r"(u[31])
       : "memory");
 }
-__device__ __forceinline__ void tmem_ld16f(uint32_t a, float* r) {
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
-      : "=f"(r[0]), "=f"(r[1]), "=f"(r[2]), "=f"(r[3]), "=f"(r[4]), "=f"(r[5]), "=f"(r[6]), "=f"(r[7]), "=f"(r[8]),
-        "=f"(r[9]), "=f"(r[10]), "=f"(r[11]), "=f"(r[12]), "=f"(r[13]), "=f"(r[14]), "=f"(r[15])
-      : "r"(a));
-}
 __device__ __forceinline__ void tmem_st8(uint32_t a, const uint32_t* u) {
   asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(a), "r"(u[0]), "r"(u[1]),
                "r"(u[2]), "r"(u[3]), "r"(u[4]), "r"(u[5]), "r"(u[6]), "r"(u[7])
@@ -878,17 +871,20 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(ChunkCfg<T, D, E4>::
         // STEP columns at a time: all 64 stay in registers from the maximum to
         // the exponentials, or, with codes, where the widening warps' code
         // fills the instruction cache, a short loop reads them from TMEM twice
-        constexpr int STEP = E4 ? 16 : 64;
+        // (8 columns: 974 us where 16 take 986 and all 64 took 1308; 2048
+        // tokens over 14000, 8 heads x 128).  The keys' scales hold the softmax
+        // scale as well: one product less a score.
+        constexpr int STEP = E4 ? 8 : 64;
         float s[STEP];
-        auto columns = [&](int c0) {
+        auto columns = [&](int c0, bool scaled) {
           if (STEP == 64) {
             tmem_ld32(sb + 64 * h, s);
             tmem_ld32(sb + 64 * h + 32, s + STEP / 2);
           } else {
-            tmem_ld16f(sb + 64 * h + c0, s);
+            tmem_ld8(sb + 64 * h + c0, s);
           }
           tmem_ld_wait();
-          if (E4) {
+          if (E4 && scaled) {
 #pragma unroll
             for (int i = 0; i < STEP / 4; ++i) {
               const float4 f = reinterpret_cast<const float4*>(ks + c0)[i];
@@ -906,11 +902,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(ChunkCfg<T, D, E4>::
         float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll 1
         for (int c0 = 0; c0 < 64; c0 += STEP) {
-          columns(c0);
+          columns(c0, true);
 #pragma unroll
           for (int i = 0; i < STEP; ++i) m4[i & 3] = fmaxf(m4[i & 3], s[i]);
         }
-        float mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * c;
+        float mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * (E4 ? 1.f : c);
         // the other half's maximum: both threads then decide alike
         mx = fmaxf(mx, exchange(mx));
         const bool grow = mx > m + kRescaleLog2 || (m == -INFINITY && mx > m);
@@ -942,12 +938,18 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(ChunkCfg<T, D, E4>::
         float l2[2] = {0.f, 0.f};
 #pragma unroll 1
         for (int c0 = 0; c0 < 64; c0 += STEP) {
-          if (STEP < 64) columns(c0);
+          if (STEP < 64) columns(c0, false);
           uint32_t pk[STEP / 2];
 #pragma unroll
           for (int q = 0; q < STEP / 2; ++q) {
             float a = s[2 * q], b = s[2 * q + 1];
-            fma2(a, b, c, -base);
+            if (E4) {
+              const float4 f = reinterpret_cast<const float4*>(ks + c0)[q >> 1];
+              if (q & 1) fma2(a, b, f.z, f.w, -base);
+              else fma2(a, b, f.x, f.y, -base);
+            } else {
+              fma2(a, b, c, -base);
+            }
             a = ex2(a);
             b = ex2(b);
             add2(l2[0], l2[1], a, b);
@@ -960,7 +962,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(ChunkCfg<T, D, E4>::
           }
           // P of a half goes over the S columns that its own threads have read
           if (STEP == 64) tmem_st32(sb + 64 * h, pk);
-          else tmem_st8(sb + 64 * h + c0 / 2, pk);
+          else tmem_st4(sb + 64 * h + c0 / 2, pk);
         }
         l += l2[0] + l2[1];
         tmem_st_wait();
@@ -1095,7 +1097,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(ChunkCfg<T, D, E4>::
         // v = f * 2^e; a scale without an exponent of its own stays whole
         const uint32_t b = __float_as_uint(cv[i]);
         const bool normal = (b & 0x7f800000u) != 0;
-        sc[32 * i] = ck[i];
+        sc[32 * i] = ck[i] * p.scale_log2;
         sc[kBlockKeys + 32 * i] = normal ? __uint_as_float((b & 0x007fffffu) | 0x3f800000u) : 1.f;
         uint32_t* e = reinterpret_cast<uint32_t*>(sc) + 2 * kBlockKeys + 32 * i;
         if (std::is_same<T, __half>::value) {

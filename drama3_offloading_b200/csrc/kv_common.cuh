@@ -75,6 +75,12 @@ __device__ __forceinline__ void fma2(float& x, float& y, float a, float b) {   /
       : "+f"(x), "+f"(y)
       : "f"(a), "f"(b));
 }
+__device__ __forceinline__ void fma2(float& x, float& y, float a, float b, float n) {   // (x * a + n, y * b + n)
+  asm("{\n\t.reg .b64 v, m, n;\n\tmov.b64 v, {%0, %1};\n\tmov.b64 m, {%2, %3};\n\tmov.b64 n, {%4, %4};\n\t"
+      "fma.rn.f32x2 v, v, m, n;\n\tmov.b64 {%0, %1}, v;\n\t}"
+      : "+f"(x), "+f"(y)
+      : "f"(a), "f"(b), "f"(n));
+}
 __device__ __forceinline__ void mul2(float& x, float& y, float a, float b) {   // (x * a, y * b)
   asm("{\n\t.reg .b64 v, m;\n\tmov.b64 v, {%0, %1};\n\tmov.b64 m, {%2, %3};\n\t"
       "mul.rn.f32x2 v, v, m;\n\tmov.b64 {%0, %1}, v;\n\t}"
