@@ -126,12 +126,12 @@ def paged_attention(q: torch.Tensor, cache: PagedKV, page_table: torch.Tensor,
     its ``kv_lens[b]`` (int32) cached tokens, so row i of n sees the keys
     ``[0, kv_lens[b] - n + i]``; a row that sees none gives zeros.  Key j lies
     in page ``page_table[b, j // page_size]`` (int32 ``[batch, pages]``); ids
-    outside the cache read as zeros.  Lengths
-    behind the table's width count as the width.  ``max_q`` and ``max_kv`` bound
-    the new tokens and the length of a sequence; they choose the launch
-    (default: one token, the table's width), and with others the answer is the
-    same, later.  ``scale`` defaults to head_dim ** -0.5.  ``out`` may be
-    ``q``; rows of it behind the last sequence are left as they were.
+    outside the cache read as zeros.  Lengths behind the table's width count as
+    the width.  ``max_q`` and ``max_kv`` bound the new tokens and the length of
+    a sequence (default: one token, the table's width); they choose the launch:
+    a sequence that exceeds them is answered too, more slowly.  ``scale``
+    defaults to head_dim ** -0.5.  ``out`` may be ``q``; rows of it behind the
+    last sequence are left as they were.
 
     Keys that a row's mask hides may hold anything.  Values are multiplied by
     zero there: an infinity or NaN in V reaches rows of the same sequence and

@@ -14,8 +14,14 @@
 // both halves: 32 bytes a cycle, and twice as many blocks fit in the ring.
 //
 // Bound: the tensor pipe for D = 256 (2048 cycles a block against about 1300
-// for the exponentials of 128 x 128 scores on one warpgroup); the
-// exponentials for D = 128.
+// for the exponentials of 128 x 128 scores on one warpgroup), the exponentials
+// for D = 128.  Measured, 2048 tokens over 14000, pages of 64: 16 heads of 256
+// over 2 in bf16 1425 TFLOP/s, 32 of 128 over 8 in fp16 975; the former, run for
+// seconds, is held by the power limit.  Pages of 16 hold 16-bit caches back
+// (1054 and 647): their loading threads issue twelve small boxes a block.
+// Codes reach 810 and 517, bound by instruction-cache misses (six of ten
+// cycles issue nothing): the widening and the softmax are different code on
+// the same schedulers, which is why their loops are kept short.
 //
 // TMEM, 512 columns: two S blocks (P of each half goes over its S) and O.  S of block
 // j + 1 is issued before P V of block j, so the tensor core works while the
@@ -36,7 +42,7 @@
 //
 // Split: as in the row kernel, the list of all (sequence, KV head, row tile,
 // key block) is cut into equal parts, one per pair; tiles that a cut goes
-// through are joined by attn_chunk_join_kernel in the parts' order.
+// through are joined by attn_join_kernel in the parts' order.
 //
 // e4m3 caches: codes are staged by TMA and widened to 16 bits in shared
 // memory.  K codes are exact there, and a key's scale multiplies a column of S

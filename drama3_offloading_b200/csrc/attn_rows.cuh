@@ -23,8 +23,10 @@
 // into gridDim.x equal parts, so ragged batches load every SM alike.  A part
 // holds whole pairs and at most two pieces of pairs, whose unnormalised sums
 // go to the workspace (two places per CTA) and are joined by
-// attn_rows_join_kernel in the order of the parts: results do not depend on
-// timing.
+// attn_join_kernel in the order of the parts: results do not depend on timing.
+// Measured: 4 tokens over 8 heads x 100000 and more keys read 6.7 TB/s, 64
+// ragged sequences of codes 4.3 (a piece costs its start and its join); one
+// token over a short context is 9 us of latency.
 //
 // e4m3 caches: codes are exact in fp16, so the products run in fp16 whatever
 // the queries' type.  bf16 queries are scaled by a power of two per row (exact
@@ -77,7 +79,7 @@ __device__ __forceinline__ void attn_error(int* err, int code) { atomicCAS(err, 
 // warp: false once it has run out, with the error recorded, or *abort is set.
 // Out of line: a kernel's roles run from different places of its code at once
 // and its many waits in line cost it instruction-cache misses (a chunk of 2048
-// over 30720: 796 us in line, 728 so; the walks out of line, with their state
+// over 30720: 796 us in line, 728 so, on one box; the walks out of line, with their state
 // in local memory, made everything slower).
 __device__ __noinline__ bool wait_on(uint32_t bar, uint32_t parity, int* err, int code, volatile int* abort) {
   const uint64_t t0 = globaltimer_ns();
