@@ -673,6 +673,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(ChunkCfg<T, D, E4>::
         asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(raw_full + pos.slot)) : "memory");
       }
       asm volatile("cp.async.wait_all;" ::: "memory");
+      // after a wait ran out: Q, too, has landed before the memory goes
+      if (!ok && qn && rank == 0) mbar_wait(q_full, (qn - 1) & 1, kAttnWaitBudgetNs);
     };
     if (warp == 9) copy(std::false_type{});
     else copy(std::true_type{});
@@ -735,6 +737,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(ChunkCfg<T, D, E4>::
         }
       }
       // after a wait ran out: what is in flight has landed before the memory goes
+      if (!ok && qn && rank == 0) mbar_wait(q_full, (qn - 1) & 1, kAttnWaitBudgetNs);
       if (!ok && (E4 || rank == 0))
 #pragma unroll 1
         for (int i = 0; i < N; ++i) mbar_wait(bars_full + i, pos.phase ^ (i <= pos.slot ? 0 : 1), kAttnWaitBudgetNs);
