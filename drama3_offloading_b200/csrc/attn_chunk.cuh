@@ -19,7 +19,7 @@
 // over 2 in bf16 1425 TFLOP/s, 32 of 128 over 8 in fp16 975; the former, run for
 // seconds, is held by the power limit.  Pages of 16 hold 16-bit caches back
 // (1054 and 647): their loading threads issue twelve small boxes a block.
-// Codes reach 810 and 517, bound by instruction-cache misses (six of ten
+// Codes reach 860 and 560, bound by instruction-cache misses (six of ten
 // cycles issue nothing): the widening and the softmax are different code on
 // the same schedulers, which is why their loops are kept short.
 //
@@ -60,9 +60,11 @@ constexpr int kAttnErrChunkLoad = 53, kAttnErrChunkMma = 54, kAttnErrChunkSoftma
 constexpr int kBlockKeys = 128;
 constexpr float kRescaleLog2 = 8.f;
 // Pages below this go into the code ring by 16-byte copies of a whole warp: a
-// TMA instruction costs its thread some 500 cycles here whatever its size, and
-// a block of 16-token pages is twelve of them.
-constexpr int kSmallPage = 64;
+// TMA instruction costs its thread some 500 cycles here whatever its size.
+// 2048 tokens over 14000, 8 heads x 128: pages of 16 take 1204 us by TMA and
+// 990 by copies, of 32 1081 and 912, of 64 996 and 901, but of 128, one
+// instruction a tile, 801 and 902.
+constexpr int kSmallPage = 128;
 
 template <typename T, int D, bool E4>
 struct ChunkCfg {
@@ -544,7 +546,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(ChunkCfg<T, D, E4>::
   const uint32_t rank = cluster_rank();
   const int ps = p.page_size;
   if (smem_u32(smem_raw) & 1023) {       // the swizzle counts on it
-    if (tid == 0) attn_error(p.err, kAttnErrChunkAlign);
+    if (tid == 0) {
+      attn_error(p.err, kAttnErrChunkAlign);
+      ws.desc[blockIdx.x | 1] = make_int4(-1, 0, 0, 0);      // nothing to join
+    }
     return;
   }
   if (tid == 0) {
