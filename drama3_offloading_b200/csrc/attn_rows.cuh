@@ -685,6 +685,9 @@ __global__ void __launch_bounds__(RowsCfg<T, D, E4, NT>::THREADS, 1)
           for (int r = w.s.kv - key0; r < 16; ++r)
             for (int x = lane; x < D * C::ES / 16; x += 32)
               asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(tile_piece(vb, col, r, x)), "r"(0) : "memory");
+          // the next load of this slot writes the same bytes through the async
+          // proxy, which the arrival that frees the slot does not order alone
+          fence_proxy_async_smem();
           __syncwarp();
         }
         if (E4) {
