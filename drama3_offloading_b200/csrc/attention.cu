@@ -124,7 +124,7 @@ static int launch_rows(const AttnParams& p, const d3_attention* a, const d3_kv_c
   const long long tiles = ((long long)a->max_kv + C::KEYS - 1) / C::KEYS;
   // the kernel counts the list in 31 bits; what it reads may be larger than max_q and max_kv say
   if (((long long)a->tokens * p.group / C::ROWS + a->batch) * c->kv_heads *
-          ((long long)a->table_pages * c->page_size / C::KEYS + 1 + kPieceUnits) >= (1LL << 31))
+          ((long long)a->table_pages * c->page_size / C::KEYS + 1 + kPieceUnits) >= kListMost)
     return fail(D3_ERR_TOO_LARGE, "d3_paged_attention: too many key tiles");
   const long long most = (tiles < 1 ? 1 : tiles) * groups * a->batch * c->kv_heads;
   const int parts = (int)(most < part_sms() ? most : part_sms());
@@ -156,7 +156,7 @@ static int launch_chunk(const AttnParams& p, const d3_attention* a, const d3_kv_
   const long long blocks = ((long long)a->max_kv + kBlockKeys - 1) / kBlockKeys;
   const long long most = (blocks < 1 ? 1 : blocks) * tiles * c->kv_heads;
   // the kernel counts the list in 31 bits; the lengths it reads may be larger than max_kv says
-  if (((long long)a->table_pages * c->page_size / kBlockKeys + 1 + kTileUnits<D>) * tiles * c->kv_heads >= (1LL << 31))
+  if (((long long)a->table_pages * c->page_size / kBlockKeys + 1 + kTileUnits<D>) * tiles * c->kv_heads >= kListMost)
     return fail(D3_ERR_TOO_LARGE, "d3_paged_attention: too many key blocks");
   const int pairs = (int)(most < part_sms() / 2 ? most : part_sms() / 2);
   D3_CUDA_TRY(launch_k(attn_chunk_kernel<T, D, E4>, dim3(2 * pairs), dim3(C::THREADS), C::SMEM, st, pdl_enabled(),

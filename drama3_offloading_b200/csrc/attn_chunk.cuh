@@ -125,8 +125,7 @@ struct ChunkPart {
 };
 // All threads of the CTA.  Each warp takes a run of sequences, 32 at a time:
 // their lanes read the lengths, and the whole warp adds up the blocks of each
-// that this launch takes.  The host has checked that the list is shorter than
-// 2^31.
+// that this launch takes.
 __device__ ChunkPart chunk_plan(const AttnParams& p, int per, int more, int part, int parts, int* s_scan,
                                 ChunkPart* s_part) {
   const int warps = blockDim.x >> 5, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -147,16 +146,17 @@ __device__ ChunkPart chunk_plan(const AttnParams& p, int per, int more, int part
     }
   };
   each([&](int, const AttnSeq& s) {
-    sum += warp_head_units(s, per, more) * p.kv_heads;
+    sum = list_add(sum, warp_head_units(s, per, more) * p.kv_heads);
     return false;
   });
   if (lane == 0) s_scan[warp] = sum;
   __syncthreads();
   int before = 0, total = 0;
   for (int w = 0; w < warps; ++w) {
-    before += w < warp ? s_scan[w] : 0;
-    total += s_scan[w];
+    if (w < warp) before = list_add(before, s_scan[w]);
+    total = list_add(total, s_scan[w]);
   }
+  total = list_total(p, total);
   const int g = min(parts, total);
   const int begin = part < g ? part_begin(total, g, part) : 0;
   const int count = part < g ? part_begin(total, g, part + 1) - begin : 0;

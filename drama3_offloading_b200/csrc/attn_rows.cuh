@@ -46,7 +46,7 @@ namespace d3 {
 
 constexpr uint64_t kAttnWaitBudgetNs = 2000000000ull;
 constexpr int kJoinThreads = 256, kJoinBlocks = 3;   // of the joining kernel: threads, blocks an SM
-constexpr int kAttnErrRowsLoad = 51, kAttnErrRowsUse = 52;
+constexpr int kAttnErrRowsLoad = 51, kAttnErrRowsUse = 52, kAttnErrOffsets = 58;
 
 struct AttnParams {
   const void* q;                 // [tokens][heads][D]
@@ -157,8 +157,18 @@ struct RowsWork {
 
 __device__ __forceinline__ int rows_tiles(int kv, int keys) { return max(1, (kv + keys - 1) / keys); }
 
-// units of sequence b over all of its KV heads and row groups.  The host has
-// checked that the list is shorter than 2^31.
+// Lengths of the list add up to kListMost at most.  The host has checked that
+// sequences which share no row stay below it; offsets that go back and forth
+// can give every sequence all of the rows.  A list that reaches it has no parts:
+// the call records an error and writes nothing.
+constexpr int kListMost = 0x7fffffff;
+__device__ __forceinline__ int list_add(int a, int b) { return (int)min((unsigned)a + (unsigned)b, (unsigned)kListMost); }
+__device__ __forceinline__ int list_total(const AttnParams& p, int total) {
+  if (total < kListMost) return total;
+  if (threadIdx.x == 0) attn_error(p.err, kAttnErrOffsets);
+  return 0;
+}
+// units of sequence b over all of its KV heads and row groups
 __device__ __forceinline__ int rows_units(const AttnParams& p, int b, int keys, int rows_per) {
   const AttnSeq s = attn_seq(p, b);
   if (s.rows == 0 || s.rows < p.min_rows || s.rows > p.max_rows) return 0;
@@ -178,20 +188,21 @@ __device__ RowsWork rows_plan(const AttnParams& p, int keys, int rows_per, int p
   const int per = (p.batch + n - 1) / n;
   const int b0 = min(p.batch, tid * per), b1 = min(p.batch, b0 + per);
   int sum = 0;
-  for (int b = b0; b < b1; ++b) sum += rows_units(p, b, keys, rows_per);
+  for (int b = b0; b < b1; ++b) sum = list_add(sum, rows_units(p, b, keys, rows_per));
   int inc = sum;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
     const int v = __shfl_up_sync(0xffffffffu, inc, o);
-    if (lane >= o) inc += v;
+    if (lane >= o) inc = list_add(inc, v);
   }
   if (lane == 31) s_scan[warp] = inc;
   __syncthreads();
   int before = inc - sum, total = 0;
   for (int w = 0; w < n / 32; ++w) {
-    if (w < warp) before += s_scan[w];
-    total += s_scan[w];
+    if (w < warp) before = list_add(before, s_scan[w]);
+    total = list_add(total, s_scan[w]);
   }
+  total = list_total(p, total);
   RowsWork r{total, 0, 0, 0, 0, {0, 0, 0, 0}};
   // no part is empty: a pair's parts are neighbours in the workspace
   const int g = min(parts, total);

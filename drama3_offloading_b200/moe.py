@@ -42,7 +42,7 @@ def error_word(device: torch.device) -> torch.Tensor:
     return t
 
 
-# device error codes: which bounded wait gave up
+# device error codes: which bounded wait gave up (or, _NOT_WAITS, what a kernel refused)
 ERROR_CODES = {
     1: "expert GEMM: the TMA producer waited for a free pipeline stage",
     2: "expert GEMM: the MMA issuer waited for loaded operands or a free accumulator",
@@ -59,7 +59,9 @@ ERROR_CODES = {
     55: "paged attention, chunk: the softmax waited for scores or for the output",
     56: "paged attention, chunk: a widening or scale warp waited for its ring",
     57: "paged attention, chunk: shared memory not on a 1024-byte boundary",
+    58: "paged attention: cu_q goes back and forth: more rows than the call has",
 }
+_NOT_WAITS = (57, 58)
 
 
 def error_message(code: int) -> str:
@@ -74,8 +76,8 @@ def check_errors(device=None) -> None:
         device = torch.device("cuda", torch.cuda.current_device())
     v = int(error_word(device).item())
     if v:
-        raise RuntimeError(f"d3 device error code {v}: {error_message(v)} (a bounded wait "
-                           "expired)")
+        wait = "" if v in _NOT_WAITS else " (a bounded wait expired)"
+        raise RuntimeError(f"d3 device error code {v}: {error_message(v)}{wait}")
 
 
 def router_topk(x: torch.Tensor, gate_w: torch.Tensor, k: int = 8, renorm: bool = True,

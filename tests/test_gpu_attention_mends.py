@@ -64,3 +64,31 @@ def test_many_ends_inside_a_tile(dim, page, dtype, kind):
     for _ in range(20):
         same &= (call(c) == out).all()
     assert bool(same)
+
+
+# ---------------------------------------------------------------- broken offsets
+
+@pytest.mark.parametrize("max_q", [1, 1000])
+def test_offsets_that_go_back_and_forth_are_refused(max_q):
+    """Every second sequence has all rows: 500 x 1000 rows over 243 million keys
+    each are more key tiles than 31 bits count.  Nothing is read or written for
+    them, the error word says why, and the next call is right."""
+    cache = kvcache.PagedKV(4, 16, 1, 128, BF, DEV)
+    q = torch.randn(1000, 1, 128, device=DEV).to(BF)
+    pages = 15_200_000
+    table = torch.zeros(1, pages, dtype=torch.int32, device=DEV).expand(1000, -1)
+    cu = torch.zeros(1001, dtype=torch.int32, device=DEV)
+    cu[1::2] = 1000
+    kv = torch.full((1000,), pages * 16, dtype=torch.int32, device=DEV)
+    out = torch.full_like(q, 5.0)
+    moe.check_errors(DEV)
+    try:
+        attention.paged_attention(q, cache, table, kv, cu, max_q=max_q, out=out)
+        with pytest.raises(RuntimeError, match="code 58: .*cu_q"):
+            moe.check_errors(DEV)
+    finally:
+        moe.error_word(DEV).zero_()
+    assert bool((out == 5.0).all())
+    lens = torch.full((1000,), 50, dtype=torch.int32, device=DEV)
+    got = attention.paged_attention(q, cache, table[:, :4], lens, max_q=max_q)
+    check(got, *ref.attention(q, cache, table[:, :4], lens))
