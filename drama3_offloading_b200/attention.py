@@ -133,7 +133,9 @@ def paged_attention(q: torch.Tensor, cache: PagedKV, page_table: torch.Tensor,
     defaults to head_dim ** -0.5.  ``out`` may be ``q``; rows of it behind the
     last sequence are left as they were.
 
-    Keys that a row's mask hides may hold anything.  Values are multiplied by
+    A row whose visible scores hold NaN or +inf, or -inf alone, gives NaN, as the
+    formula does; a score of -inf among others takes its key away.  Keys that a
+    row's mask hides may hold anything.  Values are multiplied by
     zero there: an infinity or NaN in V reaches rows of the same sequence and
     call that do not see its key."""
     if q.dim() != 3:

@@ -85,7 +85,8 @@ struct ChunkCfg {
 struct ChunkWs {           // carved from the call's workspace
   float* o;                // [pairs][2][D / 4][256][4]
   float* ml;               // [pairs][2][256][2]
-  int4* desc;              // [pairs][2]: (first query token, new tokens, KV head, row tile), (last part, or -1)
+  int4* desc;              // [pairs][2]: (first query token, new tokens, KV head, row tile), (last part or -1,
+                           // last key of the sequence's first new token, ...)
 };
 
 // key blocks that row tile i (of `per` tokens) of a sequence sees: at least one
@@ -826,7 +827,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(ChunkCfg<T, D, E4>::
     ChunkPiece w;
     uint32_t it = 0, pieces = 0;
     int4 desc = make_int4(0, 0, 0, 0);
-    int last_part = -1;
+    int last_part = -1, last_key = 0;
     const float c = p.scale_log2;
     while (walk.next(p, per, w)) {
       const int tok = w.tile * per + (int)rank * tpc + ti;       // of the sequence's new ones
@@ -1001,10 +1002,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(ChunkCfg<T, D, E4>::
           // the part that holds the tile's last block
           const long long u = (long long)part.begin + part.count + (w.nb - w.j1) - 1;
           desc = make_int4(w.s.q0, w.s.n, w.head, w.tile);
+          last_key = w.s.kv - w.s.n;
           last_part = part_of(part.total, min(pairs, part.total), u);
         }
       }
-      const float inv = l > 0.f ? 1.f / l : 0.f;
+      // the sum is NaN for a row of NaN scores, 0 for one of -inf alone; a row
+      // that sees no key is known by its mask
+      const float inv = 1.f / l;
+      const bool sees = last >= 0;
       if (idle || !ok) {
       } else if (whole) {
         // four lanes swap 16-byte pieces of their four rows, so that a store
@@ -1024,7 +1029,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(ChunkCfg<T, D, E4>::
           uint32_t u[4][4];                    // [piece][word]
 #pragma unroll
           for (int q = 0; q < 16; ++q)
-            u[q >> 2][q & 3] = l > 0.f ? Elem<T>::from_f2(o[2 * q] * inv, o[2 * q + 1] * inv) : 0u;
+            u[q >> 2][q & 3] = sees ? Elem<T>::from_f2(o[2 * q] * inv, o[2 * q + 1] * inv) : 0u;
 #pragma unroll
           for (int x = 1; x <= 2; x <<= 1) {
             const bool up = lane & x;
@@ -1066,7 +1071,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(ChunkCfg<T, D, E4>::
     }
     if (rank == 0 && tid == 0) {
       ws.desc[2 * pair] = desc;
-      ws.desc[2 * pair + 1] = make_int4(last_part, 0, 0, 0);
+      ws.desc[2 * pair + 1] = make_int4(last_part, last_key, 0, 0);
     }
   } else if (E4 && warp == 11) {
     // ---- scales: lane has columns lane + 32 i of every block, in the order
@@ -1208,7 +1213,7 @@ __device__ __forceinline__ int chunk_join_groups(const AttnParams& p, const int4
 }
 template <typename T, int D>
 __device__ __forceinline__ void chunk_join(const AttnParams& p, const ChunkWs& ws, const int4& de, int c0, int c1,
-                                           int group) {
+                                           int last_key, int group) {
   constexpr int N = D / 64;
   const int g0 = chunk_join_groups(p, de, 0), half = group >= g0, tpc = 128 / p.group;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -1244,8 +1249,8 @@ __device__ __forceinline__ void chunk_join(const AttnParams& p, const ChunkWs& w
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
       const float f = ex2(ml[k].x - base);
-      if (f == 0.f) continue;
       l = fmaf(ml[k].y, f, l);
+      if (f == 0.f) continue;
 #pragma unroll
       for (int i = 0; i < N; ++i) {
         a[i].x = fmaf(v[k][i].x, f, a[i].x);
@@ -1255,13 +1260,15 @@ __device__ __forceinline__ void chunk_join(const AttnParams& p, const ChunkWs& w
       }
     }
   }
-  const float inv = l > 0.f ? 1.f / l : 0.f;
+  const float inv = 1.f / l;
+  const bool sees = last_key + tok >= 0;
   T* dst = static_cast<T*>(p.out) + (long long)(de.x + tok) * p.out_token +
            (long long)(de.z * p.group + rr - ti * p.group) * p.out_head + x * 4;
 #pragma unroll
   for (int i = 0; i < N; ++i)
     *reinterpret_cast<uint2*>(dst + 16 * i) =
-        make_uint2(Elem<T>::from_f2(a[i].x * inv, a[i].y * inv), Elem<T>::from_f2(a[i].z * inv, a[i].w * inv));
+        sees ? make_uint2(Elem<T>::from_f2(a[i].x * inv, a[i].y * inv), Elem<T>::from_f2(a[i].z * inv, a[i].w * inv))
+             : make_uint2(0u, 0u);
 }
 
 // What the row kernel (parts [0, rows_parts)) and the chunk kernel cut.  After
@@ -1275,26 +1282,31 @@ __device__ __forceinline__ void chunk_join(const AttnParams& p, const ChunkWs& w
 template <typename T, int D>
 __global__ void __launch_bounds__(kJoinThreads, kJoinBlocks) attn_join_kernel(const __grid_constant__ AttnParams p, int rows_per,
                                                                     int rows_parts, int parts, const ChunkWs ws) {
-  __shared__ int s_sum[kJoinThreads / 32], s_c0, s_c1, s_at;
+  __shared__ int s_sum[kJoinThreads / 32], s_c0, s_c1, s_last, s_at;
   __shared__ int4 s_de;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   pdl_trigger();
   pdl_wait();
   int4 de = make_int4(0, 0, 0, 0);
-  int c1 = -1, n = 0;
+  int2 to = make_int2(-1, 0);    // last part, last key of the first new token
+  int n = 0;
+  auto read_to = [](const int4* at) {
+    const int4 v = __ldcg(at);
+    return make_int2(v.x, v.y);
+  };
   if (gridDim.y > 1) {
     const int part = blockIdx.x, row = blockIdx.y;
     de = __ldcg(p.ws_desc + 2 * part);
-    c1 = __ldcg(p.ws_desc + 2 * part + 1).x;
-    if (c1 >= 0 && de.w * rows_per + row < de.y) rows_join<T, D>(p, rows_per, de, part, c1, row);
+    to = read_to(p.ws_desc + 2 * part + 1);
+    if (to.x >= 0 && de.w * rows_per + row < de.y) rows_join<T, D>(p, rows_per, de, part, to.x, to.y, row);
     return;
   }
   const int c0 = tid < rows_parts ? tid : tid - rows_parts;
   if (tid < parts) {
     const int4* at = (tid < rows_parts ? p.ws_desc : ws.desc) + 2 * c0;
     de = __ldcg(at);
-    c1 = __ldcg(at + 1).x;
-    if (c1 >= 0)
+    to = read_to(at + 1);
+    if (to.x >= 0)
       n = tid < rows_parts ? min(rows_per, de.y - de.w * rows_per)
                            : chunk_join_groups(p, de, 0) + chunk_join_groups(p, de, 1);
   }
@@ -1316,12 +1328,13 @@ __global__ void __launch_bounds__(kJoinThreads, kJoinBlocks) attn_join_kernel(co
     if (i >= before && i < before + n) {
       s_de = de;
       s_c0 = c0 + (tid < rows_parts ? 0 : rows_parts);
-      s_c1 = c1;
+      s_c1 = to.x;
+      s_last = to.y;
       s_at = i - before;
     }
     __syncthreads();
-    if (s_c0 < rows_parts) rows_join<T, D>(p, rows_per, s_de, s_c0, s_c1, s_at);
-    else chunk_join<T, D>(p, ws, s_de, s_c0 - rows_parts, s_c1, s_at);
+    if (s_c0 < rows_parts) rows_join<T, D>(p, rows_per, s_de, s_c0, s_c1, s_last, s_at);
+    else chunk_join<T, D>(p, ws, s_de, s_c0 - rows_parts, s_c1, s_last, s_at);
     __syncthreads();
   }
 }

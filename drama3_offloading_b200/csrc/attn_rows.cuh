@@ -69,7 +69,8 @@ struct AttnParams {
   float* ws_o;                   // partial sums
   float* ws_ml;                  // their maxima and sums
   int4* ws_desc;                 // two of each part: (first query token, rows of the sequence, KV head, row
-                                 // group), (last part or -1, ...) of the pair that begins and does not end in it
+                                 // group), (last part or -1, last key of token 0, ...) of the pair that begins
+                                 // and does not end in it
   int* err;
 };
 
@@ -451,7 +452,7 @@ __global__ void __launch_bounds__(RowsCfg<T, D, E4, NT>::THREADS, 1)
     if (++slot == C::SLOTS) { slot = 0; phase ^= 1; }
   };
   int4 desc = make_int4(0, 0, 0, 0);
-  int last_part = -1;
+  int last_part = -1, last_key = 0;
   // a piece's queries are fetched while the one before runs: this warp's rows,
   // 16 bytes a lane
   constexpr int QROWS = (C::ROWS + C::WARPS - 1) / C::WARPS;
@@ -751,6 +752,7 @@ __global__ void __launch_bounds__(RowsCfg<T, D, E4, NT>::THREADS, 1)
       // the part that holds the pair's last tile
       const long long u = (long long)work.begin + work.count + (w.nt - w.t1) - 1;
       desc = make_int4(w.s.q0, w.s.rows, w.head, w.rg);
+      last_key = w.s.kv - w.s.n;
       last_part = part_of(work.total, min((int)gridDim.x, work.total), u);
     }
     float f[NT][2];    // this warp's factor of its rows
@@ -761,14 +763,17 @@ __global__ void __launch_bounds__(RowsCfg<T, D, E4, NT>::THREADS, 1)
         const int r = n * 8 + 2 * t4 + j;
         float m = -INFINITY;
         for (int x = 0; x < C::WARPS; ++x) m = fmaxf(m, s_ml[(x * C::ROWS + r) * 2]);
+        // a maximum leaves NaN out, a sum does not: a row of NaN scores has the
+        // maximum -inf and the sum NaN, and its quotient is NaN, as is that of
+        // a row whose scores are all -inf.  A row that sees no key is known by
+        // its mask alone.
+        const float base = m == -INFINITY ? 0.f : m;
         float l = 0.f;
-        for (int x = 0; x < C::WARPS; ++x) {
-          const float mw = s_ml[(x * C::ROWS + r) * 2];
-          if (mw != -INFINITY) l += s_ml[(x * C::ROWS + r) * 2 + 1] * ex2(mw - m);
-        }
-        f[n][j] = mx[n][j] == -INFINITY ? 0.f : ex2(mx[n][j] - m);
+        for (int x = 0; x < C::WARPS; ++x)
+          l += s_ml[(x * C::ROWS + r) * 2 + 1] * ex2(s_ml[(x * C::ROWS + r) * 2] - base);
+        f[n][j] = ex2(mx[n][j] - base);
         if (E4) f[n][j] *= vref;
-        if (whole) f[n][j] = l > 0.f ? f[n][j] / l : 0.f;
+        if (whole) f[n][j] = last[n][j] >= 0 ? f[n][j] / l : 0.f;
         else if (warp == 0 && g == 0) {
           p.ws_ml[(place * C::ROWS + r) * 2] = m;
           p.ws_ml[(place * C::ROWS + r) * 2 + 1] = l;
@@ -814,18 +819,20 @@ __global__ void __launch_bounds__(RowsCfg<T, D, E4, NT>::THREADS, 1)
   }
   if (tid == 0) {
     p.ws_desc[2 * blockIdx.x] = desc;
-    p.ws_desc[2 * blockIdx.x + 1] = make_int4(last_part, 0, 0, 0);
+    p.ws_desc[2 * blockIdx.x + 1] = make_int4(last_part, last_key, 0, 0);
   }
 }
 
 // Pairs that the parts' cuts go through: the sum of their parts, in the parts'
-// order.  c0 and c1 are the first and the last of its parts, r the row; the
-// threads take turns of D/4 over the parts and add up through shared
-// memory.  The workspace is read through L2: launched early, this kernel
+// order.  c0 and c1 are the first and the last of its parts, last_key that of
+// the sequence's first new token, r the row; the threads take turns of D/4 over
+// the parts and add up through shared memory.  A part's sum counts even if its
+// factor is 0: it may be NaN.  The workspace is read through L2: launched early, this kernel
 // shares SMs with the join of the call before, whose lines of the same memory
 // may still be in L1.
 template <typename T, int D>
-__device__ __forceinline__ void rows_join(const AttnParams& p, int rows_per, const int4& de, int c0, int c1, int r) {
+__device__ __forceinline__ void rows_join(const AttnParams& p, int rows_per, const int4& de, int c0, int c1, int last_key,
+                                          int r) {
   constexpr int GROUPS = kJoinThreads / (D / 4);
   __shared__ float4 s_a[GROUPS][D / 4];
   __shared__ float2 s_ml[GROUPS];
@@ -856,8 +863,8 @@ __device__ __forceinline__ void rows_join(const AttnParams& p, int rows_per, con
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
       const float f = ex2(ml[k].x - base);
-      if (f == 0.f) continue;
       l = fmaf(ml[k].y, f, l);
+      if (f == 0.f) continue;
       a.x = fmaf(v[k].x, f, a.x);
       a.y = fmaf(v[k].y, f, a.y);
       a.z = fmaf(v[k].z, f, a.z);
@@ -877,19 +884,21 @@ __device__ __forceinline__ void rows_join(const AttnParams& p, int rows_per, con
 #pragma unroll
   for (int x = 0; x < GROUPS; ++x) {
     const float f = ex2(s_ml[x].x - base);
+    l = fmaf(s_ml[x].y, f, l);
     if (f == 0.f) continue;
     const float4 v = s_a[x][d4];
-    l = fmaf(s_ml[x].y, f, l);
     a.x = fmaf(v.x, f, a.x);
     a.y = fmaf(v.y, f, a.y);
     a.z = fmaf(v.z, f, a.z);
     a.w = fmaf(v.w, f, a.w);
   }
-  const float inv = l > 0.f ? 1.f / l : 0.f;
+  const float inv = 1.f / l;
   T* dst = static_cast<T*>(p.out) + (long long)(de.x + gr / p.group) * p.out_token +
            (long long)(de.z * p.group + gr % p.group) * p.out_head + d4 * 4;
+  const bool sees = last_key + gr / p.group >= 0;
   *reinterpret_cast<uint2*>(dst) =
-      make_uint2(Elem<T>::from_f2(a.x * inv, a.y * inv), Elem<T>::from_f2(a.z * inv, a.w * inv));
+      sees ? make_uint2(Elem<T>::from_f2(a.x * inv, a.y * inv), Elem<T>::from_f2(a.z * inv, a.w * inv))
+           : make_uint2(0u, 0u);
 }
 
 }  // namespace d3

@@ -458,7 +458,8 @@ D3_API int d3_qk_norm_rope(const d3_norm_rope* a, const d3_kv_cache* cache, d3_s
  * max_kv bound the new tokens and the length of any sequence (they choose the
  * launch; a longer sequence is still computed in full, up to table_pages).
  * Rows of out behind cu_q[batch] are left as they were; out may be q.  The
- * cache has q's type or is E4M3.  heads / kv_heads <= 128.  Keys that a row's
+ * cache has q's type or is E4M3.  heads / kv_heads <= 128.  A row whose visible
+ * scores hold NaN or +inf, or -inf alone, gives NaN.  Keys that a row's
  * mask hides may hold anything; an infinity or NaN in V reaches rows of its
  * sequence that do not see it.
  * workspace: at least d3_paged_attention_workspace_size bytes, 16-byte

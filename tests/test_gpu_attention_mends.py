@@ -92,3 +92,104 @@ def test_offsets_that_go_back_and_forth_are_refused(max_q):
     lens = torch.full((1000,), 50, dtype=torch.int32, device=DEV)
     got = attention.paged_attention(q, cache, table[:, :4], lens, max_q=max_q)
     check(got, *ref.attention(q, cache, table[:, :4], lens))
+
+
+# ---------------------------------------------------------------- not finite
+
+def plain(q, cache, table, kv_lens, cu):
+    """(out, bound) in 64 bits where scores may be infinite or NaN; rows that see
+    no key are zeros.  The bound is tests/attention_reference.py's with the
+    largest |v| in the place of the weighted mean of |v|, over finite scores."""
+    T, H, D = q.shape
+    k, v = ref.values(cache)
+    G, out = H // cache.kv_heads, torch.zeros(T, H, D, dtype=torch.float64, device=DEV)
+    bound = torch.zeros_like(out)
+    step = ref.half_step(q.dtype) * (2 if cache.e4m3 else 1)
+    for b, L in enumerate(kv_lens.tolist()):
+        q0, q1 = int(cu[b]), int(cu[b + 1])
+        n = q1 - q0
+        if L == 0:
+            continue
+        at = table[b].long()
+        kk, vv = (x[at].transpose(0, 1).reshape(cache.kv_heads, -1, D)[:, :L] for x in (k, v))
+        see = torch.arange(L, device=DEV)[None] <= torch.arange(L - n, L, device=DEV)[:, None]
+        for h in range(H):
+            x = q[q0:q1, h].double()
+            s = (x @ kk[h // G].T * D ** -0.5).masked_fill(~see, -torch.inf)
+            p = torch.where(see.any(-1, keepdim=True), torch.softmax(s, -1), 0.0)
+            out[q0:q1, h] = p @ vv[h // G]
+            qk = (x.abs() @ kk[h // G].abs().T).nan_to_num(0, 0, 0).amax(-1, keepdim=True) * D ** -0.5
+            score = qk * (D + 8) * 2.0 ** -24 + 2.0 ** -21
+            bound[q0:q1, h] = vv[h // G].abs().amax() * (step + 2 * score + L * 2.0 ** -23 + 2.0 ** -24)
+    fin = torch.finfo(q.dtype)
+    return out, bound + ref.half_step(q.dtype) * out.nan_to_num().abs() + fin.smallest_normal * ref.half_step(q.dtype)
+
+
+def same_kind(out, want, bound):
+    """NaN where the formula has NaN, zeros and values where it has them."""
+    assert torch.equal(out.isnan(), want.isnan())
+    ok = ~want.isnan()
+    assert bool(((out.double() - want)[ok].abs() <= bound[ok]).all())
+    moe.check_errors(DEV)
+
+
+# one piece a sequence, and sequences that several SMs share
+WHOLE, SPLIT = [(0, 40), (2, 1), (0, 0)], [(0, 5000), (2, 1)]
+SHAPES = [(256, 8, 2, 64, BF, BF), (128, 8, 2, 16, FP, FP), (256, 8, 2, 64, BF, E4), (128, 12, 2, 32, FP, E4)]
+
+
+def some(lens, n, seed, shape):
+    """A batch whose first sequences have n new tokens (0 stands for n)."""
+    return batch(seed, [(a or n, kv) for a, kv in lens], shape[1], shape[2], shape[0], *shape[3:])
+
+
+@pytest.mark.parametrize("shape", SHAPES)
+@pytest.mark.parametrize("lens", [WHOLE, SPLIT], ids=["whole", "split"])
+@pytest.mark.parametrize("n", [1, 3, 40])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+def test_a_query_that_is_not_finite_gives_nan_to_its_row_alone(shape, lens, n, bad):
+    c = some(lens, n, 3, shape)
+    q = c[2].clone()
+    q[n - 1, 1] = bad                                  # the last row, one head of it
+    q[-1, 0, 5] = bad                                  # sequence of two rows and one key, or of n and none
+    want, bound = plain(q, c[0], c[1], c[4], c[3])
+    assert bool(want[n - 1, 1].isnan().all()) and int(want.isnan().any(-1).sum()) == (2 if lens is SPLIT else 1)
+    same_kind(call(c, q), want, bound)
+
+
+@pytest.mark.parametrize("shape", SHAPES)
+@pytest.mark.parametrize("lens", [WHOLE, SPLIT], ids=["whole", "split"])
+@pytest.mark.parametrize("n", [1, 3, 40])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), float("-inf")])
+def test_a_visible_key_that_is_not_finite(shape, lens, n, bad):
+    """NaN, or an infinite score above all others, gives NaN; a score of -inf
+    takes its key away.  Rows that do not see the key are as they were."""
+    c = some(lens, n, 4, shape)
+    q, kv, page = c[2].clone(), lens[0][1], c[0].page_size
+    q[:, ::2, 9], q[:, 1::2, 9] = 1.0, -1.0
+    for j in (kv - 2, 7):                              # the last row but one sees the former
+        k = c[0].k.clone()
+        where = (int(c[1][0, j // page]), 1, j % page)
+        if c[0].e4m3:                                  # as a row with one such element is written
+            c[0].k[where].view(torch.uint8)[9] = 0x7F
+        else:
+            c[0].k[where][9] = bad
+        want, bound = plain(q, c[0], c[1], c[4], c[3])
+        gone = want[n - 1].isnan().all(-1).sum()
+        assert int(gone) == shape[1] // shape[2] // (1 if c[0].e4m3 or bad != bad else 2)
+        same_kind(call(c, q), want, bound)
+        c[0].k.copy_(k)
+
+
+@pytest.mark.parametrize("shape", SHAPES[:2])
+@pytest.mark.parametrize("lens", [WHOLE, SPLIT], ids=["whole", "split"])
+@pytest.mark.parametrize("n", [1, 3, 40])
+def test_scores_of_minus_infinity_alone(shape, lens, n):
+    """As the quotient 0 / 0, and unlike a row that sees no key."""
+    c = some(lens, n, 5, shape)
+    c[0].k[..., 0] = float("-inf")
+    q = c[2].clone()
+    q[..., 0] = 1.0
+    want, bound = plain(q, c[0], c[1], c[4], c[3])
+    assert bool(want[:n].isnan().all())
+    same_kind(call(c, q), want, bound)
