@@ -33,7 +33,9 @@
 // but for elements 2^-24 below the row's largest); a key's scale multiplies
 // its scores in fp32; a value's scale, in units of a power of two not below any
 // scale the warp has met, multiplies the probability before it is rounded to
-// fp16.
+// fp16.  The product is at most 1 and goes into fp16 times 2^15, so that its
+// eleven bits are whole down to 2^-29 of that unit and something is left down to
+// 2^-40: a row that hardly heeds a key of far larger values keeps the others'.
 #pragma once
 
 #include "kv_common.cuh"
@@ -44,6 +46,7 @@
 
 namespace d3 {
 
+constexpr float kCodesUp = 0x1p15f;        // of probability times scale, in fp16
 constexpr uint64_t kAttnWaitBudgetNs = 2000000000ull;
 constexpr int kJoinThreads = 256, kJoinBlocks = 3;   // of the joining kernel: threads, blocks an SM
 constexpr int kAttnErrRowsLoad = 51, kAttnErrRowsUse = 52, kAttnErrOffsets = 58;
@@ -646,8 +649,8 @@ __global__ void __launch_bounds__(RowsCfg<T, D, E4, NT>::THREADS, 1)
           }
           // 1 / vref, a power of two as well, by its exponent
           const float inv = vref > 0.f ? __uint_as_float(0x7f000000u - __float_as_uint(vref)) : 0.f;
-          u0 *= inv;
-          u1 *= inv;
+          u0 = u0 * inv * kCodesUp;
+          u1 = u1 * inv * kCodesUp;
         }
         uint32_t pb[NT][2];
         float pr[NT][4], keep[NT][2], top[NT][2];
@@ -772,7 +775,7 @@ __global__ void __launch_bounds__(RowsCfg<T, D, E4, NT>::THREADS, 1)
         for (int x = 0; x < C::WARPS; ++x)
           l += s_ml[(x * C::ROWS + r) * 2 + 1] * ex2(s_ml[(x * C::ROWS + r) * 2] - base);
         f[n][j] = ex2(mx[n][j] - base);
-        if (E4) f[n][j] *= vref;
+        if (E4) f[n][j] *= vref * (1.f / kCodesUp);
         if (whole) f[n][j] = last[n][j] >= 0 ? f[n][j] / l : 0.f;
         else if (warp == 0 && g == 0) {
           p.ws_ml[(place * C::ROWS + r) * 2] = m;

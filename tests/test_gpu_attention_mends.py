@@ -193,3 +193,47 @@ def test_scores_of_minus_infinity_alone(shape, lens, n):
     want, bound = plain(q, c[0], c[1], c[4], c[3])
     assert bool(want[:n].isnan().all())
     same_kind(call(c, q), want, bound)
+
+
+# ---------------------------------------------------------------- codes
+
+@pytest.mark.parametrize("dim,heads,hk,page,dtype", [(256, 8, 2, 64, BF), (128, 8, 2, 16, FP), (256, 16, 2, 32, FP), (128, 12, 2, 128, BF)])
+@pytest.mark.parametrize("n", [1, 2, 40])
+@pytest.mark.parametrize("length", [50, 300, 4000])
+def test_values_far_above_those_that_count(dim, heads, hk, page, dtype, n, length):
+    """Every 20th key has values 2^22 times the others' and a score that takes
+    it out: what is left is theirs, with all of its bits."""
+    c = batch(7, [(n, length), (n, max(1, length // 3))], heads, hk, dim, page, dtype, E4)
+    cache, table, q, cu, kv = c
+    q[..., 0] = 20.0
+    g = torch.Generator(device=DEV).manual_seed(2)
+    for b, L in enumerate(kv.tolist()):
+        k, v = (torch.randn(L, hk, dim, generator=g, device=DEV) for _ in range(2))
+        k[..., 0] = 0.0
+        v *= 2.0 ** -7
+        loud = torch.arange(L, device=DEV) % 20 == 3
+        k[loud, :, 0] = -40.0
+        v[loud] *= 2.0 ** 22
+        i = torch.arange(L, device=DEV)
+        kvcache.write(cache, k.to(dtype), v.to(dtype).clamp(-3e4, 3e4), table[b].long()[i // page] * page + i % page)
+    want, _ = ref.attention(q, cache, table, kv, cu)
+    # as in the reference's bound, but instead of 2^-24 of the largest value a half
+    # step 2^-25 of fp16 over the unit 2^15, which is at most twice a scale, for
+    # each key: 2^-39 of the largest value
+    K, V = ref.values(cache)
+    bound = torch.zeros_like(want)
+    step = 2 * ref.half_step(dtype)
+    for b, L in enumerate(kv.tolist()):
+        r = slice(int(cu[b]), int(cu[b + 1]))
+        at = table[b].long()
+        kk, vv = (x[at].transpose(0, 1).reshape(hk, -1, dim)[:, :L] for x in (K, V))
+        see = torch.arange(L, device=DEV)[None] <= torch.arange(L - n, L, device=DEV)[:, None]
+        for h in range(heads):
+            x, kh, vh = q[r, h].double(), kk[h // (heads // hk)], vv[h // (heads // hk)]
+            p = torch.softmax((x @ kh.T * dim ** -0.5).masked_fill(~see, -torch.inf), -1).nan_to_num()
+            qk = (x.abs() @ kh.abs().T).amax(-1, keepdim=True) * dim ** -0.5
+            err = step + 2 * (qk * (dim + 8) * 2.0 ** -24 + 2.0 ** -21) + L * 2.0 ** -23
+            bound[r, h] = p @ vh.abs() * err + L * 2.0 ** -39 * vh.abs().amax()
+    fin = torch.finfo(dtype)
+    bound += ref.half_step(dtype) * want.abs() + fin.smallest_normal * ref.half_step(dtype)
+    check(call((cache, table, q, cu, kv)), want, bound)
