@@ -29,8 +29,9 @@
 // token over a short context is 9 us of latency.
 //
 // e4m3 caches: codes are exact in fp16, so the products run in fp16 whatever
-// the queries' type.  bf16 queries are scaled by a power of two per row (exact
-// but for elements 2^-24 below the row's largest); a key's scale multiplies
+// the queries' type.  bf16 queries are scaled by a power of two per row that
+// brings the largest into [2^14, 2^15), the top of fp16: their eight bits stay
+// whole but for elements 2^31 times smaller than it.  A key's scale multiplies
 // its scores in fp32; a value's scale, in units of a power of two not below any
 // scale the warp has met, multiplies the probability before it is rounded to
 // fp16.  The product is at most 1 and goes into fp16 times 2^15, so that its
@@ -520,10 +521,11 @@ __global__ void __launch_bounds__(RowsCfg<T, D, E4, NT>::THREADS, 1)
         for (int i = 0; i < 8; ++i) amax = fmaxf(amax, fabsf(x[i]));
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
-        // amax in [2^(e-1), 2^e); the factor's exponent stays inside fp32's
+        // amax in [2^(e-1), 2^e) goes to [2^14, 2^15); the factor and its inverse
+        // stay inside fp32's normal range
         int e = 0;
         if (amax > 0.f && amax < INFINITY) frexpf(amax, &e);
-        e = max(-120, min(120, e));
+        e = max(-126, e - 15);
         mul = ldexpf(1.f, -e);
         back = ldexpf(1.f, e);
       }

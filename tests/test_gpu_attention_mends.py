@@ -237,3 +237,30 @@ def test_values_far_above_those_that_count(dim, heads, hk, page, dtype, n, lengt
     fin = torch.finfo(dtype)
     bound += ref.half_step(dtype) * want.abs() + fin.smallest_normal * ref.half_step(dtype)
     check(call((cache, table, q, cu, kv)), want, bound)
+
+
+@pytest.mark.parametrize("dim,heads,hk,page", [(256, 8, 2, 64), (128, 8, 2, 16), (256, 16, 2, 32), (128, 12, 2, 128)])
+@pytest.mark.parametrize("n", [1, 2, 40])
+@pytest.mark.parametrize("top", [2.0 ** 18, 2.0 ** 24, -2.0 ** 120])
+def test_a_query_element_far_above_the_others(dim, heads, hk, page, n, top):
+    """One element of a row is huge and meets zeros in every key: the scores are
+    the other elements'.  The bound counts |q| |k|, so nothing of it is the huge
+    one's; queries that become fp16 may lose a step 2^-25 over 2^14, of the
+    largest element, of each element."""
+    c = batch(8, [(n, 300), (n, 70)], heads, hk, dim, page, BF, E4)
+    cache, table, q, cu, kv = c
+    cache.k[..., 5] = 0
+    big = q.clone()
+    big[..., 5] = top
+    want, bound = ref.attention(big, cache, table, kv, cu)
+    K, V = ref.values(cache)
+    fin = lambda x: x.nan_to_num()
+    lost = 2.0 ** -39 * abs(top) * fin(K).abs().sum(-1).amax() * dim ** -0.5
+    if top < 2.0 ** 30:
+        bound = bound + 2 * lost * fin(V).abs().amax()
+        got = call((cache, table, big, cu, kv))
+        check(got, want, bound)
+    else:       # too far above: what is left of the others is under fp16's least step or not, but finite
+        got = call((cache, table, big, cu, kv))
+        moe.check_errors(DEV)
+        assert bool(got.isfinite().all())
