@@ -75,18 +75,33 @@ def index(t: torch.Tensor, name: str, tokens: int, device: int) -> None:
         raise ValueError(f"{name} is on {t.device}, not on device {device}")
 
 
+def _free(t: torch.Tensor):
+    """(token stride, head stride) of ``t``'s rows, the stride of a dimension of
+    size 1 -- any number, of one token of an odd pitch, say -- replaced by a
+    contiguous tensor's."""
+    heads, dim = t.shape[1:]
+    s0, s1, _ = t.stride()
+    return heads * dim if t.shape[0] == 1 else s0, dim if heads == 1 else s1
+
+
 def in_place(t: torch.Tensor):
     """(``t``, address, token stride, head stride), or those of a copy if the
     rows do not lie as the kernels read them: contiguous dims, rows on 16-byte
     boundaries."""
     s0, s1, s2 = t.stride()
     at = t.data_ptr()
-    if s2 == 1 and s0 > 0 and s1 > 0 and not (s0 | s1) & 7 and not at & 15:
-        return t, at, s0, s1
+    if s2 == 1 and not at & 15:
+        if s0 > 0 and s1 > 0 and not (s0 | s1) & 7:
+            return t, at, s0, s1
+        s0, s1 = _free(t)
+        if s0 > 0 and s1 > 0 and not (s0 | s1) & 7:
+            return t, at, s0, s1
     t = t.contiguous()
     if t.data_ptr() & 15:
         t = t.clone()
-    return t, t.data_ptr(), t.stride(0), t.stride(1)
+    # (what is contiguous for torch may keep such a stride)
+    heads, dim = t.shape[1:]
+    return t, t.data_ptr(), heads * dim, dim
 
 
 def output(t: torch.Tensor, shape, dtype, device: int):
@@ -94,8 +109,11 @@ def output(t: torch.Tensor, shape, dtype, device: int):
     if t.shape == shape and t.dtype is dtype and t.get_device() == device:
         s0, s1, s2 = t.stride()
         at = t.data_ptr()
-        if s2 == 1 and s0 > 0 and s1 > 0 and not (s0 | s1) & 7 and not at & 15:
-            return t, at, s0, s1
+        if s2 == 1 and not at & 15:
+            if s0 <= 0 or s1 <= 0 or (s0 | s1) & 7:
+                s0, s1 = _free(t)
+            if s0 > 0 and s1 > 0 and not (s0 | s1) & 7:
+                return t, at, s0, s1
     raise ValueError(f"out must be {dtype} {tuple(shape)} on device {device}, its rows contiguous on "
                      "16-byte boundaries")
 

@@ -264,3 +264,42 @@ def test_a_query_element_far_above_the_others(dim, heads, hk, page, n, top):
         got = call((cache, table, big, cu, kv))
         moe.check_errors(DEV)
         assert bool(got.isfinite().all())
+
+
+# ---------------------------------------------------------------- views
+
+@pytest.mark.parametrize("kind", [BF, E4])
+@pytest.mark.parametrize("t", [slice(0, 1), slice(2, 3), slice(1, 2), slice(0, 5)])
+def test_tokens_cut_from_a_buffer_of_an_odd_pitch(kind, t):
+    """Rows 2568 bytes apart: one of them (its pitch means nothing) as several."""
+    pitch = torch.randn(5, 1284, device=DEV).to(BF)
+    x = pitch[:, :1024].view(5, 8, 128)[t]
+    q, k, v = x[:, :4], x[:, 4:6], x[:, 6:]
+    n = x.shape[0]
+    w, f = torch.ones(128, dtype=BF, device=DEV), attention.rope_frequencies(64, device=DEV)
+    pos, slots = torch.arange(n, device=DEV), torch.arange(n, device=DEV) + 3
+    table = torch.zeros(1, 1, dtype=torch.int32, device=DEV)
+    lens, cu = torch.tensor([n + 3], dtype=torch.int32, device=DEV), torch.tensor([0, n], dtype=torch.int32, device=DEV)
+
+    def run(q, k, v):
+        cache = kvcache.PagedKV(1, 16, 2, 128, kind, DEV)
+        kvcache.write(cache, k, v, slots)
+        first = kvcache.read(cache, slots, dtype=BF)
+        turned = attention.qk_norm_rope(q, k, w, w, pos, f)
+        qw = attention.qk_norm_rope_write(q, k, v, w, w, pos, f, cache, slots)
+        a = attention.paged_attention(q, cache, table, lens, cu, max_q=n)
+        return (*first, *turned, qw, a, *kvcache.read(cache, slots, dtype=BF))
+    for a, b in zip(run(q, k, v), run(q.clone(), k.clone(), v.clone())):
+        assert torch.equal(a, b)
+    if n == 1 and q.data_ptr() % 16 == 0:              # ... and as outputs
+        want = run(q, k, v)
+        cache = kvcache.PagedKV(1, 16, 2, 128, kind, DEV)
+        kvcache.write(cache, k, v, slots)
+        attention.qk_norm_rope_write(q.clone(), k, v, w, w, pos, f, cache, slots)
+        before = pitch.clone()
+        assert attention.paged_attention(q, cache, table, lens, out=q) is q
+        assert torch.equal(q, want[5])
+        back = before[:, :1024].view(5, 8, 128)[t]
+        attention.qk_norm_rope(back[:, :4], back[:, 4:6], w, w, pos, f, out=(q, k))
+        assert torch.equal(q, want[2]) and torch.equal(k, want[3])
+    moe.check_errors(DEV)
