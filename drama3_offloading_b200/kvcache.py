@@ -43,6 +43,8 @@ def elsewhere(device: int, stream) -> bool:
     arguments."""
     if device < 0:
         raise ValueError("tensors on the CPU: a CUDA device is needed")
+    if stream is not None and stream.device_index != device:
+        raise ValueError(f"stream is of device {stream.device_index}, the tensors are on {device}")
     return stream is not None or _device() != device
 
 

@@ -1,5 +1,8 @@
 """How the rows of the cache and attention calls are read and written in place,
-without a GPU: strides of dimensions of size 1 carry no meaning."""
+without a GPU: strides of dimensions of size 1 carry no meaning.  And where a
+call runs: never on a stream of another device."""
+from types import SimpleNamespace
+
 import pytest
 import torch
 
@@ -57,3 +60,11 @@ def test_outputs_of_one_token_or_head():
     for x in (pitch[:2], pitch[1:2], pitch[:1].expand(5, -1, -1), pitch[:1, :1].expand(1, 8, -1)):
         with pytest.raises(ValueError):
             kvcache.output(x, x.shape, BF, -1)
+
+
+def test_a_stream_of_another_device_is_refused():
+    """(such a call would else leave the stream for its device's current one)"""
+    for device, of in ((0, 1), (1, 0)):
+        with pytest.raises(ValueError, match="stream"):
+            kvcache.elsewhere(device, SimpleNamespace(device_index=of))
+    assert kvcache.elsewhere(1, SimpleNamespace(device_index=1))
