@@ -743,10 +743,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(ChunkCfg<T, D, E4>::
         }
       }
       // after a wait ran out: what is in flight has landed before the memory goes
-      if (!ok && qn && rank == 0) mbar_wait(q_full, (qn - 1) & 1, kAttnWaitBudgetNs);
       if (!ok && (E4 || rank == 0))
-#pragma unroll 1
-        for (int i = 0; i < N; ++i) mbar_wait(bars_full + i, pos.phase ^ (i <= pos.slot ? 0 : 1), kAttnWaitBudgetNs);
+        drain_ring(N, pos.slot, pos.phase, kAttnWaitBudgetNs,
+                   [&](int i, uint32_t par) { return mbar_try_wait(bars_full + i, par); },
+                   [] { return globaltimer_ns(); });
+      if (!ok && qn && rank == 0) mbar_wait(q_full, (qn - 1) & 1, kAttnWaitBudgetNs);
     }
   } else if (warp == 8) {
     // ---- MMAs of the pair

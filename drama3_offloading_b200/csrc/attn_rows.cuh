@@ -40,6 +40,7 @@
 #pragma once
 
 #include "kv_common.cuh"
+#include "ring_drain.h"
 
 #include <cuda.h>
 
@@ -429,11 +430,11 @@ __global__ void __launch_bounds__(RowsCfg<T, D, E4, NT>::THREADS, 1)
           if (++slot == C::SLOTS) { slot = 0; phase ^= 1; }
         }
       }
-      if (!ok) {
-        // what is still in flight has landed before the CTA's memory goes
-#pragma unroll 1
-        for (int i = 0; i < C::SLOTS; ++i) mbar_wait(full + i, phase ^ (i < slot ? 0 : 1), kAttnWaitBudgetNs);
-      }
+      // what is still in flight has landed before the CTA's memory goes
+      if (!ok)
+        drain_ring(C::SLOTS, slot, phase, kAttnWaitBudgetNs,
+                   [&](int i, uint32_t par) { return mbar_try_wait(full + i, par); },
+                   [] { return globaltimer_ns(); });
     }
     return;
   }
