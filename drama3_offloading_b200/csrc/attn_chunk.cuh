@@ -536,12 +536,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(ChunkCfg<T, D, E4>::
   uint64_t* o_free = o_done + 1;
   uint64_t* o_last = o_free + 1;
   uint64_t* all_done = o_last + 1;
-  uint64_t* x_bar = all_done + 1;        // [4]: a row's two threads
-  uint64_t* raw_full = x_bar + 4;        // codes: [RAWS]
+  uint64_t* raw_full = all_done + 1;     // codes: [RAWS]
   uint64_t* raw_empty = raw_full + C::RAWS;
   uint64_t* sc_full = raw_empty + C::RAWS;   // [SC_RING]
   uint64_t* sc_empty = sc_full + C::SC_RING;
-  static_assert(2 * C::SLOTS + 14 + 2 * C::RAWS + 2 * C::SC_RING <= 64, "barriers");
+  static_assert(2 * C::SLOTS + 10 + 2 * C::RAWS + 2 * C::SC_RING <= 64, "barriers");
   const uint32_t sq = smem_u32(smem), ss = smem_u32(s_ring);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const uint32_t rank = cluster_rank();
@@ -568,7 +567,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(ChunkCfg<T, D, E4>::
     mbar_init(o_free, 16);
     mbar_init(o_last, 1);
     mbar_init(all_done, 1);
-    for (int i = 0; i < 4; ++i) mbar_init(x_bar + i, 2);
     if (E4) {
       for (int i = 0; i < C::RAWS; ++i) {
         mbar_init(raw_full + i, ps < kSmallPage ? 32 : 1);     // 32 lanes' copies, or TMA

@@ -13,7 +13,6 @@ template <typename T>
 struct Elem;
 template <>
 struct Elem<__nv_bfloat16> {
-  using T2 = __nv_bfloat162;
   static __device__ __forceinline__ float2 to_f2(uint32_t w) {
     return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&w));
   }
@@ -24,7 +23,6 @@ struct Elem<__nv_bfloat16> {
 };
 template <>
 struct Elem<__half> {
-  using T2 = __half2;
   static __device__ __forceinline__ float2 to_f2(uint32_t w) {
     return __half22float2(*reinterpret_cast<const __half2*>(&w));
   }
