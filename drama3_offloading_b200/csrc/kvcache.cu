@@ -68,15 +68,18 @@ constexpr int kMaxHalf = 128;          // rotary pairs of the widest head
 constexpr int kMaxTokensPerCta = 8;
 
 // x / s rounded as the division is.  With r = 1 / s rounded and q = x r, the
-// remainder x - q s is exact in one fused step and q + rem r is the quotient
+// remainder q s - x is exact in one fused step and q - rem r is the quotient
 // rounded correctly (Markstein's correction): three operations, two values at
 // a time, where a division takes about ten.  The remainder must not
-// underflow: the caller sees to it that s is not far from 1.
+// underflow: the caller sees to it that s is not far from 1.  (With the
+// remainder's sign the other way round -0 would become 0.)
 __device__ __forceinline__ void div2(float& x, float& y, float s, float r) {
   float q0 = x, q1 = y;
   mul2(q0, q1, r, r);
-  fma2v(x, y, -q0, s, -q1, s);
-  fma2v(q0, q1, x, r, y, r);
+  x = -x;
+  y = -y;
+  fma2v(x, y, q0, s, q1, s);
+  fma2v(q0, q1, x, -r, y, -r);
   x = q0;
   y = q1;
 }

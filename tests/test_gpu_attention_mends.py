@@ -303,3 +303,30 @@ def test_tokens_cut_from_a_buffer_of_an_odd_pitch(kind, t):
         attention.qk_norm_rope(back[:, :4], back[:, 4:6], w, w, pos, f, out=(q, k))
         assert torch.equal(q, want[2]) and torch.equal(k, want[3])
     moe.check_errors(DEV)
+
+
+# ---------------------------------------------------------------- zeros
+
+@pytest.mark.parametrize("dim", [128, 256])
+@pytest.mark.parametrize("dtype", [BF, FP])
+def test_a_negative_zero_keeps_its_sign(dim, dtype):
+    """Codes are those of the formula bit for bit, 0x80 for -0 among them, and
+    read back as -0; in rows of zeros as in others."""
+    g = torch.Generator(device=DEV).manual_seed(1)
+    x = torch.randn(70, 2, dim, generator=g, device=DEV).to(dtype)
+    x[torch.rand(x.shape, generator=g, device=DEV) < 0.2] = -0.0
+    x[3], x[4], x[5, :, 1:] = -0.0, 0.0, -0.0
+    w, f = torch.ones(dim, dtype=dtype, device=DEV), attention.rope_frequencies(64, device=DEV)
+    slots = torch.arange(70, device=DEV)
+    code, scale = (t.to(DEV) for t in ref.quantise(x.cpu()))
+    assert int((code.view(torch.uint8) == 0x80).sum()) > 1000
+    for call in (lambda c: kvcache.write(c, x, x, slots),
+                 lambda c: attention.qk_norm_rope_write(x, x, x, w, w, slots, f, c, slots)):
+        cache = kvcache.PagedKV(5, 16, 2, dim, E4, DEV)
+        call(cache)
+        put = lambda t: t.transpose(1, 2).reshape(80, 2, *t.shape[3:])[:70]
+        assert torch.equal(put(cache.v.view(torch.uint8)), code.view(torch.uint8))
+        assert torch.equal(put(cache.v_scale), scale)
+        back = kvcache.read(cache, slots, dtype=dtype)[1]
+        want = (code.float() * scale[..., None]).to(dtype)
+        assert torch.equal(back.view(torch.int16), want.view(torch.int16))
