@@ -24,6 +24,9 @@ template <typename Filled, typename Now>
 D3_HOST_DEVICE bool drain_ring(int n, int slot, uint32_t phase, uint64_t budget_ns, Filled filled, Now now) {
   const uint64_t t0 = now();
   bool all = true;
+#ifdef __CUDACC__
+#pragma unroll 1
+#endif
   for (int i = 0; i < n; ++i) {
     const uint32_t parity = phase ^ (i < slot ? 0u : 1u);
     bool there = filled(i, parity);
