@@ -823,10 +823,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(ChunkCfg<T, D, E4>::
     };
     auto wait = [&](uint64_t* bar, uint32_t par) { wait_warp(bar, par, kAttnErrChunkSoftmax); };
     ChunkWalk walk(part, MORE);
-    ChunkPiece w;
+    ChunkPiece w{};
     uint32_t it = 0, pieces = 0;
-    int4 desc = make_int4(0, 0, 0, 0);
-    int last_part = -1, last_key = 0;
     const float c = p.scale_log2;
     while (walk.next(p, per, w)) {
       const int tok = w.tile * per + (int)rank * tpc + ti;       // of the sequence's new ones
@@ -997,13 +995,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(ChunkCfg<T, D, E4>::
       if (!whole && h == 0) {
         ws.ml[((size_t)place * 256 + row) * 2] = m;
         ws.ml[((size_t)place * 256 + row) * 2 + 1] = l;
-        if (w.j0 == 0 && tid == 0) {
-          // the part that holds the tile's last block
-          const long long u = (long long)part.begin + part.count + (w.nb - w.j1) - 1;
-          desc = make_int4(w.s.q0, w.s.n, w.head, w.tile);
-          last_key = w.s.kv - w.s.n;
-          last_part = part_of(part.total, min(pairs, part.total), u);
-        }
       }
       // the sum is NaN for a row of NaN scores, 0 for one of -inf alone; a row
       // that sees no key is known by its mask
@@ -1069,8 +1060,15 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(ChunkCfg<T, D, E4>::
       if (lane == 0) mbar_arrive_remote(mapa(smem_u32(o_free), 0));
     }
     if (rank == 0 && tid == 0) {
-      ws.desc[2 * pair] = desc;
-      ws.desc[2 * pair + 1] = make_int4(last_part, last_key, 0, 0);
+      // a tile that begins and does not end in this part is its last piece
+      if (w.j0 == 0 && w.j1 > 0 && w.j1 < w.nb) {
+        // the part that holds the tile's last block
+        const long long u = (long long)part.begin + part.count + (w.nb - w.j1) - 1;
+        ws.desc[2 * pair] = make_int4(w.s.q0, w.s.n, w.head, w.tile);
+        ws.desc[2 * pair + 1] = make_int4(part_of(part.total, min(pairs, part.total), u), w.s.kv - w.s.n, 0, 0);
+      } else {
+        ws.desc[2 * pair + 1] = make_int4(-1, 0, 0, 0);
+      }
     }
   } else if (E4 && warp == 11) {
     // ---- scales: lane has columns lane + 32 i of every block, in the order

@@ -456,8 +456,6 @@ __global__ void __launch_bounds__(RowsCfg<T, D, E4, NT>::THREADS, 1)
     if (lane == 0) mbar_arrive(empty + slot);
     if (++slot == C::SLOTS) { slot = 0; phase ^= 1; }
   };
-  int4 desc = make_int4(0, 0, 0, 0);
-  int last_part = -1, last_key = 0;
   // a piece's queries are fetched while the one before runs: this warp's rows,
   // 16 bytes a lane
   constexpr int QROWS = (C::ROWS + C::WARPS - 1) / C::WARPS;
@@ -754,13 +752,6 @@ __global__ void __launch_bounds__(RowsCfg<T, D, E4, NT>::THREADS, 1)
     const bool whole = w.t0 == 0 && w.t1 == w.nt;
     const int place = blockIdx.x * 2 + (w.t0 == 0 ? 1 : 0);
     float* wo = p.ws_o + (size_t)place * C::ROWS * D;
-    if (!whole && w.t0 == 0) {
-      // the part that holds the pair's last tile
-      const long long u = (long long)work.begin + work.count + (w.nt - w.t1) - 1;
-      desc = make_int4(w.s.q0, w.s.rows, w.head, w.rg);
-      last_key = w.s.kv - w.s.n;
-      last_part = part_of(work.total, min((int)gridDim.x, work.total), u);
-    }
     float f[NT][2];    // this warp's factor of its rows
 #pragma unroll
     for (int n = 0; n < NT; ++n)
@@ -824,8 +815,16 @@ __global__ void __launch_bounds__(RowsCfg<T, D, E4, NT>::THREADS, 1)
     }
   }
   if (tid == 0) {
-    p.ws_desc[2 * blockIdx.x] = desc;
-    p.ws_desc[2 * blockIdx.x + 1] = make_int4(last_part, last_key, 0, 0);
+    // a pair that begins and does not end in this part is its last piece
+    if (w.t0 == 0 && w.t1 > 0 && w.t1 < w.nt) {
+      // the part that holds the pair's last tile
+      const long long u = (long long)work.begin + work.count + (w.nt - w.t1) - 1;
+      p.ws_desc[2 * blockIdx.x] = make_int4(w.s.q0, w.s.rows, w.head, w.rg);
+      p.ws_desc[2 * blockIdx.x + 1] =
+          make_int4(part_of(work.total, min((int)gridDim.x, work.total), u), w.s.kv - w.s.n, 0, 0);
+    } else {
+      p.ws_desc[2 * blockIdx.x + 1] = make_int4(-1, 0, 0, 0);
+    }
   }
 }
 
