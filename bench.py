@@ -252,7 +252,9 @@ def measured_peaks() -> dict:
 # ---------------------------------------------------------------- decode
 
 def decode_config(args, capacity: int | None = None) -> dict:
-    """The decode workload's ``config`` (the same dict for both arms)."""
+    """The decode workload's ``config``: the same dict for both arms, but for the
+    K/V of ``--kv-cache bf16`` or ``e4m3``, which the reference arm does not have.
+    There it is the dense stand-in's, so those two lines are not of the same bytes."""
     from drama3_offloading_b200 import decode as dec
     cap = capacity or max(1, int(args.cache_gib * (1 << 30)) // (args.layers * EXPERT_BYTES))
     kind = args.kv_cache if args.impl == "ours" else "dense"

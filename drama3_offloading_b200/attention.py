@@ -98,7 +98,8 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor,
     head, then the first ``2 * len(inv_freq)`` dims turned by
     ``positions * inv_freq`` in pairs of halves (or, ``interleaved``, of
     neighbours).  ``weight_offset=1`` for zero-centred weights.  ``out=(q_out,
-    k_out)`` may be ``(q, k)``.  Returns (q, k)."""
+    k_out)`` may be ``(q, k)``.  The mean is float32, the angle float64;
+    len(inv_freq) is a multiple of 8.  Returns (q, k)."""
     return _norm_rope(q, k, None, q_weight, k_weight, positions, inv_freq, None, None, eps,
                       weight_offset, interleaved, out, stream)
 
@@ -137,7 +138,12 @@ def paged_attention(q: torch.Tensor, cache: PagedKV, page_table: torch.Tensor,
     formula does; a score of -inf among others takes its key away.  Keys that a
     row's mask hides may hold anything.  Values are multiplied by
     zero there: an infinity or NaN in V reaches rows of the same sequence and
-    call that do not see its key."""
+    call that do not see its key; over codes, with float16 queries and more than
+    16 rows of a KV head, that holds for values which float16 cannot hold, too.
+
+    Scores and sums are float32.  Probabilities are rounded to q's type before
+    they meet V (over codes and up to 16 rows of a KV head to float16, the values'
+    scales in them): about 1.4 times the error of rounding the result alone."""
     if q.dim() != 3:
         raise ValueError("q must be [tokens, heads, head_dim]")
     tokens, heads, dim = q.shape

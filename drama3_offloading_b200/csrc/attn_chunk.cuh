@@ -16,9 +16,9 @@
 // Bound: the tensor pipe for D = 256 (2048 cycles a block against about 1300
 // for the exponentials of 128 x 128 scores on one warpgroup), the exponentials
 // for D = 128.  Measured, 2048 tokens over 14000, pages of 64: 16 heads of 256
-// over 2 in bf16 1425 TFLOP/s, 32 of 128 over 8 in fp16 975; the former, run for
+// over 2 in bf16 1425 TFLOP/s, 32 of 128 over 8 in fp16 983; the former, run for
 // seconds, is held by the power limit.  Pages of 16 hold 16-bit caches back
-// (1054 and 647): their loading threads issue twelve small boxes a block.
+// (1095 and 635): their loading threads issue many small boxes a block.
 // Codes reach 860 and 560, bound by instruction-cache misses (six of ten
 // cycles issue nothing): the widening and the softmax are different code on
 // the same schedulers, which is why their loops are kept short.

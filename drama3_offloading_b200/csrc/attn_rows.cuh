@@ -25,8 +25,9 @@
 // go to the workspace (two places per CTA) and are joined by
 // attn_join_kernel in the order of the parts: results do not depend on timing.
 // Measured: 4 tokens over 8 heads x 100000 and more keys read 6.7 TB/s, 64
-// ragged sequences of codes 4.3 (a piece costs its start and its join); one
-// token over a short context is 9 us of latency.
+// ragged sequences of codes 4.4 (a warp's products and softmax of a tile come one
+// after the other; a piece costs its start and its join); one token over a short
+// context is 9 us of latency.
 //
 // e4m3 caches: codes are exact in fp16, so the products run in fp16 whatever
 // the queries' type.  bf16 queries are scaled by a power of two per row that

