@@ -633,9 +633,10 @@ __global__ void __launch_bounds__(RowsCfg<T, D, E4, NT>::THREADS, 1)
         const uint32_t vb = smem_u32(s_slots + (size_t)slot * C::SLOT) + mine;
         if (E4) {
           // values' scales in units of vref, a power of two not below any yet
+          // (a caller's own scales may be negative)
           u0 = key0 + g < w.s.kv ? u0 : 0.f;
           u1 = key0 + g + 8 < w.s.kv ? u1 : 0.f;
-          float vmax = fmaxf(u0, u1);
+          float vmax = fmaxf(fabsf(u0), fabsf(u1));
 #pragma unroll
           for (int x = 4; x < 32; x <<= 1) vmax = fmaxf(vmax, __shfl_xor_sync(0xffffffffu, vmax, x));
           if (vmax > vref) {

@@ -330,3 +330,17 @@ def test_a_negative_zero_keeps_its_sign(dim, dtype):
         back = kvcache.read(cache, slots, dtype=dtype)[1]
         want = (code.float() * scale[..., None]).to(dtype)
         assert torch.equal(back.view(torch.int16), want.view(torch.int16))
+
+
+@pytest.mark.parametrize("dim,heads,hk,page,dtype", [(256, 8, 2, 64, BF), (128, 8, 2, 16, FP)])
+@pytest.mark.parametrize("n", [1, 2, 40])
+@pytest.mark.parametrize("share", [0.5, 1.0])
+def test_negative_scales(dim, heads, hk, page, dtype, n, share):
+    """A caller's own cache (value = code * scale) may have them, here and there
+    or everywhere."""
+    c = batch(11, [(n, 300), (n, 70)], heads, hk, dim, page, dtype, E4)
+    g = torch.Generator(device=DEV).manual_seed(4)
+    for s in (c[0].k_scale, c[0].v_scale):
+        turn = torch.rand(s.shape, generator=g, device=DEV) < share
+        s.mul_(torch.where(turn, -1.0, 1.0)).mul_(2.0 ** torch.randint(-3, 4, s.shape, generator=g, device=DEV))
+    check(call(c), *ref.attention(c[2], c[0], c[1], c[4], c[3]))
