@@ -167,7 +167,7 @@ __device__ __forceinline__ int rows_tiles(int kv, int keys) { return max(1, (kv 
 // Lengths of the list add up to kListMost at most.  The host has checked that
 // sequences which share no row stay below it; offsets that go back and forth
 // can give every sequence all of the rows.  A list that reaches it has no parts:
-// the call records an error and writes nothing.
+// the kernel records an error and writes nothing.
 constexpr int kListMost = 0x7fffffff;
 __device__ __forceinline__ int list_add(int a, int b) { return (int)min((unsigned)a + (unsigned)b, (unsigned)kListMost); }
 __device__ __forceinline__ int list_total(const AttnParams& p, int total) {

@@ -465,8 +465,8 @@ D3_API int d3_qk_norm_rope(const d3_norm_rope* a, const d3_kv_cache* cache, d3_s
  * workspace: at least d3_paged_attention_workspace_size bytes, 16-byte
  * aligned, of this call's own until it ends.  *err_word: 51 .. 57 when a
  * bounded wait (2 s) ran out, 58 when cu_q goes back and forth so that its
- * sequences have more work than the call's rows could (nothing is written
- * then).  No counterpart in the reference. */
+ * sequences have more work than the call's rows could (the kernel that counts
+ * it writes nothing then).  No counterpart in the reference. */
 typedef struct d3_attention {
   const void* q;                        /* [tokens][heads][head_dim] */
   int64_t q_token, q_head;
